@@ -271,6 +271,72 @@ int forge_linear_small(int dtype, int M, int N, int K, const void* x, int64_t sx
                        int gain_dtype, int norm, float eps, const void* residual, int64_t sr,
                        void* out, int64_t so, void* stream);
 
+/*
+ * ---- The paged cache (no counterpart in the reference, whose cache is one slab of max_len per row).
+ * Pools k_pages, v_pages [n_pages, K, page_size, D] (strides skp, skh, sks; last dim contiguous) hold
+ * runs of page_size positions (a power of two, at least 16) of every KV head. Position s of batch row b is
+ * slot s % page_size of page page_table[b * s_table + s / page_size], int32, max_pages entries per row.
+ * An entry outside [0, n_pages) -- -1 by convention: never given, or given back -- is never read through
+ * nor written: its keys are invisible, whatever the window says. Rows may share pages (a common prefix).
+ * row_pos [B] int32: the tokens each row held before the call; new_lens [B] int32 or NULL: how many of
+ * the T new tokens of a row are real (a padded batch); NULL: all.
+ * All of it is read on the device, so a recorded graph replays with new tables, positions and lengths.
+ * 16-byte aligned tensors and strides.
+ *
+ * forge_kv_append_paged: forge_kv_append into pages. Token t < new_lens[b] of row b goes to position
+ * row_pos[b] + t; padded tokens and positions without a page are not written. k and v of one call
+ * must not name one (page, slot) twice.
+ */
+int forge_kv_append_paged(int dtype, int B, int T, int K, int D, const void* k, int64_t skb,
+                          int64_t skh, int64_t skt, const void* v, int64_t svb, int64_t svh,
+                          int64_t svt, void* k_pages, void* v_pages, int64_t sdp, int64_t sdh,
+                          int64_t sds, int n_pages, int page_size, const int32_t* page_table,
+                          int64_t s_table, int max_pages, const int32_t* row_pos,
+                          const int32_t* new_lens, const float* k_weight, float eps, int flags,
+                          const float* cos, const float* sin, int64_t s_cos_b, int64_t s_cos_t,
+                          void* stream);
+
+/*
+ * Attention of T new tokens per row over the paged cache, which holds them already: a decode step
+ * (T = 1), a verify step, a chunk of a prompt, rows of different lengths and different numbers of new
+ * tokens. Query t of row b sits at p = row_pos[b] + t and sees key s iff s <= p and
+ * (window == 0, or s > p - window, or s < sinks): with a window, the first `sinks` positions stay
+ * visible. Head dims 32, 64, 128, 256, and 512 in bf16/fp16. q as in forge_attn_decode (raw with
+ * FORGE_NORM_QK / FORGE_ROPE). max_kv_len: host upper bound on row_pos[b] + new_lens[b] (at most
+ * max_pages * page_size; positions from it on do not exist for the call). Rows t >= new_lens[b], and
+ * rows that see no key, come out as zeros.
+ * workspace: forge_attn_paged_workspace_bytes(...) bytes (256-byte aligned) of fp32 partials, where the
+ * keys of a row are split over blocks; NULL: not split. Calls that may overlap need separate ones.
+ * The order of the sums depends on the shapes and bounds of the call alone.
+ */
+size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
+                                        int64_t max_kv_len, int window, int sinks);
+int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb,
+                     int64_t sqh, int64_t sqt, const float* q_weight, float eps, int flags,
+                     const float* cos, const float* sin, int64_t s_cos_b, int64_t s_cos_t,
+                     const void* k_pages, const void* v_pages, int64_t skp, int64_t skh,
+                     int64_t sks, int n_pages, int page_size, const int32_t* page_table,
+                     int64_t s_table, int max_pages, const int32_t* row_pos,
+                     const int32_t* new_lens, int64_t max_kv_len, int window, int sinks,
+                     float scale, void* out, int64_t sob, int64_t sot, int64_t soh,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same attention over a contiguous cache [B, K, max_len, D] for sliding-window layers whose first
+ * `sinks` positions stay visible (window > 0; sinks 0: the plain window). Positions as in
+ * forge_attn_decode: row_pos, pos_dev or pos0. Any T: prompts, chunks, verify and decode steps.
+ */
+size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
+                                        int64_t max_kv_len, int window, int sinks);
+int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb,
+                     int64_t sqh, int64_t sqt, const float* q_weight, float eps, int flags,
+                     const float* cos, const float* sin, int64_t s_cos_b, int64_t s_cos_t,
+                     const void* k_cache, const void* v_cache, int64_t skb, int64_t skh,
+                     int64_t sks, int64_t max_len, const int32_t* row_pos, const int64_t* pos_dev,
+                     int64_t pos0, int64_t max_kv_len, int window, int sinks, float scale,
+                     void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,41 @@ SIGNATURES: dict[str, tuple] = {
         _p, _i64,                            # residual, row stride
         _p, _i64,                            # out, row stride
         _p]),
+    "forge_kv_append_paged": (_i, [
+        _i, _i, _i, _i, _i,                  # dtype, B, T, K, D
+        _p, _i64, _i64, _i64,                # k + strides
+        _p, _i64, _i64, _i64,                # v + strides
+        _p, _p, _i64, _i64, _i64,            # k_pages, v_pages, sdp, sdh, sds
+        _i, _i, _p, _i64, _i,                # n_pages, page_size, page_table, s_table, max_pages
+        _p, _p,                              # row_pos, new_lens
+        _p, _f, _i,                          # k_weight, eps, flags
+        _p, _p, _i64, _i64,                  # cos, sin, s_cos_b, s_cos_t
+        _p]),
+    "forge_attn_paged_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
+    "forge_attn_paged": (_i, [
+        _i, _i, _i, _i, _i, _i,              # dtype, B, T, H, K, D
+        _p, _i64, _i64, _i64,                # q + strides
+        _p, _f, _i,                          # q_weight, eps, flags
+        _p, _p, _i64, _i64,                  # cos, sin, s_cos_b, s_cos_t
+        _p, _p, _i64, _i64, _i64,            # k_pages, v_pages, skp, skh, sks
+        _i, _i, _p, _i64, _i,                # n_pages, page_size, page_table, s_table, max_pages
+        _p, _p, _i64,                        # row_pos, new_lens, max_kv_len
+        _i, _i, _f,                          # window, sinks, scale
+        _p, _i64, _i64, _i64,                # out + strides (b, t, h)
+        _p, C.c_size_t,                      # workspace, bytes
+        _p]),
+    "forge_attn_sinks_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
+    "forge_attn_sinks": (_i, [
+        _i, _i, _i, _i, _i, _i,              # dtype, B, T, H, K, D
+        _p, _i64, _i64, _i64,                # q + strides
+        _p, _f, _i,                          # q_weight, eps, flags
+        _p, _p, _i64, _i64,                  # cos, sin, s_cos_b, s_cos_t
+        _p, _p, _i64, _i64, _i64, _i64,      # k_cache, v_cache, skb, skh, sks, max_len
+        _p, _p, _i64, _i64,                  # row_pos, pos_dev, pos0, max_kv_len
+        _i, _i, _f,                          # window, sinks, scale
+        _p, _i64, _i64, _i64,                # out + strides (b, t, h)
+        _p, C.c_size_t,                      # workspace, bytes
+        _p]),
 }
 
 _lock = threading.Lock()

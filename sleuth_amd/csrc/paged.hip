@@ -1,0 +1,515 @@
+// Attention of new tokens over a paged cache, and over a contiguous one with a sliding window whose
+// first tokens stay visible (forge_attn_paged, forge_attn_sinks).
+//
+// Row b's new token t sits at position p = base_b + t and sees key s iff
+//   s <= p  and  (no window, or s > p - window, or s < sinks),
+// so a row's visible keys are one run, or two with a window: the first `sinks` keys and the window.
+// out = sum_s w_s v_s / sum_s w_s,  w_s = exp(scale q.k_s - m), m the running maximum: one pass over
+// the keys, statistics and sums in fp32. A contiguous cache is a paged one with one page per batch row.
+//
+// The G * T query rows (token, head of the group) of one KV head share its keys: row r is token r / G,
+// head r % G of the group. Both kernels below take blocks of such rows, so a key row loaded once serves
+// every head of the group, and a step of few tokens still fills matrix-core tiles.
+#include <limits.h>
+
+#include "paged.h"
+
+namespace forge {
+
+// ---------------------------------------------------------------- matrix-core steps
+// 16x16 tiles. Lane (n, g) = (lane % 16, lane / 16) gives row n of A and column n of B, k-slots of
+// group g, and receives column n, rows 4g .. 4g+3 of C. Scores are computed transposed
+// (S^T = K . Q^T: A = 16 keys, B = 16 query rows), so a lane owns ONE query row and four keys of each
+// key block: the row maximum takes two exchanges (lanes 16 and 32 away), the row sum none until the
+// end, and the weights are already where the second product O^T = V^T . P^T wants its B operand.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Mma;
+template <> struct Mma<bf16> {
+  static __device__ __forceinline__ f32x4 k32(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 k16(i16x4 a, i16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct Mma<f16> {
+  static __device__ __forceinline__ f32x4 k32(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 k16(i16x4 a, i16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mma<float> {
+  // 16 bytes are four channels: four products of one channel per group
+  static __device__ __forceinline__ f32x4 k32(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[e]), __uint_as_float(b[e]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four groups of one query row). Swapping x with
+// itself returns both halves of each pair, so both lanes combine the same two values.
+template <bool MAX> __device__ __forceinline__ float over_groups(float x) {
+  unsigned u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned a0 = a[0], a1 = a[1];
+  x = MAX ? fmaxf(__uint_as_float(a0), __uint_as_float(a1)) : __uint_as_float(a0) + __uint_as_float(a1);
+  u = __float_as_uint(x);
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned b0 = b[0], b1 = b[1];
+  return MAX ? fmaxf(__uint_as_float(b0), __uint_as_float(b1)) : __uint_as_float(b0) + __uint_as_float(b1);
+}
+
+// ---------------------------------------------------------------- split kernel
+// A block of four waves takes ROWS = 16 RB query rows of one (batch row, KV head) and a part of their
+// key tiles. Each wave streams tiles of its own (tile i goes to wave i % 4) through registers into LDS
+// that only it uses, so no wave waits for another until the end: the tile in registers is the prefetch
+// of the next one. The waves' (m, l, O) meet in LDS once, at the end.
+template <typename T, int D, int RB> struct StepTile {
+  static_assert(16 * RB <= step_rows_most(sizeof(T), D), "registers");
+  static constexpr int ROWB = D * (int)sizeof(T);        // bytes of a key row
+  static constexpr int NCH = ROWB / 16;                  // 16-byte chunks of it
+  static constexpr int KT = step_keys(sizeof(T), D, 16 * RB);  // keys per wave tile
+  static constexpr int KB = KT / 16;                     // 16-key blocks
+  static constexpr int RPI = 64 / NCH;                   // key rows per wave load instruction
+  static constexpr int NL = KT / RPI;                    // load instructions per K (or V) tile
+  static constexpr int TILEB = KT * ROWB;
+  static constexpr int RP = ROWB >= 256 ? 1 : 256 / ROWB;  // key rows per 256-byte bank line
+};
+
+// Chunk swizzles by key row. K operands: 16 rows of one chunk at a time, so the chunk index turns with
+// the row. V operands: in 16 bits 16 rows of two neighbouring chunks (32 bytes), in fp32 four rows 4
+// apart of four chunks (64 bytes).
+template <typename T, int D> __device__ __forceinline__ int step_swz_k(int row) {
+  using TL = StepTile<T, D, 1>;
+  return (row / TL::RP) & ((TL::NCH < 16 ? TL::NCH : 16) - 1);
+}
+template <typename T, int D> __device__ __forceinline__ int step_swz_v(int row) {
+  using TL = StepTile<T, D, 1>;
+  if constexpr (sizeof(T) == 4) return ((row >> 2) << 2) & ((TL::NCH < 16 ? TL::NCH : 16) - 1);
+  else return ((row / TL::RP) << 1) & ((TL::NCH < 16 ? TL::NCH : 16) - 1);
+}
+
+// Query row `row` (a row that exists) as B operands: chunk 4s + g in q[s], with RMSNorm and RoPE in
+// fp32 and one rounding.
+template <typename T, int D>
+__device__ __forceinline__ void step_load_q(const PagedParams& p, int b, int kvh, int row, int g,
+                                            u32x4 (&q)[StepTile<T, D, 1>::NCH / 4]) {
+  constexpr int NCH = StepTile<T, D, 1>::NCH, S = NCH / 4, E = 16 / sizeof(T);
+  const int t = row / p.G, h = kvh * p.G + row % p.G;
+  const T* src = static_cast<const T*>(p.q) + b * p.sqb + h * p.sqh + t * p.sqt;
+#pragma unroll
+  for (int s = 0; s < S; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + (4 * s + g) * E);
+  const bool norm = p.flags & FORGE_NORM_QK, rope = p.flags & FORGE_ROPE;
+  if (!norm && !rope) return;
+  float f[S][E];
+#pragma unroll
+  for (int s = 0; s < S; ++s) unpack16<T>(__builtin_bit_cast(uint4, q[s]), f[s]);
+  if (norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss += f[s][e] * f[s][e];
+    const float rs = rsqrtf(over_groups<false>(ss) / (float)D + p.eps);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float w[E];
+      if (p.qw) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(p.qw + (4 * s + g) * E + e);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[s][e] = p.qw ? f[s][e] * rs * w[e] : f[s][e] * rs;
+    }
+  }
+  if (rope) {
+    const float* cr = p.cos + b * p.csb + t * p.cst;
+    const float* sr = p.sin + b * p.csb + t * p.cst;
+    if constexpr (S >= 2) {  // the pair (c, c + D/2) is in one lane
+#pragma unroll
+      for (int s = 0; s < S / 2; ++s)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int c = (4 * s + g) * E + e;
+          const float a = f[s][e], z = f[s + S / 2][e];
+          f[s][e] = a * cr[c] - z * sr[c];
+          f[s + S / 2][e] = z * cr[c + D / 2] + a * sr[c + D / 2];
+        }
+    } else {  // 16 bits, head dim 32: the partner channel is two groups away
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = g * E + e;
+        const float o = __shfl_xor(f[0][e], 32, kWave);
+        f[0][e] = f[0][e] * cr[c] + (g < 2 ? -o : o) * sr[c];
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if constexpr (sizeof(T) < 4) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[s][e] = fp32_result(f[s][e]);
+    }
+    q[s] = __builtin_bit_cast(u32x4, pack16<T>(f[s]));
+  }
+}
+
+template <typename T, int D, int RB> struct StepLds {
+  using TL = StepTile<T, D, RB>;
+  static constexpr int ROWS = 16 * RB;
+  static constexpr int OUT = ROWS * D * 4;                                // a wave's output in fp32
+  static constexpr int WAVE = 2 * TL::TILEB > OUT ? 2 * TL::TILEB : OUT;  // a wave's K and V tile, later its output
+  static constexpr int BYTES = 4 * WAVE + 4 * ROWS * 8;                   // and (m, l) of every wave's rows
+  static constexpr int BLOCKS = BYTES <= 80 * 1024 && TL::KT == 32 ? 2 : 1; // per CU: by its 160 KB, and by registers
+};
+
+template <typename T, int D, int RB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(StepLds<T, D, RB>::BLOCKS)))
+void paged_step_kernel(PagedParams p) {
+  using TL = StepTile<T, D, RB>;
+  using LD = StepLds<T, D, RB>;
+  constexpr int KT = TL::KT, KB = TL::KB, NL = TL::NL, S = TL::NCH / 4, DB = D / 16, ROWS = LD::ROWS;
+  constexpr int GROUPS = KT / 16;
+
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int n = lane & 15, g = lane >> 4;
+
+  int part, rblk, b, kvh;
+  block_unit(p, (p.rows + ROWS - 1) / ROWS, part, rblk, b, kvh);
+  const RowSpan w = row_span(p, b, rblk * ROWS, ROWS, KT);
+  const int begin = part * p.tiles_per_part;
+  const int end = begin + p.tiles_per_part < w.tiles ? begin + p.tiles_per_part : w.tiles;
+  const bool whole = w.tiles <= p.tiles_per_part;
+  if (part > 0 && begin >= w.tiles) return;
+
+  // ---- key tiles of this wave: begin + wave, + 4, ...
+  u32x4 kr[NL], vr[NL];
+  const int lrow = lane / TL::NCH, lch = lane % TL::NCH;
+  const char* kb0 = static_cast<const char*>(p.k) + kvh * p.skh * (int64_t)sizeof(T);
+  const char* vb0 = static_cast<const char*>(p.v) + kvh * p.skh * (int64_t)sizeof(T);
+  const int64_t pageb = p.skp * (int64_t)sizeof(T);
+  const int rowb = (int)(p.sks * (int64_t)sizeof(T));
+  unsigned bad = 0;  // bit i: 16-key group i of the tile in kr/vr lies in no page of the pool
+  auto load = [&](int i) {
+    const int key0 = w.tile_key(i, KT);
+    const int left = w.last - key0;  // the tile's last row that exists
+    unsigned miss = 0;
+    int64_t base[GROUPS];
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      // (a group past the row's last key reads that key instead)
+      const int key = key0 + (16 * j <= left ? 16 * j : left & ~15);
+      const int page = p.page_of(b, key);
+      if (page < 0) miss |= 1u << j;
+      base[j] = page * pageb + (int64_t)(key & p.page_mask) * rowb;
+    }
+    if (miss == 0) {
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        int row = j * TL::RPI % 16 + lrow;
+        if (left < KT - 1) {
+          const int in = j * TL::RPI / 16 * 16;   // the group's first row
+          const int most = in <= left ? left - in : left & 15;
+          row = row < most ? row : most;
+        }
+        const unsigned off = (unsigned)(row * rowb + lch * 16);
+        const int64_t at = base[j * TL::RPI / 16];
+        kr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb0 + at + off));
+        vr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vb0 + at + off));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NL; ++j) {
+        int row = j * TL::RPI % 16 + lrow;
+        const int in = j * TL::RPI / 16 * 16;
+        const int most = in <= left ? left - in : left & 15;
+        row = row < most ? row : most;
+        const unsigned off = (unsigned)(row * rowb + lch * 16);
+        const int64_t at = base[j * TL::RPI / 16];
+        kr[j] = u32x4{0, 0, 0, 0};
+        vr[j] = u32x4{0, 0, 0, 0};
+        if (!(miss >> (j * TL::RPI / 16) & 1)) {
+          kr[j] = *reinterpret_cast<const u32x4*>(kb0 + at + off);
+          vr[j] = *reinterpret_cast<const u32x4*>(vb0 + at + off);
+        }
+      }
+    }
+    bad = miss;
+  };
+  int i = begin + wave;
+  constexpr bool kLate = D >= 512;  // (registers: the first tile after the query rows)
+  if (!kLate && i < end) load(i);
+
+  // ---- query rows, as B operands; rows behind the row's last one stand for that one (never written)
+  u32x4 q[RB][S];
+  int qpos[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int row = rblk * ROWS + 16 * r + n;
+    const int at = row < w.rows ? row : w.rows - 1;
+    qpos[r] = w.base + at / p.G;
+    if (w.rows > 0) step_load_q<T, D>(p, b, kvh, at, g, q[r]);
+  }
+
+  if (kLate && i < end) load(i);
+
+  f32x4 o[RB][DB];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    m[r] = kNegInf;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[r][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float c = p.scale_log2;
+  char* kt = smem + wave * LD::WAVE;
+  char* vt = kt + TL::TILEB;
+
+  for (; i < end; i += 4) {
+    const int key0 = w.tile_key(i, KT);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int row = j * TL::RPI + lrow;
+      *reinterpret_cast<u32x4*>(kt + row * TL::ROWB + ((lch ^ step_swz_k<T, D>(row)) << 4)) = kr[j];
+      *reinterpret_cast<u32x4*>(vt + row * TL::ROWB + ((lch ^ step_swz_v<T, D>(row)) << 4)) = vr[j];
+    }
+    const unsigned miss = bad;
+    if (i + 4 < end) load(i + 4);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (this wave's tile: LDS keeps a wave's order)
+    __builtin_amdgcn_wave_barrier();
+
+    f32x4 s[RB][KB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) s[r][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < S; ++st)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int row = 16 * kb + n;
+        const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * TL::ROWB + (((4 * st + g) ^ step_swz_k<T, D>(row)) << 4));
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s[r][kb] = Mma<T>::k32(a, q[r][st], s[r][kb]);
+      }
+
+    // a tile that every row of the block sees whole needs no mask
+    const bool full = miss == 0 && key0 + KT - 1 <= w.first &&
+                      (p.window <= 0 || key0 > w.last - p.window || key0 + KT <= p.sinks);
+    if (!full) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int lo = p.window > 0 ? qpos[r] - p.window : -1;  // keys above it, or first tokens
+        const int hi = qpos[r] < w.last ? qpos[r] : w.last;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = key0 + 16 * kb + 4 * g + j;
+            const bool see = key <= hi && (key > lo || key < p.sinks) && !(miss >> kb & 1);
+            s[r][kb][j] = see ? s[r][kb][j] : kNegInf;
+          }
+      }
+    }
+
+    // online softmax in base 2, the scale folded into the exponent; the reference maximum moves only
+    // when a score passes it by 2^8 (weights stay <= 2^8, safe in 16 bits), so rescaling is rare
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      float mx = s[r][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[r][kb][j]);
+      mx = over_groups<true>(mx) * c;
+      if (mx > m[r] + 8.0f) {
+        const float a = m[r] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[r] - mx);
+        l[r] *= a;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[r][d] *= a;
+        m[r] = mx;
+      }
+      const float neg = m[r] == kNegInf ? 0.0f : -m[r];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w8 = __builtin_amdgcn_exp2f(fmaf(s[r][kb][j], c, neg));
+          s[r][kb][j] = w8;
+          l[r] += w8;
+        }
+    }
+
+    // O^T += V^T . P^T; the k-slots of a lane are the keys whose weights it holds
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 16 * kb + 4 * g + j;
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const int ch = 4 * d + (n >> 2);
+            const float a = *reinterpret_cast<const float*>(vt + row * TL::ROWB + ((ch ^ step_swz_v<T, D>(row)) << 4) + 4 * (n & 3));
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+              o[r][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, s[r][kb][j], o[r][d], 0, 0, 0);
+          }
+        }
+    } else {
+      // transposing LDS reads: in each 16-lane group lane 4k + i/4 addresses 4 channels of key k and
+      // lane i receives channel i of the four keys
+      i16x4 w4[RB][KB];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          T x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(s[r][kb][j]);
+          w4[r][kb] = *reinterpret_cast<const i16x4*>(x);
+        }
+      const int vrow = 4 * g + (n >> 2);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        i16x4 a4[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const int row = 16 * kb + vrow, ch = 2 * d + ((n & 3) >> 1);
+          const unsigned at = lds_offset(vt) + row * TL::ROWB + ((ch ^ step_swz_v<T, D>(row)) << 4) + 8 * (n & 1);
+          a4[kb] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          if constexpr (KB == 2) {
+            const i16x8 a = __builtin_shufflevector(a4[0], a4[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            const i16x8 x = __builtin_shufflevector(w4[r][0], w4[r][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            o[r][d] = Mma<T>::k32(__builtin_bit_cast(u32x4, a), __builtin_bit_cast(u32x4, x), o[r][d]);
+          } else {
+            o[r][d] = Mma<T>::k16(a4[0], w4[r][0], o[r][d]);
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- the four waves' rows meet: each scales its own to the common maximum and puts it into its LDS
+  // region (16-byte pieces turned with the row), then all threads add the four
+  float2* ml = reinterpret_cast<float2*>(smem + 4 * LD::WAVE);  // [wave][ROWS]
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    l[r] = over_groups<false>(l[r]);
+    if (g == 0) ml[wave * ROWS + 16 * r + n] = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+  constexpr int Q4 = D / 4;  // float4 pieces of a row
+  float4* mine = reinterpret_cast<float4*>(smem + wave * LD::WAVE);
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int row = 16 * r + n;
+    float M = kNegInf;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, ml[x * ROWS + row].x);
+    const float a = rescale(m[r], M);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const int piece = (4 * d + g) ^ (n & (Q4 < 16 ? Q4 - 1 : 15));
+      mine[row * Q4 + piece] = make_float4(o[r][d][0] * a, o[r][d][1] * a, o[r][d][2] * a, o[r][d][3] * a);
+    }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < ROWS * Q4; x += 256) {
+    const int row = x / Q4, c4 = x % Q4;
+    const int flat = rblk * ROWS + row;
+    if (flat >= p.rows) break;
+    const bool real = flat < w.rows;
+    float M = kNegInf, L = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) M = fmaxf(M, ml[y * ROWS + row].x);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float2 e = ml[y * ROWS + row];
+      L += rescale(e.x, M) * e.y;
+      const float4 f = reinterpret_cast<const float4*>(smem + y * LD::WAVE)[row * Q4 + (c4 ^ (row & (Q4 < 16 ? Q4 - 1 : 15)))];
+      acc.x += f.x;
+      acc.y += f.y;
+      acc.z += f.z;
+      acc.w += f.w;
+    }
+    if (whole || !real) {
+      store_row<T>(p, b, kvh, flat, 4 * c4, acc, real && L > 0.0f ? 1.0f / L : 0.0f);
+    } else {
+      const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts + part;
+      *reinterpret_cast<float4*>(p.ws_o + slot * D + 4 * c4) = acc;
+      if (c4 == 0) p.ws_ml[slot] = make_float2(M, L);
+    }
+  }
+}
+
+template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hipStream_t s) {
+  using LD = StepLds<T, D, RB>;
+  static bool attr_set = false;
+  if (LD::BYTES > 64 * 1024 && !attr_set) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, LD::BYTES) != hipSuccess)
+      return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
+    attr_set = true;
+  }
+  const int64_t blocks = (int64_t)((p.rows + LD::ROWS - 1) / LD::ROWS) * p.K * p.B * p.nparts;
+  if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
+  hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)blocks), dim3(256), LD::BYTES, s, p);
+  int st = check_launch();
+  if (st == 0 && p.nparts > 1) st = launch_paged_combine<T, D>(p, LD::ROWS, StepTile<T, D, RB>::KT, s);
+  return st;
+}
+
+template <typename T, int D> static int launch_step(const PagedParams& p, const PagedPlan& plan, hipStream_t s) {
+  constexpr int MOST = step_rows_most(sizeof(T), D);
+  if (plan.rows == 16) return launch_step_rb<T, D, 1>(p, s);
+  if constexpr (MOST >= 32) {
+    if (plan.rows == 32) return launch_step_rb<T, D, 2>(p, s);
+  }
+  if constexpr (MOST >= 64) {
+    if (plan.rows == 64) return launch_step_rb<T, D, 4>(p, s);
+  }
+  return set_error("forge_attn_paged: no kernel of this row block");
+}
+
+template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
+  switch (D) {
+    case 32: return launch_step<T, 32>(p, plan, s);
+    case 64: return launch_step<T, 64>(p, plan, s);
+    case 128: return launch_step<T, 128>(p, plan, s);
+    case 256: return launch_step<T, 256>(p, plan, s);
+    case 512:
+      if constexpr (sizeof(T) == 2) return launch_step<T, 512>(p, plan, s);
+    default: return set_error("forge_attn_paged: unsupported head dim");
+  }
+}
+
+#if FORGE_PAGED_PART == 1
+template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 2
+template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 3
+template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#endif
+
+}  // namespace forge

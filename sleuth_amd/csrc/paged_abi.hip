@@ -1,0 +1,166 @@
+// Entry points of the paged cache and of attention with sinks (kernels: paged.hip): argument checks, the
+// cut of a call into blocks, the launch.
+#include <limits.h>
+
+#include "paged.h"
+
+namespace forge {
+
+extern template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+extern template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+extern template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+
+static bool paged_dim_ok(int dtype, int D) {
+  return D == 32 || D == 64 || D == 128 || D == 256 || (D == 512 && dtype != FORGE_F32);
+}
+
+// Rows per block, keys per tile and the key split of a call whose rows hold at most max_kv keys.
+static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_kv, int window, int sinks,
+                            bool split) {
+  PagedPlan plan{};
+  const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
+  const int64_t rows = (int64_t)G * T;
+  const int most = step_rows_most(es, D);
+  plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  if (plan.rows > most) plan.rows = most;
+  plan.keys = step_keys(es, D, plan.rows);
+  plan.nparts = 1;
+  // tiles that a block can have: its queries' window and the first tokens, or the whole row
+  const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
+  int64_t keys = max_kv;
+  if (window > 0 && window + tokens + sinks < keys) keys = window + tokens + sinks;
+  const int64_t tiles = (keys + plan.keys - 1) / plan.keys + 3;
+  plan.tiles_per_part = (int)tiles;
+  if (!split) return plan;
+  const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
+  const int64_t want = (4 * (int64_t)device_cus() + units - 1) / units;
+  int64_t per = (tiles + want - 1) / want;
+  if (per < 8) per = 8;  // two tiles for each wave
+  const int64_t parts = (tiles + per - 1) / per;
+  if (parts > 1) {
+    plan.nparts = (int)parts;
+    plan.tiles_per_part = (int)per;
+  }
+  return plan;
+}
+
+static size_t paged_ws_bytes(const PagedPlan& plan, int B, int T, int H, int D) {
+  if (plan.nparts < 2) return 0;
+  const size_t slots = (size_t)B * H * T * plan.nparts;
+  return (slots * 8 + 255) / 256 * 256 + slots * D * 4;
+}
+
+static bool unaligned(const void* p) { return (uintptr_t)p % 16 != 0; }
+
+// Checks what both entry points share, cuts the call and launches it.
+static int paged_run(int dtype, int D, PagedParams p, float scale, void* workspace, size_t workspace_bytes,
+                     hipStream_t s) {
+  if (dtype != FORGE_F32 && dtype != FORGE_BF16 && dtype != FORGE_F16) return set_error("unknown dtype code");
+  if (p.B < 0 || p.T < 0 || p.H <= 0 || p.K <= 0 || p.H % p.K) return set_error("bad sizes (H must be a multiple of K)");
+  if (!paged_dim_ok(dtype, D)) return set_error("head dim must be 32, 64, 128, 256 (or 512 in bf16/fp16)");
+  if (!p.q || !p.k || !p.v || !p.out) return set_error("null tensor pointer");
+  if (p.window < 0 || p.sinks < 0 || p.window > INT_MAX / 2 || p.sinks > INT_MAX / 2)
+    return set_error("window and sinks must not be negative");
+  if (p.sinks > 0 && p.window == 0) return set_error("sinks need a window (without one every key is visible)");
+  const int64_t es = dtype == FORGE_F32 ? 4 : 2, e16 = 16 / es;
+  for (const int64_t st : {p.sqb, p.sqh, p.sqt, p.skp, p.skh, p.sks, p.sob, p.soh, p.sot})
+    if (st < 0 || st % e16) return set_error("strides must be multiples of 16 bytes");
+  if (unaligned(p.q) || unaligned(p.k) || unaligned(p.v) || unaligned(p.out))
+    return set_error("q, k, v and out must be 16-byte aligned");
+  if (p.sks < D || p.sks > INT_MAX / 16 / 64) return set_error("cache positions must be head dim to 2^21 elements apart");
+  if ((p.flags & FORGE_NORM_QK) && p.qw && unaligned(p.qw)) return set_error("the norm gain must be 16-byte aligned");
+  if ((p.flags & FORGE_ROPE) && (!p.cos || !p.sin)) return set_error("FORGE_ROPE needs cos and sin");
+  p.G = p.H / p.K;
+  if ((int64_t)p.G * p.T > INT_MAX / 2) return set_error("too many query rows");
+  if (p.B == 0 || p.T == 0) return 0;
+  p.rows = p.G * p.T;
+  p.scale_log2 = scale * kLog2e;
+  const bool split = workspace != nullptr;
+  const PagedPlan plan = paged_plan(dtype, p.B, p.T, p.H, p.K, D, p.limit, p.window, p.sinks, split);
+  p.nparts = plan.nparts;
+  p.tiles_per_part = plan.tiles_per_part;
+  if (plan.nparts > 1) {
+    if (workspace_bytes < paged_ws_bytes(plan, p.B, p.T, p.H, D)) return set_error("workspace too small");
+    if ((uintptr_t)workspace % 256) return set_error("the workspace must be 256-byte aligned");
+    const size_t slots = (size_t)p.B * p.H * p.T * plan.nparts;
+    p.ws_ml = static_cast<float2*>(workspace);
+    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (slots * 8 + 255) / 256 * 256);
+  }
+  switch (dtype) {
+    case FORGE_F32: return launch_paged<float>(p, plan, D, s);
+    case FORGE_BF16: return launch_paged<bf16>(p, plan, D, s);
+    default: return launch_paged<f16>(p, plan, D, s);
+  }
+}
+
+}  // namespace forge
+
+using namespace forge;
+
+extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
+                                                   int window, int sinks) {
+  if (B <= 0 || T <= 0 || H <= 0 || K <= 0 || H % K || !paged_dim_ok(dtype, D) || max_kv_len <= 0 || window < 0 ||
+      sinks < 0)
+    return 0;
+  return paged_ws_bytes(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, true), B, T, H, D);
+}
+
+extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
+                                int64_t sqt, const float* q_weight, float eps, int flags, const float* cos,
+                                const float* sin, int64_t s_cos_b, int64_t s_cos_t, const void* k_pages,
+                                const void* v_pages, int64_t skp, int64_t skh, int64_t sks, int n_pages, int page_size,
+                                const int32_t* page_table, int64_t s_table, int max_pages, const int32_t* row_pos,
+                                const int32_t* new_lens, int64_t max_kv_len, int window, int sinks, float scale,
+                                void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
+  if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
+  if (!page_table || !row_pos) return set_error("null page table or row positions");
+  if (max_kv_len <= 0) return set_error("max_kv_len must be positive");
+  int64_t limit = (int64_t)max_pages * page_size;
+  if (max_kv_len < limit) limit = max_kv_len;
+  if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
+  PagedParams p{};
+  p.q = q; p.sqb = sqb; p.sqh = sqh; p.sqt = sqt;
+  p.qw = q_weight; p.eps = eps; p.flags = flags;
+  p.cos = cos; p.sin = sin; p.csb = s_cos_b; p.cst = s_cos_t;
+  p.k = k_pages; p.v = v_pages; p.skp = skp; p.skh = skh; p.sks = sks;
+  p.table = page_table; p.spt = s_table; p.max_pages = max_pages; p.npages = n_pages;
+  p.page_shift = __builtin_ctz((unsigned)page_size); p.page_mask = page_size - 1;
+  p.row_pos = row_pos; p.new_lens = new_lens;
+  p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
+  p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
+  return paged_run(dtype, D, p, scale, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+extern "C" size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
+                                                   int window, int sinks) {
+  return forge_attn_paged_workspace_bytes(dtype, B, T, H, K, D, max_kv_len, window, sinks);
+}
+
+extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
+                                int64_t sqt, const float* q_weight, float eps, int flags, const float* cos,
+                                const float* sin, int64_t s_cos_b, int64_t s_cos_t, const void* k_cache,
+                                const void* v_cache, int64_t skb, int64_t skh, int64_t sks, int64_t max_len,
+                                const int32_t* row_pos, const int64_t* pos_dev, int64_t pos0, int64_t max_kv_len,
+                                int window, int sinks, float scale, void* out, int64_t sob, int64_t sot, int64_t soh,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (window <= 0) return set_error("forge_attn_sinks needs a window");
+  if (max_kv_len <= 0 || max_len <= 0) return set_error("max_kv_len and max_len must be positive");
+  const int64_t limit = max_kv_len < max_len ? max_kv_len : max_len;
+  if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
+  if (!row_pos && !pos_dev && (pos0 < 0 || T < 0 || pos0 > limit - T))
+    return set_error("pos + T exceeds max_kv_len or the cache length");
+  PagedParams p{};
+  p.q = q; p.sqb = sqb; p.sqh = sqh; p.sqt = sqt;
+  p.qw = q_weight; p.eps = eps; p.flags = flags;
+  p.cos = cos; p.sin = sin; p.csb = s_cos_b; p.cst = s_cos_t;
+  p.k = k_cache; p.v = v_cache; p.skp = skb; p.skh = skh; p.sks = sks;
+  p.page_shift = 31; p.page_mask = 0x7fffffff; p.npages = B;
+  p.row_pos = row_pos; p.pos_dev = pos_dev; p.pos0 = pos0;
+  p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
+  p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
+  return paged_run(dtype, D, p, scale, workspace, workspace_bytes, (hipStream_t)stream);
+}

@@ -34,6 +34,13 @@ struct RowParams {
   const int64_t* pos_dev;
   int64_t pos0;
   int64_t dst_len;
+  // Paged destinations (forge_kv_append_paged): row drow of batch row b is slot drow % page_size of page
+  // table[b][drow / page_size], and db is the distance between pages. Tokens at or past new_lens[b]
+  // (null: T), and positions without a page of the pool, are not written.
+  const int32_t* table;
+  int64_t spt;
+  int max_pages, npages, page_shift;
+  const int32_t* new_lens;
 };
 
 template <typename T, int VEC>
@@ -59,7 +66,7 @@ __device__ __forceinline__ void store_vec(T* p, const float* in) {
 // A lane group handles RPL rows: RPL consecutive heads of one (b, t). They share the
 // token's RoPE row and the gain, so those are loaded once per group rather than once per
 // row, and the group has all RPL rows' loads in flight together.
-template <typename T, int VEC, int GW, int RPL>
+template <typename T, int VEC, int GW, int RPL, bool PAGED>
 __global__ __launch_bounds__(256) void row_norm_rope_kernel(RowParams p) {
   // No implicit contraction (fmas are written out, and a product is not folded into its
   // rounding to fp16): forge_attn_decode_append makes the same rows with the same
@@ -86,9 +93,16 @@ __global__ __launch_bounds__(256) void row_norm_rope_kernel(RowParams p) {
   const bool active = c0 < half;
 
   int64_t drow = t;
-  if (rt.at_pos) {
+  int64_t dpage = b;
+  if (PAGED || rt.at_pos) {
     drow = row_base(p.row_pos, p.pos_dev, p.pos0, b) + t;
     if (drow < 0 || drow >= p.dst_len) return;  // never write past the cache
+  }
+  if constexpr (PAGED) {
+    if (p.new_lens && t >= p.new_lens[b]) return;
+    dpage = p.table[b * p.spt + (drow >> p.page_shift)];  // (dst_len <= max_pages * page_size)
+    if (dpage < 0 || dpage >= p.npages) return;
+    drow &= ((int64_t)1 << p.page_shift) - 1;
   }
 
   const T* src = static_cast<const T*>(rt.src) + b * rt.sb + h0 * rt.sh + t * rt.st;
@@ -156,7 +170,7 @@ __global__ __launch_bounds__(256) void row_norm_rope_kernel(RowParams p) {
         z[j][i] = nz;
       }
   }
-  T* dst = static_cast<T*>(rt.dst) + b * rt.db + h0 * rt.dh + drow * rt.dt;
+  T* dst = static_cast<T*>(rt.dst) + dpage * rt.db + h0 * rt.dh + drow * rt.dt;
 #pragma unroll
   for (int j = 0; j < RPL; ++j) {
     if constexpr (sizeof(T) < 4) {
@@ -171,7 +185,7 @@ __global__ __launch_bounds__(256) void row_norm_rope_kernel(RowParams p) {
   }
 }
 
-template <typename T, int VEC, int RPL>
+template <typename T, int VEC, int RPL, bool PAGED>
 static int launch_rows_rpl(const RowParams& p, int gw, hipStream_t s) {
   const int64_t rows =
       (int64_t)p.B * p.T * (p.t[0].heads + (p.ntensors > 1 ? p.t[1].heads : 0));
@@ -181,7 +195,7 @@ static int launch_rows_rpl(const RowParams& p, int gw, hipStream_t s) {
   const dim3 grid((unsigned)((groups + gpb - 1) / gpb));
   switch (gw) {
 #define FORGE_GW(W) \
-  case W: hipLaunchKernelGGL((row_norm_rope_kernel<T, VEC, W, RPL>), grid, dim3(256), 0, s, p); break;
+  case W: hipLaunchKernelGGL((row_norm_rope_kernel<T, VEC, W, RPL, PAGED>), grid, dim3(256), 0, s, p); break;
     FORGE_GW(1) FORGE_GW(2) FORGE_GW(4) FORGE_GW(8) FORGE_GW(16) FORGE_GW(32) FORGE_GW(64)
 #undef FORGE_GW
     default: return set_error("row kernel: unsupported group width");
@@ -190,17 +204,17 @@ static int launch_rows_rpl(const RowParams& p, int gw, hipStream_t s) {
 }
 
 // Rows per lane group: 4 (or 2) consecutive heads when every tensor's head count allows.
-template <typename T, int VEC>
+template <typename T, int VEC, bool PAGED>
 static int launch_rows_vec(const RowParams& p, int gw, hipStream_t s) {
   auto divides = [&](int r) {
     return p.t[0].heads % r == 0 && (p.ntensors < 2 || p.t[1].heads % r == 0);
   };
-  if (divides(4)) return launch_rows_rpl<T, VEC, 4>(p, gw, s);
-  if (divides(2)) return launch_rows_rpl<T, VEC, 2>(p, gw, s);
-  return launch_rows_rpl<T, VEC, 1>(p, gw, s);
+  if (divides(4)) return launch_rows_rpl<T, VEC, 4, PAGED>(p, gw, s);
+  if (divides(2)) return launch_rows_rpl<T, VEC, 2, PAGED>(p, gw, s);
+  return launch_rows_rpl<T, VEC, 1, PAGED>(p, gw, s);
 }
 
-template <typename T>
+template <typename T, bool PAGED>
 static int launch_rows(const RowParams& p, hipStream_t s) {
   const int half = p.D / 2;
   constexpr int V16 = 16 / sizeof(T);
@@ -211,16 +225,20 @@ static int launch_rows(const RowParams& p, hipStream_t s) {
   int gw = 1;
   while (gw < lanes) gw <<= 1;
   if (gw > 64) return set_error("head dim too large for the row kernel (max 64 lanes per row)");
-  if (vec == V16) return launch_rows_vec<T, V16>(p, gw, s);
-  if (vec == 2) return launch_rows_vec<T, 2>(p, gw, s);
-  return launch_rows_vec<T, 1>(p, gw, s);
+  if (vec == V16) return launch_rows_vec<T, V16, PAGED>(p, gw, s);
+  if constexpr (!PAGED) {
+    if (vec == 2) return launch_rows_vec<T, 2, false>(p, gw, s);
+    return launch_rows_vec<T, 1, false>(p, gw, s);
+  }
+  return set_error("head dim: half of it must be a multiple of 16 bytes");
 }
 
+template <bool PAGED = false>
 static int dispatch_rows(int dtype, const RowParams& p, hipStream_t s) {
   switch (dtype) {
-    case FORGE_F32: return launch_rows<float>(p, s);
-    case FORGE_BF16: return launch_rows<bf16>(p, s);
-    case FORGE_F16: return launch_rows<f16>(p, s);
+    case FORGE_F32: return launch_rows<float, PAGED>(p, s);
+    case FORGE_BF16: return launch_rows<bf16, PAGED>(p, s);
+    case FORGE_F16: return launch_rows<f16, PAGED>(p, s);
     default: return set_error("unknown dtype code");
   }
 }
@@ -289,4 +307,47 @@ extern "C" int forge_kv_append(int dtype, int B, int T, int K, int D, const void
   p.pos0 = pos0;
   p.dst_len = dst_len;
   return dispatch_rows(dtype, p, (hipStream_t)stream);
+}
+
+extern "C" int forge_kv_append_paged(int dtype, int B, int T, int K, int D, const void* k, int64_t skb, int64_t skh,
+                                     int64_t skt, const void* v, int64_t svb, int64_t svh, int64_t svt, void* k_pages,
+                                     void* v_pages, int64_t sdp, int64_t sdh, int64_t sds, int n_pages, int page_size,
+                                     const int32_t* page_table, int64_t s_table, int max_pages, const int32_t* row_pos,
+                                     const int32_t* new_lens, const float* k_weight, float eps, int flags,
+                                     const float* cos, const float* sin, int64_t s_cos_b, int64_t s_cos_t,
+                                     void* stream) {
+  clear_error();
+  if (B < 0 || K <= 0 || T < 0) return set_error("bad sizes");
+  const int es = dtype == FORGE_F32 ? 4 : 2, e16 = 16 / es;
+  if (D <= 0 || D % (2 * e16) || D > 128 * e16) return set_error("head dim: half of it must be a multiple of 16 bytes, at most 1 KB");
+  if (!k || !v || !k_pages || !v_pages || !page_table || !row_pos) return set_error("null tensor pointer");
+  if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
+  if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
+  for (const int64_t st : {skb, skh, skt, svb, svh, svt, sdp, sdh, sds})
+    if (st < 0 || st % e16) return set_error("strides must be multiples of 16 bytes");
+  for (const void* x : {k, v, (const void*)k_pages, (const void*)v_pages})
+    if ((uintptr_t)x % 16) return set_error("k, v and the pages must be 16-byte aligned");
+  const bool rope = flags & FORGE_ROPE;
+  if (rope && (!cos || !sin)) return set_error("FORGE_ROPE needs cos and sin");
+  RowParams p{};
+  p.t[0] = RowTensor{k, skb, skh, skt, k_pages, sdp, sdh, sds, k_weight, K, (flags & FORGE_NORM_QK) ? 1 : 0, rope ? 1 : 0, 1};
+  p.t[1] = RowTensor{v, svb, svh, svt, v_pages, sdp, sdh, sds, nullptr, K, (flags & FORGE_NORM_V) ? 1 : 0, 0, 1};
+  p.ntensors = 2;
+  p.B = B;
+  p.T = T;
+  p.D = D;
+  p.eps = eps;
+  p.cos = cos;
+  p.sin = sin;
+  p.csb = s_cos_b;
+  p.cst = s_cos_t;
+  p.row_pos = row_pos;
+  p.dst_len = (int64_t)max_pages * page_size;
+  p.table = page_table;
+  p.spt = s_table;
+  p.max_pages = max_pages;
+  p.npages = n_pages;
+  p.page_shift = __builtin_ctz((unsigned)page_size);
+  p.new_lens = new_lens;
+  return dispatch_rows<true>(dtype, p, (hipStream_t)stream);
 }

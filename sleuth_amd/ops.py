@@ -12,6 +12,8 @@ outputs [B,T,H,D] (attention.py:155).
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -527,5 +529,193 @@ def linear_small(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
     return r if r.__class__ is not int else check(r, "forge_linear_small")
 
 
+# ---------------------------------------------------------------- the paged cache, windows with sinks
+def _guard(dev: torch.device):
+    """Launches go to the tensors' GPU, whichever is current."""
+    return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
+
+
+def _aligned(t: torch.Tensor) -> bool:
+    """16-byte aligned: the pointer and every stride of a dimension that has one (the last one contiguous)."""
+    e = 16 // t.element_size()
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+        all(st % e == 0 and st >= 0 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
+
+
+def _strides3(t: torch.Tensor) -> tuple[int, int, int]:
+    """The three leading strides, 0 where a dimension has one element (torch keeps any number there)."""
+    return tuple(st if n > 1 else 0 for st, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+def _int32_rows(t: torch.Tensor | None, B: int, dev: torch.device, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.shape != (B,) or t.device != dev:
+        raise ValueError(f"{name} must be an int32 [B] tensor on {dev}")
+    return t.contiguous()
+
+
+def _pages(k_pages, v_pages, page_table, B: int, dev: torch.device):
+    """Checks the pools [n_pages, K, page_size, D] and the table [B, max_pages]."""
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must be [n_pages, K, page_size, D]")
+    n, _, size, _ = k_pages.shape
+    if size < 16 or size & (size - 1) or n < 1:
+        raise ValueError(f"pages hold a power of two of at least 16 positions, not {size}")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must have one dtype")
+    if _strides3(k_pages) != _strides3(v_pages) or not _aligned(k_pages) or not _aligned(v_pages):
+        raise ValueError("k_pages and v_pages must have the same strides, the last dimension contiguous, 16-byte aligned")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] < 1 or \
+            page_table.device != dev:
+        raise ValueError(f"page_table must be int32 [B, max_pages] with B={B} on {dev}")
+    return page_table if page_table.stride(1) == 1 else page_table.contiguous()
+
+
+def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    page_table: torch.Tensor, row_pos: torch.Tensor, *, new_lens: torch.Tensor | None = None,
+                    k_weight: torch.Tensor | None = None, eps: float = 1e-6, norm_k: bool = False,
+                    norm_v: bool = False, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None) -> None:
+    """kv_append into a paged cache: k, v [B,K,T,D] get their norm and RoPE as there, and token t of row b goes to
+    position row_pos[b] + t, i.e. slot position % page_size of page page_table[b, position // page_size] of the pools
+    [n_pages, K, page_size, D]. Tokens t >= new_lens[b] (a padded batch) and positions without a page (an entry
+    outside the pool, or past the table's end) are not written. Lengths, table and positions are int32 on the GPU."""
+    if k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [B, K, T, D]")
+    B, K, T, D = k.shape
+    dev = _need_device(k, v, k_pages, v_pages, page_table, row_pos, new_lens, cos, sin, k_weight if norm_k else None)
+    table = _pages(k_pages, v_pages, page_table, B, dev)
+    if k_pages.shape[1] != K or k_pages.shape[3] != D:
+        raise ValueError(f"pages {tuple(k_pages.shape)} do not fit new k {tuple(k.shape)}")
+    e16 = 16 // k_pages.element_size()
+    if D % (2 * e16) or D > 128 * e16:
+        raise ValueError(f"head dim {D}: pages take multiples of {2 * e16} up to {128 * e16} in {k_pages.dtype}")
+    k, v = (x if x.dtype == k_pages.dtype and _aligned(x) else x.to(k_pages.dtype).clone(memory_format=torch.contiguous_format)
+            for x in (k, v))
+    rp, nl = _int32_rows(row_pos, B, dev, "row_pos"), _int32_rows(new_lens, B, dev, "new_lens")
+    c, s, s_b, s_t = _rope_tables(cos, sin, B, T, D)
+    flags = (NORM_QK if norm_k else 0) | (ROPE if c is not None else 0) | (NORM_V if norm_v else 0)
+    w = _weight(k_weight, D) if norm_k else None
+    with _guard(dev):
+        st = lib().forge_kv_append_paged(dtype_code(k_pages), B, T, K, D, _ptr(k), *_strides3(k), _ptr(v), *_strides3(v),
+                                         _ptr(k_pages), _ptr(v_pages), *_strides3(k_pages), k_pages.shape[0],
+                                         k_pages.shape[2], _ptr(table), table.stride(0) if B > 1 else 0, table.shape[1],
+                                         _ptr(rp), _ptr(nl), _ptr(w), float(eps), flags, _ptr(c), _ptr(s), s_b, s_t,
+                                         _stream(dev))
+    check(st, "forge_kv_append_paged")
+
+
+def paged_supported(dtype: torch.dtype, D: int) -> bool:
+    """attn_paged and attn_sinks take this dtype and head dim."""
+    return dtype in _DTYPES and (D in (32, 64, 128, 256) or (D == 512 and dtype != torch.float32))
+
+
+def _new_token_args(q, cache, q_weight, eps, norm_q, cos, sin, window, sinks, out):
+    """Checks what attn_paged and attn_sinks share; (q, C arguments from dtype to s_cos_t, out)."""
+    if q.dim() != 4 or q.shape[1] % cache.shape[1] or q.shape[3] != cache.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)} does not fit the cache {tuple(cache.shape)}")
+    B, H, T, D = q.shape
+    if q.dtype != cache.dtype:
+        raise ValueError(f"q is {q.dtype} but the cache is {cache.dtype}")
+    if not paged_supported(q.dtype, D):
+        raise ValueError(f"head dim {D} in {q.dtype}: 32, 64, 128, 256, and 512 in 16 bits")
+    if window < 0 or sinks < 0 or (sinks and not window):
+        raise ValueError("window and sinks must not be negative, and sinks need a window")
+    dev = q.device
+    if not _aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
+    elif out.shape != (B, T, H, D) or out.dtype != q.dtype or out.device != dev or not _aligned(out):
+        raise ValueError(f"out must be a 16-byte aligned [B,T,H,D] = {(B, T, H, D)} {q.dtype} on {dev}")
+    c, s, s_b, s_t = _rope_tables(cos, sin, B, T, D)
+    w = _weight(q_weight, D) if norm_q else None
+    if w is not None and w.data_ptr() % 16:
+        w = w.clone()
+    flags = (NORM_QK if norm_q else 0) | (ROPE if c is not None else 0)
+    keep = (q, w, c, s)   # alive until the launch
+    return keep, (dtype_code(q), B, T, H, cache.shape[1], D, _ptr(q), *_strides3(q), _ptr(w), float(eps), flags, _ptr(c),
+                  _ptr(s), s_b, s_t), out
+
+
+def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+               row_pos: torch.Tensor, *, scale: float, new_lens: torch.Tensor | None = None,
+               max_kv_len: int | None = None, window: int = 0, sinks: int = 0, q_weight: torch.Tensor | None = None,
+               eps: float = 1e-6, norm_q: bool = False, cos: torch.Tensor | None = None,
+               sin: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new tokens q [B,H,T,D] over the paged cache (kv_append_paged), which holds their keys
+    already: one token per row or a chunk of thousands, rows of any lengths. Query t of row b sits at
+    p = row_pos[b] + t and sees keys s <= p; with a window those with s > p - window, and the first `sinks` positions.
+    Keys whose table entry lies outside the pool (-1: given back) are invisible. Returns [B,T,H,D]; rows
+    t >= new_lens[b] and rows that see nothing are zeros. max_kv_len: an upper bound on row_pos[b] + new_lens[b]
+    (default: what the table can hold); it sizes the launch."""
+    dev = _need_device(q, k_pages, v_pages, page_table, row_pos, new_lens, cos, sin, q_weight if norm_q else None, out)
+    B, T = q.shape[0], q.shape[2]
+    table = _pages(k_pages, v_pages, page_table, B, dev)
+    rp, nl = _int32_rows(row_pos, B, dev, "row_pos"), _int32_rows(new_lens, B, dev, "new_lens")
+    size = k_pages.shape[2]
+    most = table.shape[1] * size
+    max_kv_len = most if max_kv_len is None else min(int(max_kv_len), most)
+    if max_kv_len < 1:
+        raise ValueError("max_kv_len must be positive")
+    keep, args, out = _new_token_args(q, k_pages, q_weight, eps, norm_q, cos, sin, window, sinks, out)
+    with _guard(dev):
+        need = lib().forge_attn_paged_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks))
+        ws = _partials(need, dev)
+        st = lib().forge_attn_paged(*args, _ptr(k_pages), _ptr(v_pages), *_strides3(k_pages), k_pages.shape[0], size,
+                                    _ptr(table), table.stride(0) if B > 1 else 0, table.shape[1], _ptr(rp), _ptr(nl),
+                                    max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
+                                    _ptr(ws), need, _stream(dev))
+    check(st, "forge_attn_paged")
+    return out
+
+
+def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, scale: float, window: int,
+               sinks: int, pos: int | None = None, pos_dev: torch.Tensor | None = None,
+               row_pos: torch.Tensor | None = None, max_kv_len: int | None = None,
+               q_weight: torch.Tensor | None = None, eps: float = 1e-6, norm_q: bool = False,
+               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Sliding-window attention whose first `sinks` positions stay visible, over a contiguous cache
+    [B,K,max_len,D] that holds the new keys already: query t of row b sits at p = base_b + t (row_pos, pos_dev or
+    pos, as attn_decode) and sees keys s <= p with s > p - window or s < sinks. Any T: whole prompts, chunks, verify and
+    decode steps. Returns [B,T,H,D]."""
+    dev = _need_device(q, k_cache, v_cache, pos_dev, row_pos, cos, sin, q_weight if norm_q else None, out)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.dtype != v_cache.dtype or q.shape[0] != k_cache.shape[0]:
+        raise ValueError(f"q {tuple(q.shape)} does not fit caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if _strides3(k_cache) != _strides3(v_cache) or not _aligned(k_cache) or not _aligned(v_cache):
+        raise ValueError("k and v caches must have the same strides, the last dimension contiguous, 16-byte aligned")
+    if window < 1:
+        raise ValueError("attn_sinks needs a window (attn_decode and attn_prefill see every key)")
+    B, T, max_len = q.shape[0], q.shape[2], k_cache.shape[2]
+    rp, pd, p0 = _positions(pos, pos_dev, row_pos, B, dev)
+    if rp is None and pd is None:
+        if not 0 <= p0 <= max_len - T:
+            raise ValueError(f"pos {p0} + {T} tokens do not fit a cache of {max_len}")
+        max_kv_len = p0 + T
+    max_kv_len = max_len if max_kv_len is None else min(int(max_kv_len), max_len)
+    if max_kv_len < 1:
+        if B == 0 or T == 0:
+            max_kv_len = 1
+        else:
+            raise ValueError("max_kv_len must be positive")
+    keep, args, out = _new_token_args(q, k_cache, q_weight, eps, norm_q, cos, sin, window, sinks, out)
+    with _guard(dev):
+        need = lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks))
+        ws = _partials(need, dev)
+        st = lib().forge_attn_sinks(*args, _ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache), max_len, _ptr(rp), _ptr(pd),
+                                    p0, max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
+                                    _ptr(ws), need, _stream(dev))
+    check(st, "forge_attn_sinks")
+    return out
+
+
+def _cache_strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """_strides3 with a positions' stride the kernels accept where there is one position."""
+    b, h, s = _strides3(t)
+    return b, h, s or t.shape[3]
+
+
 __all__ = ["head_norm_rope", "kv_append", "attn_decode", "attn_decode_append", "attn_decode_noalloc", "attn_prefill", "attn_prefill_f32", "decode_chunk",
-           "decode_workspace_bytes", "attn_drafter", "prefill_supported", "dtype_code", "_lib"]
+           "decode_workspace_bytes", "attn_drafter", "prefill_supported", "kv_append_paged",
+           "attn_paged", "attn_sinks", "paged_supported", "dtype_code", "_lib"]
