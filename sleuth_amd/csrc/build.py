@@ -22,7 +22,7 @@ LIB_NAME = "libforge_attn.so"
 HOST_NAME = "_forge_host.so"
 # (source, defines, object name); decode.hip's and paged.hip's kernels are built per dtype, side by side
 SOURCES = [("abi.hip", [], "abi"), ("prep.hip", [], "prep"), ("prefill.hip", [], "prefill"), ("linear.hip", [], "linear"),
-           ("paged_abi.hip", [], "paged_abi"), *(("paged.hip", [f"-DFORGE_PAGED_PART={n}"], f"paged{n}") for n in range(1, 4)),
+           ("paged_abi.hip", [], "paged_abi"), ("paged_chunk.hip", [], "paged_chunk"), *(("paged.hip", [f"-DFORGE_PAGED_PART={n}"], f"paged{n}") for n in range(1, 4)),
            *(("decode.hip", [f"-DFORGE_DECODE_PART={n}"], f"decode{n}") for n in range(4))]
 ARCH = "gfx950"
 

@@ -25,7 +25,7 @@ struct PagedParams {
   int64_t skp, skh, sks;  // elements between pages (contiguous: batch rows), heads, positions
   const int32_t* table;   // [B][max_pages] page ids, or null: contiguous, batch row b is page b
   int64_t spt;
-  int max_pages, npages;
+  int npages;
   int page_shift, page_mask;  // contiguous: 31 and 0x7fffffff
   const int32_t* row_pos;
   const int64_t* pos_dev;
@@ -44,12 +44,11 @@ struct PagedParams {
   float2* ws_ml;  // [B][K][rows][nparts]
   float* ws_o;    // ... [D]
 
-  // The page that holds position `key` of batch row b; -1 where the table names none of the pool.
+  // The page that holds position `key` (below limit, so the table has an entry for it) of batch row b; -1
+  // where the table names none of the pool.
   __device__ __forceinline__ int page_of(int b, int key) const {
     if (!table) return b;
-    const int at = key >> page_shift;
-    if (at >= max_pages) return -1;
-    const int id = scalar_load(table + b * spt + at);
+    const int id = scalar_load(table + b * spt + (key >> page_shift));
     return (unsigned)id < (unsigned)npages ? id : -1;
   }
 };
@@ -63,6 +62,7 @@ constexpr int step_keys(int esize, int D, int rows) { return esize * D * (rows /
 
 // How the host cuts a call: rows per block, keys per tile, parts.
 struct PagedPlan {
+  bool chunk;  // paged_chunk.hip's kernel (rows 128), or paged.hip's
   int rows, keys;
   int nparts, tiles_per_part;
 };
@@ -169,5 +169,6 @@ static int launch_paged_combine(const PagedParams& p, int block_rows, int KT, hi
 }
 
 template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
+template <typename T> int launch_paged_chunk(const PagedParams& p, int D, hipStream_t s);
 
 }  // namespace forge

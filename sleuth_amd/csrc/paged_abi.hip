@@ -8,6 +8,8 @@ namespace forge {
 
 extern template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+extern template int launch_paged_chunk<bf16>(const PagedParams&, int, hipStream_t);
+extern template int launch_paged_chunk<f16>(const PagedParams&, int, hipStream_t);
 extern template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 
 static bool paged_dim_ok(int dtype, int D) {
@@ -24,6 +26,11 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   if (plan.rows > most) plan.rows = most;
   plan.keys = step_keys(es, D, plan.rows);
+  if (es == 2 && D >= 64 && D <= 256 && rows > 64) {
+    plan.chunk = true;
+    plan.rows = 128;
+    plan.keys = D == 256 ? 32 : 64;
+  }
   plan.nparts = 1;
   // tiles that a block can have: its queries' window and the first tokens, or the whole row
   const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
@@ -33,7 +40,7 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.tiles_per_part = (int)tiles;
   if (!split) return plan;
   const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
-  const int64_t want = (4 * (int64_t)device_cus() + units - 1) / units;
+  const int64_t want = ((plan.chunk ? 2 : 4) * (int64_t)device_cus() + units - 1) / units;
   int64_t per = (tiles + want - 1) / want;
   if (per < 8) per = 8;  // two tiles for each wave
   const int64_t parts = (tiles + per - 1) / per;
@@ -88,8 +95,8 @@ static int paged_run(int dtype, int D, PagedParams p, float scale, void* workspa
   }
   switch (dtype) {
     case FORGE_F32: return launch_paged<float>(p, plan, D, s);
-    case FORGE_BF16: return launch_paged<bf16>(p, plan, D, s);
-    default: return launch_paged<f16>(p, plan, D, s);
+    case FORGE_BF16: return plan.chunk ? launch_paged_chunk<bf16>(p, D, s) : launch_paged<bf16>(p, plan, D, s);
+    default: return plan.chunk ? launch_paged_chunk<f16>(p, D, s) : launch_paged<f16>(p, plan, D, s);
   }
 }
 
@@ -126,7 +133,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   p.qw = q_weight; p.eps = eps; p.flags = flags;
   p.cos = cos; p.sin = sin; p.csb = s_cos_b; p.cst = s_cos_t;
   p.k = k_pages; p.v = v_pages; p.skp = skp; p.skh = skh; p.sks = sks;
-  p.table = page_table; p.spt = s_table; p.max_pages = max_pages; p.npages = n_pages;
+  p.table = page_table; p.spt = s_table; p.npages = n_pages;
   p.page_shift = __builtin_ctz((unsigned)page_size); p.page_mask = page_size - 1;
   p.row_pos = row_pos; p.new_lens = new_lens;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;

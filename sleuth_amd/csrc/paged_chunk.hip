@@ -1,0 +1,383 @@
+// Chunks of many query rows over a paged cache, or over a contiguous one with a window and first tokens:
+// bf16/fp16, head dims 64, 128, 256, on v_mfma_f32_32x32x16 (the split kernel of paged.hip serves the rest).
+//
+// A block of 4 waves owns 128 query rows of one (batch row, KV head) -- row r is token r / G, head r % G of the
+// group, so the heads of a group share each key tile they read -- and streams that row's visible key tiles through
+// two LDS stages, as the causal prefill kernel does: direct loads into LDS in swizzled chunk order, S^T = K . Q^T
+// with Q^T in registers, one lane per query row (two lanes share a row's keys), P^T fed to O^T = V^T . P^T straight
+// from the score registers. See prefill.hip for the operand layouts; what differs here:
+//   * A wave loads RW = BN / 4 consecutive key rows of a tile, which never straddle pages (pages are multiples of 16
+//     positions), so a tile costs each wave one table entry: a scalar load, issued one tile ahead.
+//   * A page id outside the pool leaves zeros in LDS and a flag for the stage; its keys are masked.
+//   * With a window, the tiles that hold first tokens come before those of the window.
+#include <limits.h>
+
+#include "paged.h"
+#include "prefill_tile.h"
+
+namespace forge {
+
+// Query row (b, h, t) as MFMA B operands, RMSNorm and RoPE in fp32 with one rounding: channels 16s + 8hi + e.
+template <typename T, int D>
+__device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h, int t, int hi,
+                                             typename Mfma<T>::vec (&q)[D / 16]) {
+  using V8 = typename Mfma<T>::vec;
+  constexpr int S = D / 16;
+  const T* src = static_cast<const T*>(p.q) + b * p.sqb + h * p.sqh + t * p.sqt;
+  const bool norm = p.flags & FORGE_NORM_QK, rope = p.flags & FORGE_ROPE;
+  if (!norm && !rope) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) q[s] = *reinterpret_cast<const V8*>(src + 16 * s + 8 * hi);
+    return;
+  }
+  float f[S][8];
+#pragma unroll
+  for (int s = 0; s < S; ++s) unpack16<T>(load16(src + 16 * s + 8 * hi), f[s]);
+  if (norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss += f[s][e] * f[s][e];
+    ss += __shfl_xor(ss, 32, kWave);
+    const float rs = rsqrtf(ss / (float)D + p.eps);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      float w[8];
+      if (p.qw) load_f32x8(p.qw + 16 * s + 8 * hi, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[s][e] = p.qw ? f[s][e] * rs * w[e] : f[s][e] * rs;
+    }
+  }
+  if (rope) {
+    const float* cr = p.cos + b * p.csb + t * p.cst;
+    const float* sr = p.sin + b * p.csb + t * p.cst;
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = 16 * s + 8 * hi + e;
+        const float a = f[s][e], z = f[s + S / 2][e];
+        f[s][e] = a * cr[c] - z * sr[c];
+        f[s + S / 2][e] = z * cr[c + D / 2] + a * sr[c + D / 2];
+      }
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[s][e] = from_f32<T>(fp32_result(f[s][e]));
+}
+
+template <int D> constexpr int chunk_lds() { return Tile<D>::LDS_BYTES + 64; }  // and the stages' flags
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void paged_chunk_kernel(PagedParams p) {
+  using V8 = typename Mfma<T>::vec;
+  using TL = Tile<D>;
+  constexpr int BN = TL::BN, BM = TL::BM;
+  constexpr int KB = BN / 32, KSTEPS = D / 16, DB = D / 32, HALVES = BN / 16;
+  constexpr int RW = BN / TL::WAVES;      // key rows of a tile that a wave loads
+  constexpr int RL = kWave / TL::NCH;     // of which one load instruction covers RL
+  static_assert(TL::STAGES == 2 && RW == RL * TL::LOADS && RW <= 16, "a wave's rows lie in one page");
+
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stage][K|V][TILEB], then the flags [stage][wave]
+  int* flags = reinterpret_cast<int*>(smem + TL::LDS_BYTES);
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int lane = threadIdx.x % kWave;
+  const int n = lane & 31, hi = lane >> 5;
+
+  int part, rblk, b, kvh;
+  block_unit(p, (p.rows + BM - 1) / BM, part, rblk, b, kvh);
+  const RowSpan w = row_span(p, b, rblk * BM, BM, BN);
+  const int begin = part * p.tiles_per_part;
+  const int end = begin + p.tiles_per_part < w.tiles ? begin + p.tiles_per_part : w.tiles;
+  const bool whole = w.tiles <= p.tiles_per_part;
+  if (part > 0 && begin >= w.tiles) return;
+
+  // rows without a real token come out as zeros
+  if (part == 0 && w.rows < rblk * BM + BM) {
+    const int r0 = w.rows > rblk * BM ? w.rows : rblk * BM;
+    const int r1 = rblk * BM + BM < p.rows ? rblk * BM + BM : p.rows;
+    for (int x = threadIdx.x; x < (r1 - r0) * (D / 4); x += 256)
+      store_row<T>(p, b, kvh, r0 + x / (D / 4), 4 * (x % (D / 4)), make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+  }
+  if (w.tiles == 0) return;
+
+  // ---- key tiles: load i of this wave fills LDS slots (wave * LOADS + i) * 64 + lane, key rows RL * i + lane / NCH
+  // of the wave's RW, in swizzled chunk order (kept offsets up to head dim 128; one xor each from shared registers
+  // at 256, where registers are short)
+  constexpr bool KEEP = D < 256;
+  const int64_t pageb = p.skp * 2;
+  const int rowb = (int)p.sks * 2;
+  const char* kgb = static_cast<const char*>(p.k) + kvh * p.skh * 2;
+  const char* vgb = static_cast<const char*>(p.v) + kvh * p.skh * 2;
+  const int ld_row = lane / TL::NCH, pch = lane % TL::NCH;
+  const int wr0 = wave * RW;
+  const int ld_k = (pch ^ swz_k<D>(ld_row)) << 4, ld_v = (pch ^ swz_v<D>(ld_row)) << 4;
+  int kept_k[KEEP ? TL::LOADS : 1], kept_v[KEEP ? TL::LOADS : 1];
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int i = 0; i < TL::LOADS; ++i) {
+      const int in = RL * i + ld_row;
+      kept_k[i] = in * rowb + ((pch ^ swz_k<D>(wr0 + in)) << 4);
+      kept_v[i] = in * rowb + ((pch ^ swz_v<D>(wr0 + in)) << 4);
+    }
+  }
+  int flagged[2] = {0, 0};   // what this wave's flag of each stage holds
+  if (lane < 2) flags[4 * lane + wave] = 0;
+  // first row of the wave's part of tile i; where the row's keys end before it, of the part that holds the last key
+  auto part_key = [&](int i) {
+    const int key0 = w.tile_key(i, BN), left = w.last - key0;
+    return key0 + (wr0 <= left ? wr0 : left & ~(RW - 1));
+  };
+  auto issue = [&](int i, int stage, int page) {
+    const unsigned kdst = lds_offset(smem + (2 * stage) * TL::TILEB + wave * TL::LOADS * 1024);
+    const unsigned vdst = kdst + TL::TILEB;
+    const int miss = page < 0;
+    if (miss != flagged[stage]) {
+      if (lane == 0) flags[4 * stage + wave] = miss;
+      flagged[stage] = miss;
+    }
+    if (miss) {
+      char* kd = smem + (2 * stage) * TL::TILEB + wave * TL::LOADS * 1024 + lane * 16;
+#pragma unroll
+      for (int x = 0; x < TL::LOADS; ++x) {
+        *reinterpret_cast<uint4*>(kd + x * 1024) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(kd + TL::TILEB + x * 1024) = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
+    const int key = part_key(i);
+    const int64_t at = page * pageb + (int64_t)(key & p.page_mask) * rowb;
+    const int most = w.last - key;  // rows of the part past it re-read it (masked)
+    const char* ks = kgb + at;
+    const char* vs = vgb + at;
+    int lk = ld_k, lv = ld_v;
+    if constexpr (!KEEP) asm volatile("" : "+v"(lk), "+v"(lv));  // (not kept over the loop)
+    if (most >= RW - 1) {
+#pragma unroll
+      for (int x = 0; x < TL::LOADS; ++x) {
+        if constexpr (KEEP) {
+          lds_dma16(ks, (unsigned)kept_k[x], kdst + x * 1024);
+          lds_dma16(vs, (unsigned)kept_v[x], vdst + x * 1024);
+        } else {
+          const int r0 = wr0 + RL * x;
+          const unsigned lo = (unsigned)(ld_row * rowb);
+          lds_dma16(ks + RL * x * rowb, lo + (lk ^ (swz_k<D>(r0) << 4)), kdst + x * 1024);
+          lds_dma16(vs + RL * x * rowb, lo + (lv ^ (swz_v<D>(r0) << 4)), vdst + x * 1024);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < TL::LOADS; ++x) {
+        const int in = RL * x + ld_row, row = in < most ? in : most;
+        lds_dma16(ks, (unsigned)(row * rowb + ((pch ^ swz_k<D>(wr0 + in)) << 4)), kdst + x * 1024);
+        lds_dma16(vs, (unsigned)(row * rowb + ((pch ^ swz_v<D>(wr0 + in)) << 4)), vdst + x * 1024);
+      }
+    }
+  };
+  issue(begin, 0, p.page_of(b, part_key(begin)));
+  int page = p.page_of(b, part_key(begin + 1 < end ? begin + 1 : begin));
+
+  // ---- this lane's query row; the wave's span of positions
+  const int w_row = rblk * BM + wave * 32;
+  const bool wave_any = w_row < w.rows;
+  const int flat = w_row + n;
+  const bool valid = flat < w.rows;
+  const int t = (valid ? flat : w.rows - 1) / p.G, h = kvh * p.G + (valid ? flat : w.rows - 1) % p.G;
+  const int qpos = w.base + t;
+  const int wq_lo = w.base + w_row / p.G;
+  const int wq_hi = w.base + (w_row + 31 < w.rows ? w_row + 31 : w.rows - 1) / p.G;
+  V8 qreg[KSTEPS];
+  chunk_load_q<T, D>(p, b, h, t, hi, qreg);
+
+  // LDS read offsets of a lane within a stage's K and V tiles (prefill.hip)
+  const int g = lane >> 4, kq = (lane >> 2) & 3, qq = lane & 3;
+  const int v_row = 4 * (g >> 1) + kq;
+  const unsigned k_rd = n * TL::ROWB + ((hi ^ swz_k<D>(n)) << 4);
+  const unsigned v_rd = v_row * TL::ROWB + (((2 * (g & 1) + (qq >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (qq & 1);
+  const unsigned lds0 = lds_offset(smem);
+
+  floatx16 oacc[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) oacc[d][x] = 0.0f;
+  float m_run = kNegInf, l_run = 0.0f;
+  const float c = p.scale_log2;
+
+  for (int it = begin; it < end; ++it) {
+    const int stage = (it - begin) & 1;
+    wait_vm<0>();
+    __syncthreads();  // tile `it` is in LDS for every wave; the other stage is free
+    if (it + 1 < end) {
+      issue(it + 1, stage ^ 1, page);
+      page = p.page_of(b, part_key(it + 2 < end ? it + 2 : it + 1));
+    }
+    const int key0 = w.tile_key(it, BN);
+    const bool needed = wave_any && key0 <= wq_hi &&
+                        (p.window <= 0 || key0 + BN - 1 > wq_lo - p.window || key0 < p.sinks);
+    if (!needed) continue;
+    const unsigned bad = p.table ? (unsigned)__ballot(flags[4 * stage + (lane & 3)] != 0) & 15u : 0u;
+    const bool full = bad == 0 && key0 + BN - 1 <= wq_lo &&
+                      (p.window <= 0 || wq_hi - key0 < p.window || key0 + BN <= p.sinks);
+
+    const unsigned kl = lds0 + (2 * stage) * TL::TILEB + k_rd;
+    const unsigned vl = lds0 + (2 * stage + 1) * TL::TILEB + v_rd;
+
+    // S^T = K . Q^T, K operands read two steps ahead (pinned: left alone each step waits for its reads)
+    floatx16 sacc[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) sacc[kb][x] = 0.0f;
+    {
+      auto kread = [&](int kb, int st) {
+        return *(__attribute__((address_space(3))) const V8*)((kl ^ (32 * (st & 7))) + 256 * (st >> 3) +
+                                                              kb * 32 * TL::ROWB);
+      };
+      V8 a0[KB], a1[KB], a2[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) a0[kb] = kread(kb, 0);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) a1[kb] = kread(kb, 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * KB, 0);
+#pragma unroll
+      for (int st = 0; st < KSTEPS; ++st) {
+        if (st + 2 < KSTEPS) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) a2[kb] = kread(kb, st + 2);
+          __builtin_amdgcn_sched_group_barrier(0x100, KB, 0);
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) sacc[kb] = Mfma<T>::run(a0[kb], qreg[st], sacc[kb]);
+        __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          a0[kb] = a1[kb];
+          a1[kb] = a2[kb];
+        }
+      }
+    }
+
+    // element (kb, x) of this lane is key key0 + 4hi + ce, ce = 32kb + 8(x/4) + x%4
+    if (!full) {
+      const int base = key0 + 4 * hi;
+      const int lim_hi = (qpos < w.last ? qpos : w.last) - base;
+      const int lim_lo = p.window > 0 ? qpos - p.window + 1 - base : -(1 << 30);
+      const int lim_sink = p.sinks - base;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int ce = 32 * kb + 8 * (x >> 2) + (x & 3);
+          const bool gone = bad >> ((32 * kb + 8 * (x >> 2)) / RW) & 1;
+          sacc[kb][x] = ce <= lim_hi && (ce >= lim_lo || ce < lim_sink) && !gone ? sacc[kb][x] : kNegInf;
+        }
+    }
+
+    // online softmax in base 2, the scale in the exponent's fma; the maximum moves when a score passes it by 2^8
+    float mxp[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      mxp[i] = sacc[0][4 * i];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = (kb == 0 ? 1 : 0); j < 4; ++j) mxp[i] = fmaxf(mxp[i], sacc[kb][4 * i + j]);
+    }
+    const float mxc = max_xor32(fmaxf(fmaxf(mxp[0], mxp[1]), fmaxf(mxp[2], mxp[3]))) * c;
+    if (mxc > m_run + kLazyLog2) {
+      const float alpha = m_run == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m_run - mxc);
+      l_run *= alpha;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) oacc[d][x] *= alpha;
+      m_run = mxc;
+    }
+    const float neg_m = m_run == kNegInf ? 0.0f : -m_run;
+    float rs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float pv = __builtin_amdgcn_exp2f(fmaf(sacc[kb][x], c, neg_m));
+        sacc[kb][x] = pv;
+        rs[x & 3] += pv;
+      }
+    l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+
+    // O^T += V^T . P^T (weights rounded to the type: the matrix cores take nothing wider beside 16-bit values)
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf) {
+      const int kb = hf >> 1, half = hf & 1;
+      V8 pb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pb[e] = from_f32<T>(sacc[kb][8 * half + e]);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const unsigned va = (vl ^ (64 * (d & 3))) + 256 * (d >> 2) + 16 * hf * TL::ROWB;
+        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)va);
+        const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) i16x4*)(va + 8 * TL::ROWB));
+        typedef short i16x8 __attribute__((ext_vector_type(8)));
+        const i16x8 av = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+        oacc[d] = Mfma<T>::run(__builtin_bit_cast(V8, av), pb, oacc[d]);
+      }
+    }
+  }
+
+  l_run += __shfl_xor(l_run, 32, kWave);
+  if (!valid) return;
+  if (!whole) {
+    const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts + part;
+    float* po = p.ws_o + slot * D + 4 * hi;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(po + d * 32 + 8 * i) =
+            make_float4(oacc[d][4 * i], oacc[d][4 * i + 1], oacc[d][4 * i + 2], oacc[d][4 * i + 3]);
+    if (hi == 0) p.ws_ml[slot] = make_float2(m_run, l_run);
+    return;
+  }
+  const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store_row<T>(p, b, kvh, flat, d * 32 + 8 * i + 4 * hi,
+                   make_float4(oacc[d][4 * i], oacc[d][4 * i + 1], oacc[d][4 * i + 2], oacc[d][4 * i + 3]), inv);
+}
+
+template <typename T, int D> static int launch_chunk_d(const PagedParams& p, hipStream_t s) {
+  using TL = Tile<D>;
+  static bool attr_set = false;
+  if (chunk_lds<D>() > 64 * 1024 && !attr_set) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D>),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<D>()) != hipSuccess)
+      return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
+    attr_set = true;
+  }
+  const int64_t blocks = (int64_t)((p.rows + TL::BM - 1) / TL::BM) * p.K * p.B * p.nparts;
+  if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), dim3((unsigned)blocks), dim3(256), chunk_lds<D>(), s, p);
+  const int st = check_launch();
+  return st || p.nparts < 2 ? st : launch_paged_combine<T, D>(p, TL::BM, TL::BN, s);
+}
+
+template <typename T> int launch_paged_chunk(const PagedParams& p, int D, hipStream_t s) {
+  switch (D) {
+    case 64: return launch_chunk_d<T, 64>(p, s);
+    case 128: return launch_chunk_d<T, 128>(p, s);
+    case 256: return launch_chunk_d<T, 256>(p, s);
+    default: return set_error("forge_attn_paged: unsupported head dim");
+  }
+}
+template int launch_paged_chunk<bf16>(const PagedParams&, int, hipStream_t);
+template int launch_paged_chunk<f16>(const PagedParams&, int, hipStream_t);
+
+}  // namespace forge
