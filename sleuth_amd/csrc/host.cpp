@@ -370,6 +370,202 @@ PyObject* tensors_are_impl(PyObject* const* a) {
   Py_RETURN_TRUE;
 }
 
+// A tensor [.., .., .., D] that the paged kernels take as it is: the last dimension contiguous, pointer and strides
+// multiples of 16 bytes (ops._aligned), its strides with 0 for dimensions of one element (ops._strides3).
+bool strides16(const Tensor& t, int64_t (&s)[3]) {
+  const int64_t e16 = 16 / t.element_size();
+  if (t.dim() != 4 || t.stride(3) != 1 || (uintptr_t)t.const_data_ptr() % 16) return false;
+  for (int i = 0; i < 3; ++i) {
+    s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (s[i] < 0 || s[i] % e16) return false;
+  }
+  return true;
+}
+
+// int32 [B] on dev
+bool rows_ok(const Tensor& t, int64_t B, c10::Device dev) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == B && t.is_contiguous() && t.device() == dev;
+}
+
+struct Pages {
+  int64_t s[3], B, size, max, stride;
+  int n;
+};
+
+// pools [n, K, size, D] and table [B, max] of one cache (ops._pages)
+bool pages_ok(const Tensor& kp, const Tensor& vp, const Tensor& table, int64_t B, c10::Device dev, Pages& p) {
+  int64_t sv[3];
+  if (kp.dim() != 4 || kp.sizes() != vp.sizes() || kp.scalar_type() != vp.scalar_type() || kp.device() != dev ||
+      vp.device() != dev || !strides16(kp, p.s) || !strides16(vp, sv) || !std::equal(p.s, p.s + 3, sv))
+    return false;
+  p.size = kp.size(2);
+  if (p.size < 16 || p.size > INT_MAX || (p.size & (p.size - 1)) || kp.size(0) < 1 || kp.size(0) > INT_MAX) return false;
+  if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(0) != B || table.size(1) < 1 ||
+      table.size(1) > INT_MAX || table.stride(1) != 1 || table.device() != dev)
+    return false;
+  p.n = (int)kp.size(0);
+  p.max = table.size(1);
+  p.stride = B > 1 ? table.stride(0) : 0;
+  return p.stride >= 0;
+}
+
+// kv_append_paged(k, v, k_pages, v_pages, table, row_pos, new_lens | None, k_weight | None, eps, norm_k, norm_v,
+//                 cos | None, sin | None)
+PyObject* kv_append_paged_impl(PyObject* const* a) {
+  Tensor k, v, kp, vp, table, row_pos, news, kw, cos, sin;
+  if (!take(a[0], k) || !take(a[1], v) || !take(a[2], kp) || !take(a[3], vp) || !take(a[4], table) ||
+      !take(a[5], row_pos) || !take_opt(a[6], news) || !take_opt(a[7], kw) || !take_opt(a[11], cos) || !take_opt(a[12], sin))
+    return nullptr;
+  float eps;
+  if (!as_float(a[8], eps) || k.dim() != 4 || k.sizes() != v.sizes()) return nullptr;
+  const bool norm_k = a[9] == Py_True, norm_v = a[10] == Py_True;
+  const int64_t B = k.size(0), K = k.size(1), T = k.size(2), D = k.size(3);
+  const int dt = dtype_of(kp);
+  const c10::Device dev = k.device();
+  Pages p;
+  int64_t sk[3], sv[3];
+  if (dt < 0 || k.scalar_type() != kp.scalar_type() || v.scalar_type() != kp.scalar_type() || v.device() != dev ||
+      c10::hip::current_device() != dev.index() || !strides16(k, sk) || !strides16(v, sv) ||
+      !pages_ok(kp, vp, table, B, dev, p) || kp.size(1) != K || kp.size(3) != D || !rows_ok(row_pos, B, dev) ||
+      (news.defined() && !rows_ok(news, B, dev)))
+    return nullptr;
+  Rope r;
+  if (!rope_ok(cos, sin, B, T, D, dev, r) || !gain_ok(kw, D, dev)) return nullptr;
+  const int flags = (norm_k ? FORGE_NORM_QK : 0) | (r.cos ? FORGE_ROPE : 0) | (norm_v ? FORGE_NORM_V : 0);
+  int st;
+  {
+    NoGil unlocked;
+    st = forge_kv_append_paged(dt, (int)B, (int)T, (int)K, (int)D, ptr(k), sk[0], sk[1], sk[2], ptr(v), sv[0], sv[1], sv[2],
+                               kp.data_ptr(), vp.data_ptr(), p.s[0], p.s[1], p.s[2], p.n, (int)p.size,
+                               static_cast<const int32_t*>(ptr(table)), p.stride, (int)p.max,
+                               static_cast<const int32_t*>(ptr(row_pos)), static_cast<const int32_t*>(ptr(news)),
+                               norm_k ? static_cast<const float*>(ptr(kw)) : nullptr, eps, flags, r.cos, r.sin, r.sb, r.st,
+                               c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return st >= 0 ? PyLong_FromLong(st) : nullptr;   // (a rejected call gets its error the Python way)
+}
+
+// What attn_paged and attn_sinks have in common: q, its norm and tables, window and sinks, the output and the partials.
+struct NewTokens {
+  Tensor q, qw, cos, sin, out, ws;
+  float scale, eps;
+  int64_t window, sinks, sq[3], B, H, T, D;
+  int dt, flags;
+  const float* w;
+  Rope r;
+  size_t need = 0;
+
+  bool take_args(const Tensor& cache) {
+    if (q.dim() != 4 || cache.dim() != 4 || !strides16(q, sq)) return false;
+    B = q.size(0), H = q.size(1), T = q.size(2), D = q.size(3);
+    dt = dtype_of(q);
+    const c10::Device dev = q.device();
+    const int64_t K = cache.size(1);
+    if (dt < 0 || K <= 0 || H % K || cache.size(3) != D || cache.scalar_type() != q.scalar_type() || B < 1 || T < 1 ||
+        B > INT_MAX || H > INT_MAX || T > INT_MAX || window < 0 || sinks < 0 || window > INT_MAX / 2 ||
+        sinks > INT_MAX / 2 || (sinks && !window) || c10::hip::current_device() != dev.index())
+      return false;
+    if (!rope_ok(cos, sin, B, T, D, dev, r) || !gain_ok(qw, D, dev) || (uintptr_t)ptr(qw) % 16) return false;
+    return true;
+  }
+  void set_flags(bool norm_q) {
+    flags = (norm_q ? FORGE_NORM_QK : 0) | (r.cos ? FORGE_ROPE : 0);
+    w = norm_q ? static_cast<const float*>(ptr(qw)) : nullptr;
+  }
+  // (without the GIL) the output, and memory for the partials of a split launch; without it nothing is split
+  void allocate(int64_t K, int64_t max_kv) {
+    const auto opts = q.options().requires_grad(false);
+    out = at::empty({B, T, H, D}, opts);
+    need = forge_attn_paged_workspace_bytes(dt, (int)B, (int)T, (int)H, (int)K, (int)D, max_kv, (int)window, (int)sinks);
+    if (!need) return;
+    try {
+      ws = at::empty({(int64_t)need}, opts.dtype(at::kByte));
+    } catch (const c10::OutOfMemoryError&) {
+    }
+  }
+};
+
+// attn_paged(q, k_pages, v_pages, table, row_pos, new_lens | None, scale, max_kv_len | None, window, sinks,
+//            q_weight | None, eps, norm_q, cos | None, sin | None)
+PyObject* attn_paged_impl(PyObject* const* a) {
+  NewTokens n;
+  Tensor kp, vp, table, row_pos, news;
+  int64_t max_kv = 0;
+  if (!take(a[0], n.q) || !take(a[1], kp) || !take(a[2], vp) || !take(a[3], table) || !take(a[4], row_pos) ||
+      !take_opt(a[5], news) || !as_float(a[6], n.scale) || (a[7] != Py_None && !as_int(a[7], max_kv)) ||
+      !as_int(a[8], n.window) || !as_int(a[9], n.sinks) || !take_opt(a[10], n.qw) || !as_float(a[11], n.eps) ||
+      !take_opt(a[13], n.cos) || !take_opt(a[14], n.sin))
+    return nullptr;
+  if (!n.take_args(kp)) return nullptr;
+  const c10::Device dev = n.q.device();
+  Pages p;
+  if (!pages_ok(kp, vp, table, n.B, dev, p) || !rows_ok(row_pos, n.B, dev) || (news.defined() && !rows_ok(news, n.B, dev)))
+    return nullptr;
+  const int64_t most = p.max * p.size, K = kp.size(1);
+  max_kv = a[7] == Py_None ? most : std::min(max_kv, most);
+  if (max_kv < 1) return nullptr;
+  n.set_flags(a[12] == Py_True);
+  int st;
+  {
+    NoGil unlocked;
+    n.allocate(K, max_kv);
+    st = forge_attn_paged(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w,
+                          n.eps, n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kp), ptr(vp), p.s[0], p.s[1], p.s[2], p.n,
+                          (int)p.size, static_cast<const int32_t*>(ptr(table)), p.stride, (int)p.max,
+                          static_cast<const int32_t*>(ptr(row_pos)), static_cast<const int32_t*>(ptr(news)), max_kv,
+                          (int)n.window, (int)n.sinks, n.scale, n.out.data_ptr(), n.out.stride(0), n.out.stride(1),
+                          n.out.stride(2), n.ws.defined() ? n.ws.data_ptr() : nullptr, n.need,
+                          c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return st < 0 ? nullptr : result(st, n.out);
+}
+
+// attn_sinks(q, k_cache, v_cache, scale, window, sinks, pos | None, pos_dev | None, row_pos | None, max_kv_len | None,
+//            q_weight | None, eps, norm_q, cos | None, sin | None)
+PyObject* attn_sinks_impl(PyObject* const* a) {
+  NewTokens n;
+  Tensor kc, vc, pos_dev, row_pos;
+  int64_t pos = 0, max_kv = -1, sk[3], sv[3];
+  if (!take(a[0], n.q) || !take(a[1], kc) || !take(a[2], vc) || !as_float(a[3], n.scale) || !as_int(a[4], n.window) ||
+      !as_int(a[5], n.sinks) || (a[6] != Py_None && !as_int(a[6], pos)) || !take_opt(a[7], pos_dev) ||
+      !take_opt(a[8], row_pos) || (a[9] != Py_None && !as_int(a[9], max_kv)) || !take_opt(a[10], n.qw) ||
+      !as_float(a[11], n.eps) || !take_opt(a[13], n.cos) || !take_opt(a[14], n.sin))
+    return nullptr;
+  if (!n.take_args(kc) || n.window < 1) return nullptr;
+  const c10::Device dev = n.q.device();
+  if (kc.sizes() != vc.sizes() || kc.scalar_type() != vc.scalar_type() || kc.device() != dev || vc.device() != dev ||
+      kc.size(0) != n.B || !strides16(kc, sk) || !strides16(vc, sv) || !std::equal(sk, sk + 3, sv))
+    return nullptr;
+  const int64_t K = kc.size(1), max_len = kc.size(2);
+  if (row_pos.defined()) {
+    if (!rows_ok(row_pos, n.B, dev)) return nullptr;
+    pos_dev.reset();
+    pos = 0;
+  } else if (pos_dev.defined()) {
+    if (pos_dev.scalar_type() != at::kLong || pos_dev.numel() < 1 || pos_dev.device() != dev) return nullptr;
+    pos = 0;
+  } else {
+    if (pos < 0 || pos > max_len - n.T) return nullptr;
+    max_kv = pos + n.T;
+  }
+  max_kv = max_kv < 0 ? max_len : std::min(max_kv, max_len);
+  if (max_kv < 1) return nullptr;
+  n.set_flags(a[12] == Py_True);
+  int st;
+  {
+    NoGil unlocked;
+    n.allocate(K, max_kv);
+    st = forge_attn_sinks(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w,
+                          n.eps, n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kc), ptr(vc), sk[0], sk[1],
+                          max_len > 1 ? sk[2] : n.D, max_len, static_cast<const int32_t*>(ptr(row_pos)),
+                          static_cast<const int64_t*>(ptr(pos_dev)), pos, max_kv, (int)n.window, (int)n.sinks, n.scale,
+                          n.out.data_ptr(), n.out.stride(0), n.out.stride(1), n.out.stride(2),
+                          n.ws.defined() ? n.ws.data_ptr() : nullptr, n.need,
+                          c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return st < 0 ? nullptr : result(st, n.out);
+}
+
 // An exception on the way (out of memory, for one) goes the Python way too, which raises it there.
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -391,7 +587,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&entry<NAME##_impl, N>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     FORGE_ENTRY(decode_append, 21), FORGE_ENTRY(kv_append, 11), FORGE_ENTRY(prefill, 11),
-    FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), {nullptr, nullptr, 0, nullptr},
+    FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), FORGE_ENTRY(kv_append_paged, 13),
+    FORGE_ENTRY(attn_paged, 15),    FORGE_ENTRY(attn_sinks, 15), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_forge_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -580,6 +580,10 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     position row_pos[b] + t, i.e. slot position % page_size of page page_table[b, position // page_size] of the pools
     [n_pages, K, page_size, D]. Tokens t >= new_lens[b] (a padded batch) and positions without a page (an entry
     outside the pool, or past the table's end) are not written. Lengths, table and positions are int32 on the GPU."""
+    st = host().kv_append_paged(k, v, k_pages, v_pages, page_table, row_pos, new_lens, k_weight, float(eps), bool(norm_k),
+                                bool(norm_v), cos, sin)
+    if st is not None:
+        return check(st, "forge_kv_append_paged")
     if k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [B, K, T, D]")
     B, K, T, D = k.shape
@@ -649,6 +653,11 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     Keys whose table entry lies outside the pool (-1: given back) are invisible. Returns [B,T,H,D]; rows
     t >= new_lens[b] and rows that see nothing are zeros. max_kv_len: an upper bound on row_pos[b] + new_lens[b]
     (default: what the table can hold); it sizes the launch."""
+    if out is None:
+        r = host().attn_paged(q, k_pages, v_pages, page_table, row_pos, new_lens, float(scale), max_kv_len, window, sinks,
+                              q_weight, float(eps), bool(norm_q), cos, sin)
+        if r is not None:
+            return r if r.__class__ is not int else check(r, "forge_attn_paged")
     dev = _need_device(q, k_pages, v_pages, page_table, row_pos, new_lens, cos, sin, q_weight if norm_q else None, out)
     B, T = q.shape[0], q.shape[2]
     table = _pages(k_pages, v_pages, page_table, B, dev)
@@ -680,6 +689,11 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
     [B,K,max_len,D] that holds the new keys already: query t of row b sits at p = base_b + t (row_pos, pos_dev or
     pos, as attn_decode) and sees keys s <= p with s > p - window or s < sinks. Any T: whole prompts, chunks, verify and
     decode steps. Returns [B,T,H,D]."""
+    if out is None:
+        r = host().attn_sinks(q, k_cache, v_cache, float(scale), window, sinks, pos, pos_dev, row_pos, max_kv_len, q_weight,
+                              float(eps), bool(norm_q), cos, sin)
+        if r is not None:
+            return r if r.__class__ is not int else check(r, "forge_attn_sinks")
     dev = _need_device(q, k_cache, v_cache, pos_dev, row_pos, cos, sin, q_weight if norm_q else None, out)
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.dtype != v_cache.dtype or q.shape[0] != k_cache.shape[0]:
         raise ValueError(f"q {tuple(q.shape)} does not fit caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
