@@ -38,9 +38,9 @@ struct PagedParams {
   float scale_log2;
   void* out;
   int64_t sob, sot, soh;
-  // Key split: a row block's tiles go to ceil(tiles / tiles_per_part) blocks, at most nparts, each
-  // writing an fp32 partial that the combine kernel merges in part order.
-  int nparts, tiles_per_part;
+  // Key split: a row block's tiles go to ceil(tiles / part_tiles) blocks (at most nparts) in equal shares, each
+  // writing an fp32 partial that the combine kernel merges in part order. nparts 1: no split.
+  int nparts, part_tiles;
   float2* ws_ml;  // [B][K][rows][nparts]
   float* ws_o;    // ... [D]
 
@@ -59,19 +59,36 @@ constexpr int step_rows_most(int esize, int D) {
   return esize == 4 ? (D <= 64 ? 64 : D == 128 ? 32 : 16) : D <= 128 ? 64 : D == 256 ? 32 : 16;
 }
 constexpr int step_keys(int esize, int D, int rows) { return esize * D * (rows / 16) >= 1024 ? 16 : 32; }
+// Its blocks per CU (registers, and 160 KB of LDS).
+constexpr int step_blocks_per_cu(int esize, int D, int rows) {
+  const int bytes = esize * D * (rows == 64 ? 2 : 1);
+  return bytes <= 128 && rows == 16 ? 4 : bytes <= 256 ? 2 : 1;
+}
 
 // How the host cuts a call: rows per block, keys per tile, parts.
 struct PagedPlan {
   bool chunk;  // paged_chunk.hip's kernel (rows 128), or paged.hip's
   int rows, keys;
-  int nparts, tiles_per_part;
+  int nparts, part_tiles;
 };
 
-// The keys of query rows row0 .. row0 + nrows - 1 of batch row b, as tiles of KT keys: the tiles that
-// hold first tokens (from key 0 on), then those from the first query's window to the last query.
+// Batch row b: the position of its first new token, and its real query rows (new_lens * G). A position
+// outside the cache leaves nothing visible, and tokens past `limit` are not real.
+__device__ __forceinline__ void row_extent(const PagedParams& p, int b, int& base, int& rows) {
+  int64_t at = p.row_pos ? (int64_t)p.row_pos[b] : p.pos_dev ? *p.pos_dev : p.pos0;
+  if (at < 0 || at > p.limit) at = p.limit;
+  base = (int)at;
+  int nl = p.new_lens ? p.new_lens[b] : p.T;
+  nl = nl < 0 ? 0 : nl < p.T ? nl : p.T;
+  if (nl > p.limit - base) nl = p.limit - base;
+  rows = nl * p.G;
+}
+
+// The keys of query rows row0 .. row0 + nrows - 1 of a batch row, as tiles of KT keys: the tiles that hold
+// first tokens (from key 0 on), then those from the first query's window to the last query.
 struct RowSpan {
   int base;         // position of the row's first new token
-  int rows;         // query rows of the batch row that are real (new_lens * G)
+  int rows;         // query rows of the batch row that are real
   int first, last;  // positions of the block's first and last real query
   int sink_tiles, main_tile, tiles;
   __device__ __forceinline__ int tile_key(int i, int KT) const {
@@ -79,23 +96,16 @@ struct RowSpan {
   }
 };
 
-__device__ __forceinline__ RowSpan row_span(const PagedParams& p, int b, int row0, int nrows, int KT) {
+__device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int rows, int row0, int nrows, int KT) {
   RowSpan w;
-  int64_t base = p.row_pos ? (int64_t)p.row_pos[b] : p.pos_dev ? *p.pos_dev : p.pos0;
-  // (a position outside the cache leaves nothing visible)
-  if (base < 0 || base > p.limit) base = p.limit;
-  w.base = __builtin_amdgcn_readfirstlane((int)base);
-  int nl = p.new_lens ? p.new_lens[b] : p.T;
-  nl = __builtin_amdgcn_readfirstlane(nl < 0 ? 0 : nl < p.T ? nl : p.T);
-  if (w.base >= p.limit) nl = 0;
-  else if (nl > p.limit - w.base) nl = p.limit - w.base;
-  w.rows = nl * p.G;
+  w.base = base;
+  w.rows = rows;
   w.sink_tiles = w.main_tile = w.tiles = 0;
   w.first = w.last = 0;
-  if (row0 >= w.rows) return w;
-  const int row1 = (row0 + nrows < w.rows ? row0 + nrows : w.rows) - 1;
-  w.first = w.base + row0 / p.G;
-  w.last = w.base + row1 / p.G;
+  if (row0 >= rows) return w;
+  const int row1 = (row0 + nrows < rows ? row0 + nrows : rows) - 1;
+  w.first = base + row0 / p.G;
+  w.last = base + row1 / p.G;
   const int lo = p.window > 0 && w.first >= p.window ? w.first - p.window + 1 : 0;
   w.main_tile = lo / KT;
   const int se = p.sinks < lo ? p.sinks : lo;
@@ -103,6 +113,21 @@ __device__ __forceinline__ RowSpan row_span(const PagedParams& p, int b, int row
   w.sink_tiles = st < w.main_tile ? st : w.main_tile;
   w.tiles = w.sink_tiles + w.last / KT - w.main_tile + 1;
   return w;
+}
+
+// The same for batch row b of a block (uniform: scalar registers).
+__device__ __forceinline__ RowSpan row_span(const PagedParams& p, int b, int row0, int nrows, int KT) {
+  int base, rows;
+  row_extent(p, b, base, rows);
+  return make_span(p, __builtin_amdgcn_readfirstlane(base), __builtin_amdgcn_readfirstlane(rows), row0, nrows, KT);
+}
+
+// Part `part` of a row block's tiles; how many parts it has (0 or 1: no partials).
+__device__ __forceinline__ int take_tiles(const PagedParams& p, const RowSpan& w, int part, int& begin, int& end) {
+  const int parts = p.nparts < 2 ? 1 : (w.tiles + p.part_tiles - 1) / p.part_tiles;
+  begin = (int)((int64_t)part * w.tiles / (parts > 1 ? parts : 1));
+  end = (int)((int64_t)(part + 1) * w.tiles / (parts > 1 ? parts : 1));
+  return parts;
 }
 
 // blockIdx.x -> (part, row block, batch row, KV head). Late row blocks first (a causal chunk's have the
@@ -137,10 +162,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int b
   const int flat = (int)blockIdx.x / (p.B * p.K) * (256 / LPR) + threadIdx.x / LPR;
   const int x = 4 * (threadIdx.x % LPR);
   const int kvh = pair % p.K, b = pair / p.K;
-  if (flat >= p.rows) return;
-  const RowSpan w = row_span(p, b, flat / block_rows * block_rows, block_rows, KT);
-  if (flat >= w.rows || w.tiles <= p.tiles_per_part) return;  // written by its block
-  const int parts = (w.tiles + p.tiles_per_part - 1) / p.tiles_per_part;
+  int base, rows;
+  row_extent(p, b, base, rows);
+  if (flat >= rows) return;
+  const RowSpan w = make_span(p, base, rows, flat / block_rows * block_rows, block_rows, KT);
+  const int parts = (w.tiles + p.part_tiles - 1) / p.part_tiles;
+  if (parts < 2) return;  // written by its block
   const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts;
   float M = kNegInf;
   for (int i = 0; i < parts; ++i) M = fmaxf(M, p.ws_ml[slot + i].x);

@@ -170,12 +170,18 @@ template <typename T, int D, int RB> struct StepLds {
   static constexpr int ROWS = 16 * RB;
   static constexpr int OUT = ROWS * D * 4;                                // a wave's output in fp32
   static constexpr int WAVE = 2 * TL::TILEB > OUT ? 2 * TL::TILEB : OUT;  // a wave's K and V tile, later its output
-  static constexpr int BYTES = 4 * WAVE + 4 * ROWS * 8;                   // and (m, l) of every wave's rows
-  static constexpr int BLOCKS = BYTES <= 80 * 1024 && TL::KT == 32 ? 2 : 1; // per CU: by its 160 KB, and by registers
+  // The query operands are read from LDS in each tile where the output and the tile in flight take the
+  // registers: a reload of a spilled one would wait for the tile loads it queues behind.
+  static constexpr bool Q_LDS = TL::ROWB * RB >= 1024;
+  static constexpr int ML = 4 * ROWS * 8;                                 // (m, l) of every wave's rows
+  static constexpr int Q_OFF = 4 * WAVE + ML;
+  static constexpr int BYTES = Q_OFF + (Q_LDS ? ROWS * TL::ROWB : 0);
+  static constexpr int BLOCKS = step_blocks_per_cu(sizeof(T), D, ROWS);
+  static_assert(BLOCKS * BYTES <= 160 * 1024, "LDS");
 };
 
 template <typename T, int D, int RB>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(StepLds<T, D, RB>::BLOCKS)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(StepLds<T, D, RB>::BLOCKS >= 2 ? 2 : 1)))
 void paged_step_kernel(PagedParams p) {
   using TL = StepTile<T, D, RB>;
   using LD = StepLds<T, D, RB>;
@@ -190,10 +196,10 @@ void paged_step_kernel(PagedParams p) {
   int part, rblk, b, kvh;
   block_unit(p, (p.rows + ROWS - 1) / ROWS, part, rblk, b, kvh);
   const RowSpan w = row_span(p, b, rblk * ROWS, ROWS, KT);
-  const int begin = part * p.tiles_per_part;
-  const int end = begin + p.tiles_per_part < w.tiles ? begin + p.tiles_per_part : w.tiles;
-  const bool whole = w.tiles <= p.tiles_per_part;
-  if (part > 0 && begin >= w.tiles) return;
+  int begin, end;
+  const int parts = take_tiles(p, w, part, begin, end);
+  const bool whole = parts < 2;
+  if (part > 0 && part >= parts) return;
 
   // ---- key tiles of this wave: begin + wave, + 4, ...
   u32x4 kr[NL], vr[NL];
@@ -250,21 +256,29 @@ void paged_step_kernel(PagedParams p) {
     bad = miss;
   };
   int i = begin + wave;
-  constexpr bool kLate = D >= 512;  // (registers: the first tile after the query rows)
-  if (!kLate && i < end) load(i);
+  if (i < end) load(i);
 
   // ---- query rows, as B operands; rows behind the row's last one stand for that one (never written)
-  u32x4 q[RB][S];
+  u32x4 q[LD::Q_LDS ? 1 : RB][S];
   int qpos[RB];
+  char* ql = smem + LD::Q_OFF;  // [ROWS][chunks turned with the row]
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int row = rblk * ROWS + 16 * r + n;
     const int at = row < w.rows ? row : w.rows - 1;
     qpos[r] = w.base + at / p.G;
-    if (w.rows > 0) step_load_q<T, D>(p, b, kvh, at, g, q[r]);
+    if constexpr (LD::Q_LDS) {
+      if (r % 4 == wave && w.rows > 0) {
+        step_load_q<T, D>(p, b, kvh, at, g, q[0]);
+#pragma unroll
+        for (int st = 0; st < S; ++st)
+          *reinterpret_cast<u32x4*>(ql + (16 * r + n) * TL::ROWB + (((4 * st + g) ^ n) << 4)) = q[0][st];
+      }
+    } else if (w.rows > 0) {
+      step_load_q<T, D>(p, b, kvh, at, g, q[r]);
+    }
   }
-
-  if (kLate && i < end) load(i);
+  if constexpr (LD::Q_LDS) __syncthreads();
 
   f32x4 o[RB][DB];
   float m[RB], l[RB];
@@ -304,7 +318,12 @@ void paged_step_kernel(PagedParams p) {
         const int row = 16 * kb + n;
         const u32x4 a = *reinterpret_cast<const u32x4*>(kt + row * TL::ROWB + (((4 * st + g) ^ step_swz_k<T, D>(row)) << 4));
 #pragma unroll
-        for (int r = 0; r < RB; ++r) s[r][kb] = Mma<T>::k32(a, q[r][st], s[r][kb]);
+        for (int r = 0; r < RB; ++r) {
+          u32x4 x;
+          if constexpr (LD::Q_LDS) x = *reinterpret_cast<const u32x4*>(ql + (16 * r + n) * TL::ROWB + (((4 * st + g) ^ n) << 4));
+          else x = q[r][st];
+          s[r][kb] = Mma<T>::k32(a, x, s[r][kb]);
+        }
       }
 
     // a tile that every row of the block sees whole needs no mask

@@ -22,9 +22,9 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   PagedPlan plan{};
   const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
   const int64_t rows = (int64_t)G * T;
-  const int most = step_rows_most(es, D);
+  const int row_most = step_rows_most(es, D);
   plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  if (plan.rows > most) plan.rows = most;
+  if (plan.rows > row_most) plan.rows = row_most;
   plan.keys = step_keys(es, D, plan.rows);
   if (es == 2 && D >= 64 && D <= 256 && rows > 64) {
     plan.chunk = true;
@@ -32,21 +32,25 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     plan.keys = D == 256 ? 32 : 64;
   }
   plan.nparts = 1;
-  // tiles that a block can have: its queries' window and the first tokens, or the whole row
-  const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
-  int64_t keys = max_kv;
-  if (window > 0 && window + tokens + sinks < keys) keys = window + tokens + sinks;
-  const int64_t tiles = (keys + plan.keys - 1) / plan.keys + 3;
-  plan.tiles_per_part = (int)tiles;
   if (!split) return plan;
+  // tiles that a block can have: its queries' window and the first tokens (whose ends may lie inside tiles), or
+  // the whole row
+  const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
+  int64_t tiles = (max_kv + plan.keys - 1) / plan.keys;
+  if (window > 0) {
+    const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
+    if (seen < tiles) tiles = seen;
+  }
+  const int64_t slots = (int64_t)device_cus() * (plan.chunk ? 2 : step_blocks_per_cu(es, D, plan.rows));
   const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
-  const int64_t want = ((plan.chunk ? 2 : 4) * (int64_t)device_cus() + units - 1) / units;
-  int64_t per = (tiles + want - 1) / want;
-  if (per < 8) per = 8;  // two tiles for each wave
+  const int64_t least = 8, most = plan.chunk ? 1 << 20 : 64;
+  int64_t per = (units * tiles + slots - 1) / slots;
+  if (per > most) per = most;
+  if (per < least) per = least;
   const int64_t parts = (tiles + per - 1) / per;
   if (parts > 1) {
     plan.nparts = (int)parts;
-    plan.tiles_per_part = (int)per;
+    plan.part_tiles = (int)((tiles + parts - 1) / parts);
   }
   return plan;
 }
@@ -85,7 +89,7 @@ static int paged_run(int dtype, int D, PagedParams p, float scale, void* workspa
   const bool split = workspace != nullptr;
   const PagedPlan plan = paged_plan(dtype, p.B, p.T, p.H, p.K, D, p.limit, p.window, p.sinks, split);
   p.nparts = plan.nparts;
-  p.tiles_per_part = plan.tiles_per_part;
+  p.part_tiles = plan.part_tiles;
   if (plan.nparts > 1) {
     if (workspace_bytes < paged_ws_bytes(plan, p.B, p.T, p.H, D)) return set_error("workspace too small");
     if ((uintptr_t)workspace % 256) return set_error("the workspace must be 256-byte aligned");

@@ -91,10 +91,10 @@ void paged_chunk_kernel(PagedParams p) {
   int part, rblk, b, kvh;
   block_unit(p, (p.rows + BM - 1) / BM, part, rblk, b, kvh);
   const RowSpan w = row_span(p, b, rblk * BM, BM, BN);
-  const int begin = part * p.tiles_per_part;
-  const int end = begin + p.tiles_per_part < w.tiles ? begin + p.tiles_per_part : w.tiles;
-  const bool whole = w.tiles <= p.tiles_per_part;
-  if (part > 0 && begin >= w.tiles) return;
+  int begin, end;
+  const int parts = take_tiles(p, w, part, begin, end);
+  const bool whole = parts < 2;
+  if (part > 0 && part >= parts) return;
 
   // rows without a real token come out as zeros
   if (part == 0 && w.rows < rblk * BM + BM) {
