@@ -11,6 +11,11 @@ __device__ __forceinline__ int scalar_load(const int32_t* p) {
   return *(const __attribute__((address_space(4))) int32_t*)p;
 }
 
+// A block's share of a planned call: part `part` of `parts` of row block `pair` (b * row blocks + row block).
+struct PagedItem {
+  int pair, part, parts, slot;
+};
+
 struct PagedParams {
   const void* q;
   int64_t sqb, sqh, sqt;
@@ -41,8 +46,13 @@ struct PagedParams {
   // Key split: a row block's tiles go to ceil(tiles / part_tiles) blocks (at most nparts) in equal shares, each
   // writing an fp32 partial that the combine kernel merges in part order. nparts 1: no split.
   int nparts, part_tiles;
-  float2* ws_ml;  // [B][K][rows][nparts]
-  float* ws_o;    // ... [D]
+  // Planned calls (the chunk kernel, rows of different lengths): block x takes item items[x / K] of KV head
+  // x % K; the pairs say where the merge finds a row block's partials. Null: the static split above.
+  const PagedItem* items;
+  const int2* pairs;  // [B][row blocks]: (its first slot, parts)
+  int slots;          // blocks that the device holds at a time
+  float2* ws_ml;      // [slot][block's rows]
+  float* ws_o;        // ... [D]
 
   // The page that holds position `key` (below limit, so the table has an entry for it) of batch row b; -1
   // where the table names none of the pool.
@@ -67,10 +77,14 @@ constexpr int step_blocks_per_cu(int esize, int D, int rows) {
 
 // How the host cuts a call: rows per block, keys per tile, parts.
 struct PagedPlan {
-  bool chunk;  // paged_chunk.hip's kernel (rows 128), or paged.hip's
+  bool chunk;    // paged_chunk.hip's kernel (rows 128), or paged.hip's
+  bool planned;  // the parts are planned on the device
   int rows, keys;
   int nparts, part_tiles;
+  int slots;   // blocks that the device holds at a time
+  int nitems;  // planned: room for this many
 };
+constexpr int kPlanPairs = 4096;  // row blocks (of all batch rows) that a plan can hold
 
 // Batch row b: the position of its first new token, and its real query rows (new_lens * G). A position
 // outside the cache leaves nothing visible, and tokens past `limit` are not real.
@@ -122,26 +136,51 @@ __device__ __forceinline__ RowSpan row_span(const PagedParams& p, int b, int row
   return make_span(p, __builtin_amdgcn_readfirstlane(base), __builtin_amdgcn_readfirstlane(rows), row0, nrows, KT);
 }
 
-// Part `part` of a row block's tiles; how many parts it has (0 or 1: no partials).
-__device__ __forceinline__ int take_tiles(const PagedParams& p, const RowSpan& w, int part, int& begin, int& end) {
-  const int parts = p.nparts < 2 ? 1 : (w.tiles + p.part_tiles - 1) / p.part_tiles;
-  begin = (int)((int64_t)part * w.tiles / (parts > 1 ? parts : 1));
-  end = (int)((int64_t)(part + 1) * w.tiles / (parts > 1 ? parts : 1));
-  return parts;
-}
+// What a block does: part `part` of `parts` (0 or 1: the whole) of row block rblk of (b, kvh); its tiles, and the
+// slot that its partial goes to.
+struct BlockWork {
+  int b, kvh, rblk, part, parts, begin, end, slot;
+  RowSpan span;
+  bool none;  // nothing to do
+};
 
-// blockIdx.x -> (part, row block, batch row, KV head). Late row blocks first (a causal chunk's have the
-// most keys). The (batch row, KV head, part) triples follow each other, so where they are a multiple of 8
-// in number all blocks that read the same keys run on one XCD and meet in its L2.
-__device__ __forceinline__ void block_unit(const PagedParams& p, int nrb, int& part, int& rblk, int& b, int& kvh) {
-  const int pairs = p.B * p.K;
+// Late row blocks first (a causal chunk's have the most keys). The (batch row, KV head, part) triples follow
+// each other, so where they are a multiple of 8 in number all blocks that read the same keys run on one XCD and
+// meet in its L2. A row block's tiles go to its parts in equal shares.
+template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const PagedParams& p) {
+  BlockWork w;
+  const int nrb = (p.rows + BM - 1) / BM;
   const int x = blockIdx.x;
-  rblk = nrb - 1 - x / (pairs * p.nparts);
-  const int y = x % (pairs * p.nparts);
-  const int pair = y % pairs;
-  part = y / pairs;
-  b = pair / p.K;
-  kvh = pair % p.K;
+  w.none = true;
+  if (p.items) {
+    w.kvh = x % p.K;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 it = *(const __attribute__((address_space(4))) i32x4*)(p.items + x / p.K);
+    w.part = it[1];
+    w.parts = it[2];
+    w.slot = it[3] * p.K + w.kvh;
+    w.b = it[0] / nrb;
+    w.rblk = it[0] % nrb;
+    if (w.parts < 0) return w;  // behind the last item
+    w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
+  } else {
+    const int pairs = p.B * p.K;
+    w.rblk = nrb - 1 - x / (pairs * p.nparts);
+    const int y = x % (pairs * p.nparts);
+    const int pair = y % pairs;
+    w.part = y / pairs;
+    w.b = pair / p.K;
+    w.kvh = pair % p.K;
+    w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
+    w.parts = p.nparts < 2 ? 1 : (w.span.tiles + p.part_tiles - 1) / p.part_tiles;
+    w.slot = (pair * nrb + w.rblk) * p.nparts + w.part;
+    if (w.part > 0 && w.part >= w.parts) return w;
+  }
+  w.none = false;
+  const int n = w.parts > 1 ? w.parts : 1;
+  w.begin = (int)((int64_t)w.part * w.span.tiles / n);
+  w.end = (int)((int64_t)(w.part + 1) * w.span.tiles / n);
+  return w;
 }
 
 // Four output channels of query row `flat` of (b, kvh).
@@ -153,49 +192,87 @@ __device__ __forceinline__ void store_row(const PagedParams& p, int b, int kvh, 
   else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
 }
 
+// Rows of a merging block: 256 threads of D / 4 lanes a row, within one row block.
+constexpr int combine_rows(int D, int BM) { return 1024 / D < BM ? 1024 / D : BM; }
+
 // Merges the parts of the rows whose tiles were split: D / 4 lanes per row, four channels each, the
 // parts in order.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int block_rows, int KT) {
-  constexpr int LPR = D / 4;
-  const int pair = (int)blockIdx.x % (p.B * p.K);
-  const int flat = (int)blockIdx.x / (p.B * p.K) * (256 / LPR) + threadIdx.x / LPR;
+template <typename T, int D, int BM, int KT>
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int subs) {
+  constexpr int LPR = D / 4, RPB = combine_rows(D, BM);
+  const int nrb = (p.rows + BM - 1) / BM;
+  const int kvh = (int)blockIdx.x % p.K, r = (int)blockIdx.x / p.K;
+  const int sub = r % subs, pair = r / subs;
+  const int b = pair / nrb, rblk = pair % nrb;
+  const int in = sub * RPB + threadIdx.x / LPR, flat = rblk * BM + in;
   const int x = 4 * (threadIdx.x % LPR);
-  const int kvh = pair % p.K, b = pair / p.K;
   int base, rows;
   row_extent(p, b, base, rows);
   if (flat >= rows) return;
-  const RowSpan w = make_span(p, base, rows, flat / block_rows * block_rows, block_rows, KT);
-  const int parts = (w.tiles + p.part_tiles - 1) / p.part_tiles;
+  int parts, stride;
+  int64_t slot;
+  if (p.items) {
+    const int2 e = p.pairs[pair];
+    parts = e.y;
+    slot = (int64_t)e.x * p.K + kvh;
+    stride = p.K;
+  } else {
+    const RowSpan w = make_span(p, base, rows, rblk * BM, BM, KT);
+    parts = (w.tiles + p.part_tiles - 1) / p.part_tiles;
+    slot = ((int64_t)(b * p.K + kvh) * nrb + rblk) * p.nparts;
+    stride = 1;
+  }
   if (parts < 2) return;  // written by its block
-  const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts;
-  float M = kNegInf;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, p.ws_ml[slot + i].x);
-  float L = 0.0f;
+  // eight parts' loads go out together; the running maximum as in the kernels
+  constexpr int U = 8;
+  const float2* ml = p.ws_ml + slot * BM + in;
+  const float* po = p.ws_o + (slot * BM + in) * D + x;
+  const int64_t step = (int64_t)stride * BM;
+  float M = kNegInf, L = 0.0f;
   float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i = 0; i < parts; ++i) {
-    const float2 e = p.ws_ml[slot + i];
-    const float4 o = *reinterpret_cast<const float4*>(p.ws_o + (slot + i) * D + x);
-    const float a = rescale(e.x, M);
-    L += a * e.y;
-    O.x += a * o.x;
-    O.y += a * o.y;
-    O.z += a * o.z;
-    O.w += a * o.w;
+  for (int i0 = 0; i0 < parts; i0 += U) {
+    float2 e[U];
+    float4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (i0 + u < parts ? i0 + u : parts - 1) * step;
+      e[u] = ml[at];
+      o[u] = *reinterpret_cast<const float4*>(po + at * D);
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, e[u].x);
+    const float keep = rescale(M, top);
+    L *= keep;
+    O.x *= keep;
+    O.y *= keep;
+    O.z *= keep;
+    O.w *= keep;
+    M = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float a = i0 + u < parts ? rescale(e[u].x, M) : 0.0f;
+      L += a * e[u].y;
+      O.x += a * o[u].x;
+      O.y += a * o[u].y;
+      O.z += a * o[u].z;
+      O.w += a * o[u].w;
+    }
   }
   store_row<T>(p, b, kvh, flat, x, O, L > 0.0f ? 1.0f / L : 0.0f);
 }
 
-template <typename T, int D>
-static int launch_paged_combine(const PagedParams& p, int block_rows, int KT, hipStream_t s) {
-  constexpr int RPB = 256 / (D / 4);
-  const int64_t blocks = (int64_t)((p.rows + RPB - 1) / RPB) * p.K * p.B;
+template <typename T, int D, int BM, int KT> static int launch_paged_combine(const PagedParams& p, hipStream_t s) {
+  constexpr int RPB = combine_rows(D, BM);
+  const int64_t nrb = (p.rows + BM - 1) / BM;
+  const int subs = p.rows < BM ? (p.rows + RPB - 1) / RPB : BM / RPB;  // (blocks of a row block)
+  const int64_t blocks = nrb * subs * p.K * p.B;
   if (blocks > 0x7fffffff) return set_error("forge_attn_paged: grid too large");
-  hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3((unsigned)blocks), dim3(256), 0, s, p, block_rows, KT);
+  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT>), dim3((unsigned)blocks), dim3(RPB * (D / 4)), 0, s, p, subs);
   return check_launch();
 }
 
 template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
-template <typename T> int launch_paged_chunk(const PagedParams& p, int D, hipStream_t s);
+template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
 
 }  // namespace forge

@@ -193,13 +193,11 @@ void paged_step_kernel(PagedParams p) {
   const int lane = threadIdx.x % kWave;
   const int n = lane & 15, g = lane >> 4;
 
-  int part, rblk, b, kvh;
-  block_unit(p, (p.rows + ROWS - 1) / ROWS, part, rblk, b, kvh);
-  const RowSpan w = row_span(p, b, rblk * ROWS, ROWS, KT);
-  int begin, end;
-  const int parts = take_tiles(p, w, part, begin, end);
-  const bool whole = parts < 2;
-  if (part > 0 && part >= parts) return;
+  const BlockWork work = block_work<ROWS, KT>(p);
+  if (work.none) return;
+  const RowSpan w = work.span;
+  const int b = work.b, kvh = work.kvh, rblk = work.rblk, begin = work.begin, end = work.end;
+  const bool whole = work.parts < 2;
 
   // ---- key tiles of this wave: begin + wave, + 4, ...
   u32x4 kr[NL], vr[NL];
@@ -475,7 +473,7 @@ void paged_step_kernel(PagedParams p) {
     if (whole || !real) {
       store_row<T>(p, b, kvh, flat, 4 * c4, acc, real && L > 0.0f ? 1.0f / L : 0.0f);
     } else {
-      const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts + part;
+      const int64_t slot = (int64_t)work.slot * ROWS + row;
       *reinterpret_cast<float4*>(p.ws_o + slot * D + 4 * c4) = acc;
       if (c4 == 0) p.ws_ml[slot] = make_float2(M, L);
     }
@@ -495,7 +493,7 @@ template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hi
   if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
   hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)blocks), dim3(256), LD::BYTES, s, p);
   int st = check_launch();
-  if (st == 0 && p.nparts > 1) st = launch_paged_combine<T, D>(p, LD::ROWS, StepTile<T, D, RB>::KT, s);
+  if (st == 0 && p.nparts > 1) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
   return st;
 }
 

@@ -8,8 +8,8 @@ namespace forge {
 
 extern template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged_chunk<bf16>(const PagedParams&, int, hipStream_t);
-extern template int launch_paged_chunk<f16>(const PagedParams&, int, hipStream_t);
+extern template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+extern template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 
 static bool paged_dim_ok(int dtype, int D) {
@@ -17,8 +17,9 @@ static bool paged_dim_ok(int dtype, int D) {
 }
 
 // Rows per block, keys per tile and the key split of a call whose rows hold at most max_kv keys.
+// ragged: the rows may have different lengths (row_pos).
 static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_kv, int window, int sinks,
-                            bool split) {
+                            bool ragged, bool split) {
   PagedPlan plan{};
   const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
   const int64_t rows = (int64_t)G * T;
@@ -41,9 +42,16 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
     if (seen < tiles) tiles = seen;
   }
-  const int64_t slots = (int64_t)device_cus() * (plan.chunk ? 2 : step_blocks_per_cu(es, D, plan.rows));
+  plan.slots = device_cus() * (plan.chunk ? 2 : step_blocks_per_cu(es, D, plan.rows));
+  const int64_t slots = plan.slots;
   const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
-  const int64_t least = 8, most = plan.chunk ? 1 << 20 : 64;
+  const int64_t blocks = units / K;
+  if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots) {
+    plan.planned = true;
+    plan.nitems = (int)(slots / K + blocks);
+    return plan;
+  }
+  const int64_t least = 8, most = E("FORGE_MOST", plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys);
   int64_t per = (units * tiles + slots - 1) / slots;
   if (per > most) per = most;
   if (per < least) per = least;
@@ -55,17 +63,28 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   return plan;
 }
 
-static size_t paged_ws_bytes(const PagedPlan& plan, int B, int T, int H, int D) {
-  if (plan.nparts < 2) return 0;
-  const size_t slots = (size_t)B * H * T * plan.nparts;
-  return (slots * 8 + 255) / 256 * 256 + slots * D * 4;
+// The workspace: [items | row blocks' parts] of a planned call, then (m, l) and the output of every slot's rows.
+struct PagedWs {
+  size_t pairs, ml, o, bytes;
+};
+static PagedWs paged_ws(const PagedPlan& plan, int B, int T, int H, int K, int D) {
+  PagedWs w{};
+  if (plan.nparts < 2 && !plan.planned) return w;
+  const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t blocks = (size_t)B * (((size_t)(H / K) * T + plan.rows - 1) / plan.rows);
+  const size_t rows = (plan.planned ? (size_t)plan.nitems : blocks * plan.nparts) * K * plan.rows;
+  w.pairs = plan.planned ? up(plan.nitems * sizeof(PagedItem)) : 0;
+  w.ml = w.pairs + (plan.planned ? up(blocks * sizeof(int2)) : 0);
+  w.o = w.ml + up(rows * sizeof(float2));
+  w.bytes = w.o + rows * D * sizeof(float);
+  return w;
 }
 
 static bool unaligned(const void* p) { return (uintptr_t)p % 16 != 0; }
 
 // Checks what both entry points share, cuts the call and launches it.
-static int paged_run(int dtype, int D, PagedParams p, float scale, void* workspace, size_t workspace_bytes,
-                     hipStream_t s) {
+static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scale, void* workspace,
+                     size_t workspace_bytes, hipStream_t s) {
   if (dtype != FORGE_F32 && dtype != FORGE_BF16 && dtype != FORGE_F16) return set_error("unknown dtype code");
   if (p.B < 0 || p.T < 0 || p.H <= 0 || p.K <= 0 || p.H % p.K) return set_error("bad sizes (H must be a multiple of K)");
   if (!paged_dim_ok(dtype, D)) return set_error("head dim must be 32, 64, 128, 256 (or 512 in bf16/fp16)");
@@ -87,20 +106,26 @@ static int paged_run(int dtype, int D, PagedParams p, float scale, void* workspa
   p.rows = p.G * p.T;
   p.scale_log2 = scale * kLog2e;
   const bool split = workspace != nullptr;
-  const PagedPlan plan = paged_plan(dtype, p.B, p.T, p.H, p.K, D, p.limit, p.window, p.sinks, split);
+  const PagedPlan plan = paged_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, p.row_pos != nullptr, split);
   p.nparts = plan.nparts;
   p.part_tiles = plan.part_tiles;
-  if (plan.nparts > 1) {
-    if (workspace_bytes < paged_ws_bytes(plan, p.B, p.T, p.H, D)) return set_error("workspace too small");
+  p.slots = plan.slots;
+  const PagedWs ws = paged_ws(plan, p.B, p.T, p.H, p.K, D);
+  if (ws.bytes) {
+    if (workspace_bytes < ws.bytes) return set_error("workspace too small");
     if ((uintptr_t)workspace % 256) return set_error("the workspace must be 256-byte aligned");
-    const size_t slots = (size_t)p.B * p.H * p.T * plan.nparts;
-    p.ws_ml = static_cast<float2*>(workspace);
-    p.ws_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (slots * 8 + 255) / 256 * 256);
+    char* at = static_cast<char*>(workspace);
+    if (plan.planned) {
+      p.items = reinterpret_cast<PagedItem*>(at);
+      p.pairs = reinterpret_cast<int2*>(at + ws.pairs);
+    }
+    p.ws_ml = reinterpret_cast<float2*>(at + ws.ml);
+    p.ws_o = reinterpret_cast<float*>(at + ws.o);
   }
   switch (dtype) {
     case FORGE_F32: return launch_paged<float>(p, plan, D, s);
-    case FORGE_BF16: return plan.chunk ? launch_paged_chunk<bf16>(p, D, s) : launch_paged<bf16>(p, plan, D, s);
-    default: return plan.chunk ? launch_paged_chunk<f16>(p, D, s) : launch_paged<f16>(p, plan, D, s);
+    case FORGE_BF16: return plan.chunk ? launch_paged_chunk<bf16>(p, plan, D, s) : launch_paged<bf16>(p, plan, D, s);
+    default: return plan.chunk ? launch_paged_chunk<f16>(p, plan, D, s) : launch_paged<f16>(p, plan, D, s);
   }
 }
 
@@ -111,9 +136,12 @@ using namespace forge;
 extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
                                                    int window, int sinks) {
   if (B <= 0 || T <= 0 || H <= 0 || K <= 0 || H % K || !paged_dim_ok(dtype, D) || max_kv_len <= 0 || window < 0 ||
-      sinks < 0)
+      sinks < 0 || max_kv_len > INT_MAX)
     return 0;
-  return paged_ws_bytes(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, true), B, T, H, D);
+  // (calls with and without row positions may be cut differently: what either needs)
+  const size_t a = paged_ws(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, true, true), B, T, H, K, D).bytes;
+  const size_t b = paged_ws(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, false, true), B, T, H, K, D).bytes;
+  return a > b ? a : b;
 }
 
 extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
@@ -132,6 +160,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   int64_t limit = (int64_t)max_pages * page_size;
   if (max_kv_len < limit) limit = max_kv_len;
   if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
+  if (max_kv_len > INT_MAX) max_kv_len = limit;
   PagedParams p{};
   p.q = q; p.sqb = sqb; p.sqh = sqh; p.sqt = sqt;
   p.qw = q_weight; p.eps = eps; p.flags = flags;
@@ -142,7 +171,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   p.row_pos = row_pos; p.new_lens = new_lens;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
-  return paged_run(dtype, D, p, scale, workspace, workspace_bytes, (hipStream_t)stream);
+  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 extern "C" size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
@@ -173,5 +202,5 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   p.row_pos = row_pos; p.pos_dev = pos_dev; p.pos0 = pos0;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
-  return paged_run(dtype, D, p, scale, workspace, workspace_bytes, (hipStream_t)stream);
+  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, (hipStream_t)stream);
 }

@@ -88,13 +88,11 @@ void paged_chunk_kernel(PagedParams p) {
   const int lane = threadIdx.x % kWave;
   const int n = lane & 31, hi = lane >> 5;
 
-  int part, rblk, b, kvh;
-  block_unit(p, (p.rows + BM - 1) / BM, part, rblk, b, kvh);
-  const RowSpan w = row_span(p, b, rblk * BM, BM, BN);
-  int begin, end;
-  const int parts = take_tiles(p, w, part, begin, end);
-  const bool whole = parts < 2;
-  if (part > 0 && part >= parts) return;
+  const BlockWork work = block_work<BM, BN>(p);
+  if (work.none) return;
+  const RowSpan w = work.span;
+  const int b = work.b, kvh = work.kvh, rblk = work.rblk, part = work.part, begin = work.begin, end = work.end;
+  const bool whole = work.parts < 2;
 
   // rows without a real token come out as zeros
   if (part == 0 && w.rows < rblk * BM + BM) {
@@ -333,7 +331,7 @@ void paged_chunk_kernel(PagedParams p) {
   l_run += __shfl_xor(l_run, 32, kWave);
   if (!valid) return;
   if (!whole) {
-    const int64_t slot = (((int64_t)b * p.K + kvh) * p.rows + flat) * p.nparts + part;
+    const int64_t slot = (int64_t)work.slot * BM + wave * 32 + n;
     float* po = p.ws_o + slot * D + 4 * hi;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -353,7 +351,94 @@ void paged_chunk_kernel(PagedParams p) {
                    make_float4(oacc[d][4 * i], oacc[d][4 * i + 1], oacc[d][4 * i + 2], oacc[d][4 * i + 3]), inv);
 }
 
-template <typename T, int D> static int launch_chunk_d(const PagedParams& p, hipStream_t s) {
+// Plans a call whose rows have different lengths, which only the device knows: one block, a thread per row
+// block. Each row block's tiles are cut into equal parts of at most `per` tiles, the smallest `per` of 16 tried
+// (wave w tries one, over the row blocks in turn) with which all parts are resident at once; the parts go out
+// longest first (64 classes of length), so that a CU that got a long one gets a short one beside it.
+constexpr int kPlanThreads = 1024;
+template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedParams p, PagedItem* items,
+                                                                                        int2* pairs, int nitems) {
+  __shared__ int tiles[kPlanPairs];
+  __shared__ int wave_of[16], wave_tot[16], cls[64], pick;
+  const int nrb = (p.rows + BM - 1) / BM, n = p.B * nrb;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  if (threadIdx.x < 64) cls[threadIdx.x] = 0;
+  int sum = 0;
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    int base, rows;
+    row_extent(p, i / nrb, base, rows);
+    tiles[i] = make_span(p, base, rows, i % nrb * BM, BM, KT).tiles;
+    sum += tiles[i];
+  }
+  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d, kWave);
+  if (lane == 0) wave_tot[wave] = sum;
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < 16; ++w) total += wave_tot[w];
+  // equal shares of all slots, and up to 2.5 times that; fewer than 8 tiles a part cost more than they even out
+  const int room = p.slots / p.K;
+  const int least = max(8, (total + room - 1) / room);
+  auto per_of = [&](int w) { return w == 15 ? 1 << 30 : least + (int)((int64_t)least * w / 10); };
+  {
+    const int per = per_of(wave);
+    int parts = 0;
+    for (int i = lane; i < n; i += kWave) parts += (tiles[i] + per - 1) / per;
+    for (int d = 1; d < kWave; d <<= 1) parts += __shfl_xor(parts, d, kWave);
+    if (lane == 0) wave_of[wave] = parts;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int w = 0;
+    while (w < 15 && wave_of[w] > room) ++w;
+    pick = w;
+  }
+  __syncthreads();
+  const int per = per_of(pick);
+  // lengths relative to the longest part: class 0 is the longest; a row block without a real query is one part
+  // of no tiles, which writes its zeros
+  auto parts_of = [&](int i) { return tiles[i] > 0 ? (tiles[i] + per - 1) / per : 1; };
+  auto class_of = [&](int i, int parts) {
+    const int len = tiles[i] / parts;
+    const int scale = per < (1 << 30) ? per : p.limit / KT + 1;
+    return 63 - (int)min((int64_t)63, (int64_t)len * 64 / (scale + 1));
+  };
+  int mine = 0;
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int parts = parts_of(i);
+    mine += parts;
+    atomicAdd(&cls[class_of(i, parts)], parts);
+  }
+  // slots: row blocks in the order of the threads that hold them
+  int before = mine;
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int y = __shfl_up(before, d, kWave);
+    if (lane >= d) before += y;
+  }
+  if (lane == kWave - 1) wave_tot[wave] = before;
+  before -= mine;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) before += wave_tot[w];
+  if (threadIdx.x == 0) {
+    int at = 0;
+    for (int c = 0; c < 64; ++c) {
+      const int k = cls[c];
+      cls[c] = at;
+      at += k;
+    }
+    pick = at;  // all parts
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+    const int parts = parts_of(i);
+    pairs[i] = make_int2(before, parts);
+    const int at = atomicAdd(&cls[class_of(i, parts)], parts);
+    for (int j = 0; j < parts; ++j) items[at + j] = PagedItem{i, j, parts, before + j};
+    before += parts;
+  }
+  for (int i = pick + threadIdx.x; i < nitems; i += kPlanThreads) items[i] = PagedItem{0, 0, -1, 0};
+}
+
+template <typename T, int D> static int launch_chunk_d(PagedParams p, const PagedPlan& plan, hipStream_t s) {
   using TL = Tile<D>;
   static bool attr_set = false;
   if (chunk_lds<D>() > 64 * 1024 && !attr_set) {
@@ -362,22 +447,29 @@ template <typename T, int D> static int launch_chunk_d(const PagedParams& p, hip
       return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
     attr_set = true;
   }
-  const int64_t blocks = (int64_t)((p.rows + TL::BM - 1) / TL::BM) * p.K * p.B * p.nparts;
+  int64_t blocks = (int64_t)((p.rows + TL::BM - 1) / TL::BM) * p.K * p.B * p.nparts;
+  if (plan.planned) {
+    blocks = (int64_t)plan.nitems * p.K;
+    hipLaunchKernelGGL((paged_plan_kernel<TL::BM, TL::BN>), dim3(1), dim3(kPlanThreads), 0, s, p,
+                       const_cast<PagedItem*>(p.items), const_cast<int2*>(p.pairs), plan.nitems);
+    const int st = check_launch();
+    if (st) return st;
+  }
   if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
   hipLaunchKernelGGL((paged_chunk_kernel<T, D>), dim3((unsigned)blocks), dim3(256), chunk_lds<D>(), s, p);
   const int st = check_launch();
-  return st || p.nparts < 2 ? st : launch_paged_combine<T, D>(p, TL::BM, TL::BN, s);
+  return st || (p.nparts < 2 && !plan.planned) ? st : launch_paged_combine<T, D, TL::BM, TL::BN>(p, s);
 }
 
-template <typename T> int launch_paged_chunk(const PagedParams& p, int D, hipStream_t s) {
+template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
   switch (D) {
-    case 64: return launch_chunk_d<T, 64>(p, s);
-    case 128: return launch_chunk_d<T, 128>(p, s);
-    case 256: return launch_chunk_d<T, 256>(p, s);
+    case 64: return launch_chunk_d<T, 64>(p, plan, s);
+    case 128: return launch_chunk_d<T, 128>(p, plan, s);
+    case 256: return launch_chunk_d<T, 256>(p, plan, s);
     default: return set_error("forge_attn_paged: unsupported head dim");
   }
 }
-template int launch_paged_chunk<bf16>(const PagedParams&, int, hipStream_t);
-template int launch_paged_chunk<f16>(const PagedParams&, int, hipStream_t);
+template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 
 }  // namespace forge
