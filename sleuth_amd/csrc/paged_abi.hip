@@ -51,7 +51,7 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     plan.nitems = (int)(slots / K + blocks);
     return plan;
   }
-  const int64_t least = 8, most = E("FORGE_MOST", plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys);
+  const int64_t least = 8, most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
   int64_t per = (units * tiles + slots - 1) / slots;
   if (per > most) per = most;
   if (per < least) per = least;
