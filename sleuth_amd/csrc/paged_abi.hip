@@ -102,7 +102,6 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   if ((p.flags & FORGE_ROPE) && (!p.cos || !p.sin)) return set_error("FORGE_ROPE needs cos and sin");
   p.G = p.H / p.K;
   if ((int64_t)p.G * p.T > INT_MAX / 2) return set_error("too many query rows");
-  if (p.B == 0 || p.T == 0) return 0;
   p.rows = p.G * p.T;
   p.scale_log2 = scale * kLog2e;
   const bool split = workspace != nullptr;
@@ -155,8 +154,9 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   clear_error();
   if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
   if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
-  if (!page_table || !row_pos) return set_error("null page table or row positions");
   if (max_kv_len <= 0) return set_error("max_kv_len must be positive");
+  if (B == 0 || T == 0) return 0;  // (torch's empty tensors have no address)
+  if (!page_table || !row_pos) return set_error("null page table or row positions");
   int64_t limit = (int64_t)max_pages * page_size;
   if (max_kv_len < limit) limit = max_kv_len;
   if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
@@ -191,6 +191,7 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   if (max_kv_len <= 0 || max_len <= 0) return set_error("max_kv_len and max_len must be positive");
   const int64_t limit = max_kv_len < max_len ? max_kv_len : max_len;
   if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
+  if (B == 0 || T == 0) return 0;
   if (!row_pos && !pos_dev && (pos0 < 0 || T < 0 || pos0 > limit - T))
     return set_error("pos + T exceeds max_kv_len or the cache length");
   PagedParams p{};

@@ -320,6 +320,7 @@ extern "C" int forge_kv_append_paged(int dtype, int B, int T, int K, int D, cons
   if (B < 0 || K <= 0 || T < 0) return set_error("bad sizes");
   const int es = dtype == FORGE_F32 ? 4 : 2, e16 = 16 / es;
   if (D <= 0 || D % (2 * e16) || D > 128 * e16) return set_error("head dim: half of it must be a multiple of 16 bytes, at most 1 KB");
+  if (B == 0 || T == 0) return 0;  // (torch's empty tensors have no address)
   if (!k || !v || !k_pages || !v_pages || !page_table || !row_pos) return set_error("null tensor pointer");
   if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
   if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
