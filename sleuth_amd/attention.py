@@ -16,6 +16,9 @@ of head_norm_rope + cache.update + SDPA):
                         (MFMA flash) with the q norm + RoPE in its q load;
       T > 16, fp32, head dim 32-128:          forge_kv_append, then forge_attn_prefill_f32
                         (the same on fp32 MFMA; from 49 keys on);
+      a paged cache (PagedKVCache):           forge_kv_append_paged, then forge_attn_paged;
+      a window with first tokens that stay visible (spec.sinks): forge_kv_append, then
+                        forge_attn_sinks;
       otherwise         forge_attn_decode_append: the cache write and the split-K
                         attention (decode, verify, static steps, other head sizes)
                         in one launch, the q norm + RoPE fused into the q load.
@@ -81,15 +84,16 @@ def doc_block_mask(doc_ids: torch.Tensor):
     return create_block_mask(mask_mod, B, None, T, T, device=doc_ids.device)
 
 
-def causal_mask(T: int, S: int, offset: int, window: int, device) -> torch.Tensor:
+def causal_mask(T: int, S: int, offset: int, window: int, device, sinks: int = 0) -> torch.Tensor:
     """[T, S] bool, True = may attend: query t sits at position offset + t, key s at s; keys
     after the query are hidden, and with a window those window or more positions before it
-    (attention.py:160-169)."""
+    (attention.py:160-169) but for the first `sinks`."""
     qpos = torch.arange(T, device=device)[:, None] + offset
     kpos = torch.arange(S, device=device)[None, :]
     mask = kpos <= qpos
     if window:
-        mask &= qpos - kpos < window
+        near = qpos - kpos < window
+        mask &= near | (kpos < sinks) if sinks else near
     return mask
 
 
@@ -208,6 +212,7 @@ class Attention(nn.Module):
         self.kind = spec.kind
         self.n_heads, self.n_kv, self.hd = cfg.n_heads, spec.kv_heads, spec.head_dim
         self.window = spec.window
+        self.sinks = getattr(spec, "sinks", 0) if spec.window else 0   # (the host's AttnSpec has none)
         self.scale = cfg.attn_scale or 1.0 / math.sqrt(self.hd)
         self.eps = cfg.norm_eps
         self.use_rope = cfg.pos_type == "rope"
@@ -304,7 +309,7 @@ class Attention(nn.Module):
         if same_doc is not None:
             from . import ops
 
-            if cache is not None or q.shape[2] <= DECODE_MAX_T or not ops.prefill_supported(q) or \
+            if cache is not None or self.sinks or q.shape[2] <= DECODE_MAX_T or not ops.prefill_supported(q) or \
                     torch.cuda.is_current_stream_capturing():
                 return False, None
             docs = _doc_starts(same_doc, q.shape[0], q.shape[2])
@@ -393,6 +398,16 @@ class Attention(nn.Module):
         if q.stride(-1) != 1:
             q = q.contiguous()
 
+        if getattr(cache, "paged", False):
+            # PagedKVCache: rows of any lengths, a different number of new tokens each (cache.new_lens)
+            cache.reserve(T)
+            where = (cache.page_table, cache.seq_lens)
+            kp, vp = cache.k[self.layer_idx], cache.v[self.layer_idx]
+            ops.kv_append_paged(k, v, kp, vp, *where, new_lens=cache.new_lens, norm_v=norm_v, **k_args)
+            self.last_path = "hip-paged"
+            return ops.attn_paged(q, kp, vp, *where, scale=self.scale, new_lens=cache.new_lens, max_kv_len=cache.top(T),
+                                  window=self.window, sinks=self.sinks, **q_args)
+
         if cache is None:
             kc = torch.empty(B, self.n_kv, T, hd, device=q.device, dtype=q.dtype)
             vc = torch.empty_like(kc)
@@ -418,6 +433,11 @@ class Attention(nn.Module):
             chunk = ops.decode_chunk(q.dtype, B, 1, H, self.n_kv, hd, cache.max_len, self.window,
                                      uniform="row_pos" not in pos_kw)
 
+        if self.sinks:
+            ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)
+            self.last_path = "hip-sinks"
+            return ops.attn_sinks(q, kc, vc, scale=self.scale, window=self.window, sinks=self.sinks, max_kv_len=max_kv,
+                                  **pos_kw, **q_args)
         if T > DECODE_MAX_T and offset is not None and ops.prefill_supported(q) and \
                 (q_args["cos"] is None or q_args["cos"].dim() == 2):
             ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)
@@ -459,8 +479,10 @@ class Attention(nn.Module):
         offset = S - q.shape[2]
         if getattr(cache, "static", False) and not tap_active(self.tap_pattern):
             kwargs = {"enable_gqa": True} if self.n_kv != self.n_heads else {}
-            return F.scaled_dot_product_attention(q, k, v, attn_mask=cache.attn_mask(self.window),
-                                                  scale=self.scale, **kwargs)
+            mask = cache.attn_mask(self.window)
+            if self.sinks:
+                mask = mask | (cache.attn_mask(0) & (torch.arange(S, device=q.device) < self.sinks))
+            return F.scaled_dot_product_attention(q, k, v, attn_mask=mask, scale=self.scale, **kwargs)
         if _is_block_mask(same_doc):
             # FlexAttention document mask (doc_block_mask, attention.py:54-64): the reference
             # hands it to flex_attention and allows no pattern tap, window or cached prefix
@@ -479,6 +501,11 @@ class Attention(nn.Module):
         """Per-row torch attention for a cache with per-row lengths."""
         T = q.shape[2]
         lens = list(cache.seq_lens_host)
+        if getattr(cache, "paged", False):
+            if same_doc is not None:
+                raise NotImplementedError("document masks are for whole windows: no paged cache")
+            cache.update(self.layer_idx, k, v)
+            return self._paged_torch(q, cache)
         cache.update(self.layer_idx, k, v)
         out = []
         for b, L in enumerate(lens):
@@ -488,9 +515,26 @@ class Attention(nn.Module):
             out.append(fn(q[b:b + 1], kb, vb, L, same_doc))
         return torch.cat(out, 0)
 
+    def _paged_torch(self, q, cache):
+        """Per-row torch attention over a paged cache that holds the new keys: rows past a row's new
+        tokens are zeros, positions without a page are invisible, as in ops.attn_paged."""
+        out = torch.zeros_like(q)
+        for b, (L, n) in enumerate(zip(cache.seq_lens_host, cache.new_tokens(q.shape[2]))):
+            if not n:
+                continue
+            kb, vb, held = cache.row(self.layer_idx, b, L + n)
+            rep = self.n_heads // self.n_kv
+            scores = (q[b, :, :n].float() @ kb.repeat_interleave(rep, 0).float().transpose(-2, -1)) * self.scale
+            see = self._mask(n, L + n, L, q.device) & held
+            probs = scores.masked_fill(~see, float("-inf")).softmax(-1).nan_to_num(0.0)
+            if tap_active(self.tap_pattern):
+                probs = self.tap_pattern(probs[None])[0]
+            out[b, :, :n] = (probs @ vb.repeat_interleave(rep, 0).float()).to(q.dtype)
+        return out
+
     def _mask(self, T: int, S: int, offset: int, device) -> torch.Tensor:
         """[T, S] bool, True = may attend (attention.py:160-169)."""
-        return causal_mask(T, S, offset, self.window, device)
+        return causal_mask(T, S, offset, self.window, device, self.sinks)
 
     def _fused(self, q, k, v, offset, same_doc=None):
         T, S = q.shape[2], k.shape[2]

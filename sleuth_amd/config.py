@@ -20,6 +20,7 @@ class AttnSpec:
     rope_theta: float
     window: int      # 0 = sees the whole context
     v_from_k: bool   # no v_proj: values come from the keys
+    sinks: int = 0   # first tokens that stay visible beside the window
 
 
 @dataclass
@@ -42,6 +43,7 @@ class ModelConfig:
     attn_scale: float = 0.0       # 0 = 1/sqrt(head_dim)
     layer_types: list[str] = field(default_factory=list)
     sliding_window: int = 0
+    sink_tokens: int = 0          # first tokens that sliding layers keep seeing (0: the window alone)
     swa_head_size: int = 0
     swa_kv_heads: int = 0
     swa_rope_theta: float = 0.0
@@ -63,6 +65,8 @@ class ModelConfig:
             (len(kinds) != n, "layer_types needs one entry per layer"),
             (not set(kinds) <= {"full", "sliding"}, "layer_types entries are 'full' or 'sliding'"),
             ("sliding" in kinds and self.sliding_window <= 0, "sliding layers need sliding_window > 0"),
+            (self.sink_tokens < 0 or (self.sink_tokens > 0 and "sliding" not in kinds),
+             "sink_tokens must not be negative and need sliding layers"),
             (self.pos_type not in ("rope", "none", "learned"), "pos_type is 'rope', 'none' or 'learned'"),
             (bool(self.shared_layers) and len(self.shared_layers) != n, "shared_layers needs one entry per layer"),
         ]
@@ -86,7 +90,7 @@ class ModelConfig:
         """The attention shape of layer i: sliding layers take the swa_* overrides."""
         if self.layer_type(i) == "sliding":
             return AttnSpec("sliding", self.swa_head_size or self.head_dim, self.swa_kv_heads or self.kv_heads,
-                            self.swa_rope_theta or self.rope_theta, self.sliding_window, False)
+                            self.swa_rope_theta or self.rope_theta, self.sliding_window, False, self.sink_tokens)
         return AttnSpec("full", self.head_dim, self.kv_heads, self.rope_theta, 0, self.full_v_from_k)
 
     @property

@@ -7,6 +7,9 @@ generate()             the decode loop of sleuth/forge/infer/generate.py:49-136:
 speculative_generate() greedy draft-then-verify as in speculative.py:83-277: [pending] + k
                        guesses in one forward at offset cache.pos, the agreeing prefix kept by
                        moving pos back (the rewind the reference's keep() does)
+generate_batch()       several prompts of different lengths at once over a paged cache: their chunks
+                       of new tokens padded to one batch, then one token per step for the rows
+                       still running; pages come back as rows end or leave every layer's sight
 GraphDecoder           decode/verify steps replayed from a HIP graph (the role of
                        cuda_graph.py:67-144), built for kernels that read the live length on
                        the device: the attention reads only the keys below pos_t + T, whatever
@@ -25,6 +28,7 @@ from typing import Callable
 import torch
 
 from .kv_cache import KVCache
+from .paged_cache import PagedKVCache
 
 
 @dataclass
@@ -158,6 +162,61 @@ def generate(model, prompt_ids: list[int], max_new_tokens: int = 32, temperature
     if dec is not None:
         stats["graph_replays"] = dec.replays
     return GenerationResult(list(prompt_ids), new, reason, stats)
+
+
+@torch.no_grad()
+def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, temperature: float = 0.0,
+                   stop_ids: set[int] | None = None, seed: int | None = None, chunk: int = 512, page_size: int = 64,
+                   n_pages: int | None = None, cache_dtype: torch.dtype | None = None) -> list[GenerationResult]:
+    """generate() for a batch of prompts of any lengths over a paged cache: every pass takes up to `chunk` tokens of
+    each prompt that has some left (the batch is padded to the longest), then each running row decodes one token per
+    pass. A row's pages come back when it ends, and, where every layer slides, as they leave the windows (the first
+    cfg.sink_tokens positions stay)."""
+    if not prompts or not all(prompts):
+        raise ValueError("every prompt must contain at least one token")
+    if chunk < 1:
+        raise ValueError("chunk must be positive")
+    cfg, dev = model.cfg, next(model.parameters()).device
+    cache = PagedKVCache.for_model(model, len(prompts), cfg.max_seq_len, cache_dtype, page_size, n_pages)
+    gen = torch.Generator(device=dev).manual_seed(seed or 0)
+    specs = [cfg.attn_spec(i) for i in range(cfg.n_layers)]
+    window = max(s.window for s in specs) if all(s.window for s in specs) else 0
+    model.eval()
+    left = [list(p) for p in prompts]                 # tokens that no pass has taken yet
+    results = [GenerationResult(list(p), [], "max_new_tokens") for p in prompts]
+    running = [max_new_tokens > 0] * len(prompts)
+    passes, most_pages = 0, 0
+    while any(running):
+        new = [min(len(x), chunk) if run else 0 for x, run in zip(left, running)]
+        T = max(new)
+        ids = torch.tensor([x[:n] + [0] * (T - n) for x, n in zip(left, new)], device=dev)
+        cache.set_new(new)
+        logits = model(ids, cache=cache).logits
+        passes, most_pages = passes + 1, max(most_pages, cache.n_pages - cache.free_pages)
+        last = logits[torch.arange(len(new), device=dev), torch.tensor(new, device=dev).clamp(min=1) - 1]
+        tokens = _pick(last, temperature, gen).tolist()
+        for b, n in enumerate(new):
+            left[b] = left[b][n:]
+            if not n or left[b]:
+                continue                              # not running, or more of its prompt to come
+            r = results[b]
+            r.new_ids.append(tokens[b])
+            if stop_ids and tokens[b] in stop_ids:
+                r.stop_reason = "stop_token"
+            elif len(r.new_ids) == max_new_tokens:
+                r.stop_reason = "max_new_tokens"
+            elif cache.seq_lens_host[b] >= cfg.max_seq_len:
+                r.stop_reason = "context_full"
+            else:
+                left[b] = [tokens[b]]
+                continue
+            running[b] = False
+            cache.release(b)
+        if window:
+            cache.release_unseen(window, cfg.sink_tokens)
+    for r in results:
+        r.stats = {"kv_cache_mb": round(cache.nbytes() / 1e6, 2), "passes": passes, "most_pages": most_pages}
+    return results
 
 
 def ngram_draft(max_ngram: int = 3) -> Callable[[list[int], int], list[int]]:

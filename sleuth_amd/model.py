@@ -148,6 +148,8 @@ class Transformer(nn.Module):
                         getattr(self, f"rope_sin_{k}").index_select(0, pos)) for k in self._rope_kinds()}
         if getattr(cache, "ragged", False):
             idx = cache.seq_lens.long()[:, None] + torch.arange(T, device=cache.seq_lens.device)[None, :]
+            if getattr(cache, "paged", False):
+                idx = idx.clamp(max=self.cfg.max_seq_len - 1)   # (the padding of a padded batch)
             return {k: (getattr(self, f"rope_cos_{k}")[idx], getattr(self, f"rope_sin_{k}")[idx])
                     for k in self._rope_kinds()}
         return {k: (getattr(self, f"rope_cos_{k}")[offset:offset + T],
@@ -156,8 +158,9 @@ class Transformer(nn.Module):
     def forward(self, idx: torch.Tensor, cache=None, return_hidden: bool = False) -> ModelOutput:
         B, T = idx.shape
         offset = cache.pos if cache is not None else 0
-        if offset + T > self.cfg.max_seq_len:
-            raise ValueError(f"sequence length {offset + T} exceeds max_seq_len {self.cfg.max_seq_len}")
+        longest = cache.top(T) if getattr(cache, "paged", False) else offset + T
+        if longest > self.cfg.max_seq_len:
+            raise ValueError(f"sequence length {longest} exceeds max_seq_len {self.cfg.max_seq_len}")
         if getattr(cache, "static", False):
             cache.new_step()
         # (fp32 rows of 16-bit tables, made once per pass: a model cast to bf16 holds its tables in bf16,

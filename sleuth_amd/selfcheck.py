@@ -75,6 +75,21 @@ def self_check(device: torch.device, dtype: torch.dtype) -> None:
             want = _ref_attention(qp, kc[:1], vc[:1], 0, 0, 0.125)
             if not _close(got, want, tol):
                 raise ForgeError("MFMA prefill disagrees with torch")
+        # pages of 16 in another order: the cache above cut up, then the same windowed with first tokens
+        table = torch.tensor([[2, 0, 1], [5, 3, 4]], dtype=torch.int32, device=dev)
+        kp, vp = (torch.zeros(6, K, 16, D, dtype=dtype, device=dev) for _ in range(2))
+        at = torch.tensor([10, 10], dtype=torch.int32, device=dev)
+        for b in range(B):
+            for j in range(2):
+                kp[table[b, j]], vp[table[b, j]] = kc[b, :, 16 * j:16 * j + 16], vc[b, :, 16 * j:16 * j + 16]
+        ops.kv_append_paged(knew, vnew, kp, vp, table, at, k_weight=w, eps=1e-6, norm_k=True, cos=c, sin=s)
+        qq = q[:, :, :T]
+        got = ops.attn_paged(qq, kp, vp, table, at, scale=0.125)
+        if not _close(got, _ref_attention(qq, kc[:, :, :13], vc[:, :, :13], 10, 0, 0.125), tol):
+            raise ForgeError("paged attention disagrees with torch")
+        same = ops.attn_sinks(qq, kc, vc, scale=0.125, pos=10, window=5, sinks=2)
+        if not _close(ops.attn_paged(qq, kp, vp, table, at, scale=0.125, window=5, sinks=2), same, tol):
+            raise ForgeError("paged and contiguous attention with first tokens disagree")
         torch.cuda.synchronize(device)
     except ForgeError as e:
         raise ForgeError(f"HIP attention self-check failed on {device} ({dtype}): {e}") from e
