@@ -330,14 +330,19 @@ void paged_step_kernel(PagedParams p) {
     if (!full) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        const int lo = p.window > 0 ? qpos[r] - p.window : -1;  // keys above it, or first tokens
-        const int hi = qpos[r] < w.last ? qpos[r] : w.last;
+        // visible: [lo, lo + len), and the first tokens up to the query (no branch per element)
+        const int base = key0 + 4 * g;
+        int lo = (p.window > 0 ? qpos[r] - p.window + 1 : 0) - base;
+        if (lo < -base) lo = -base;
+        const int top = (qpos[r] < w.last ? qpos[r] : w.last) - base + 1;
+        const unsigned len = (unsigned)(top - lo);
+        const int first = p.sinks - base;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int key = key0 + 16 * kb + 4 * g + j;
-            const bool see = key <= hi && (key > lo || key < p.sinks) && !(miss >> kb & 1);
+            const int ce = 16 * kb + j;
+            const bool see = (((unsigned)(ce - lo) < len) | ((ce < first) & (ce < top))) & !(miss >> kb & 1);
             s[r][kb][j] = see ? s[r][kb][j] : kNegInf;
           }
       }
