@@ -64,9 +64,9 @@ struct PagedParams {
 };
 
 // The split kernel's largest row block and its keys per wave tile, by element size and head dim: what the
-// registers hold (fewer keys in flight with more rows or wider ones).
+// registers hold (fewer keys in flight with more rows or wider ones), and what it is asked for (paged_plan).
 constexpr int step_rows_most(int esize, int D) {
-  return esize == 4 ? (D <= 64 ? 64 : D == 128 ? 32 : 16) : D <= 128 ? 64 : D == 256 ? 32 : 16;
+  return esize == 4 ? (D <= 64 ? 64 : D == 128 ? 32 : 16) : D == 32 ? 64 : D <= 256 ? 32 : 16;
 }
 constexpr int step_keys(int esize, int D, int rows) { return esize * D * (rows / 16) >= 1024 ? 16 : 32; }
 // Its blocks per CU (registers, and 160 KB of LDS).

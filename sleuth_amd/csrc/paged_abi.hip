@@ -27,7 +27,11 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   if (plan.rows > row_most) plan.rows = row_most;
   plan.keys = step_keys(es, D, plan.rows);
-  if (es == 2 && D >= 64 && D <= 256 && rows > 64) {
+  // More than 32 rows go to the chunk kernel, whose four waves share each key tile; up to 32 the split kernel's
+  // waves keep more bytes in flight. us, split / chunk: 34 rows (8 batch rows of 2,000 keys, 8 KV heads, head dim
+  // 128) 27.8 / 23.9, 40 rows (32 of 8,000) 239 / 194, 32 rows 183 / 196; head dim 256, one KV head, 16 batch rows of
+  // 8,000: 40 rows 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118.
+  if (es == 2 && D >= 64 && D <= 256 && rows > 32) {
     plan.chunk = true;
     plan.rows = 128;
     plan.keys = D == 256 ? 32 : 64;
@@ -42,13 +46,14 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
     if (seen < tiles) tiles = seen;
   }
-  plan.slots = device_cus() * (plan.chunk ? 2 : step_blocks_per_cu(es, D, plan.rows));
+  // (three chunk blocks per CU at head dim 64: a 512-token chunk at 15,360, 12 q / 4 KV heads, 53 -> 45 us)
+  plan.slots = device_cus() * (plan.chunk ? (D == 64 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
   const int64_t slots = plan.slots;
   const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
   const int64_t blocks = units / K;
   if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots) {
     plan.planned = true;
-    plan.nitems = (int)(slots / K + blocks);
+    plan.nitems = (int)(plan.slots / K + blocks);
     return plan;
   }
   const int64_t least = 8, most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
