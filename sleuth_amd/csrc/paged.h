@@ -37,7 +37,8 @@ struct PagedParams {
   int64_t pos0;
   const int32_t* new_lens;  // or null: T each
   int B, T, H, K, G;
-  int rows;   // G * T
+  unsigned g_inv;  // ceil(2^32 / G): the token of a query row is one high product (rows * G < 2^32)
+  int rows;        // G * T
   int limit;  // keys at or past it do not exist
   int window, sinks;
   float scale_log2;
@@ -53,6 +54,9 @@ struct PagedParams {
   int slots;          // blocks that the device holds at a time
   float2* ws_ml;      // [slot][block's rows]
   float* ws_o;        // ... [D]
+
+  // Token of query row r (r / G).
+  __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((unsigned)r, g_inv); }
 
   // The page that holds position `key` (below limit, so the table has an entry for it) of batch row b; -1
   // where the table names none of the pool.
@@ -118,8 +122,8 @@ __device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int
   w.first = w.last = 0;
   if (row0 >= rows) return w;
   const int row1 = (row0 + nrows < rows ? row0 + nrows : rows) - 1;
-  w.first = base + row0 / p.G;
-  w.last = base + row1 / p.G;
+  w.first = base + p.token(row0);
+  w.last = base + p.token(row1);
   const int lo = p.window > 0 && w.first >= p.window ? w.first - p.window + 1 : 0;
   w.main_tile = lo / KT;
   const int se = p.sinks < lo ? p.sinks : lo;
@@ -144,17 +148,17 @@ struct BlockWork {
   bool none;  // nothing to do
 };
 
-// Late row blocks first (a causal chunk's have the most keys). The (batch row, KV head, part) triples follow
-// each other, so where they are a multiple of 8 in number all blocks that read the same keys run on one XCD and
-// meet in its L2. A row block's tiles go to its parts in equal shares.
+// Grid: x (batch row, KV head), y part, z row block, late ones first (a causal chunk's have the most keys). Blocks
+// start in that order, x first, so where (batch row, KV head) pairs times parts are a multiple of 8 all blocks that
+// read the same keys run on one XCD and meet in its L2.
 template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const PagedParams& p) {
   BlockWork w;
   const int nrb = (p.rows + BM - 1) / BM;
-  const int x = blockIdx.x;
   w.none = true;
   if (p.items) {
-    w.kvh = x % p.K;
     typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const int x = blockIdx.x;
+    w.kvh = x % p.K;
     const i32x4 it = *(const __attribute__((address_space(4))) i32x4*)(p.items + x / p.K);
     w.part = it[1];
     w.parts = it[2];
@@ -164,29 +168,32 @@ template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const 
     if (w.parts < 0) return w;  // behind the last item
     w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
   } else {
-    const int pairs = p.B * p.K;
-    w.rblk = nrb - 1 - x / (pairs * p.nparts);
-    const int y = x % (pairs * p.nparts);
-    const int pair = y % pairs;
-    w.part = y / pairs;
+    const int pair = blockIdx.x;
+    w.part = blockIdx.y;
+    w.rblk = nrb - 1 - (int)blockIdx.z;
     w.b = pair / p.K;
-    w.kvh = pair % p.K;
+    w.kvh = pair - w.b * p.K;
     w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
     w.parts = p.nparts < 2 ? 1 : (w.span.tiles + p.part_tiles - 1) / p.part_tiles;
     w.slot = (pair * nrb + w.rblk) * p.nparts + w.part;
     if (w.part > 0 && w.part >= w.parts) return w;
   }
   w.none = false;
-  const int n = w.parts > 1 ? w.parts : 1;
-  w.begin = (int)((int64_t)w.part * w.span.tiles / n);
-  w.end = (int)((int64_t)(w.part + 1) * w.span.tiles / n);
+  w.begin = 0;
+  w.end = w.span.tiles;
+  if (w.parts > 1) {  // equal shares: the first `more` parts take one tile more
+    const int per = w.span.tiles / w.parts, more = w.span.tiles - per * w.parts;
+    w.begin = w.part * per + (w.part < more ? w.part : more);
+    w.end = w.begin + per + (w.part < more);
+  }
   return w;
 }
 
 // Four output channels of query row `flat` of (b, kvh).
 template <typename T>
 __device__ __forceinline__ void store_row(const PagedParams& p, int b, int kvh, int flat, int ch, float4 a, float f) {
-  T* dst = static_cast<T*>(p.out) + b * p.sob + (int64_t)(flat / p.G) * p.sot + (kvh * p.G + flat % p.G) * p.soh + ch;
+  const int t = p.token(flat);
+  T* dst = static_cast<T*>(p.out) + b * p.sob + (int64_t)t * p.sot + (kvh * p.G + flat - t * p.G) * p.soh + ch;
   T v[4] = {from_f32<T>(a.x * f), from_f32<T>(a.y * f), from_f32<T>(a.z * f), from_f32<T>(a.w * f)};
   if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<float4*>(v);
   else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
@@ -198,12 +205,11 @@ constexpr int combine_rows(int D, int BM) { return 1024 / D < BM ? 1024 / D : BM
 // Merges the parts of the rows whose tiles were split: D / 4 lanes per row, four channels each, the
 // parts in order.
 template <typename T, int D, int BM, int KT>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p, int subs) {
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   constexpr int LPR = D / 4, RPB = combine_rows(D, BM);
   const int nrb = (p.rows + BM - 1) / BM;
-  const int kvh = (int)blockIdx.x % p.K, r = (int)blockIdx.x / p.K;
-  const int sub = r % subs, pair = r / subs;
-  const int b = pair / nrb, rblk = pair % nrb;
+  const int b = (int)blockIdx.x / p.K, kvh = (int)blockIdx.x - b * p.K;
+  const int sub = blockIdx.y, rblk = blockIdx.z, pair = b * nrb + rblk;
   const int in = sub * RPB + threadIdx.x / LPR, flat = rblk * BM + in;
   const int x = 4 * (threadIdx.x % LPR);
   int base, rows;
@@ -266,9 +272,9 @@ template <typename T, int D, int BM, int KT> static int launch_paged_combine(con
   constexpr int RPB = combine_rows(D, BM);
   const int64_t nrb = (p.rows + BM - 1) / BM;
   const int subs = p.rows < BM ? (p.rows + RPB - 1) / RPB : BM / RPB;  // (blocks of a row block)
-  const int64_t blocks = nrb * subs * p.K * p.B;
-  if (blocks > 0x7fffffff) return set_error("forge_attn_paged: grid too large");
-  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT>), dim3((unsigned)blocks), dim3(RPB * (D / 4)), 0, s, p, subs);
+  if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
+  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
+                     0, s, p);
   return check_launch();
 }
 

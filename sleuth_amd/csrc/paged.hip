@@ -106,7 +106,7 @@ template <typename T, int D>
 __device__ __forceinline__ void step_load_q(const PagedParams& p, int b, int kvh, int row, int g,
                                             u32x4 (&q)[StepTile<T, D, 1>::NCH / 4]) {
   constexpr int NCH = StepTile<T, D, 1>::NCH, S = NCH / 4, E = 16 / sizeof(T);
-  const int t = row / p.G, h = kvh * p.G + row % p.G;
+  const int t = p.token(row), h = kvh * p.G + row - t * p.G;
   const T* src = static_cast<const T*>(p.q) + b * p.sqb + h * p.sqh + t * p.sqt;
 #pragma unroll
   for (int s = 0; s < S; ++s) q[s] = *reinterpret_cast<const u32x4*>(src + (4 * s + g) * E);
@@ -264,7 +264,7 @@ void paged_step_kernel(PagedParams p) {
   for (int r = 0; r < RB; ++r) {
     const int row = rblk * ROWS + 16 * r + n;
     const int at = row < w.rows ? row : w.rows - 1;
-    qpos[r] = w.base + at / p.G;
+    qpos[r] = w.base + p.token(at);
     if constexpr (LD::Q_LDS) {
       if (r % 4 == wave && w.rows > 0) {
         step_load_q<T, D>(p, b, kvh, at, g, q[0]);
@@ -494,9 +494,9 @@ template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hi
       return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
     attr_set = true;
   }
-  const int64_t blocks = (int64_t)((p.rows + LD::ROWS - 1) / LD::ROWS) * p.K * p.B * p.nparts;
-  if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
-  hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)blocks), dim3(256), LD::BYTES, s, p);
+  const int nrb = (p.rows + LD::ROWS - 1) / LD::ROWS;
+  if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
+  hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
   int st = check_launch();
   if (st == 0 && p.nparts > 1) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
   return st;

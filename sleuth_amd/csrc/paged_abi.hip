@@ -60,7 +60,8 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   int64_t per = (units * tiles + slots - 1) / slots;
   if (per > most) per = most;
   if (per < least) per = least;
-  const int64_t parts = (tiles + per - 1) / per;
+  int64_t parts = (tiles + per - 1) / per;
+  if (parts > 65535) parts = 65535;  // (the grid's)
   if (parts > 1) {
     plan.nparts = (int)parts;
     plan.part_tiles = (int)((tiles + parts - 1) / parts);
@@ -106,7 +107,8 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   if ((p.flags & FORGE_NORM_QK) && p.qw && unaligned(p.qw)) return set_error("the norm gain must be 16-byte aligned");
   if ((p.flags & FORGE_ROPE) && (!p.cos || !p.sin)) return set_error("FORGE_ROPE needs cos and sin");
   p.G = p.H / p.K;
-  if ((int64_t)p.G * p.T > INT_MAX / 2) return set_error("too many query rows");
+  if ((int64_t)p.G * p.G * p.T > INT_MAX || (int64_t)p.B * p.K > INT_MAX) return set_error("too many query rows");
+  p.g_inv = (unsigned)(((1ull << 32) + p.G - 1) / p.G);
   p.rows = p.G * p.T;
   p.scale_log2 = scale * kLog2e;
   const bool split = workspace != nullptr;

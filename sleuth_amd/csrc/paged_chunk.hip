@@ -184,10 +184,10 @@ void paged_chunk_kernel(PagedParams p) {
   const bool wave_any = w_row < w.rows;
   const int flat = w_row + n;
   const bool valid = flat < w.rows;
-  const int t = (valid ? flat : w.rows - 1) / p.G, h = kvh * p.G + (valid ? flat : w.rows - 1) % p.G;
+  const int t = p.token(valid ? flat : w.rows - 1), h = kvh * p.G + (valid ? flat : w.rows - 1) - t * p.G;
   const int qpos = w.base + t;
-  const int wq_lo = w.base + w_row / p.G;
-  const int wq_hi = w.base + (w_row + 31 < w.rows ? w_row + 31 : w.rows - 1) / p.G;
+  const int wq_lo = w.base + p.token(w_row);
+  const int wq_hi = w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
   V8 qreg[KSTEPS];
   chunk_load_q<T, D>(p, b, h, t, hi, qreg);
 
@@ -468,16 +468,17 @@ template <typename T, int D> static int launch_chunk_d(PagedParams p, const Page
       return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
     attr_set = true;
   }
-  int64_t blocks = (int64_t)((p.rows + TL::BM - 1) / TL::BM) * p.K * p.B * p.nparts;
+  const int nrb = (p.rows + TL::BM - 1) / TL::BM;
+  if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
+  dim3 grid((unsigned)(p.B * p.K), p.nparts, nrb);
   if (plan.planned) {
-    blocks = (int64_t)plan.nitems * p.K;
+    grid = dim3((unsigned)(plan.nitems * p.K));
     hipLaunchKernelGGL((paged_plan_kernel<TL::BM, TL::BN>), dim3(1), dim3(kPlanThreads), 0, s, p,
                        const_cast<PagedItem*>(p.items), const_cast<int2*>(p.pairs), plan.nitems);
     const int st = check_launch();
     if (st) return st;
   }
-  if (blocks > INT_MAX) return set_error("forge_attn_paged: grid too large");
-  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), dim3((unsigned)blocks), dim3(256), chunk_lds<D>(), s, p);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(256), chunk_lds<D>(), s, p);
   const int st = check_launch();
   return st || (p.nparts < 2 && !plan.planned) ? st : launch_paged_combine<T, D, TL::BM, TL::BN>(p, s);
 }
