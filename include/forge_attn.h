@@ -307,8 +307,12 @@ int forge_kv_append_paged(int dtype, int B, int T, int K, int D, const void* k, 
  * rows that see no key, come out as zeros.
  * workspace: forge_attn_paged_workspace_bytes(...) bytes (256-byte aligned) of fp32 partials, where the
  * keys of a row are split over blocks; NULL: not split. Calls that may overlap need separate ones.
- * The order of the sums depends on the shapes and bounds of the call alone.
+ * ws_flags = FORGE_WS_ZEROED promises that its first FORGE_PAGED_COUNTER_BYTES bytes hold zero: small merges
+ * then need no launch of their own (the block that finishes a row last does them). Every call leaves these bytes
+ * zero, so a workspace cleared once before its first use keeps the promise for the calls that follow it
+ * on one stream. The order of the sums depends on the shapes and bounds of the call alone.
  */
+#define FORGE_PAGED_COUNTER_BYTES (64 * 1024)
 size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
                                         int64_t max_kv_len, int window, int sinks);
 int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb,
@@ -319,7 +323,7 @@ int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q
                      int64_t s_table, int max_pages, const int32_t* row_pos,
                      const int32_t* new_lens, int64_t max_kv_len, int window, int sinks,
                      float scale, void* out, int64_t sob, int64_t sot, int64_t soh,
-                     void* workspace, size_t workspace_bytes, void* stream);
+                     void* workspace, size_t workspace_bytes, int ws_flags, void* stream);
 
 /*
  * The same attention over a contiguous cache [B, K, max_len, D] for sliding-window layers whose first
@@ -335,7 +339,7 @@ int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q
                      int64_t sks, int64_t max_len, const int32_t* row_pos, const int64_t* pos_dev,
                      int64_t pos0, int64_t max_kv_len, int window, int sinks, float scale,
                      void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
-                     size_t workspace_bytes, void* stream);
+                     size_t workspace_bytes, int ws_flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -155,7 +155,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, _p, _i64,                        # row_pos, new_lens, max_kv_len
         _i, _i, _f,                          # window, sinks, scale
         _p, _i64, _i64, _i64,                # out + strides (b, t, h)
-        _p, C.c_size_t,                      # workspace, bytes
+        _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
         _p]),
     "forge_attn_sinks_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
     "forge_attn_sinks": (_i, [
@@ -167,7 +167,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, _p, _i64, _i64,                  # row_pos, pos_dev, pos0, max_kv_len
         _i, _i, _f,                          # window, sinks, scale
         _p, _i64, _i64, _i64,                # out + strides (b, t, h)
-        _p, C.c_size_t,                      # workspace, bytes
+        _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
         _p]),
 }
 

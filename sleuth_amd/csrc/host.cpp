@@ -468,16 +468,21 @@ struct NewTokens {
     if (!rope_ok(cos, sin, B, T, D, dev, r) || !gain_ok(qw, D, dev) || (uintptr_t)ptr(qw) % 16) return false;
     return true;
   }
+  void size(int64_t K, int64_t max_kv) {
+    need = forge_attn_paged_workspace_bytes(dt, (int)B, (int)T, (int)H, (int)K, (int)D, max_kv, (int)window, (int)sinks);
+  }
+  // Calls of few partials outside graph capture use their stream's workspace (ops._PagedPartials)
+  bool keep() const { return need && need <= ((size_t)32 << 20) && !capturing(); }
   void set_flags(bool norm_q) {
     flags = (norm_q ? FORGE_NORM_QK : 0) | (r.cos ? FORGE_ROPE : 0);
     w = norm_q ? static_cast<const float*>(ptr(qw)) : nullptr;
   }
-  // (without the GIL) the output, and memory for the partials of a split launch; without it nothing is split
-  void allocate(int64_t K, int64_t max_kv) {
+  // (without the GIL) the output, and memory for the partials of a split launch where the stream's workspace does not
+  // serve; without it nothing is split
+  void allocate(bool kept) {
     const auto opts = q.options().requires_grad(false);
     out = at::empty({B, T, H, D}, opts);
-    need = forge_attn_paged_workspace_bytes(dt, (int)B, (int)T, (int)H, (int)K, (int)D, max_kv, (int)window, (int)sinks);
-    if (!need) return;
+    if (!need || kept) return;
     try {
       ws = at::empty({(int64_t)need}, opts.dtype(at::kByte));
     } catch (const c10::OutOfMemoryError&) {
@@ -485,16 +490,16 @@ struct NewTokens {
   }
 };
 
-// attn_paged(q, k_pages, v_pages, table, row_pos, new_lens | None, scale, max_kv_len | None, window, sinks,
+// attn_paged(table of workspaces, q, k_pages, v_pages, table, row_pos, new_lens | None, scale, max_kv_len | None, window, sinks,
 //            q_weight | None, eps, norm_q, cos | None, sin | None)
 PyObject* attn_paged_impl(PyObject* const* a) {
   NewTokens n;
   Tensor kp, vp, table, row_pos, news;
   int64_t max_kv = 0;
-  if (!take(a[0], n.q) || !take(a[1], kp) || !take(a[2], vp) || !take(a[3], table) || !take(a[4], row_pos) ||
-      !take_opt(a[5], news) || !as_float(a[6], n.scale) || (a[7] != Py_None && !as_int(a[7], max_kv)) ||
-      !as_int(a[8], n.window) || !as_int(a[9], n.sinks) || !take_opt(a[10], n.qw) || !as_float(a[11], n.eps) ||
-      !take_opt(a[13], n.cos) || !take_opt(a[14], n.sin))
+  if (!take(a[1], n.q) || !take(a[2], kp) || !take(a[3], vp) || !take(a[4], table) || !take(a[5], row_pos) ||
+      !take_opt(a[6], news) || !as_float(a[7], n.scale) || (a[8] != Py_None && !as_int(a[8], max_kv)) ||
+      !as_int(a[9], n.window) || !as_int(a[10], n.sinks) || !take_opt(a[11], n.qw) || !as_float(a[12], n.eps) ||
+      !take_opt(a[14], n.cos) || !take_opt(a[15], n.sin))
     return nullptr;
   if (!n.take_args(kp)) return nullptr;
   const c10::Device dev = n.q.device();
@@ -502,34 +507,40 @@ PyObject* attn_paged_impl(PyObject* const* a) {
   if (!pages_ok(kp, vp, table, n.B, dev, p) || !rows_ok(row_pos, n.B, dev) || (news.defined() && !rows_ok(news, n.B, dev)))
     return nullptr;
   const int64_t most = p.max * p.size, K = kp.size(1);
-  max_kv = a[7] == Py_None ? most : std::min(max_kv, most);
+  max_kv = a[8] == Py_None ? most : std::min(max_kv, most);
   if (max_kv < 1) return nullptr;
-  n.set_flags(a[12] == Py_True);
+  n.set_flags(a[13] == Py_True);
+  n.size(K, max_kv);
+  const bool kept = n.keep();
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  StreamWorkspace ws(a[0], dev.index(), stream, kept ? n.need : 0);
+  if (kept && !ws.ptr) return nullptr;   // (made the Python way)
   int st;
   {
     NoGil unlocked;
-    n.allocate(K, max_kv);
+    n.allocate(kept);
     st = forge_attn_paged(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w,
                           n.eps, n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kp), ptr(vp), p.s[0], p.s[1], p.s[2], p.n,
                           (int)p.size, static_cast<const int32_t*>(ptr(table)), p.stride, (int)p.max,
                           static_cast<const int32_t*>(ptr(row_pos)), static_cast<const int32_t*>(ptr(news)), max_kv,
                           (int)n.window, (int)n.sinks, n.scale, n.out.data_ptr(), n.out.stride(0), n.out.stride(1),
-                          n.out.stride(2), n.ws.defined() ? n.ws.data_ptr() : nullptr, n.need,
-                          c10::hip::getCurrentHIPStream(dev.index()).stream());
+                          n.out.stride(2), kept ? ws.ptr : n.ws.defined() ? n.ws.data_ptr() : nullptr,
+                          kept ? ws.bytes : n.need, kept ? FORGE_WS_ZEROED : 0, stream);
   }
+  if (st == 0) ws.put_back();
   return st < 0 ? nullptr : result(st, n.out);
 }
 
-// attn_sinks(q, k_cache, v_cache, scale, window, sinks, pos | None, pos_dev | None, row_pos | None, max_kv_len | None,
+// attn_sinks(table of workspaces, q, k_cache, v_cache, scale, window, sinks, pos | None, pos_dev | None, row_pos | None, max_kv_len | None,
 //            q_weight | None, eps, norm_q, cos | None, sin | None)
 PyObject* attn_sinks_impl(PyObject* const* a) {
   NewTokens n;
   Tensor kc, vc, pos_dev, row_pos;
   int64_t pos = 0, max_kv = -1, sk[3], sv[3];
-  if (!take(a[0], n.q) || !take(a[1], kc) || !take(a[2], vc) || !as_float(a[3], n.scale) || !as_int(a[4], n.window) ||
-      !as_int(a[5], n.sinks) || (a[6] != Py_None && !as_int(a[6], pos)) || !take_opt(a[7], pos_dev) ||
-      !take_opt(a[8], row_pos) || (a[9] != Py_None && !as_int(a[9], max_kv)) || !take_opt(a[10], n.qw) ||
-      !as_float(a[11], n.eps) || !take_opt(a[13], n.cos) || !take_opt(a[14], n.sin))
+  if (!take(a[1], n.q) || !take(a[2], kc) || !take(a[3], vc) || !as_float(a[4], n.scale) || !as_int(a[5], n.window) ||
+      !as_int(a[6], n.sinks) || (a[7] != Py_None && !as_int(a[7], pos)) || !take_opt(a[8], pos_dev) ||
+      !take_opt(a[9], row_pos) || (a[10] != Py_None && !as_int(a[10], max_kv)) || !take_opt(a[11], n.qw) ||
+      !as_float(a[12], n.eps) || !take_opt(a[14], n.cos) || !take_opt(a[15], n.sin))
     return nullptr;
   if (!n.take_args(kc) || n.window < 1) return nullptr;
   const c10::Device dev = n.q.device();
@@ -550,19 +561,25 @@ PyObject* attn_sinks_impl(PyObject* const* a) {
   }
   max_kv = max_kv < 0 ? max_len : std::min(max_kv, max_len);
   if (max_kv < 1) return nullptr;
-  n.set_flags(a[12] == Py_True);
+  n.set_flags(a[13] == Py_True);
+  n.size(K, max_kv);
+  const bool kept = n.keep();
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  StreamWorkspace ws(a[0], dev.index(), stream, kept ? n.need : 0);
+  if (kept && !ws.ptr) return nullptr;   // (made the Python way)
   int st;
   {
     NoGil unlocked;
-    n.allocate(K, max_kv);
+    n.allocate(kept);
     st = forge_attn_sinks(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w,
                           n.eps, n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kc), ptr(vc), sk[0], sk[1],
                           max_len > 1 ? sk[2] : n.D, max_len, static_cast<const int32_t*>(ptr(row_pos)),
                           static_cast<const int64_t*>(ptr(pos_dev)), pos, max_kv, (int)n.window, (int)n.sinks, n.scale,
                           n.out.data_ptr(), n.out.stride(0), n.out.stride(1), n.out.stride(2),
-                          n.ws.defined() ? n.ws.data_ptr() : nullptr, n.need,
-                          c10::hip::getCurrentHIPStream(dev.index()).stream());
+                          kept ? ws.ptr : n.ws.defined() ? n.ws.data_ptr() : nullptr,
+                          kept ? ws.bytes : n.need, kept ? FORGE_WS_ZEROED : 0, stream);
   }
+  if (st == 0) ws.put_back();
   return st < 0 ? nullptr : result(st, n.out);
 }
 
@@ -588,7 +605,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     FORGE_ENTRY(decode_append, 21), FORGE_ENTRY(kv_append, 11), FORGE_ENTRY(prefill, 11),
     FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), FORGE_ENTRY(kv_append_paged, 13),
-    FORGE_ENTRY(attn_paged, 15),    FORGE_ENTRY(attn_sinks, 15), {nullptr, nullptr, 0, nullptr},
+    FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 16), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_forge_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

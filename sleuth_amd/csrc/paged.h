@@ -54,6 +54,9 @@ struct PagedParams {
   int slots;          // blocks that the device holds at a time
   float2* ws_ml;      // [slot][block's rows]
   float* ws_o;        // ... [D]
+  // Arrival counters [row block of a (batch row, KV head)], all zero between calls: the last part of a row block
+  // merges it. Null: the combine kernel does, launched behind.
+  unsigned* counters;
 
   // Token of query row r (r / G).
   __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((unsigned)r, g_inv); }
@@ -199,6 +202,64 @@ __device__ __forceinline__ void store_row(const PagedParams& p, int b, int kvh, 
   else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(v);
 }
 
+// Memory that blocks on other XCDs, with L2 caches of their own, write or read in the same launch: agent-scope
+// accesses go past those caches.
+__device__ __forceinline__ float2 load_shared(const float2* p) {
+  const uint64_t u = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)u), __uint_as_float((unsigned)(u >> 32)));
+}
+__device__ __forceinline__ void store_shared(float2* p, float x, float y) {
+  const uint64_t u = __float_as_uint(x) | (uint64_t)__float_as_uint(y) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Merges a row's parts, in part order, over four channels: (m, l) at ml[i * step], outputs at o[i * step * D].
+// Returns the sum of the weights. SHARED: written in this launch.
+template <int D, bool SHARED>
+__device__ __forceinline__ float merge_parts(const float2* ml, const float* po, int parts, int64_t step, float4& O) {
+  // eight parts' loads go out together; the running maximum as in the kernels
+  constexpr int U = 8;
+  float M = kNegInf, L = 0.0f;
+  O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = 0; i0 < parts; i0 += U) {
+    float2 e[U];
+    float4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (i0 + u < parts ? i0 + u : parts - 1) * step;
+      if constexpr (SHARED) {
+        e[u] = load_shared(ml + at);
+        const float2 x = load_shared(reinterpret_cast<const float2*>(po + at * D));
+        const float2 y = load_shared(reinterpret_cast<const float2*>(po + at * D) + 1);
+        o[u] = make_float4(x.x, x.y, y.x, y.y);
+      } else {
+        e[u] = ml[at];
+        o[u] = *reinterpret_cast<const float4*>(po + at * D);
+      }
+    }
+    float top = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, e[u].x);
+    const float keep = rescale(M, top);
+    L *= keep;
+    O.x *= keep;
+    O.y *= keep;
+    O.z *= keep;
+    O.w *= keep;
+    M = top;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float a = i0 + u < parts ? rescale(e[u].x, M) : 0.0f;
+      L += a * e[u].y;
+      O.x += a * o[u].x;
+      O.y += a * o[u].y;
+      O.z += a * o[u].z;
+      O.w += a * o[u].w;
+    }
+  }
+  return L;
+}
+
 // Rows of a merging block: 256 threads of D / 4 lanes a row, within one row block.
 constexpr int combine_rows(int D, int BM) { return 1024 / D < BM ? 1024 / D : BM; }
 
@@ -229,42 +290,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
     stride = 1;
   }
   if (parts < 2) return;  // written by its block
-  // eight parts' loads go out together; the running maximum as in the kernels
-  constexpr int U = 8;
-  const float2* ml = p.ws_ml + slot * BM + in;
-  const float* po = p.ws_o + (slot * BM + in) * D + x;
-  const int64_t step = (int64_t)stride * BM;
-  float M = kNegInf, L = 0.0f;
-  float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i0 = 0; i0 < parts; i0 += U) {
-    float2 e[U];
-    float4 o[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (i0 + u < parts ? i0 + u : parts - 1) * step;
-      e[u] = ml[at];
-      o[u] = *reinterpret_cast<const float4*>(po + at * D);
-    }
-    float top = M;
-#pragma unroll
-    for (int u = 0; u < U; ++u) top = fmaxf(top, e[u].x);
-    const float keep = rescale(M, top);
-    L *= keep;
-    O.x *= keep;
-    O.y *= keep;
-    O.z *= keep;
-    O.w *= keep;
-    M = top;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float a = i0 + u < parts ? rescale(e[u].x, M) : 0.0f;
-      L += a * e[u].y;
-      O.x += a * o[u].x;
-      O.y += a * o[u].y;
-      O.z += a * o[u].z;
-      O.w += a * o[u].w;
-    }
-  }
+  float4 O;
+  const float L = merge_parts<D, false>(p.ws_ml + slot * BM + in, p.ws_o + (slot * BM + in) * D + x, parts,
+                                        (int64_t)stride * BM, O);
   store_row<T>(p, b, kvh, flat, x, O, L > 0.0f ? 1.0f / L : 0.0f);
 }
 

@@ -479,9 +479,37 @@ void paged_step_kernel(PagedParams p) {
       store_row<T>(p, b, kvh, flat, 4 * c4, acc, real && L > 0.0f ? 1.0f / L : 0.0f);
     } else {
       const int64_t slot = (int64_t)work.slot * ROWS + row;
-      *reinterpret_cast<float4*>(p.ws_o + slot * D + 4 * c4) = acc;
-      if (c4 == 0) p.ws_ml[slot] = make_float2(M, L);
+      float* po = p.ws_o + slot * D + 4 * c4;
+      if (p.counters) {
+        store_shared(reinterpret_cast<float2*>(po), acc.x, acc.y);
+        store_shared(reinterpret_cast<float2*>(po) + 1, acc.z, acc.w);
+        if (c4 == 0) store_shared(p.ws_ml + slot, M, L);
+      } else {
+        *reinterpret_cast<float4*>(po) = acc;
+        if (c4 == 0) p.ws_ml[slot] = make_float2(M, L);
+      }
     }
+  }
+  if (whole || !p.counters) return;
+
+  // ---- the part that arrives last merges the row block (the others' partials are where agent-scope accesses find
+  // them once their stores are acknowledged; the counter wraps to zero for the next call)
+  __shared__ int last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int unit = work.slot / p.nparts;
+    last = atomicInc(p.counters + unit, (unsigned)work.parts - 1) == (unsigned)work.parts - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  const int here = w.rows - rblk * ROWS < ROWS ? w.rows - rblk * ROWS : ROWS;
+  const int64_t slot0 = (int64_t)(work.slot - work.part) * ROWS;
+  for (int x = threadIdx.x; x < here * Q4; x += 256) {
+    const int row = x / Q4, ch = 4 * (x % Q4);
+    float4 O;
+    const float L = merge_parts<D, true>(p.ws_ml + slot0 + row, p.ws_o + (slot0 + row) * D + ch, work.parts, ROWS, O);
+    store_row<T>(p, b, kvh, rblk * ROWS + row, ch, O, L > 0.0f ? 1.0f / L : 0.0f);
   }
 }
 
@@ -498,7 +526,7 @@ template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hi
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
   hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
   int st = check_launch();
-  if (st == 0 && p.nparts > 1) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
+  if (st == 0 && p.nparts > 1 && !p.counters) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
   return st;
 }
 

@@ -69,9 +69,10 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   return plan;
 }
 
-// The workspace: [items | row blocks' parts] of a planned call, then (m, l) and the output of every slot's rows.
+// The workspace: the counters, [items | row blocks' parts] of a planned call, then (m, l) and the output of every
+// slot's rows.
 struct PagedWs {
-  size_t pairs, ml, o, bytes;
+  size_t items, pairs, ml, o, bytes;
 };
 static PagedWs paged_ws(const PagedPlan& plan, int B, int T, int H, int K, int D) {
   PagedWs w{};
@@ -79,7 +80,8 @@ static PagedWs paged_ws(const PagedPlan& plan, int B, int T, int H, int K, int D
   const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t blocks = (size_t)B * (((size_t)(H / K) * T + plan.rows - 1) / plan.rows);
   const size_t rows = (plan.planned ? (size_t)plan.nitems : blocks * plan.nparts) * K * plan.rows;
-  w.pairs = plan.planned ? up(plan.nitems * sizeof(PagedItem)) : 0;
+  w.items = FORGE_PAGED_COUNTER_BYTES;
+  w.pairs = w.items + (plan.planned ? up(plan.nitems * sizeof(PagedItem)) : 0);
   w.ml = w.pairs + (plan.planned ? up(blocks * sizeof(int2)) : 0);
   w.o = w.ml + up(rows * sizeof(float2));
   w.bytes = w.o + rows * D * sizeof(float);
@@ -90,7 +92,7 @@ static bool unaligned(const void* p) { return (uintptr_t)p % 16 != 0; }
 
 // Checks what both entry points share, cuts the call and launches it.
 static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scale, void* workspace,
-                     size_t workspace_bytes, hipStream_t s) {
+                     size_t workspace_bytes, int ws_flags, hipStream_t s) {
   if (dtype != FORGE_F32 && dtype != FORGE_BF16 && dtype != FORGE_F16) return set_error("unknown dtype code");
   if (p.B < 0 || p.T < 0 || p.H <= 0 || p.K <= 0 || p.H % p.K) return set_error("bad sizes (H must be a multiple of K)");
   if (!paged_dim_ok(dtype, D)) return set_error("head dim must be 32, 64, 128, 256 (or 512 in bf16/fp16)");
@@ -122,11 +124,18 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
     if ((uintptr_t)workspace % 256) return set_error("the workspace must be 256-byte aligned");
     char* at = static_cast<char*>(workspace);
     if (plan.planned) {
-      p.items = reinterpret_cast<PagedItem*>(at);
+      p.items = reinterpret_cast<PagedItem*>(at + ws.items);
       p.pairs = reinterpret_cast<int2*>(at + ws.pairs);
     }
     p.ws_ml = reinterpret_cast<float2*>(at + ws.ml);
     p.ws_o = reinterpret_cast<float*>(at + ws.o);
+    // The last part merges where that is little for one block; else the combine kernel spreads it over many. us, last
+    // part / combine: 4 rows of 1,000 keys (6 KB) 7.3 / 9.4, 16 rows of 1,024-key windows (4 KB) 18.1 / 19.2; one row
+    // of 8,000 keys (32 KB) 15.2 / 13.7, one KV head of 256 with 32 query rows (288 KB) 29.4 / 17.7.
+    const int64_t units = (int64_t)p.B * p.K * ((p.rows + plan.rows - 1) / plan.rows);
+    const int64_t bytes = (int64_t)(p.rows < plan.rows ? p.rows : plan.rows) * D * 4 * plan.nparts;
+    if ((ws_flags & FORGE_WS_ZEROED) && !plan.chunk && units <= FORGE_PAGED_COUNTER_BYTES / 4 && bytes <= 16 * 1024)
+      p.counters = reinterpret_cast<unsigned*>(at);
   }
   switch (dtype) {
     case FORGE_F32: return launch_paged<float>(p, plan, D, s);
@@ -157,7 +166,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
                                 const int32_t* page_table, int64_t s_table, int max_pages, const int32_t* row_pos,
                                 const int32_t* new_lens, int64_t max_kv_len, int window, int sinks, float scale,
                                 void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
-                                size_t workspace_bytes, void* stream) {
+                                size_t workspace_bytes, int ws_flags, void* stream) {
   clear_error();
   if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
   if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
@@ -178,7 +187,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   p.row_pos = row_pos; p.new_lens = new_lens;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
-  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, (hipStream_t)stream);
+  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
 }
 
 extern "C" size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
@@ -192,7 +201,7 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
                                 const void* v_cache, int64_t skb, int64_t skh, int64_t sks, int64_t max_len,
                                 const int32_t* row_pos, const int64_t* pos_dev, int64_t pos0, int64_t max_kv_len,
                                 int window, int sinks, float scale, void* out, int64_t sob, int64_t sot, int64_t soh,
-                                void* workspace, size_t workspace_bytes, void* stream) {
+                                void* workspace, size_t workspace_bytes, int ws_flags, void* stream) {
   clear_error();
   if (window <= 0) return set_error("forge_attn_sinks needs a window");
   if (max_kv_len <= 0 || max_len <= 0) return set_error("max_kv_len and max_len must be positive");
@@ -210,5 +219,5 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   p.row_pos = row_pos; p.pos_dev = pos_dev; p.pos0 = pos0;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
-  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, (hipStream_t)stream);
+  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
 }

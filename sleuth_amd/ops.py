@@ -244,10 +244,11 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *
 
 
 _STREAM_WS: dict = {}
+_PAGED_WS: dict = {}      # the same for attn_paged and attn_sinks, whose workspaces begin with other counters
 _STREAM_WS_MAX = 16   # streams whose workspace is kept (the oldest is dropped beyond that)
 
 
-def _take_stream_workspace(dev: torch.device, need: int) -> tuple[tuple, torch.Tensor]:
+def _take_stream_workspace(dev: torch.device, need: int, table: dict = _STREAM_WS) -> tuple[tuple, torch.Tensor]:
     """A split-K workspace per (device, stream), cleared when it is made: every call leaves
     its work ticket zero, so calls ordered on that stream may skip the ticket reset. Grown
     (a new cleared buffer) when a call needs more. It is out of the table until the call is
@@ -255,16 +256,16 @@ def _take_stream_workspace(dev: torch.device, need: int) -> tuple[tuple, torch.T
     rather than launch between this call's kernels. Dropping a buffer is safe while its calls
     are in flight: torch's allocator reuses the memory only in that stream's order."""
     key = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
-    ws = _STREAM_WS.pop(key, None)
+    ws = table.pop(key, None)
     if ws is None or ws.numel() < need:
         ws = torch.zeros(max(need, 1 << 20), dtype=torch.uint8, device=dev)
     return key, ws
 
 
-def _put_back_stream_workspace(key: tuple, ws: torch.Tensor) -> None:
-    _STREAM_WS[key] = ws   # most recently used last
-    for old in list(_STREAM_WS)[:-_STREAM_WS_MAX]:
-        _STREAM_WS.pop(old, None)
+def _put_back_stream_workspace(key: tuple, ws: torch.Tensor, table: dict = _STREAM_WS) -> None:
+    table[key] = ws   # most recently used last
+    for old in list(table)[:-_STREAM_WS_MAX]:
+        table.pop(old, None)
 
 
 def attn_decode_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
@@ -530,6 +531,32 @@ def linear_small(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = N
 
 
 # ---------------------------------------------------------------- the paged cache, windows with sinks
+# Partials of up to this many bytes stay with their stream (a decode or verify step's); a chunk's larger ones are
+# allocated for the call
+_PAGED_WS_KEPT = 32 << 20
+
+
+class _PagedPartials:
+    """The workspace of one attn_paged or attn_sinks call: the stream's cleared one (its counters are zero between
+    calls), or memory for this call alone where it is large or a graph is being recorded (a graph keeps its own);
+    None where nothing is split or memory is short."""
+
+    def __init__(self, dev: torch.device, need: int):
+        self.key, self.ws, self.need, self.flags = None, None, need, 0
+        if need and need <= _PAGED_WS_KEPT and not torch.cuda.is_current_stream_capturing():
+            self.key, self.ws = _take_stream_workspace(dev, need, _PAGED_WS)
+            self.flags = WS_ZEROED
+        elif need:
+            self.ws = _partials(need, dev)
+
+    def args(self) -> tuple:
+        return _ptr(self.ws), 0 if self.ws is None else self.ws.numel(), self.flags
+
+    def launched(self) -> None:
+        if self.key is not None:
+            _put_back_stream_workspace(self.key, self.ws, _PAGED_WS)
+
+
 def _guard(dev: torch.device):
     """Launches go to the tensors' GPU, whichever is current."""
     return torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else contextlib.nullcontext()
@@ -654,7 +681,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     t >= new_lens[b] and rows that see nothing are zeros. max_kv_len: an upper bound on row_pos[b] + new_lens[b]
     (default: what the table can hold); it sizes the launch."""
     if out is None:
-        r = host().attn_paged(q, k_pages, v_pages, page_table, row_pos, new_lens, float(scale), max_kv_len, window, sinks,
+        r = host().attn_paged(_PAGED_WS, q, k_pages, v_pages, page_table, row_pos, new_lens, float(scale), max_kv_len, window, sinks,
                               q_weight, float(eps), bool(norm_q), cos, sin)
         if r is not None:
             return r if r.__class__ is not int else check(r, "forge_attn_paged")
@@ -669,13 +696,13 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
         raise ValueError("max_kv_len must be positive")
     keep, args, out = _new_token_args(q, k_pages, q_weight, eps, norm_q, cos, sin, window, sinks, out)
     with _guard(dev):
-        need = lib().forge_attn_paged_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks))
-        ws = _partials(need, dev)
+        ws = _PagedPartials(dev, lib().forge_attn_paged_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
         st = lib().forge_attn_paged(*args, _ptr(k_pages), _ptr(v_pages), *_strides3(k_pages), k_pages.shape[0], size,
                                     _ptr(table), table.stride(0) if B > 1 else 0, table.shape[1], _ptr(rp), _ptr(nl),
                                     max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
-                                    _ptr(ws), need, _stream(dev))
+                                    *ws.args(), _stream(dev))
     check(st, "forge_attn_paged")
+    ws.launched()
     return out
 
 
@@ -690,7 +717,7 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
     pos, as attn_decode) and sees keys s <= p with s > p - window or s < sinks. Any T: whole prompts, chunks, verify and
     decode steps. Returns [B,T,H,D]."""
     if out is None:
-        r = host().attn_sinks(q, k_cache, v_cache, float(scale), window, sinks, pos, pos_dev, row_pos, max_kv_len, q_weight,
+        r = host().attn_sinks(_PAGED_WS, q, k_cache, v_cache, float(scale), window, sinks, pos, pos_dev, row_pos, max_kv_len, q_weight,
                               float(eps), bool(norm_q), cos, sin)
         if r is not None:
             return r if r.__class__ is not int else check(r, "forge_attn_sinks")
@@ -715,12 +742,12 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
             raise ValueError("max_kv_len must be positive")
     keep, args, out = _new_token_args(q, k_cache, q_weight, eps, norm_q, cos, sin, window, sinks, out)
     with _guard(dev):
-        need = lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks))
-        ws = _partials(need, dev)
+        ws = _PagedPartials(dev, lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
         st = lib().forge_attn_sinks(*args, _ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache), max_len, _ptr(rp), _ptr(pd),
                                     p0, max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
-                                    _ptr(ws), need, _stream(dev))
+                                    *ws.args(), _stream(dev))
     check(st, "forge_attn_sinks")
+    ws.launched()
     return out
 
 

@@ -523,7 +523,7 @@ def test_without_a_workspace():
         st = _lib.lib().forge_attn_paged(_lib.BF16, 1, T, 16, 8, 128, q.data_ptr(), *q.stride()[:3], None, 0.0, 0, None, None,
                                          0, 0, kp.data_ptr(), vp.data_ptr(), *kp.stride()[:3], kp.shape[0], 16,
                                          table.data_ptr(), 0, table.shape[1], rp.data_ptr(), None, 2500 + T, 0, 0, 0.09,
-                                         out.data_ptr(), *out.stride()[:3], None, 0,
+                                         out.data_ptr(), *out.stride()[:3], None, 0, 0,
                                          torch.cuda.current_stream().cuda_stream)
         assert st == 0
         assert_close(out, *cache.want(q.cpu(), [2500], [T], 0, 0, 0.09))
@@ -644,7 +644,7 @@ def _paged_call(**over):
     a = dict(dtype=_lib.BF16, B=2, T=1, H=8, K=4, D=64, q=_P, sqb=512, sqh=64, sqt=512, qw=None, eps=1e-6, flags=0, cos=None,
              sin=None, scb=0, sct=0, kp=_P, vp=_P, skp=4096, skh=1024, sks=64, n_pages=4, page=16, table=_P, spt=2, max_pages=2,
              row_pos=_P, new=None, max_kv=32, window=0, sinks=0, scale=1.0, out=_P, sob=512, sot=512, soh=64, ws=None, wsb=0,
-             stream=None)
+             wsf=0, stream=None)
     a.update(over)
     return _lib.lib().forge_attn_paged(*a.values())
 
@@ -668,7 +668,7 @@ def test_c_refusals(what, over):
 def test_c_refusals_of_the_others():
     lib = _lib.lib()
     base = [_lib.BF16, 2, 1, 8, 4, 64, _P, 512, 64, 512, None, 1e-6, 0, None, None, 0, 0, _P, _P, 8192, 2048, 64, 32, _P, None,
-            0, 32, 8, 2, 1.0, _P, 512, 512, 64, None, 0, None]
+            0, 32, 8, 2, 1.0, _P, 512, 512, 64, None, 0, 0, None]
     for what, at, value in (("window", 27, 0), ("max_kv_len", 26, 0), ("max_len", 22, 0), ("head dim", 5, 80)):
         a = list(base)
         a[at] = value
@@ -693,3 +693,51 @@ def test_workspace_bytes():
     assert f(_lib.BF16, 1, 1, 16, 8, 128, 32768, 16, 0) == 0             # a short window is not
     assert f(_lib.BF16, 1, 1, 16, 8, 96, 32768, 0, 0) == 0 and f(9, 1, 1, 6, 4, 64, 100, 0, 0) == 0
     assert _lib.lib().forge_attn_sinks_workspace_bytes(_lib.F32, 4, 1, 8, 4, 64, 9000, 4096, 4) > 0
+
+
+@pytest.mark.gpu
+def test_merges_by_the_last_part_equal_the_combine_launch():
+    """Split decode calls with the stream's workspace (the part that ends last merges) and under a recorded graph (a
+    launch of its own merges): the same bits, many times over, and the counters are zero afterwards."""
+    g = gen(14)
+    for dtype, H, K, D, pasts, T in ((BF, 16, 8, 128, [1500, 700, 0], 1), (HF, 12, 4, 64, [1000] * 4, 1),
+                                     (SF, 8, 4, 32, [3000, 12], 2), (BF, 8, 4, 256, [900, 300], 1), (BF, 16, 1, 512, [200], 1)):
+        cache = Paged(g, [p + T for p in pasts], K, D, 16, dtype)
+        B = len(pasts)
+        q = torch.randn(B, T, H, D, generator=g).to(dtype).transpose(1, 2)
+        args = (q.cuda(), cache.kp.cuda(), cache.vp.cuda(), cache.table.cuda(), i32(pasts))
+        want, bound = cache.want(q, pasts, [T] * B, 0, 0, 0.1)
+        first = ops.attn_paged(*args, scale=0.1)
+        assert_close(first, want, bound)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.attn_paged(*args, scale=0.1)
+        for _ in range(20):
+            assert torch.equal(ops.attn_paged(*args, scale=0.1), first)
+            graph.replay()
+            assert torch.equal(out, first)
+    key = (0, torch.cuda.current_stream().cuda_stream)
+    assert not ops._PAGED_WS[key][:64 * 1024].any()
+
+
+@pytest.mark.gpu
+def test_threads_on_one_stream():
+    """Two threads that call on the same stream at once use workspaces of their own."""
+    import threading
+
+    g = gen(15)
+    cache = Paged(g, [900, 2000], 8, 128, 16, BF)
+    q = torch.randn(2, 1, 16, 128, generator=g).to(BF).transpose(1, 2).cuda()
+    args = (q, cache.kp.cuda(), cache.vp.cuda(), cache.table.cuda(), i32([899, 1999]))
+    first = ops.attn_paged(*args, scale=0.1)
+    torch.cuda.synchronize()
+    outs = {}
+
+    def work(i):
+        outs[i] = [ops.attn_paged(*args, scale=0.1) for _ in range(200)]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for i in range(4) for o in outs[i])
