@@ -173,7 +173,7 @@ template <typename T, int D, int RB> struct StepLds {
   // The query operands are read from LDS in each tile where the output and the tile in flight take the
   // registers: a reload of a spilled one would wait for the tile loads it queues behind.
   static constexpr bool Q_LDS = TL::ROWB * RB >= 1024;
-  static constexpr int ML = 4 * ROWS * 8;                                 // (m, l) of every wave's rows
+  static constexpr int ML = 5 * ROWS * 8;                                 // (m, l) of every wave's rows, and of all
   static constexpr int Q_OFF = 4 * WAVE + ML;
   static constexpr int BYTES = Q_OFF + (Q_LDS ? ROWS * TL::ROWB : 0);
   static constexpr int BLOCKS = step_blocks_per_cu(sizeof(T), D, ROWS);
@@ -441,52 +441,70 @@ void paged_step_kernel(PagedParams p) {
   }
   __syncthreads();
   constexpr int Q4 = D / 4;  // float4 pieces of a row
+  const int row0 = rblk * ROWS;
+  const int here = w.rows - row0 < ROWS ? w.rows - row0 : ROWS;   // real rows of the block, and those that exist
+  const int exist = p.rows - row0 < ROWS ? p.rows - row0 : ROWS;
   float4* mine = reinterpret_cast<float4*>(smem + wave * LD::WAVE);
+  float2* all = ml + 4 * ROWS;  // [ROWS] of the four together
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int row = 16 * r + n;
-    float M = kNegInf;
+    float2 e[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) M = fmaxf(M, ml[x * ROWS + row].x);
+    for (int y = 0; y < 4; ++y) e[y] = ml[y * ROWS + row];
+    const float M = fmaxf(fmaxf(e[0].x, e[1].x), fmaxf(e[2].x, e[3].x));
     const float a = rescale(m[r], M);
+    if (row < here) {
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      const int piece = (4 * d + g) ^ (n & (Q4 < 16 ? Q4 - 1 : 15));
-      mine[row * Q4 + piece] = make_float4(o[r][d][0] * a, o[r][d][1] * a, o[r][d][2] * a, o[r][d][3] * a);
+      for (int d = 0; d < DB; ++d) {
+        const int piece = (4 * d + g) ^ (n & (Q4 < 16 ? Q4 - 1 : 15));
+        mine[row * Q4 + piece] = make_float4(o[r][d][0] * a, o[r][d][1] * a, o[r][d][2] * a, o[r][d][3] * a);
+      }
+    }
+    if (wave == 0 && g == 0) {
+      float L = 0.0f;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) L += rescale(e[y].x, M) * e[y].y;
+      all[row] = make_float2(M, L);
     }
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < ROWS * Q4; x += 256) {
-    const int row = x / Q4, c4 = x % Q4;
-    const int flat = rblk * ROWS + row;
-    if (flat >= p.rows) break;
-    const bool real = flat < w.rows;
-    float M = kNegInf, L = 0.0f;
+  constexpr int PIECES = ROWS * Q4, PER = PIECES < 256 ? 1 : PIECES / 256;   // of a thread
+  constexpr int BATCH = PER < 4 ? PER : 4;                                   // whose reads go out together
 #pragma unroll
-    for (int y = 0; y < 4; ++y) M = fmaxf(M, ml[y * ROWS + row].x);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int x0 = 0; x0 < PER; x0 += BATCH) {
+    if (x0 * 256 / Q4 >= exist) break;
+    float4 f[BATCH][4];
+    float2 e[BATCH];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const float2 e = ml[y * ROWS + row];
-      L += rescale(e.x, M) * e.y;
-      const float4 f = reinterpret_cast<const float4*>(smem + y * LD::WAVE)[row * Q4 + (c4 ^ (row & (Q4 < 16 ? Q4 - 1 : 15)))];
-      acc.x += f.x;
-      acc.y += f.y;
-      acc.z += f.z;
-      acc.w += f.w;
+    for (int x = 0; x < BATCH; ++x) {
+      const int at = ((x0 + x) * 256 + (int)threadIdx.x) % PIECES, row = at / Q4, c4 = at % Q4;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        f[x][y] = reinterpret_cast<const float4*>(smem + y * LD::WAVE)[row * Q4 + (c4 ^ (row & (Q4 < 16 ? Q4 - 1 : 15)))];
+      e[x] = all[row];
     }
-    if (whole || !real) {
-      store_row<T>(p, b, kvh, flat, 4 * c4, acc, real && L > 0.0f ? 1.0f / L : 0.0f);
-    } else {
-      const int64_t slot = (int64_t)work.slot * ROWS + row;
-      float* po = p.ws_o + slot * D + 4 * c4;
-      if (p.counters) {
-        store_shared(reinterpret_cast<float2*>(po), acc.x, acc.y);
-        store_shared(reinterpret_cast<float2*>(po) + 1, acc.z, acc.w);
-        if (c4 == 0) store_shared(p.ws_ml + slot, M, L);
+#pragma unroll
+    for (int x = 0; x < BATCH; ++x) {
+      const int at = (x0 + x) * 256 + (int)threadIdx.x, row = at / Q4, c4 = at % Q4;
+      if (row >= exist) continue;
+      const float4 acc = make_float4((f[x][0].x + f[x][1].x) + (f[x][2].x + f[x][3].x), (f[x][0].y + f[x][1].y) + (f[x][2].y + f[x][3].y),
+                                     (f[x][0].z + f[x][1].z) + (f[x][2].z + f[x][3].z), (f[x][0].w + f[x][1].w) + (f[x][2].w + f[x][3].w));
+      if (row >= here) {
+        store_row<T>(p, b, kvh, row0 + row, 4 * c4, make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
+      } else if (whole) {
+        store_row<T>(p, b, kvh, row0 + row, 4 * c4, acc, e[x].y > 0.0f ? 1.0f / e[x].y : 0.0f);
       } else {
-        *reinterpret_cast<float4*>(po) = acc;
-        if (c4 == 0) p.ws_ml[slot] = make_float2(M, L);
+        const int64_t slot = (int64_t)work.slot * ROWS + row;
+        float* po = p.ws_o + slot * D + 4 * c4;
+        if (p.counters) {
+          store_shared(reinterpret_cast<float2*>(po), acc.x, acc.y);
+          store_shared(reinterpret_cast<float2*>(po) + 1, acc.z, acc.w);
+          if (c4 == 0) store_shared(p.ws_ml + slot, e[x].x, e[x].y);
+        } else {
+          *reinterpret_cast<float4*>(po) = acc;
+          if (c4 == 0) p.ws_ml[slot] = e[x];
+        }
       }
     }
   }
@@ -503,13 +521,12 @@ void paged_step_kernel(PagedParams p) {
   }
   __syncthreads();
   if (!last) return;
-  const int here = w.rows - rblk * ROWS < ROWS ? w.rows - rblk * ROWS : ROWS;
   const int64_t slot0 = (int64_t)(work.slot - work.part) * ROWS;
   for (int x = threadIdx.x; x < here * Q4; x += 256) {
     const int row = x / Q4, ch = 4 * (x % Q4);
     float4 O;
     const float L = merge_parts<D, true>(p.ws_ml + slot0 + row, p.ws_o + (slot0 + row) * D + ch, work.parts, ROWS, O);
-    store_row<T>(p, b, kvh, rblk * ROWS + row, ch, O, L > 0.0f ? 1.0f / L : 0.0f);
+    store_row<T>(p, b, kvh, row0 + row, ch, O, L > 0.0f ? 1.0f / L : 0.0f);
   }
 }
 
