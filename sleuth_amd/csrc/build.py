@@ -20,9 +20,10 @@ ROOT = PKG.parent
 LIB_DIR = PKG / "_lib"
 LIB_NAME = "libforge_attn.so"
 HOST_NAME = "_forge_host.so"
-# (source, defines, object name); decode.hip's and paged.hip's kernels are built per dtype, side by side
+# (source, defines, object name); decode.hip's and the paged kernels are built per dtype, side by side
 SOURCES = [("abi.hip", [], "abi"), ("prep.hip", [], "prep"), ("prefill.hip", [], "prefill"), ("linear.hip", [], "linear"),
-           ("paged_abi.hip", [], "paged_abi"), ("paged_chunk.hip", [], "paged_chunk"), *(("paged.hip", [f"-DFORGE_PAGED_PART={n}"], f"paged{n}") for n in range(1, 4)),
+           ("paged_abi.hip", [], "paged_abi"),
+           *((f"{k}.hip", [f"-DFORGE_PAGED_PART={n}"], f"{k}{n}") for k in ("paged", "paged_chunk") for n in range(1, 4)),
            *(("decode.hip", [f"-DFORGE_DECODE_PART={n}"], f"decode{n}") for n in range(4))]
 ARCH = "gfx950"
 

@@ -192,6 +192,15 @@ template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const 
   return w;
 }
 
+// The low n bits (none for n <= 0, all for n >= 32), and a score where its bit is set, else -inf.
+__device__ __forceinline__ unsigned low_bits(int n) {
+  return (unsigned)((1ull << (n < 0 ? 0 : n < 32 ? n : 32)) - 1);
+}
+__device__ __forceinline__ float masked(float s, unsigned see, int bit) {
+  const int keep = (int)__builtin_amdgcn_sbfe((int)see, bit, 1);
+  return __int_as_float((__float_as_int(s) & keep) | (__float_as_int(kNegInf) & ~keep));
+}
+
 // Four output channels of query row `flat` of (b, kvh).
 template <typename T>
 __device__ __forceinline__ void store_row(const PagedParams& p, int b, int kvh, int flat, int ch, float4 a, float f) {

@@ -330,21 +330,18 @@ void paged_step_kernel(PagedParams p) {
     if (!full) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
-        // visible: [lo, lo + len), and the first tokens up to the query (no branch per element)
+        // bits of the keys from key0 + 4g on: the window up to the query, and the first tokens up to it
         const int base = key0 + 4 * g;
-        int lo = (p.window > 0 ? qpos[r] - p.window + 1 : 0) - base;
-        if (lo < -base) lo = -base;
         const int top = (qpos[r] < w.last ? qpos[r] : w.last) - base + 1;
-        const unsigned len = (unsigned)(top - lo);
-        const int first = p.sinks - base;
+        const int lo = (p.window > 0 ? qpos[r] - p.window + 1 : 0) - base;
+        const int first = p.sinks - base < top ? p.sinks - base : top;
+        unsigned see = (low_bits(top) & ~low_bits(lo)) | low_bits(first);
+        if (miss & 1) see &= ~0xffffu;
+        if (miss & 2) see &= 0xffffu;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int ce = 16 * kb + j;
-            const bool see = (((unsigned)(ce - lo) < len) | ((ce < first) & (ce < top))) & !(miss >> kb & 1);
-            s[r][kb][j] = see ? s[r][kb][j] : kNegInf;
-          }
+          for (int j = 0; j < 4; ++j) s[r][kb][j] = masked(s[r][kb][j], see, 16 * kb + j);
       }
     }
 

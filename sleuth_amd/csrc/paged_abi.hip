@@ -10,6 +10,7 @@ extern template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int
 extern template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+extern template int launch_paged_chunk<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 extern template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 
 static bool paged_dim_ok(int dtype, int D) {
@@ -30,11 +31,13 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   // More than 32 rows go to the chunk kernel, whose four waves share each key tile; up to 32 the split kernel's
   // waves keep more bytes in flight. us, split / chunk: 34 rows (8 batch rows of 2,000 keys, 8 KV heads, head dim
   // 128) 27.8 / 23.9, 40 rows (32 of 8,000) 239 / 194, 32 rows 183 / 196; head dim 256, one KV head, 16 batch rows of
-  // 8,000: 40 rows 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118.
-  if (es == 2 && D >= 64 && D <= 256 && rows > 32) {
+  // 8,000: 40 rows 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118. In fp32, where a tile's products take 3.4 us a
+  // wave, from 65 rows and head dim 64 on: 80 rows (8 of 2,000) 111 / 85, 40 rows 64.7 / 79; 600 new tokens 143 / 127,
+  // 700 at head dim 256 116 / 92; head dim 32 (2 rows of 333) 15.5 / 23.8.
+  if (es == 2 ? D >= 64 && D <= 256 && rows > 32 : D >= 64 && rows > 64) {
     plan.chunk = true;
     plan.rows = 128;
-    plan.keys = D == 256 ? 32 : 64;
+    plan.keys = es * D >= 512 ? 32 : 64;
   }
   plan.nparts = 1;
   if (!split) return plan;
@@ -47,7 +50,7 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     if (seen < tiles) tiles = seen;
   }
   // (three chunk blocks per CU at head dim 64: a 512-token chunk at 15,360, 12 q / 4 KV heads, 53 -> 45 us)
-  plan.slots = device_cus() * (plan.chunk ? (D == 64 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
+  plan.slots = device_cus() * (plan.chunk ? (es * D >= 1024 ? 1 : es * D <= 128 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
   const int64_t slots = plan.slots;
   const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
   const int64_t blocks = units / K;
@@ -56,7 +59,9 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     plan.nitems = (int)(plan.slots / K + blocks);
     return plan;
   }
-  const int64_t least = 8, most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
+  // (two tiles for each wave of the split kernel, eight for a chunk block: 96 rows of 8,000 keys at head dim 256
+  // take 39.6 / 29.6 / 29.2 / 37.5 us at 2 / 4 / 8 / 16; one of the long tiles in fp32: 100 tokens 14 us, not 35)
+  const int64_t least = es == 4 && plan.chunk ? 1 : 8, most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
   int64_t per = (units * tiles + slots - 1) / slots;
   if (per > most) per = most;
   if (per < least) per = least;
@@ -138,7 +143,7 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
       p.counters = reinterpret_cast<unsigned*>(at);
   }
   switch (dtype) {
-    case FORGE_F32: return launch_paged<float>(p, plan, D, s);
+    case FORGE_F32: return plan.chunk ? launch_paged_chunk<float>(p, plan, D, s) : launch_paged<float>(p, plan, D, s);
     case FORGE_BF16: return plan.chunk ? launch_paged_chunk<bf16>(p, plan, D, s) : launch_paged<bf16>(p, plan, D, s);
     default: return plan.chunk ? launch_paged_chunk<f16>(p, plan, D, s) : launch_paged<f16>(p, plan, D, s);
   }

@@ -1,5 +1,6 @@
 // Chunks of many query rows over a paged cache, or over a contiguous one with a window and first tokens:
-// bf16/fp16, head dims 64, 128, 256, on v_mfma_f32_32x32x16 (the split kernel of paged.hip serves the rest).
+// bf16/fp16, head dims 64, 128, 256, on v_mfma_f32_32x32x16, and fp32, head dims 64 to 256, on v_mfma_f32_32x32x2
+// (the split kernel of paged.hip serves the rest).
 //
 // A block of 4 waves owns 128 query rows of one (batch row, KV head) -- row r is token r / G, head r % G of the
 // group, so the heads of a group share each key tile they read -- and streams that row's visible key tiles through
@@ -17,36 +18,60 @@
 
 namespace forge {
 
-// Query row (b, h, t) as MFMA B operands, RMSNorm and RoPE in fp32 with one rounding: channels 16s + 8hi + e.
+// Block shape: 128 query rows, BN keys per tile, two LDS stages of a K and a V tile.
+template <typename T, int D> struct ChunkTile {
+  static constexpr int WAVES = 4, STAGES = 2, BM = 128;
+  static constexpr int ROWB = D * (int)sizeof(T);        // bytes per key row
+  static constexpr int NCH = ROWB / 16;                  // 16-byte chunks of it
+  static constexpr int BN = ROWB >= 512 ? 32 : 64;
+  static constexpr int TILEB = BN * ROWB;
+  static constexpr int LOADS = TILEB / (WAVES * 1024);   // 16-byte loads per lane per tile
+  static constexpr int LDS_BYTES = STAGES * 2 * TILEB + 64;  // and the stages' flags
+  static constexpr int QS = D * (int)sizeof(T) / 32;     // 16-byte pieces of a lane's half of a query row
+  static constexpr int BLOCKS = ROWB >= 1024 ? 1 : 2;    // per CU
+};
+// Chunk swizzles by key row: as prefill_tile.h's in 16 bits; in fp32 a V read is 32 channels of two rows 4 apart.
+template <typename T, int D> __device__ __forceinline__ int chunk_swz_k(int row) {
+  constexpr int NCH = ChunkTile<T, D>::NCH;
+  return row & ((NCH >= 16 ? 16 : NCH) - 1);
+}
+template <typename T, int D> __device__ __forceinline__ int chunk_swz_v(int row) {
+  if constexpr (sizeof(T) == 2) return swz_v<D>(row);
+  else return ((row >> 2) & 1) << 3;
+}
+
+// Query row (b, h, t) as MFMA B operands, RMSNorm and RoPE in fp32 with one rounding: lane half hi holds the
+// 16-byte pieces 2s + hi (in 16 bits the k-slots of one product, in fp32 of four).
 template <typename T, int D>
 __device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h, int t, int hi,
-                                             typename Mfma<T>::vec (&q)[D / 16]) {
-  using V8 = typename Mfma<T>::vec;
-  constexpr int S = D / 16;
+                                             uint4 (&q)[ChunkTile<T, D>::QS]) {
+  constexpr int S = ChunkTile<T, D>::QS, E = 16 / sizeof(T);
   const T* src = static_cast<const T*>(p.q) + b * p.sqb + h * p.sqh + t * p.sqt;
+#pragma unroll
+  for (int s = 0; s < S; ++s) q[s] = load16(src + (2 * s + hi) * E);
   const bool norm = p.flags & FORGE_NORM_QK, rope = p.flags & FORGE_ROPE;
-  if (!norm && !rope) {
+  if (!norm && !rope) return;
+  float f[S][E];
 #pragma unroll
-    for (int s = 0; s < S; ++s) q[s] = *reinterpret_cast<const V8*>(src + 16 * s + 8 * hi);
-    return;
-  }
-  float f[S][8];
-#pragma unroll
-  for (int s = 0; s < S; ++s) unpack16<T>(load16(src + 16 * s + 8 * hi), f[s]);
+  for (int s = 0; s < S; ++s) unpack16<T>(q[s], f[s]);
   if (norm) {
     float ss = 0.0f;
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss += f[s][e] * f[s][e];
+      for (int e = 0; e < E; ++e) ss += f[s][e] * f[s][e];
     ss += __shfl_xor(ss, 32, kWave);
     const float rs = rsqrtf(ss / (float)D + p.eps);
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      float w[8];
-      if (p.qw) load_f32x8(p.qw + 16 * s + 8 * hi, w);
+      float w[E];
+      if (p.qw) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[s][e] = p.qw ? f[s][e] * rs * w[e] : f[s][e] * rs;
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(p.qw + (2 * s + hi) * E + e);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[s][e] = p.qw ? f[s][e] * rs * w[e] : f[s][e] * rs;
     }
   }
   if (rope) {
@@ -55,34 +80,48 @@ __device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h,
 #pragma unroll
     for (int s = 0; s < S / 2; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int c = 16 * s + 8 * hi + e;
+      for (int e = 0; e < E; ++e) {
+        const int c = (2 * s + hi) * E + e;
         const float a = f[s][e], z = f[s + S / 2][e];
         f[s][e] = a * cr[c] - z * sr[c];
         f[s + S / 2][e] = z * cr[c + D / 2] + a * sr[c + D / 2];
       }
   }
 #pragma unroll
-  for (int s = 0; s < S; ++s)
+  for (int s = 0; s < S; ++s) {
+    if constexpr (sizeof(T) < 4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[s][e] = from_f32<T>(fp32_result(f[s][e]));
+      for (int e = 0; e < E; ++e) f[s][e] = fp32_result(f[s][e]);
+    }
+    q[s] = pack16<T>(f[s]);
+  }
 }
 
-template <int D> constexpr int chunk_lds() { return Tile<D>::LDS_BYTES + 64; }  // and the stages' flags
+// One step of S^T: 16 bytes of K against 16 bytes of Q^T.
+template <typename T> __device__ __forceinline__ floatx16 chunk_score(uint4 a, uint4 b, floatx16 c) {
+  if constexpr (sizeof(T) == 2) {
+    using V8 = typename Mfma<T>::vec;
+    return Mfma<T>::run(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c);
+  } else {
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+  }
+}
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkTile<T, D>::BLOCKS)))
 void paged_chunk_kernel(PagedParams p) {
-  using V8 = typename Mfma<T>::vec;
-  using TL = Tile<D>;
+  using TL = ChunkTile<T, D>;
   constexpr int BN = TL::BN, BM = TL::BM;
-  constexpr int KB = BN / 32, KSTEPS = D / 16, DB = D / 32, HALVES = BN / 16;
+  constexpr int KB = BN / 32, KSTEPS = TL::QS, DB = D / 32;
   constexpr int RW = BN / TL::WAVES;      // key rows of a tile that a wave loads
   constexpr int RL = kWave / TL::NCH;     // of which one load instruction covers RL
   static_assert(TL::STAGES == 2 && RW == RL * TL::LOADS && RW <= 16, "a wave's rows lie in one page");
 
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stage][K|V][TILEB], then the flags [stage][wave]
-  int* flags = reinterpret_cast<int*>(smem + TL::LDS_BYTES);
+  int* flags = reinterpret_cast<int*>(smem + TL::STAGES * 2 * TL::TILEB);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
@@ -104,23 +143,24 @@ void paged_chunk_kernel(PagedParams p) {
   if (w.tiles == 0) return;
 
   // ---- key tiles: load i of this wave fills LDS slots (wave * LOADS + i) * 64 + lane, key rows RL * i + lane / NCH
-  // of the wave's RW, in swizzled chunk order (kept offsets up to head dim 128; one xor each from shared registers
-  // at 256, where registers are short)
-  constexpr bool KEEP = D < 256;
-  const int64_t pageb = p.skp * 2;
-  const int rowb = (int)p.sks * 2;
-  const char* kgb = static_cast<const char*>(p.k) + kvh * p.skh * 2;
-  const char* vgb = static_cast<const char*>(p.v) + kvh * p.skh * 2;
+  // of the wave's RW, in swizzled chunk order (kept offsets; in 16 bits at head dim 256, where registers are short,
+  // one xor each from shared ones)
+  constexpr bool KEEP = !(sizeof(T) == 2 && D == 256);
+  constexpr int ES = sizeof(T);
+  const int64_t pageb = p.skp * ES;
+  const int rowb = (int)p.sks * ES;
+  const char* kgb = static_cast<const char*>(p.k) + kvh * p.skh * ES;
+  const char* vgb = static_cast<const char*>(p.v) + kvh * p.skh * ES;
   const int ld_row = lane / TL::NCH, pch = lane % TL::NCH;
   const int wr0 = wave * RW;
-  const int ld_k = (pch ^ swz_k<D>(ld_row)) << 4, ld_v = (pch ^ swz_v<D>(ld_row)) << 4;
+  const int ld_k = (pch ^ chunk_swz_k<T, D>(ld_row)) << 4, ld_v = (pch ^ chunk_swz_v<T, D>(ld_row)) << 4;
   int kept_k[KEEP ? TL::LOADS : 1], kept_v[KEEP ? TL::LOADS : 1];
   if constexpr (KEEP) {
 #pragma unroll
     for (int i = 0; i < TL::LOADS; ++i) {
       const int in = RL * i + ld_row;
-      kept_k[i] = in * rowb + ((pch ^ swz_k<D>(wr0 + in)) << 4);
-      kept_v[i] = in * rowb + ((pch ^ swz_v<D>(wr0 + in)) << 4);
+      kept_k[i] = in * rowb + ((pch ^ chunk_swz_k<T, D>(wr0 + in)) << 4);
+      kept_v[i] = in * rowb + ((pch ^ chunk_swz_v<T, D>(wr0 + in)) << 4);
     }
   }
   int flagged[2] = {0, 0};   // what this wave's flag of each stage holds
@@ -163,16 +203,16 @@ void paged_chunk_kernel(PagedParams p) {
         } else {
           const int r0 = wr0 + RL * x;
           const unsigned lo = (unsigned)(ld_row * rowb);
-          lds_dma16(ks + RL * x * rowb, lo + (lk ^ (swz_k<D>(r0) << 4)), kdst + x * 1024);
-          lds_dma16(vs + RL * x * rowb, lo + (lv ^ (swz_v<D>(r0) << 4)), vdst + x * 1024);
+          lds_dma16(ks + RL * x * rowb, lo + (lk ^ (chunk_swz_k<T, D>(r0) << 4)), kdst + x * 1024);
+          lds_dma16(vs + RL * x * rowb, lo + (lv ^ (chunk_swz_v<T, D>(r0) << 4)), vdst + x * 1024);
         }
       }
     } else {
 #pragma unroll
       for (int x = 0; x < TL::LOADS; ++x) {
         const int in = RL * x + ld_row, row = in < most ? in : most;
-        lds_dma16(ks, (unsigned)(row * rowb + ((pch ^ swz_k<D>(wr0 + in)) << 4)), kdst + x * 1024);
-        lds_dma16(vs, (unsigned)(row * rowb + ((pch ^ swz_v<D>(wr0 + in)) << 4)), vdst + x * 1024);
+        lds_dma16(ks, (unsigned)(row * rowb + ((pch ^ chunk_swz_k<T, D>(wr0 + in)) << 4)), kdst + x * 1024);
+        lds_dma16(vs, (unsigned)(row * rowb + ((pch ^ chunk_swz_v<T, D>(wr0 + in)) << 4)), vdst + x * 1024);
       }
     }
   };
@@ -188,14 +228,20 @@ void paged_chunk_kernel(PagedParams p) {
   const int qpos = w.base + t;
   const int wq_lo = w.base + p.token(w_row);
   const int wq_hi = w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
-  V8 qreg[KSTEPS];
+  uint4 qreg[KSTEPS];
   chunk_load_q<T, D>(p, b, h, t, hi, qreg);
 
-  // LDS read offsets of a lane within a stage's K and V tiles (prefill.hip)
-  const int g = lane >> 4, kq = (lane >> 2) & 3, qq = lane & 3;
-  const int v_row = 4 * (g >> 1) + kq;
-  const unsigned k_rd = n * TL::ROWB + ((hi ^ swz_k<D>(n)) << 4);
-  const unsigned v_rd = v_row * TL::ROWB + (((2 * (g & 1) + (qq >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (qq & 1);
+  // LDS read offsets of a lane within a stage's K and V tiles: in 16 bits prefill.hip's; in fp32 a V operand is channel
+  // 32d + n of key 8i + 4hi + j, whose swizzle is the lane's own bit hi
+  const unsigned k_rd = n * TL::ROWB + ((hi ^ chunk_swz_k<T, D>(n)) << 4);
+  unsigned v_rd;
+  if constexpr (ES == 2) {
+    const int g = lane >> 4, kq = (lane >> 2) & 3, qq = lane & 3;
+    const int v_row = 4 * (g >> 1) + kq;
+    v_rd = v_row * TL::ROWB + (((2 * (g & 1) + (qq >> 1)) ^ chunk_swz_v<T, D>(v_row)) << 4) + 8 * (qq & 1);
+  } else {
+    v_rd = 4 * hi * TL::ROWB + (((n >> 2) ^ chunk_swz_v<T, D>(4 * hi)) << 4) + 4 * (n & 3);
+  }
   const unsigned lds0 = lds_offset(smem);
 
   floatx16 oacc[DB];
@@ -233,10 +279,11 @@ void paged_chunk_kernel(PagedParams p) {
       for (int x = 0; x < 16; ++x) sacc[kb][x] = 0.0f;
     {
       auto kread = [&](int kb, int st) {
-        return *(__attribute__((address_space(3))) const V8*)((kl ^ (32 * (st & 7))) + 256 * (st >> 3) +
-                                                              kb * 32 * TL::ROWB);
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        return __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) const u32x4*)((kl ^ (32 * (st & 7))) + 256 * (st >> 3) +
+                                                                                           kb * 32 * TL::ROWB));
       };
-      V8 a0[KB], a1[KB], a2[KB];
+      uint4 a0[KB], a1[KB], a2[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) a0[kb] = kread(kb, 0);
 #pragma unroll
@@ -250,8 +297,8 @@ void paged_chunk_kernel(PagedParams p) {
           __builtin_amdgcn_sched_group_barrier(0x100, KB, 0);
         }
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) sacc[kb] = Mfma<T>::run(a0[kb], qreg[st], sacc[kb]);
-        __builtin_amdgcn_sched_group_barrier(0x008, KB, 0);
+        for (int kb = 0; kb < KB; ++kb) sacc[kb] = chunk_score<T>(a0[kb], qreg[st], sacc[kb]);
+        __builtin_amdgcn_sched_group_barrier(0x008, KB * (ES == 4 ? 4 : 1), 0);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
           a0[kb] = a1[kb];
@@ -260,40 +307,25 @@ void paged_chunk_kernel(PagedParams p) {
       }
     }
 
-    // element (kb, x) of this lane is key key0 + 4hi + ce, ce = 32kb + 8(x/4) + x%4: visible iff it lies in
-    // [lo, lo + len), or before the end of the first tokens (one compare each, and no branch: written with && and ||
-    // this was a branch per element: two prompts of 4,093 tokens, window 1,024, head dim 64 took 55 us, not 48)
+    // Element (kb, x) of this lane is key key0 + 4hi + 32kb + ce, ce = 8(x/4) + x%4. What its query sees of the 32 from
+    // there on is a mask of bits: the run from the window's first key to the query, and the first tokens (up to the
+    // query). An element then takes two instructions, where compares took three and a branch each when written with
+    // && and || (two prompts of 4,093 tokens, window 1,024, head dim 64: 55 us with the branches, 46 with compares, 45).
     if (!full) {
       const int base = key0 + 4 * hi;
-      int lo = p.window > 0 ? qpos - p.window + 1 - base : -base;
-      if (lo < -base) lo = -base;
-      const unsigned len = (unsigned)((qpos < w.last ? qpos : w.last) - base - lo + 1);
-      if (key0 >= p.sinks) {
+      const int top = (qpos < w.last ? qpos : w.last) - base + 1;   // past the last visible key
+      const int lo = (p.window > 0 ? qpos - p.window + 1 : 0) - base;
+      const int first = p.sinks - base < top ? p.sinks - base : top;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+      for (int kb = 0; kb < KB; ++kb) {
+        unsigned see = (low_bits(top - 32 * kb) & ~low_bits(lo - 32 * kb)) | low_bits(first - 32 * kb);
+        if (bad) {
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int ce = 32 * kb + 8 * (x >> 2) + (x & 3);
-            sacc[kb][x] = (unsigned)(ce - lo) < len ? sacc[kb][x] : kNegInf;
-          }
-      } else {
-        const int first = p.sinks - base;
-        const int top = lo + (int)len;  // (first tokens after the query are not visible either)
+          for (int x = 0; x < 16; x += 4)
+            if (bad >> ((32 * kb + 2 * x) / RW) & 1) see &= ~(0xffu << (2 * x));
+        }
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const int ce = 32 * kb + 8 * (x >> 2) + (x & 3);
-            const bool see = ((unsigned)(ce - lo) < len) | ((ce < first) & (ce < top));
-            sacc[kb][x] = see ? sacc[kb][x] : kNegInf;
-          }
-      }
-      if (bad) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int x = 0; x < 16; ++x)
-            if (bad >> ((32 * kb + 8 * (x >> 2)) / RW) & 1) sacc[kb][x] = kNegInf;
+        for (int x = 0; x < 16; ++x) sacc[kb][x] = masked(sacc[kb][x], see, 8 * (x >> 2) + (x & 3));
       }
     }
 
@@ -329,22 +361,37 @@ void paged_chunk_kernel(PagedParams p) {
       }
     l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
 
-    // O^T += V^T . P^T (weights rounded to the type: the matrix cores take nothing wider beside 16-bit values)
+    // O^T += V^T . P^T (16-bit weights are rounded to the type: the matrix cores take nothing wider beside V)
+    if constexpr (ES == 4) {
 #pragma unroll
-    for (int hf = 0; hf < HALVES; ++hf) {
-      const int kb = hf >> 1, half = hf & 1;
-      V8 pb;
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pb[e] = from_f32<T>(sacc[kb][8 * half + e]);
+        for (int x = 0; x < 16; ++x) {
+          const unsigned row = (32 * kb + 8 * (x >> 2) + (x & 3)) * TL::ROWB;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const unsigned va = (vl ^ (64 * (d & 3))) + 256 * (d >> 2) + 16 * hf * TL::ROWB;
-        const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)va);
-        const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4*)(va + 8 * TL::ROWB));
-        typedef short i16x8 __attribute__((ext_vector_type(8)));
-        const i16x8 av = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
-        oacc[d] = Mfma<T>::run(__builtin_bit_cast(V8, av), pb, oacc[d]);
+          for (int d = 0; d < DB; ++d) {
+            const float a = *(__attribute__((address_space(3))) const float*)((vl ^ (128 * (d & 1))) + 256 * (d >> 1) + row);
+            oacc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, sacc[kb][x], oacc[d], 0, 0, 0);
+          }
+        }
+    } else {
+      using V8 = typename Mfma<T>::vec;
+#pragma unroll
+      for (int hf = 0; hf < BN / 16; ++hf) {
+        const int kb = hf >> 1, half = hf & 1;
+        V8 pb;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pb[e] = from_f32<T>(sacc[kb][8 * half + e]);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const unsigned va = (vl ^ (64 * (d & 3))) + 256 * (d >> 2) + 16 * hf * TL::ROWB;
+          const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)va);
+          const i16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) i16x4*)(va + 8 * TL::ROWB));
+          typedef short i16x8 __attribute__((ext_vector_type(8)));
+          const i16x8 av = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+          oacc[d] = Mfma<T>::run(__builtin_bit_cast(V8, av), pb, oacc[d]);
+        }
       }
     }
   }
@@ -460,11 +507,11 @@ template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_
 }
 
 template <typename T, int D> static int launch_chunk_d(PagedParams p, const PagedPlan& plan, hipStream_t s) {
-  using TL = Tile<D>;
+  using TL = ChunkTile<T, D>;
   static bool attr_set = false;
-  if (chunk_lds<D>() > 64 * 1024 && !attr_set) {
+  if (TL::LDS_BYTES > 64 * 1024 && !attr_set) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, chunk_lds<D>()) != hipSuccess)
+                            hipFuncAttributeMaxDynamicSharedMemorySize, TL::LDS_BYTES) != hipSuccess)
       return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
     attr_set = true;
   }
@@ -478,7 +525,7 @@ template <typename T, int D> static int launch_chunk_d(PagedParams p, const Page
     const int st = check_launch();
     if (st) return st;
   }
-  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(256), chunk_lds<D>(), s, p);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(256), TL::LDS_BYTES, s, p);
   const int st = check_launch();
   return st || (p.nparts < 2 && !plan.planned) ? st : launch_paged_combine<T, D, TL::BM, TL::BN>(p, s);
 }
@@ -488,10 +535,15 @@ template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPl
     case 64: return launch_chunk_d<T, 64>(p, plan, s);
     case 128: return launch_chunk_d<T, 128>(p, plan, s);
     case 256: return launch_chunk_d<T, 256>(p, plan, s);
-    default: return set_error("forge_attn_paged: unsupported head dim");
   }
+  return set_error("forge_attn_paged: unsupported head dim");
 }
+#if FORGE_PAGED_PART == 1
 template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 2
 template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 3
+template int launch_paged_chunk<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#endif
 
 }  // namespace forge

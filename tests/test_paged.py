@@ -55,6 +55,12 @@ CASES = [
     (HF, 8, 4, 32, 16, [0], 300, None, 0, 0),
     (BF, 28, 4, 128, 32, [64], 45, None, 0, 0),
     (BF, 6, 2, 128, 16, [64, 3], 45, None, 0, 0),
+    # fp32 chunks of more than 64 rows: two and three row blocks, tiles that the row's end cuts
+    (SF, 16, 8, 128, 32, [70, 0], 130, None, 0, 0),
+    (SF, 12, 4, 64, 16, [333], 100, None, 0, 0),
+    (SF, 8, 1, 256, 16, [37], 21, None, 0, 0),
+    (SF, 16, 8, 128, 16, [500, 20], 60, [60, 7], 100, 9),
+    (SF, 8, 4, 256, 64, [90], 130, None, 33, 40),
     # padded batches: no new token, one, some, all
     (BF, 16, 8, 128, 16, [100, 50, 0, 700], 9, [9, 0, 1, 4], 0, 0),
     (HF, 12, 4, 64, 16, [30, 8, 0], 90, [90, 1, 0], 0, 0),
