@@ -50,7 +50,7 @@ struct PagedParams {
   // Planned calls (the chunk kernel, rows of different lengths): block x takes item items[x / K] of KV head
   // x % K; the pairs say where the merge finds a row block's partials. Null: the static split above.
   const PagedItem* items;
-  const int2* pairs;  // [B][row blocks]: (its first slot, parts)
+  const int4* pairs;  // [B][row blocks]: (its first slot, parts, the batch row's real query rows)
   int slots;          // blocks that the device holds at a time
   float2* ws_ml;      // [slot][block's rows]
   float* ws_o;        // ... [D]
@@ -224,10 +224,9 @@ __device__ __forceinline__ void store_shared(float2* p, float x, float y) {
 
 // Merges a row's parts, in part order, over four channels: (m, l) at ml[i * step], outputs at o[i * step * D].
 // Returns the sum of the weights. SHARED: written in this launch.
-template <int D, bool SHARED>
+template <int D, int U, bool SHARED>
 __device__ __forceinline__ float merge_parts(const float2* ml, const float* po, int parts, int64_t step, float4& O) {
-  // eight parts' loads go out together; the running maximum as in the kernels
-  constexpr int U = 8;
+  // U parts' loads go out together; the running maximum as in the kernels
   float M = kNegInf, L = 0.0f;
   O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int i0 = 0; i0 < parts; i0 += U) {
@@ -282,25 +281,25 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   const int sub = blockIdx.y, rblk = blockIdx.z, pair = b * nrb + rblk;
   const int in = sub * RPB + threadIdx.x / LPR, flat = rblk * BM + in;
   const int x = 4 * (threadIdx.x % LPR);
-  int base, rows;
-  row_extent(p, b, base, rows);
-  if (flat >= rows) return;
-  int parts, stride;
+  int rows, parts, stride;
   int64_t slot;
   if (p.items) {
-    const int2 e = p.pairs[pair];
-    parts = e.y;
-    slot = (int64_t)e.x * p.K + kvh;
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const i32x4 e = *(const __attribute__((address_space(4))) i32x4*)(p.pairs + pair);
+    slot = (int64_t)e[0] * p.K + kvh;
+    parts = e[1];
+    rows = e[2];
     stride = p.K;
   } else {
-    const RowSpan w = make_span(p, base, rows, rblk * BM, BM, KT);
+    const RowSpan w = row_span(p, b, rblk * BM, BM, KT);
+    rows = w.rows;
     parts = (w.tiles + p.part_tiles - 1) / p.part_tiles;
     slot = ((int64_t)(b * p.K + kvh) * nrb + rblk) * p.nparts;
     stride = 1;
   }
-  if (parts < 2) return;  // written by its block
+  if (parts < 2 || flat >= rows) return;  // written by its block
   float4 O;
-  const float L = merge_parts<D, false>(p.ws_ml + slot * BM + in, p.ws_o + (slot * BM + in) * D + x, parts,
+  const float L = merge_parts<D, BM >= 128 ? 4 : 8, false>(p.ws_ml + slot * BM + in, p.ws_o + (slot * BM + in) * D + x, parts,
                                         (int64_t)stride * BM, O);
   store_row<T>(p, b, kvh, flat, x, O, L > 0.0f ? 1.0f / L : 0.0f);
 }

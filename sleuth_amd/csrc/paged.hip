@@ -522,7 +522,7 @@ void paged_step_kernel(PagedParams p) {
   for (int x = threadIdx.x; x < here * Q4; x += 256) {
     const int row = x / Q4, ch = 4 * (x % Q4);
     float4 O;
-    const float L = merge_parts<D, true>(p.ws_ml + slot0 + row, p.ws_o + (slot0 + row) * D + ch, work.parts, ROWS, O);
+    const float L = merge_parts<D, 8, true>(p.ws_ml + slot0 + row, p.ws_o + (slot0 + row) * D + ch, work.parts, ROWS, O);
     store_row<T>(p, b, kvh, row0 + row, ch, O, L > 0.0f ? 1.0f / L : 0.0f);
   }
 }

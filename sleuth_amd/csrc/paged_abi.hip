@@ -87,7 +87,7 @@ static PagedWs paged_ws(const PagedPlan& plan, int B, int T, int H, int K, int D
   const size_t rows = (plan.planned ? (size_t)plan.nitems : blocks * plan.nparts) * K * plan.rows;
   w.items = FORGE_PAGED_COUNTER_BYTES;
   w.pairs = w.items + (plan.planned ? up(plan.nitems * sizeof(PagedItem)) : 0);
-  w.ml = w.pairs + (plan.planned ? up(blocks * sizeof(int2)) : 0);
+  w.ml = w.pairs + (plan.planned ? up(blocks * sizeof(int4)) : 0);
   w.o = w.ml + up(rows * sizeof(float2));
   w.bytes = w.o + rows * D * sizeof(float);
   return w;
@@ -130,7 +130,7 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
     char* at = static_cast<char*>(workspace);
     if (plan.planned) {
       p.items = reinterpret_cast<PagedItem*>(at + ws.items);
-      p.pairs = reinterpret_cast<int2*>(at + ws.pairs);
+      p.pairs = reinterpret_cast<int4*>(at + ws.pairs);
     }
     p.ws_ml = reinterpret_cast<float2*>(at + ws.ml);
     p.ws_o = reinterpret_cast<float*>(at + ws.o);

@@ -425,7 +425,7 @@ void paged_chunk_kernel(PagedParams p) {
 // longest first (64 classes of length), so that a CU that got a long one gets a short one beside it.
 constexpr int kPlanThreads = 1024;
 template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedParams p, PagedItem* items,
-                                                                                        int2* pairs, int nitems) {
+                                                                                        int4* pairs, int nitems) {
   __shared__ int tiles[kPlanPairs];
   __shared__ int wave_of[16], wave_tot[16], cls[64], pick;
   const int nrb = (p.rows + BM - 1) / BM, n = p.B * nrb;
@@ -498,7 +498,9 @@ template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     const int parts = parts_of(i);
-    pairs[i] = make_int2(before, parts);
+    int base, rows;
+    row_extent(p, i / nrb, base, rows);
+    pairs[i] = make_int4(before, parts, rows, 0);
     const int at = atomicAdd(&cls[class_of(i, parts)], parts);
     for (int j = 0; j < parts; ++j) items[at + j] = PagedItem{i, j, parts, before + j};
     before += parts;
@@ -521,7 +523,7 @@ template <typename T, int D> static int launch_chunk_d(PagedParams p, const Page
   if (plan.planned) {
     grid = dim3((unsigned)(plan.nitems * p.K));
     hipLaunchKernelGGL((paged_plan_kernel<TL::BM, TL::BN>), dim3(1), dim3(kPlanThreads), 0, s, p,
-                       const_cast<PagedItem*>(p.items), const_cast<int2*>(p.pairs), plan.nitems);
+                       const_cast<PagedItem*>(p.items), const_cast<int4*>(p.pairs), plan.nitems);
     const int st = check_launch();
     if (st) return st;
   }
