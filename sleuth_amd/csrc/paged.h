@@ -272,8 +272,9 @@ __device__ __forceinline__ float merge_parts(const float2* ml, const float* po, 
 constexpr int combine_rows(int D, int BM) { return 1024 / D < BM ? 1024 / D : BM; }
 
 // Merges the parts of the rows whose tiles were split: D / 4 lanes per row, four channels each, the
-// parts in order.
-template <typename T, int D, int BM, int KT>
+// parts in order, eight at a time; four in planned calls, whose many rows of few parts want the registers for more
+// waves.
+template <typename T, int D, int BM, int KT, bool PLANNED>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   constexpr int LPR = D / 4, RPB = combine_rows(D, BM);
   const int nrb = (p.rows + BM - 1) / BM;
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   const int x = 4 * (threadIdx.x % LPR);
   int rows, parts, stride;
   int64_t slot;
-  if (p.items) {
+  if constexpr (PLANNED) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     const i32x4 e = *(const __attribute__((address_space(4))) i32x4*)(p.pairs + pair);
     slot = (int64_t)e[0] * p.K + kvh;
@@ -299,17 +300,18 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   }
   if (parts < 2 || flat >= rows) return;  // written by its block
   float4 O;
-  const float L = merge_parts<D, BM >= 128 ? 4 : 8, false>(p.ws_ml + slot * BM + in, p.ws_o + (slot * BM + in) * D + x, parts,
-                                        (int64_t)stride * BM, O);
+  const float2* ml = p.ws_ml + slot * BM + in;
+  const float* po = p.ws_o + (slot * BM + in) * D + x;
+  const float L = merge_parts<D, PLANNED ? 4 : 8, false>(ml, po, parts, (int64_t)stride * BM, O);
   store_row<T>(p, b, kvh, flat, x, O, L > 0.0f ? 1.0f / L : 0.0f);
 }
 
-template <typename T, int D, int BM, int KT> static int launch_paged_combine(const PagedParams& p, hipStream_t s) {
+template <typename T, int D, int BM, int KT, bool PLANNED = false> static int launch_paged_combine(const PagedParams& p, hipStream_t s) {
   constexpr int RPB = combine_rows(D, BM);
   const int64_t nrb = (p.rows + BM - 1) / BM;
   const int subs = p.rows < BM ? (p.rows + RPB - 1) / RPB : BM / RPB;  // (blocks of a row block)
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
-  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
+  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT, PLANNED>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
                      0, s, p);
   return check_launch();
 }

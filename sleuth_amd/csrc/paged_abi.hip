@@ -28,13 +28,15 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   if (plan.rows > row_most) plan.rows = row_most;
   plan.keys = step_keys(es, D, plan.rows);
-  // More than 32 rows go to the chunk kernel, whose four waves share each key tile; up to 32 the split kernel's
-  // waves keep more bytes in flight. us, split / chunk: 34 rows (8 batch rows of 2,000 keys, 8 KV heads, head dim
-  // 128) 27.8 / 23.9, 40 rows (32 of 8,000) 239 / 194, 32 rows 183 / 196; head dim 256, one KV head, 16 batch rows of
-  // 8,000: 40 rows 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118. In fp32, where a tile's products take 3.4 us a
-  // wave, from 65 rows and head dim 64 on: 80 rows (8 of 2,000) 111 / 85, 40 rows 64.7 / 79; 600 new tokens 143 / 127,
-  // 700 at head dim 256 116 / 92; head dim 32 (2 rows of 333) 15.5 / 23.8.
-  if (es == 2 ? D >= 64 && D <= 256 && rows > 32 : D >= 64 && rows > 64) {
+  // More than 32 rows go to the chunk kernel, whose waves share each key tile; up to 32 the split kernel's waves keep
+  // more bytes in flight. us, split / chunk: 34 rows (8 batch rows of 2,000 keys, 8 KV heads, head dim 128) 27.8 / 23.9,
+  // 40 rows (32 of 8,000) 239 / 194, 32 rows 183 / 196; head dim 256, one KV head, 16 batch rows of 8,000: 40 rows
+  // 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118. Head dim 512, where the split kernel has room for 16 rows, from 17
+  // on: 32 rows (8 batch rows of 4,000) 30.1 / 26.9, 48 of 500 18.0 / 15.6, 8,192 (1 of 4,600) 404 / 113; its worst are
+  // 320 rows of 300 keys, 18.7 / 23.1. In fp32, where a tile's products take 3.4 us a wave, from 65 rows and head dim
+  // 64 on: 80 rows (8 of 2,000) 111 / 85, 40 rows 64.7 / 79; 600 new tokens 143 / 127, 700 at head dim 256 116 / 92; head
+  // dim 32 (2 rows of 333) 15.5 / 23.8.
+  if (es == 2 ? D >= 64 && rows > (D == 512 ? 16 : 32) : D >= 64 && rows > 64) {
     plan.chunk = true;
     plan.rows = 128;
     plan.keys = es * D >= 512 ? 32 : 64;
@@ -59,9 +61,19 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     plan.nitems = (int)(plan.slots / K + blocks);
     return plan;
   }
-  // (two tiles for each wave of the split kernel, eight for a chunk block: 96 rows of 8,000 keys at head dim 256
-  // take 39.6 / 29.6 / 29.2 / 37.5 us at 2 / 4 / 8 / 16; one of the long tiles in fp32: 100 tokens 14 us, not 35)
-  const int64_t least = es == 4 && plan.chunk ? 1 : 8, most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
+  // The least tiles of a part. Split kernel: two for each wave. Chunk kernel: a part's tiles run one after the other
+  // and so do the parts in the merge, an eighth of a tile's time each, so n tiles in parts of p take about
+  // p + n / (8 p), least at p = sqrt(n / 8); up to four tiles a second launch costs more than it saves. us with parts
+  // of eight or more / with these: 100 new tokens behind 2,000 at head dim 128 18.6 / 15.0, two rows of 100 behind 900
+  // at head dim 64 15.3 / 10.1, 3 tokens behind 500 at head dim 512 27.1 / 15.7; 96 query rows of 8,000 keys at head dim
+  // 256 25.3 / 24.7 (twice as many a part 25.0). One of the long tiles in fp32: 100 tokens 14 us, not 35.
+  int64_t least = 8;
+  if (plan.chunk) {
+    least = 1;
+    while (es == 2 && least * least * 8 < tiles) ++least;
+    if (es == 2 && tiles <= 4) least = tiles;
+  }
+  const int64_t most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
   int64_t per = (units * tiles + slots - 1) / slots;
   if (per > most) per = most;
   if (per < least) per = least;

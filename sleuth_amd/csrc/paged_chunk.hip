@@ -1,13 +1,13 @@
 // Chunks of many query rows over a paged cache, or over a contiguous one with a window and first tokens:
-// bf16/fp16, head dims 64, 128, 256, on v_mfma_f32_32x32x16, and fp32, head dims 64 to 256, on v_mfma_f32_32x32x2
+// bf16/fp16, head dims 64 to 512, on v_mfma_f32_32x32x16, and fp32, head dims 64 to 256, on v_mfma_f32_32x32x2
 // (the split kernel of paged.hip serves the rest).
 //
-// A block of 4 waves owns 128 query rows of one (batch row, KV head) -- row r is token r / G, head r % G of the
+// A block of 4 waves (8 at head dim 512) owns 128 query rows of one (batch row, KV head) -- row r is token r / G, head r % G of the
 // group, so the heads of a group share each key tile they read -- and streams that row's visible key tiles through
 // two LDS stages, as the causal prefill kernel does: direct loads into LDS in swizzled chunk order, S^T = K . Q^T
 // with Q^T in registers, one lane per query row (two lanes share a row's keys), P^T fed to O^T = V^T . P^T straight
 // from the score registers. See prefill.hip for the operand layouts; what differs here:
-//   * A wave loads RW = BN / 4 consecutive key rows of a tile, which never straddle pages (pages are multiples of 16
+//   * A wave loads RW (BN / 4, or / 8) consecutive key rows of a tile, which never straddle pages (pages are multiples of 16
 //     positions), so a tile costs each wave one table entry: a scalar load, issued one tile ahead.
 //   * A page id outside the pool leaves zeros in LDS and a flag for the stage; its keys are masked.
 //   * With a window, the tiles that hold first tokens come before those of the window.
@@ -18,17 +18,25 @@
 
 namespace forge {
 
-// Block shape: 128 query rows, BN keys per tile, two LDS stages of a K and a V tile.
+// Block shape: 128 query rows, BN keys per tile, two LDS stages of a K and a V tile. At head dim 512 a wave's
+// registers hold the queries and the output of 256 channels, so two waves share 32 rows: each sums the scores of its
+// half of the channels, the two exchange those sums, and each takes the products with its half of V. (One wave with all
+// 512 would need 384 registers for them: the compiler spills the queries.) 16 heads, one KV head: 4,096 tokens behind
+// 4,096 959 us, 860 TFLOP/s; 512 behind 4,096 113 us, 404 on the split kernel.
+constexpr int chunk_halves(int D) { return D > 256 ? 2 : 1; }
 template <typename T, int D> struct ChunkTile {
-  static constexpr int WAVES = 4, STAGES = 2, BM = 128;
+  static constexpr int HALVES = chunk_halves(D);
+  static constexpr int WAVES = 4 * HALVES, STAGES = 2, BM = 128;
+  static constexpr int THREADS = WAVES * 64;
   static constexpr int ROWB = D * (int)sizeof(T);        // bytes per key row
   static constexpr int NCH = ROWB / 16;                  // 16-byte chunks of it
   static constexpr int BN = ROWB >= 512 ? 32 : 64;
   static constexpr int TILEB = BN * ROWB;
   static constexpr int LOADS = TILEB / (WAVES * 1024);   // 16-byte loads per lane per tile
-  static constexpr int LDS_BYTES = STAGES * 2 * TILEB + 64;  // and the stages' flags
-  static constexpr int QS = D * (int)sizeof(T) / 32;     // 16-byte pieces of a lane's half of a query row
+  static constexpr int LDS_BYTES = STAGES * 2 * TILEB + (HALVES == 2 ? WAVES * 4096 : 64);  // and sums, or flags
+  static constexpr int QS = D / HALVES * (int)sizeof(T) / 32;  // 16-byte pieces of a lane's share of a query row
   static constexpr int BLOCKS = ROWB >= 1024 ? 1 : 2;    // per CU
+  static_assert(BLOCKS * LDS_BYTES <= 160 * 1024, "LDS");
 };
 // Chunk swizzles by key row: as prefill_tile.h's in 16 bits; in fp32 a V read is 32 channels of two rows 4 apart.
 template <typename T, int D> __device__ __forceinline__ int chunk_swz_k(int row) {
@@ -41,14 +49,18 @@ template <typename T, int D> __device__ __forceinline__ int chunk_swz_v(int row)
 }
 
 // Query row (b, h, t) as MFMA B operands, RMSNorm and RoPE in fp32 with one rounding: lane half hi holds the
-// 16-byte pieces 2s + hi (in 16 bits the k-slots of one product, in fp32 of four).
+// 16-byte pieces 2s + hi (in 16 bits the k-slots of one product, in fp32 of four). Of two waves that share the
+// row, wave `half` takes half of each half of the channels, so that RoPE's pairs stay together.
 template <typename T, int D>
-__device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h, int t, int hi,
+__device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h, int t, int hi, int half,
                                              uint4 (&q)[ChunkTile<T, D>::QS]) {
-  constexpr int S = ChunkTile<T, D>::QS, E = 16 / sizeof(T);
+  constexpr int S = ChunkTile<T, D>::QS, E = 16 / sizeof(T), HALVES = ChunkTile<T, D>::HALVES;
   const T* src = static_cast<const T*>(p.q) + b * p.sqb + h * p.sqh + t * p.sqt;
+  const auto channel = [&](int s, int of) {  // first channel of piece s of wave `of`
+    return HALVES == 1 ? (2 * s + hi) * E : (2 * (s % (S / 2)) + hi) * E + s / (S / 2) * (D / 2) + of * (D / 4);
+  };
 #pragma unroll
-  for (int s = 0; s < S; ++s) q[s] = load16(src + (2 * s + hi) * E);
+  for (int s = 0; s < S; ++s) q[s] = load16(src + channel(s, half));
   const bool norm = p.flags & FORGE_NORM_QK, rope = p.flags & FORGE_ROPE;
   if (!norm && !rope) return;
   float f[S][E];
@@ -60,6 +72,15 @@ __device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h,
     for (int s = 0; s < S; ++s)
 #pragma unroll
       for (int e = 0; e < E; ++e) ss += f[s][e] * f[s][e];
+    if constexpr (HALVES == 2) {  // (the other wave's channels)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        float o[E];
+        unpack16<T>(load16(src + channel(s, half ^ 1)), o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss += o[e] * o[e];
+      }
+    }
     ss += __shfl_xor(ss, 32, kWave);
     const float rs = rsqrtf(ss / (float)D + p.eps);
 #pragma unroll
@@ -68,7 +89,7 @@ __device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h,
       if (p.qw) {
 #pragma unroll
         for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(p.qw + (2 * s + hi) * E + e);
+          *reinterpret_cast<float4*>(w + e) = *reinterpret_cast<const float4*>(p.qw + channel(s, half) + e);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) f[s][e] = p.qw ? f[s][e] * rs * w[e] : f[s][e] * rs;
@@ -81,7 +102,7 @@ __device__ __forceinline__ void chunk_load_q(const PagedParams& p, int b, int h,
     for (int s = 0; s < S / 2; ++s)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int c = (2 * s + hi) * E + e;
+        const int c = channel(s, half) + e;
         const float a = f[s][e], z = f[s + S / 2][e];
         f[s][e] = a * cr[c] - z * sr[c];
         f[s + S / 2][e] = z * cr[c + D / 2] + a * sr[c + D / 2];
@@ -117,21 +138,25 @@ template <typename T, typename V> __device__ __forceinline__ float pair_sum(V a,
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(ChunkTile<T, D>::BLOCKS)))
+__global__ __launch_bounds__(256 * chunk_halves(D))
+__attribute__((amdgpu_waves_per_eu(ChunkTile<T, D>::BLOCKS * chunk_halves(D))))
 void paged_chunk_kernel(PagedParams p) {
   using TL = ChunkTile<T, D>;
   constexpr int BN = TL::BN, BM = TL::BM;
-  constexpr int KB = BN / 32, KSTEPS = TL::QS, DB = D / 32;
+  constexpr int HALVES = TL::HALVES;
+  constexpr int KB = BN / 32, KSTEPS = TL::QS, DB = D / HALVES / 32;
   constexpr int RW = BN / TL::WAVES;      // key rows of a tile that a wave loads
   constexpr int RL = kWave / TL::NCH;     // of which one load instruction covers RL
   static_assert(TL::STAGES == 2 && RW == RL * TL::LOADS && RW <= 16, "a wave's rows lie in one page");
 
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // [stage][K|V][TILEB], then the flags [stage][wave]
   int* flags = reinterpret_cast<int*>(smem + TL::STAGES * 2 * TL::TILEB);
+  float4* sums = reinterpret_cast<float4*>(smem + TL::STAGES * 2 * TL::TILEB);  // (two halves) [wave][4][lane]
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int n = lane & 31, hi = lane >> 5;
+  const int half = HALVES == 2 ? wave >> 2 : 0;
 
   const BlockWork work = block_work<BM, BN>(p);
   if (work.none) return;
@@ -143,7 +168,7 @@ void paged_chunk_kernel(PagedParams p) {
   if (part == 0 && w.rows < rblk * BM + BM) {
     const int r0 = w.rows > rblk * BM ? w.rows : rblk * BM;
     const int r1 = rblk * BM + BM < p.rows ? rblk * BM + BM : p.rows;
-    for (int x = threadIdx.x; x < (r1 - r0) * (D / 4); x += 256)
+    for (int x = threadIdx.x; x < (r1 - r0) * (D / 4); x += TL::THREADS)
       store_row<T>(p, b, kvh, r0 + x / (D / 4), 4 * (x % (D / 4)), make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f);
   }
   if (w.tiles == 0) return;
@@ -151,7 +176,7 @@ void paged_chunk_kernel(PagedParams p) {
   // ---- key tiles: load i of this wave fills LDS slots (wave * LOADS + i) * 64 + lane, key rows RL * i + lane / NCH
   // of the wave's RW, in swizzled chunk order (kept offsets; in 16 bits at head dim 256, where registers are short,
   // one xor each from shared ones)
-  constexpr bool KEEP = !(sizeof(T) == 2 && D == 256);
+  constexpr bool KEEP = !(sizeof(T) == 2 && D >= 256);
   constexpr int ES = sizeof(T);
   const int64_t pageb = p.skp * ES;
   const int rowb = (int)p.sks * ES;
@@ -169,18 +194,31 @@ void paged_chunk_kernel(PagedParams p) {
       kept_v[i] = in * rowb + ((pch ^ chunk_swz_v<T, D>(wr0 + in)) << 4);
     }
   }
-  int flagged[2] = {0, 0};   // what this wave's flag of each stage holds
-  if (lane < 2) flags[4 * lane + wave] = 0;
+  // Whose rows of a stage are zeros: each wave's flag, or, where a tile has only two groups of 16 rows (the least
+  // that a page holds) and the sums take the LDS, bits that every wave looks up itself.
+  int flagged[2] = {0, 0};   // what this wave's flag of each stage holds, or the stage's bits
+  if (HALVES == 1 && lane < 2) flags[4 * lane + wave] = 0;
   // first row of the wave's part of tile i; where the row's keys end before it, of the part that holds the last key
   auto part_key = [&](int i) {
     const int key0 = w.tile_key(i, BN), left = w.last - key0;
     return key0 + (wr0 <= left ? wr0 : left & ~(RW - 1));
   };
+  unsigned groups = 0;  // (two halves) bit j: group j of the tile that `page` belongs to has no page
+  auto page_at = [&](int i) {
+    if constexpr (HALVES == 1) return p.page_of(b, part_key(i));
+    const int key0 = w.tile_key(i, BN), left = w.last - key0;
+    const int p0 = p.page_of(b, key0), p1 = p.page_of(b, key0 + (left >= 16 ? 16 : 0));
+    groups = (unsigned)(p0 < 0) | (unsigned)(p1 < 0) << 1;
+    return part_key(i) - key0 < 16 ? p0 : p1;
+  };
   auto issue = [&](int i, int stage, int page) {
     const unsigned kdst = lds_offset(smem + (2 * stage) * TL::TILEB + wave * TL::LOADS * 1024);
     const unsigned vdst = kdst + TL::TILEB;
     const int miss = page < 0;
-    if (miss != flagged[stage]) {
+    if constexpr (HALVES == 2) {
+      if (stage == 0) flagged[0] = (int)groups;
+      else flagged[1] = (int)groups;
+    } else if (miss != flagged[stage]) {
       if (lane == 0) flags[4 * stage + wave] = miss;
       flagged[stage] = miss;
     }
@@ -222,11 +260,12 @@ void paged_chunk_kernel(PagedParams p) {
       }
     }
   };
-  issue(begin, 0, p.page_of(b, part_key(begin)));
-  int page = p.page_of(b, part_key(begin + 1 < end ? begin + 1 : begin));
+  int page = page_at(begin);
+  issue(begin, 0, page);
+  page = page_at(begin + 1 < end ? begin + 1 : begin);
 
   // ---- this lane's query row; the wave's span of positions
-  const int w_row = rblk * BM + wave * 32;
+  const int w_row = rblk * BM + (wave & 3) * 32;
   const bool wave_any = w_row < w.rows;
   const int flat = w_row + n;
   const bool valid = flat < w.rows;
@@ -235,7 +274,7 @@ void paged_chunk_kernel(PagedParams p) {
   const int wq_lo = w.base + p.token(w_row);
   const int wq_hi = w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
   uint4 qreg[KSTEPS];
-  chunk_load_q<T, D>(p, b, h, t, hi, qreg);
+  chunk_load_q<T, D>(p, b, h, t, hi, half, qreg);
 
   // LDS read offsets of a lane within a stage's K and V tiles: in 16 bits prefill.hip's; in fp32 a V operand is channel
   // 32d + n of key 8i + 4hi + j, whose swizzle is the lane's own bit hi
@@ -264,18 +303,20 @@ void paged_chunk_kernel(PagedParams p) {
     __syncthreads();  // tile `it` is in LDS for every wave; the other stage is free
     if (it + 1 < end) {
       issue(it + 1, stage ^ 1, page);
-      page = p.page_of(b, part_key(it + 2 < end ? it + 2 : it + 1));
+      page = page_at(it + 2 < end ? it + 2 : it + 1);
     }
     const int key0 = w.tile_key(it, BN);
     const bool needed = wave_any && key0 <= wq_hi &&
                         (p.window <= 0 || key0 + BN - 1 > wq_lo - p.window || key0 < p.sinks);
-    if (!needed) continue;
-    const unsigned bad = p.table ? (unsigned)__ballot(flags[4 * stage + (lane & 3)] != 0) & 15u : 0u;
+    if (HALVES == 1 && !needed) continue;
+    unsigned bad = 0;
+    if constexpr (HALVES == 2) bad = (unsigned)(stage ? flagged[1] : flagged[0]);
+    else if (p.table) bad = (unsigned)__ballot(flags[4 * stage + (lane & 3)] != 0) & 15u;
     const bool full = bad == 0 && key0 + BN - 1 <= wq_lo &&
                       (p.window <= 0 || wq_hi - key0 < p.window || key0 + BN <= p.sinks);
 
-    const unsigned kl = lds0 + (2 * stage) * TL::TILEB + k_rd;
-    const unsigned vl = lds0 + (2 * stage + 1) * TL::TILEB + v_rd;
+    const unsigned kl = lds0 + (2 * stage) * TL::TILEB + k_rd + 256 * half;
+    const unsigned vl = lds0 + (2 * stage + 1) * TL::TILEB + v_rd + 512 * half;
 
     // S^T = K . Q^T, K operands read two steps ahead (pinned: left alone each step waits for its reads)
     floatx16 sacc[KB];
@@ -283,11 +324,11 @@ void paged_chunk_kernel(PagedParams p) {
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int x = 0; x < 16; ++x) sacc[kb][x] = 0.0f;
-    {
+    if (HALVES == 1 || needed) {
       auto kread = [&](int kb, int st) {
         typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-        return __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) const u32x4*)((kl ^ (32 * (st & 7))) + 256 * (st >> 3) +
-                                                                                           kb * 32 * TL::ROWB));
+        return __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) const u32x4*)((kl ^ (32 * (st & 7))) +
+                                                                                           256 * HALVES * (st >> 3) + kb * 32 * TL::ROWB));
       };
       uint4 a0[KB], a1[KB], a2[KB];
 #pragma unroll
@@ -312,6 +353,26 @@ void paged_chunk_kernel(PagedParams p) {
         }
       }
     }
+    if constexpr (HALVES == 2) {
+      // the sums of the other half of the channels (every wave meets here, whatever it needs)
+      float4* mine = sums + wave * 256 + lane;
+      if (needed) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mine[64 * i] = make_float4(sacc[0][4 * i], sacc[0][4 * i + 1], sacc[0][4 * i + 2], sacc[0][4 * i + 3]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (LDS only: the next tile's loads go on)
+      if (!needed) continue;
+      const float4* other = sums + (wave ^ 4) * 256 + lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 z = other[64 * i];
+        sacc[0][4 * i] += z.x;
+        sacc[0][4 * i + 1] += z.y;
+        sacc[0][4 * i + 2] += z.z;
+        sacc[0][4 * i + 3] += z.w;
+      }
+    }
 
     // Element (kb, x) of this lane is key key0 + 4hi + 32kb + ce, ce = 8(x/4) + x%4. What its query sees of the 32 from
     // there on is a mask of bits: the run from the window's first key to the query, and the first tokens (up to the
@@ -328,7 +389,7 @@ void paged_chunk_kernel(PagedParams p) {
         if (bad) {
 #pragma unroll
           for (int x = 0; x < 16; x += 4)
-            if (bad >> ((32 * kb + 2 * x) / RW) & 1) see &= ~(0xffu << (2 * x));
+            if (bad >> ((32 * kb + 2 * x) / (HALVES == 2 ? 16 : RW)) & 1) see &= ~(0xffu << (2 * x));
         }
 #pragma unroll
         for (int x = 0; x < 16; ++x) sacc[kb][x] = masked(sacc[kb][x], see, 8 * (x >> 2) + (x & 3));
@@ -406,15 +467,15 @@ void paged_chunk_kernel(PagedParams p) {
   l_run += __shfl_xor(l_run, 32, kWave);
   if (!valid) return;
   if (!whole) {
-    const int64_t slot = (int64_t)work.slot * BM + wave * 32 + n;
-    float* po = p.ws_o + slot * D + 4 * hi;
+    const int64_t slot = (int64_t)work.slot * BM + (wave & 3) * 32 + n;
+    float* po = p.ws_o + slot * D + half * (D / 2) + 4 * hi;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<float4*>(po + d * 32 + 8 * i) =
             make_float4(oacc[d][4 * i], oacc[d][4 * i + 1], oacc[d][4 * i + 2], oacc[d][4 * i + 3]);
-    if (hi == 0) p.ws_ml[slot] = make_float2(m_run, l_run);
+    if (hi == 0 && half == 0) p.ws_ml[slot] = make_float2(m_run, l_run);
     return;
   }
   const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
@@ -422,7 +483,7 @@ void paged_chunk_kernel(PagedParams p) {
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      store_row<T>(p, b, kvh, flat, d * 32 + 8 * i + 4 * hi,
+      store_row<T>(p, b, kvh, flat, half * (D / 2) + d * 32 + 8 * i + 4 * hi,
                    make_float4(oacc[d][4 * i], oacc[d][4 * i + 1], oacc[d][4 * i + 2], oacc[d][4 * i + 3]), inv);
 }
 
@@ -534,9 +595,11 @@ template <typename T, int D> static int launch_chunk_d(PagedParams p, const Page
     const int st = check_launch();
     if (st) return st;
   }
-  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(256), TL::LDS_BYTES, s, p);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(TL::THREADS), TL::LDS_BYTES, s, p);
   const int st = check_launch();
-  return st || (p.nparts < 2 && !plan.planned) ? st : launch_paged_combine<T, D, TL::BM, TL::BN>(p, s);
+  if (st) return st;
+  if (plan.planned) return launch_paged_combine<T, D, TL::BM, TL::BN, true>(p, s);
+  return p.nparts > 1 ? launch_paged_combine<T, D, TL::BM, TL::BN>(p, s) : 0;
 }
 
 template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
@@ -544,6 +607,8 @@ template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPl
     case 64: return launch_chunk_d<T, 64>(p, plan, s);
     case 128: return launch_chunk_d<T, 128>(p, plan, s);
     case 256: return launch_chunk_d<T, 256>(p, plan, s);
+    case 512:
+      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 512>(p, plan, s);
   }
   return set_error("forge_attn_paged: unsupported head dim");
 }

@@ -78,6 +78,12 @@ CASES = [
     (SF, 8, 4, 32, 16, [200], 80, None, 33, 2),
     (BF, 16, 1, 512, 16, [150], 20, None, 48, 3),
     (BF, 8, 4, 256, 16, [400], 66, None, 64, 16),
+    # head dim 512, chunks: part of a row block, several, a padded batch, a window, one KV head and two
+    (BF, 8, 4, 512, 16, [100, 0], 45, [45, 7], 0, 0),
+    (HF, 16, 2, 512, 16, [2, 300, 1000], 4, None, 0, 0),
+    (BF, 16, 1, 512, 64, [500, 30], 9, None, 100, 9),
+    (HF, 16, 1, 512, 128, [700, 3, 90], 33, [1, 33, 0], 20, 64),
+    (BF, 4, 2, 512, 32, [15, 16, 31], 140, None, 0, 0),
 ]
 
 
@@ -318,6 +324,21 @@ def test_entries_outside_the_pool_are_invisible(T, bad, page):
     for i in range(kp.shape[0]):
         if i not in named:
             assert torch.equal(kp[i].cpu().nan_to_num(7.0), cache.kp[i].nan_to_num(7.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 32])
+def test_missing_pages_at_head_dim_512(page):
+    """The same where every wave looks up both groups of 16 keys of a tile: one of them missing, the other, both."""
+    g = gen(21)
+    T, pasts = 21, [500, 70]
+    cache = Paged(g, [p + T for p in pasts], 1, 512, page, BF)
+    for b, j in ((0, 0), (0, 3), (0, 6), (0, 7), (1, 1)):
+        cache.table[b, j] = -1 - j
+        cache.held[b][j * page:(j + 1) * page] = False
+    q = torch.randn(2, T, 16, 512, generator=g).to(BF).transpose(1, 2)
+    got = ops.attn_paged(q.cuda(), cache.kp.cuda(), cache.vp.cuda(), cache.table.cuda(), i32(pasts), scale=0.04)
+    assert_close(got, *cache.want(q, pasts, [T, T], 0, 0, 0.04))
 
 
 @pytest.mark.gpu
