@@ -310,7 +310,9 @@ int forge_kv_append_paged(int dtype, int B, int T, int K, int D, const void* k, 
  * ws_flags = FORGE_WS_ZEROED promises that its first FORGE_PAGED_COUNTER_BYTES bytes hold zero: small merges
  * then need no launch of their own (the block that finishes a row last does them). Every call leaves these bytes
  * zero, so a workspace cleared once before its first use keeps the promise for the calls that follow it
- * on one stream. The order of the sums depends on the shapes and bounds of the call alone.
+ * on one stream. The order of the sums depends on the call's sizes, bounds and row lengths alone.
+ * A key that no query of a row sees is never used. One that some query of it sees and another does not has
+ * weight 0 for the second: 0 * Inf or 0 * NaN of its value reaches that query, as in a masked product.
  */
 #define FORGE_PAGED_COUNTER_BYTES (64 * 1024)
 size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
