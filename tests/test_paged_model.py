@@ -366,3 +366,15 @@ def test_a_served_batch_in_bf16():
                 a, w = outs[0][b, :n], outs[1][b, :n]
                 assert ((a - w).norm() / w.norm()).item() < 40 * 2 ** -8
     assert c.free_pages == d.free_pages and c.seq_lens.tolist() == d.seq_lens_host
+
+
+def test_gated_attention_refuses_a_paged_cache():
+    """Its paths read cache.k[layer] as [B, K, max_len, hd]: a pool of pages must not get there."""
+    from types import SimpleNamespace
+
+    from sleuth_amd.gated import GatedAttention
+
+    m = GatedAttention(SimpleNamespace(n_heads=4, n_kv_heads=2, head_dim=32, n_rot=32, norm_eps=1e-6), 0)
+    cache = PagedKVCache([(2, 32)], 1, 32, "cpu", torch.float32)
+    with pytest.raises(NotImplementedError, match="paged"):
+        m(torch.zeros(1, 1, 16), torch.ones(1, 32), torch.zeros(1, 32), cache)
