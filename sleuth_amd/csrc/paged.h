@@ -1,6 +1,8 @@
 // What the parts of the paged / windowed attention share: its parameters, a block's keys, the merge.
 #pragma once
 
+#include <atomic>
+
 #include "common.h"
 #include "forge_internal.h"
 
@@ -314,6 +316,19 @@ template <typename T, int D, int BM, int KT, bool PLANNED = false> static int la
   hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT, PLANNED>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
                      0, s, p);
   return check_launch();
+}
+
+// Lets a kernel have `bytes` of LDS on the current device; `done` remembers on which devices (a bit each) it has them.
+inline int reserve_lds(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  if (bytes <= 64 * 1024) return 0;
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return set_error("forge_attn_paged: no current device");
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return 0;
 }
 
 template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);

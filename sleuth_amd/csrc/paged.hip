@@ -529,13 +529,8 @@ void paged_step_kernel(PagedParams p) {
 
 template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hipStream_t s) {
   using LD = StepLds<T, D, RB>;
-  static bool attr_set = false;
-  if (LD::BYTES > 64 * 1024 && !attr_set) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, LD::BYTES) != hipSuccess)
-      return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
-    attr_set = true;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB>), LD::BYTES, done)) return st;
   const int nrb = (p.rows + LD::ROWS - 1) / LD::ROWS;
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
   hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);

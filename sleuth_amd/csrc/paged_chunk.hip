@@ -578,13 +578,8 @@ template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_
 
 template <typename T, int D> static int launch_chunk_d(PagedParams p, const PagedPlan& plan, hipStream_t s) {
   using TL = ChunkTile<T, D>;
-  static bool attr_set = false;
-  if (TL::LDS_BYTES > 64 * 1024 && !attr_set) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D>),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, TL::LDS_BYTES) != hipSuccess)
-      return set_error("forge_attn_paged: cannot reserve the LDS the kernel needs");
-    attr_set = true;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D>), TL::LDS_BYTES, done)) return st;
   const int nrb = (p.rows + TL::BM - 1) / TL::BM;
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
   dim3 grid((unsigned)(p.B * p.K), p.nparts, nrb);
