@@ -606,7 +606,8 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     """kv_append into a paged cache: k, v [B,K,T,D] get their norm and RoPE as there, and token t of row b goes to
     position row_pos[b] + t, i.e. slot position % page_size of page page_table[b, position // page_size] of the pools
     [n_pages, K, page_size, D]. Tokens t >= new_lens[b] (a padded batch) and positions without a page (an entry
-    outside the pool, or past the table's end) are not written. Lengths, table and positions are int32 on the GPU."""
+    outside the pool, or past the table's end) are not written. Lengths, table and positions are int32 on the GPU. Rows
+    may share the pages of a common prefix, but no two tokens of a call may go to one slot."""
     st = host().kv_append_paged(k, v, k_pages, v_pages, page_table, row_pos, new_lens, k_weight, float(eps), bool(norm_k),
                                 bool(norm_v), cos, sin)
     if st is not None:
@@ -652,6 +653,8 @@ def _new_token_args(q, cache, q_weight, eps, norm_q, cos, sin, window, sinks, ou
         raise ValueError(f"head dim {D} in {q.dtype}: 32, 64, 128, 256, and 512 in 16 bits")
     if window < 0 or sinks < 0 or (sinks and not window):
         raise ValueError("window and sinks must not be negative, and sinks need a window")
+    if max(window, sinks) >= 1 << 30:
+        raise ValueError("window and sinks must be below 2^30 (a window of 0 sees every key)")
     dev = q.device
     if not _aligned(q):
         q = q.clone(memory_format=torch.contiguous_format)

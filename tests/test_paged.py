@@ -586,6 +586,26 @@ def test_empty_calls():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 70)])
+def test_planned_chunks_at_head_dim_512(window, sinks):
+    """A large call whose rows differ, its parts planned on the device (with a window: too few tiles, not planned)."""
+    _run_paged(BF, 16, 1, 512, 32, [2700, 40, 1500], 130, [130, 128, 0] if window else None, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(window=1 << 30), dict(window=(1 << 32) + 4), dict(window=4, sinks=1 << 30)])
+def test_windows_past_the_range_are_refused(kw):
+    q, kp = torch.zeros(2, 8, 1, 64, dtype=BF, device="cuda"), torch.zeros(4, 4, 16, 64, dtype=BF, device="cuda")
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.attn_paged(q, kp, kp, torch.zeros(2, 2, dtype=torch.int32, device="cuda"), i32([0, 0]), scale=1.0, **kw)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.attn_sinks(q, kp[:2], kp[:2], scale=1.0, pos=0, **{"sinks": 0, **kw})
+    widest = ops.attn_paged(q, kp, kp, torch.zeros(2, 2, dtype=torch.int32, device="cuda"), i32([0, 0]), scale=1.0,
+                            window=(1 << 30) - 1, sinks=(1 << 30) - 1)
+    assert not widest.any()
+
+
+@pytest.mark.gpu
 def test_large_scores_and_infinite_keys_out_of_sight():
     """Scores of hundreds (the running maximum moves), infinities where the mask hides them."""
     g = gen(13)
