@@ -2,6 +2,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "forge_internal.h"
 
 namespace forge {
@@ -23,10 +25,13 @@ int check_launch() {
 }
 
 int device_cus() {
+  static std::atomic<int> known[64];  // by device (a query takes longer than the rest of a small call's checks)
   int ncu = 0, dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess ||
-      hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || ncu <= 0)
-    ncu = 256;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  std::atomic<int>* slot = dev < 64 ? &known[dev] : nullptr;
+  if (slot && (ncu = slot->load(std::memory_order_relaxed)) > 0) return ncu;
+  if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || ncu <= 0) return 256;
+  if (slot) slot->store(ncu, std::memory_order_relaxed);
   return ncu;
 }
 

@@ -73,15 +73,12 @@ struct PagedParams {
 };
 
 // The split kernel's largest row block and its keys per wave tile, by element size and head dim: what the
-// registers hold (fewer keys in flight with more rows or wider ones), and what it is asked for (paged_plan).
-constexpr int step_rows_most(int esize, int D) {
-  return esize == 4 ? (D <= 64 ? 64 : D == 128 ? 32 : 16) : D == 32 ? 64 : D <= 256 ? 32 : 16;
-}
+// registers hold (fewer keys in flight with more rows or wider ones).
+constexpr int step_rows_most(int esize, int D) { return esize * D <= 512 ? 32 : 16; }
 constexpr int step_keys(int esize, int D, int rows) { return esize * D * (rows / 16) >= 1024 ? 16 : 32; }
 // Its blocks per CU (registers, and 160 KB of LDS).
 constexpr int step_blocks_per_cu(int esize, int D, int rows) {
-  const int bytes = esize * D * (rows == 64 ? 2 : 1);
-  return bytes <= 128 && rows == 16 ? 4 : bytes <= 256 ? 2 : 1;
+  return esize * D <= 128 && rows == 16 ? 4 : esize * D <= 256 ? 2 : 1;
 }
 
 // How the host cuts a call: rows per block, keys per tile, parts.

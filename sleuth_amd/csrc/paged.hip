@@ -540,14 +540,10 @@ template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hi
 }
 
 template <typename T, int D> static int launch_step(const PagedParams& p, const PagedPlan& plan, hipStream_t s) {
-  constexpr int MOST = step_rows_most(sizeof(T), D);
-  if (plan.rows == 16) return launch_step_rb<T, D, 1>(p, s);
-  if constexpr (MOST >= 32) {
+  if constexpr (step_rows_most(sizeof(T), D) >= 32) {
     if (plan.rows == 32) return launch_step_rb<T, D, 2>(p, s);
   }
-  if constexpr (MOST >= 64) {
-    if (plan.rows == 64) return launch_step_rb<T, D, 4>(p, s);
-  }
+  if (plan.rows == 16) return launch_step_rb<T, D, 1>(p, s);
   return set_error("forge_attn_paged: no kernel of this row block");
 }
 

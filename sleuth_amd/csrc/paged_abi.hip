@@ -22,52 +22,64 @@ static bool paged_dim_ok(int dtype, int D) {
 static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_kv, int window, int sinks,
                             bool ragged, bool split) {
   PagedPlan plan{};
-  const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
+  const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K, cus = device_cus();
   const int64_t rows = (int64_t)G * T;
-  const int row_most = step_rows_most(es, D);
-  plan.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-  if (plan.rows > row_most) plan.rows = row_most;
-  plan.keys = step_keys(es, D, plan.rows);
+  // tiles that a block can have: its queries' window and the first tokens (whose ends may lie inside tiles), or
+  // the whole row; and the call's blocks
+  const auto tiles_of = [&] {
+    const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
+    const int64_t all = (max_kv + plan.keys - 1) / plan.keys;
+    if (window <= 0) return all;
+    const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
+    return seen < all ? seen : all;
+  };
+  const auto units_of = [&] { return (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows); };
+  plan.rows = 16;
+  plan.keys = step_keys(es, D, 16);
+  const int64_t work = units_of() * tiles_of(), round = (int64_t)cus * step_blocks_per_cu(es, D, 16);
   // More than 32 rows go to the chunk kernel, whose waves share each key tile; up to 32 the split kernel's waves keep
   // more bytes in flight. us, split / chunk: 34 rows (8 batch rows of 2,000 keys, 8 KV heads, head dim 128) 27.8 / 23.9,
   // 40 rows (32 of 8,000) 239 / 194, 32 rows 183 / 196; head dim 256, one KV head, 16 batch rows of 8,000: 40 rows
   // 50.6 / 45.4, 32 rows (64 batch rows) 99.6 / 118. Head dim 512, where the split kernel has room for 16 rows, from 17
-  // on: 32 rows (8 batch rows of 4,000) 30.1 / 26.9, 48 of 500 18.0 / 15.6, 8,192 (1 of 4,600) 404 / 113; its worst are
-  // 320 rows of 300 keys, 18.7 / 23.1. In fp32, where a tile's products take 3.4 us a wave, from 65 rows and head dim
-  // 64 on: 80 rows (8 of 2,000) 111 / 85, 40 rows 64.7 / 79; 600 new tokens 143 / 127, 700 at head dim 256 116 / 92; head
-  // dim 32 (2 rows of 333) 15.5 / 23.8.
-  if (es == 2 ? D >= 64 && rows > (D == 512 ? 16 : 32) : D >= 64 && rows > 64) {
+  // on: 32 rows (8 batch rows of 4,000) 30.1 / 26.9, 8,192 (1 of 4,600) 404 / 113. In fp32, where a tile's products take
+  // 3.4 us a wave, from 65 rows and head dim 64 on: 80 rows (8 of 2,000) 111 / 85, 40 rows 64.7 / 79; 600 new tokens 143 /
+  // 127, 700 at head dim 256 116 / 92; head dim 32 (2 rows of 333) 15.5 / 23.8.
+  // A call whose 16-row blocks have few tiles is a matter of latency, and goes to them whatever its rows: up to six
+  // tiles for each block that the device holds. us, split / chunk: 256 new tokens at head dim 256 12.1 / 16.7 (4 tiles
+  // each), 12 behind 8,000 22.2 / 24.6 (5.9), 60 behind 300 at head dim 512 21.2 / 26.7 (5.6); four rows of 48 behind 500
+  // at head dim 256 23.9 / 17.4 (6.8), 100 fp32 tokens behind 500 26.0 / 21.3 (7.7).
+  if (work > 6 * round && rows > (es == 4 ? 64 : D == 512 ? 16 : 32) && D >= 64) {
     plan.chunk = true;
     plan.rows = 128;
     plan.keys = es * D >= 512 ? 32 : 64;
+  } else if (rows > 16 && work > 16 * round && step_rows_most(es, D) >= 32) {
+    // 32 rows a block read the keys half as often, 16 rows make twice the blocks: up to 16 tiles for each that the device
+    // holds. us, 16 / 32 rows: 32 query rows over 1,500 keys at head dim 256 14.1 / 17.6, over 8,000 (15.6 tiles each)
+    // 24.7 / 27.0; 16 batch rows of 1,024-key windows at head dim 128 (17 tiles) 27.1 / 21.2, 32 of 8,000 341 / 182;
+    // 333 tokens at head dim 32 in fp32 12.6 / 13.1, 2,000 in bf16 37.9 / 29.2 (64 rows a block 31.8).
+    plan.rows = 32;
+    plan.keys = step_keys(es, D, 32);
   }
   plan.nparts = 1;
   if (!split) return plan;
-  // tiles that a block can have: its queries' window and the first tokens (whose ends may lie inside tiles), or
-  // the whole row
-  const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
-  int64_t tiles = (max_kv + plan.keys - 1) / plan.keys;
-  if (window > 0) {
-    const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
-    if (seen < tiles) tiles = seen;
-  }
+  const int64_t tiles = tiles_of(), units = units_of();
   // (three chunk blocks per CU at head dim 64: a 512-token chunk at 15,360, 12 q / 4 KV heads, 53 -> 45 us)
-  plan.slots = device_cus() * (plan.chunk ? (es * D >= 1024 ? 1 : es * D <= 128 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
+  plan.slots = cus * (plan.chunk ? (es * D >= 1024 ? 1 : es * D <= 128 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
   const int64_t slots = plan.slots;
-  const int64_t units = (int64_t)B * K * ((rows + plan.rows - 1) / plan.rows);
   const int64_t blocks = units / K;
   if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots) {
     plan.planned = true;
     plan.nitems = (int)(plan.slots / K + blocks);
     return plan;
   }
-  // The least tiles of a part. Split kernel: two for each wave. Chunk kernel: a part's tiles run one after the other
-  // and so do the parts in the merge, an eighth of a tile's time each, so n tiles in parts of p take about
-  // p + n / (8 p), least at p = sqrt(n / 8); up to four tiles a second launch costs more than it saves. us with parts
-  // of eight or more / with these: 100 new tokens behind 2,000 at head dim 128 18.6 / 15.0, two rows of 100 behind 900
-  // at head dim 64 15.3 / 10.1, 3 tokens behind 500 at head dim 512 27.1 / 15.7; 96 query rows of 8,000 keys at head dim
-  // 256 25.3 / 24.7 (twice as many a part 25.0). One of the long tiles in fp32: 100 tokens 14 us, not 35.
-  int64_t least = 8;
+  // The least tiles of a part. Split kernel: two for each wave, one of the long ones from 512 bytes a key on (us, two /
+  // one: 32 rows of 1,500 keys at head dim 256 15.7 / 14.1, 2 rows of 800 at head dim 512 19.2 / 16.3, but one of 8,000 at
+  // 128 14.2 / 15.8). Chunk kernel: a part's tiles run one after the other and so do the parts in the merge, an eighth of
+  // a tile's time each, so n tiles in parts of p take about p + n / (8 p), least at p = sqrt(n / 8); up to four tiles a
+  // second launch costs more than it saves. us with parts of eight or more / with these: 100 new tokens behind 2,000 at
+  // head dim 128 18.6 / 15.0, two rows of 100 behind 900 at head dim 64 15.3 / 10.1; 96 query rows of 8,000 keys at head
+  // dim 256 25.3 / 24.7 (twice as many a part 25.0). One of the long tiles in fp32.
+  int64_t least = es * D >= 512 ? 4 : 8;
   if (plan.chunk) {
     least = 1;
     while (es == 2 && least * least * 8 < tiles) ++least;
@@ -170,9 +182,15 @@ extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int 
   if (B <= 0 || T <= 0 || H <= 0 || K <= 0 || H % K || !paged_dim_ok(dtype, D) || max_kv_len <= 0 || window < 0 ||
       sinks < 0 || max_kv_len > INT_MAX)
     return 0;
-  // (calls with and without row positions may be cut differently: what either needs)
-  const size_t a = paged_ws(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, true, true), B, T, H, K, D).bytes;
-  const size_t b = paged_ws(paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, false, true), B, T, H, K, D).bytes;
+  const auto bytes = [&](bool ragged, bool* planned) {
+    const PagedPlan plan = paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, ragged, true);
+    *planned = plan.planned;
+    return paged_ws(plan, B, T, H, K, D).bytes;
+  };
+  bool planned;
+  const size_t a = bytes(true, &planned);
+  if (!planned) return a;
+  const size_t b = bytes(false, &planned);  // (without row positions nothing is planned: what either needs)
   return a > b ? a : b;
 }
 

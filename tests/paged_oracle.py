@@ -37,7 +37,8 @@ def attend64(q, k, v, see, scale):
       - a weight exp2(c s - m): s is a sum of D products (error at most (D + 2) u a, u = 2^-24, a = scale sum |q k|), the
         exponent one fma (u |x|), exp2 a few steps: relative error e = 2 (D + 4) u a + 8 u, and the quotient has it twice;
       - sums of n weights and products: n u each, twice;
-      - 16-bit weights for the second product: half a step of the type, h; in fp16 2^-25 more per key below its range."""
+      - 16-bit weights for the second product: half a step of the type, h (also where the sum takes the rounded
+        weights: the error is then sum w d (v - out), |d| <= h, and sum w |v - out| is at most the largest |v|); in fp16 2^-25 more per key below its range."""
     H, T, D = q.shape
     G = H // k.shape[0]
     keep = see.any(0)

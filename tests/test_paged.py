@@ -585,11 +585,75 @@ def test_empty_calls():
         assert ops.attn_sinks(q, c, c, scale=0.1, window=4, sinks=1, pos=0).shape == (B, T, 8, 64)
 
 
+# How a call is cut follows from what its table can hold, so tables far wider than the rows send small calls, in
+# every form above, to the kernel of large chunks: cut on the host (4,000 keys), or planned on the device (200,000)
+@pytest.fixture(params=[4000, 200000])
+def wide_tables(request, monkeypatch):
+    plain = Paged.__init__
+
+    def widened(self, *args, **kw):
+        plain(self, *args, **kw)
+        page = self.kp.shape[2]
+        self.table = torch.nn.functional.pad(self.table, (0, request.param // page - self.table.shape[1]), value=-1)
+
+    monkeypatch.setattr(Paged, "__init__", widened)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [c for c in CASES if c[6] > 1], ids=_id)
+def test_chunks_with_wide_tables(wide_tables, case):
+    got, want, bound = _run_paged(*case)
+    assert_close(got, want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["norm", "rope", "both"])
+@pytest.mark.parametrize("dtype,H,K,D,T", [(BF, 16, 8, 128, 80), (HF, 8, 4, 256, 40), (BF, 16, 1, 512, 12), (BF, 12, 4, 64, 70),
+                                           (SF, 16, 8, 128, 40), (SF, 8, 1, 256, 12), (SF, 12, 4, 64, 30)])
+def test_fused_q_with_wide_tables(wide_tables, dtype, H, K, D, T, what):
+    test_fused_q(dtype, H, K, D, T, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64])
+def test_pages_with_wide_tables(wide_tables, page):
+    for T in (90, 300):
+        test_entries_outside_the_pool_are_invisible(T, -1, page)
+    test_a_row_without_any_page_is_zero()
+    test_rows_may_share_pages(70)
+    test_missing_pages_at_head_dim_512(32)
+    test_strided_and_unaligned_inputs(100)
+    test_large_scores_and_infinite_keys_out_of_sight()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # long enough for the kernel of large chunks with the caches' own lengths
+    (BF, 16, 8, 128, 64, [2500, 300], 200, None, 0, 0), (HF, 12, 4, 64, 16, [1500], 700, None, 0, 0),
+    (BF, 8, 4, 256, 32, [900, 30], 300, [300, 299], 0, 0), (SF, 16, 8, 128, 64, [700], 260, None, 0, 0),
+    (SF, 8, 4, 64, 16, [300, 900, 0], 400, [400, 1, 77], 256, 33), (BF, 28, 4, 128, 16, [1000, 90], 200, None, 300, 20),
+    (HF, 16, 1, 512, 32, [600], 150, None, 0, 0), (SF, 8, 1, 256, 16, [1200], 90, None, 0, 0)], ids=_id)
+def test_longer_chunks(case):
+    got, want, bound = _run_paged(*case)
+    assert_close(got, want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    (HF, 12, 4, 64, [0], 2000, 300, 4, "pos"), (BF, 16, 8, 128, [0], 900, 100, 64, "pos"),
+    (BF, 16, 8, 128, [500], 700, 129, 1, "dev"), (BF, 8, 4, 256, [40, 40], 500, 70, 9, "pos"), (SF, 8, 4, 64, [0], 1100, 200, 3, "pos"),
+    (BF, 16, 1, 512, [0], 220, 250, 3, "pos"), (BF, 16, 16, 64, [100, 900], 400, 5000, 10, "rows"), (BF, 28, 4, 128, [7, 300], 300, 64, 17, "rows")],
+    ids=_id)
+def test_longer_windows(case):
+    test_attn_sinks(case)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("window,sinks", [(0, 0), (900, 70)])
 def test_planned_chunks_at_head_dim_512(window, sinks):
     """A large call whose rows differ, its parts planned on the device (with a window: too few tiles, not planned)."""
-    _run_paged(BF, 16, 1, 512, 32, [2700, 40, 1500], 130, [130, 128, 0] if window else None, window, sinks)
+    got, want, bound = _run_paged(BF, 16, 1, 512, 32, [2700, 40, 1500], 130, [130, 128, 0] if window else None, window, sinks)
+    assert_close(got, want, bound)
 
 
 @pytest.mark.gpu
