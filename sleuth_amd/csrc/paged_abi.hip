@@ -1,6 +1,7 @@
 // Entry points of the paged cache and of attention with sinks (kernels: paged.hip): argument checks, the
 // cut of a call into blocks, the launch.
 #include <limits.h>
+#include <math.h>
 
 #include "paged.h"
 
@@ -72,23 +73,27 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     plan.nitems = (int)(plan.slots / K + blocks);
     return plan;
   }
-  // The least tiles of a part. Split kernel: two for each wave, one of the long ones from 512 bytes a key on (us, two /
-  // one: 32 rows of 1,500 keys at head dim 256 15.7 / 14.1, 2 rows of 800 at head dim 512 19.2 / 16.3, but one of 8,000 at
-  // 128 14.2 / 15.8). Chunk kernel: a part's tiles run one after the other and so do the parts in the merge, an eighth of
-  // a tile's time each, so n tiles in parts of p take about p + n / (8 p), least at p = sqrt(n / 8); up to four tiles a
-  // second launch costs more than it saves. us with parts of eight or more / with these: 100 new tokens behind 2,000 at
-  // head dim 128 18.6 / 15.0, two rows of 100 behind 900 at head dim 64 15.3 / 10.1; 96 query rows of 8,000 keys at head
-  // dim 256 25.3 / 24.7 (twice as many a part 25.0). One of the long tiles in fp32.
-  int64_t least = es * D >= 512 ? 4 : 8;
+  // Parts that are on the device together: one more would wait for a whole part of the others (us, with parts rounded
+  // up / down: 1,548 tokens, window 882, 32 q / 8 KV heads 52.0 / 32.2; 56 at head dim 512 28.3 / 14.3).
+  const int64_t fit = slots / units < 1 ? 1 : slots / units;
+  int64_t per = (tiles + fit - 1) / fit;
   if (plan.chunk) {
-    least = 1;
-    while (es == 2 && least * least * 8 < tiles) ++least;
-    if (es == 2 && tiles <= 4) least = tiles;
+    // n tiles in p parts take n / p of a tile's time, then the merge: p of its steps one after the other, the partials
+    // of all units, and a launch; in 16 bits about p (4 + units) / 64 + 3 tiles' time, an eighth of the long ones' in
+    // fp32. us, eight tiles at least / so: 100 new tokens behind 2,000 at head dim 128 18.6 / 15.1, 234 behind 319 at 256
+    // 22.7 / 20.1, 788 with a window of 256 24.3 / 22.6; at 7 rows of 432 (window 256) two parts 31.5, one 17.2.
+    const int64_t tile = es == 4 ? 512 : 64;
+    int64_t p = (int64_t)sqrt((double)(tile * tiles) / (double)(4 + units));
+    p = p < 1 ? 1 : p < fit ? p : fit;
+    const int64_t n = (tiles + p - 1) / p;
+    per = n * tile + p * (4 + units) + 192 < tiles * tile ? n : tiles;
+  } else {
+    // two tiles at least for each wave, one of the long ones from 512 bytes a key on (us, two / one: 32 rows of 1,500 keys
+    // at head dim 256 15.7 / 14.1, 2 rows of 800 at head dim 512 19.2 / 16.3, but one of 8,000 at 128 14.2 / 15.8)
+    const int64_t least = es * D >= 512 ? 4 : 8, most = (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
+    if (per > most) per = most;
+    if (per < least) per = least;
   }
-  const int64_t most = plan.chunk ? 1 << 20 : (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
-  int64_t per = (units * tiles + slots - 1) / slots;
-  if (per > most) per = most;
-  if (per < least) per = least;
   int64_t parts = (tiles + per - 1) / per;
   if (parts > 65535) parts = 65535;  // (the grid's)
   if (parts > 1) {
