@@ -40,8 +40,8 @@ template <typename T, int D> struct ChunkTile {
 };
 // Chunk swizzles by key row: as prefill_tile.h's in 16 bits; in fp32 a V read is 32 channels of two rows 4 apart.
 template <typename T, int D> __device__ __forceinline__ int chunk_swz_k(int row) {
-  constexpr int NCH = ChunkTile<T, D>::NCH;
-  return row & ((NCH >= 16 ? 16 : NCH) - 1);
+  constexpr int NCH = ChunkTile<T, D>::NCH, RP = NCH >= 16 ? 1 : 16 / NCH;  // key rows per 256-byte bank line
+  return (row / RP) & ((NCH >= 16 ? 16 : NCH) - 1);
 }
 template <typename T, int D> __device__ __forceinline__ int chunk_swz_v(int row) {
   if constexpr (sizeof(T) == 2) return swz_v<D>(row);
