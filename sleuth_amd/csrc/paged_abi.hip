@@ -49,7 +49,10 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   // tiles for each block that the device holds. us, split / chunk: 256 new tokens at head dim 256 12.1 / 16.7 (4 tiles
   // each), 12 behind 8,000 22.2 / 24.6 (5.9), 60 behind 300 at head dim 512 21.2 / 26.7 (5.6); four rows of 48 behind 500
   // at head dim 256 23.9 / 17.4 (6.8), 100 fp32 tokens behind 500 26.0 / 21.3 (7.7).
-  if (work > 6 * round && rows > (es == 4 ? 64 : D == 512 ? 16 : 32) && D >= 64) {
+  // Head dim 32 in 16 bits, four split blocks a CU, from 60 tiles each on: 6 rows of 3,898 tokens, window 897, 62.5 /
+  // 44.3, 500 tokens behind 8,000 24.2 / 20.1; four prompts of 700 (30 tiles) 8.7 / 13.5.
+  const bool rows_enough = rows > (es == 4 ? 64 : D == 512 ? 16 : 32);
+  if (rows_enough && (D >= 64 ? work > 6 * round : es == 2 && work > 60 * round)) {
     plan.chunk = true;
     plan.rows = 128;
     plan.keys = es * D >= 512 ? 32 : 64;

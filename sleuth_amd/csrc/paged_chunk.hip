@@ -1,5 +1,5 @@
 // Chunks of many query rows over a paged cache, or over a contiguous one with a window and first tokens:
-// bf16/fp16, head dims 64 to 512, on v_mfma_f32_32x32x16, and fp32, head dims 64 to 256, on v_mfma_f32_32x32x2
+// bf16/fp16, head dims 32 to 512, on v_mfma_f32_32x32x16, and fp32, head dims 64 to 256, on v_mfma_f32_32x32x2
 // (the split kernel of paged.hip serves the rest).
 //
 // A block of 4 waves (8 at head dim 512) owns 128 query rows of one (batch row, KV head) -- row r is token r / G, head r % G of the
@@ -44,7 +44,7 @@ template <typename T, int D> __device__ __forceinline__ int chunk_swz_k(int row)
   return (row / RP) & ((NCH >= 16 ? 16 : NCH) - 1);
 }
 template <typename T, int D> __device__ __forceinline__ int chunk_swz_v(int row) {
-  if constexpr (sizeof(T) == 2) return swz_v<D>(row);
+  if constexpr (sizeof(T) == 2) return D == 32 ? 0 : swz_v<D>(row);
   else return ((row >> 2) & 1) << 3;
 }
 
@@ -599,6 +599,9 @@ template <typename T, int D> static int launch_chunk_d(PagedParams p, const Page
 
 template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
   switch (D) {
+    case 32:
+      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 32>(p, plan, s);
+      break;
     case 64: return launch_chunk_d<T, 64>(p, plan, s);
     case 128: return launch_chunk_d<T, 128>(p, plan, s);
     case 256: return launch_chunk_d<T, 256>(p, plan, s);

@@ -84,6 +84,8 @@ CASES = [
     (BF, 16, 1, 512, 64, [500, 30], 9, None, 100, 9),
     (HF, 16, 1, 512, 128, [700, 3, 90], 33, [1, 33, 0], 20, 64),
     (BF, 4, 2, 512, 32, [15, 16, 31], 140, None, 0, 0),
+    (BF, 8, 4, 32, 32, [40, 7], 90, [90, 33], 0, 0),
+    (HF, 8, 4, 32, 16, [300], 150, None, 60, 5),
 ]
 
 
@@ -608,7 +610,7 @@ def test_chunks_with_wide_tables(wide_tables, case):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("what", ["norm", "rope", "both"])
-@pytest.mark.parametrize("dtype,H,K,D,T", [(BF, 16, 8, 128, 80), (HF, 8, 4, 256, 40), (BF, 16, 1, 512, 12), (BF, 12, 4, 64, 70),
+@pytest.mark.parametrize("dtype,H,K,D,T", [(BF, 16, 8, 128, 80), (HF, 8, 4, 256, 40), (BF, 16, 1, 512, 12), (BF, 12, 4, 64, 70), (HF, 8, 4, 32, 60),
                                            (SF, 16, 8, 128, 40), (SF, 8, 1, 256, 12), (SF, 12, 4, 64, 30)])
 def test_fused_q_with_wide_tables(wide_tables, dtype, H, K, D, T, what):
     test_fused_q(dtype, H, K, D, T, what)
@@ -642,7 +644,8 @@ def test_longer_chunks(case):
 @pytest.mark.parametrize("case", [
     (HF, 12, 4, 64, [0], 2000, 300, 4, "pos"), (BF, 16, 8, 128, [0], 900, 100, 64, "pos"),
     (BF, 16, 8, 128, [500], 700, 129, 1, "dev"), (BF, 8, 4, 256, [40, 40], 500, 70, 9, "pos"), (SF, 8, 4, 64, [0], 1100, 200, 3, "pos"),
-    (BF, 16, 1, 512, [0], 220, 250, 3, "pos"), (BF, 16, 16, 64, [100, 900], 400, 5000, 10, "rows"), (BF, 28, 4, 128, [7, 300], 300, 64, 17, "rows")],
+    (BF, 16, 1, 512, [0], 220, 250, 3, "pos"), (BF, 16, 16, 64, [100, 900], 400, 5000, 10, "rows"), (BF, 28, 4, 128, [7, 300], 300, 64, 17, "rows"),
+    (HF, 8, 4, 32, [5], 3001, 1400, 7, "pos")],
     ids=_id)
 def test_longer_windows(case):
     test_attn_sinks(case)
