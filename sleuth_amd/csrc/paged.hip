@@ -75,6 +75,11 @@ template <bool MAX> __device__ __forceinline__ float over_groups(float x) {
 // key tiles. Each wave streams tiles of its own (tile i goes to wave i % 4) through registers into LDS
 // that only it uses, so no wave waits for another until the end: the tile in registers is the prefetch
 // of the next one. The waves' (m, l, O) meet in LDS once, at the end.
+//
+// Bound by the keys' bytes where there are many, 710 us (6.5 TB/s) for one token of 64 rows of 1,024 to 32,767 keys, 8 KV
+// heads of 128 in bf16, as fast as a streaming read; by latency where there are few, 7 us for one row of 212 keys:
+// position, page, keys, a tile or two a wave and the merge follow one another. 16 rows a block leave the matrix units
+// half empty at a step, but nothing waits for them; a second register tile in flight per wave gained nothing.
 template <typename T, int D, int RB> struct StepTile {
   static_assert(16 * RB <= step_rows_most(sizeof(T), D), "registers");
   static constexpr int ROWB = D * (int)sizeof(T);        // bytes of a key row
