@@ -110,9 +110,23 @@ struct RowSpan {
   int base;         // position of the row's first new token
   int rows;         // query rows of the batch row that are real
   int first, last;  // positions of the block's first and last real query
+  int lo, se;       // what the block's queries see: keys below se (first tokens) and those from lo to last
   int sink_tiles, main_tile, tiles;
   __device__ __forceinline__ int tile_key(int i, int KT) const {
     return (i < sink_tiles ? i : main_tile + i - sink_tiles) * KT;
+  }
+  // A tile's ends may hold keys that no query of the block sees: past the last one, between the first tokens and the
+  // window. Their weights are 0, but 0 * NaN of such a value would be NaN, so rows of keys that are seen are read in
+  // their place (and a page behind the window costs no traffic). Of R keys from `group` on (a multiple of R) in the
+  // tile that starts at key0: where the R keys to read start, and the key to read for `key` among those.
+  template <int R> __device__ __forceinline__ int group_from(int group, int key0) const {
+    if (group > last) return last & ~(R - 1);
+    if (group >= se && group + R <= lo) return (key0 < se ? se - 1 : lo) & ~(R - 1);
+    return group;
+  }
+  __device__ __forceinline__ int row_key(int from, int key) const {
+    key = key < last ? key : last;
+    return key >= se && key < lo ? (from < se ? se - 1 : lo) : key;
   }
 };
 
@@ -121,15 +135,15 @@ __device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int
   w.base = base;
   w.rows = rows;
   w.sink_tiles = w.main_tile = w.tiles = 0;
-  w.first = w.last = 0;
+  w.first = w.last = w.lo = w.se = 0;
   if (row0 >= rows) return w;
   const int row1 = (row0 + nrows < rows ? row0 + nrows : rows) - 1;
   w.first = base + p.token(row0);
   w.last = base + p.token(row1);
-  const int lo = p.window > 0 && w.first >= p.window ? w.first - p.window + 1 : 0;
-  w.main_tile = lo / KT;
-  const int se = p.sinks < lo ? p.sinks : lo;
-  const int st = (se + KT - 1) / KT;
+  w.lo = p.window > 0 && w.first >= p.window ? w.first - p.window + 1 : 0;
+  w.main_tile = w.lo / KT;
+  w.se = p.sinks < w.lo ? p.sinks : w.lo;
+  const int st = (w.se + KT - 1) / KT;
   w.sink_tiles = st < w.main_tile ? st : w.main_tile;
   w.tiles = w.sink_tiles + w.last / KT - w.main_tile + 1;
   return w;

@@ -214,45 +214,38 @@ void paged_step_kernel(PagedParams p) {
   unsigned bad = 0;  // bit i: 16-key group i of the tile in kr/vr lies in no page of the pool
   auto load = [&](int i) {
     const int key0 = w.tile_key(i, KT);
-    const int left = w.last - key0;  // the tile's last row that exists
+    const bool edge = w.last - key0 < KT - 1 || key0 < w.lo;  // rows of it stand for keys that no query sees
     unsigned miss = 0;
+    int from[GROUPS];
     int64_t base[GROUPS];
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) {
-      // (a group past the row's last key reads that key instead)
-      const int key = key0 + (16 * j <= left ? 16 * j : left & ~15);
-      const int page = p.page_of(b, key);
+      from[j] = edge ? w.group_from<16>(key0 + 16 * j, key0) : key0 + 16 * j;
+      const int page = p.page_of(b, from[j]);
       if (page < 0) miss |= 1u << j;
-      base[j] = page * pageb + (int64_t)(key & p.page_mask) * rowb;
+      base[j] = page * pageb + (int64_t)(from[j] & p.page_mask) * rowb;
     }
     if (miss == 0) {
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
+        const int in = j * TL::RPI / 16;   // the load's group
         int row = j * TL::RPI % 16 + lrow;
-        if (left < KT - 1) {
-          const int in = j * TL::RPI / 16 * 16;   // the group's first row
-          const int most = in <= left ? left - in : left & 15;
-          row = row < most ? row : most;
-        }
+        if (edge) row = w.row_key(from[in], from[in] + row) - from[in];
         const unsigned off = (unsigned)(row * rowb + lch * 16);
-        const int64_t at = base[j * TL::RPI / 16];
-        kr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb0 + at + off));
-        vr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vb0 + at + off));
+        kr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb0 + base[in] + off));
+        vr[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vb0 + base[in] + off));
       }
     } else {
 #pragma unroll
       for (int j = 0; j < NL; ++j) {
-        int row = j * TL::RPI % 16 + lrow;
-        const int in = j * TL::RPI / 16 * 16;
-        const int most = in <= left ? left - in : left & 15;
-        row = row < most ? row : most;
+        const int in = j * TL::RPI / 16;
+        const int row = w.row_key(from[in], from[in] + j * TL::RPI % 16 + lrow) - from[in];
         const unsigned off = (unsigned)(row * rowb + lch * 16);
-        const int64_t at = base[j * TL::RPI / 16];
         kr[j] = u32x4{0, 0, 0, 0};
         vr[j] = u32x4{0, 0, 0, 0};
-        if (!(miss >> (j * TL::RPI / 16) & 1)) {
-          kr[j] = *reinterpret_cast<const u32x4*>(kb0 + at + off);
-          vr[j] = *reinterpret_cast<const u32x4*>(vb0 + at + off);
+        if (!(miss >> in & 1)) {
+          kr[j] = *reinterpret_cast<const u32x4*>(kb0 + base[in] + off);
+          vr[j] = *reinterpret_cast<const u32x4*>(vb0 + base[in] + off);
         }
       }
     }

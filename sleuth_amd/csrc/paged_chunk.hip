@@ -201,10 +201,10 @@ void paged_chunk_kernel(PagedParams p) {
   // that a page holds) and the sums take the LDS, bits that every wave looks up itself.
   int flagged[2] = {0, 0};   // what this wave's flag of each stage holds, or the stage's bits
   if (HALVES == 1 && lane < 2) flags[4 * lane + wave] = 0;
-  // first row of the wave's part of tile i; where the row's keys end before it, of the part that holds the last key
+  // first row of the wave's part of tile i, or of the part that stands for it where no query sees its keys
   auto part_key = [&](int i) {
-    const int key0 = w.tile_key(i, BN), left = w.last - key0;
-    return key0 + (wr0 <= left ? wr0 : left & ~(RW - 1));
+    const int key0 = w.tile_key(i, BN);
+    return w.group_from<RW>(key0 + wr0, key0);
   };
   unsigned groups = 0;  // (two halves) bit j: group j of the tile that `page` belongs to has no page
   auto page_at = [&](int i) {
@@ -236,12 +236,12 @@ void paged_chunk_kernel(PagedParams p) {
     }
     const int key = part_key(i);
     const int64_t at = page * pageb + (int64_t)(key & p.page_mask) * rowb;
-    const int most = w.last - key;  // rows of the part past it re-read it (masked)
+    const bool edge = w.last - key < RW - 1 || w.tile_key(i, BN) < w.lo;  // rows of it may stand for others (masked)
     const char* ks = kgb + at;
     const char* vs = vgb + at;
     int lk = ld_k, lv = ld_v;
     if constexpr (!KEEP) asm volatile("" : "+v"(lk), "+v"(lv));  // (not kept over the loop)
-    if (most >= RW - 1) {
+    if (!edge) {
 #pragma unroll
       for (int x = 0; x < TL::LOADS; ++x) {
         if constexpr (KEEP) {
@@ -257,7 +257,7 @@ void paged_chunk_kernel(PagedParams p) {
     } else {
 #pragma unroll
       for (int x = 0; x < TL::LOADS; ++x) {
-        const int in = RL * x + ld_row, row = in < most ? in : most;
+        const int in = RL * x + ld_row, row = w.row_key(key, key + in) - key;
         lds_dma16(ks, (unsigned)(row * rowb + ((pch ^ chunk_swz_k<T, D>(wr0 + in)) << 4)), kdst + x * 1024);
         lds_dma16(vs, (unsigned)(row * rowb + ((pch ^ chunk_swz_v<T, D>(wr0 + in)) << 4)), vdst + x * 1024);
       }

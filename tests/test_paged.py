@@ -855,3 +855,44 @@ def test_threads_on_one_stream():
     [t.join() for t in threads]
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for i in range(4) for o in outs[i])
+
+
+# ---------------------------------------------------------------- keys that no query sees
+HIDDEN = [
+    # (dtype, H, K, D, page, pasts, T, window, sinks): steps, 32-row blocks, chunks; the window starts in the tile of
+    # the first tokens (70, 75), or far behind it
+    (BF, 16, 8, 128, 16, [700, 75, 70], 1, 64, 4), (HF, 12, 4, 64, 64, [300, 90], 5, 50, 20), (SF, 8, 4, 32, 16, [200, 40], 3, 33, 2),
+    (BF, 8, 1, 256, 32, [333], 4, 100, 33), (BF, 16, 1, 512, 16, [150, 77], 1, 48, 3), (BF, 16, 8, 128, 16, [700], 1, 1, 0),
+    (HF, 8, 4, 32, 64, [900], 1500, 700, 4), (BF, 16, 8, 128, 64, [500], 900, 100, 40), (HF, 12, 4, 64, 16, [777], 2000, 300, 4),
+    (BF, 8, 4, 256, 32, [400, 90], 500, 70, 9), (SF, 8, 4, 64, 16, [333], 1100, 200, 3), (BF, 16, 1, 512, 32, [600], 220, 250, 3),
+    (HF, 8, 4, 32, 16, [1500], 3001, 1400, 7), (BF, 16, 16, 64, 128, [900], 700, 129, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+@pytest.mark.parametrize("case", HIDDEN, ids=_id)
+def test_keys_that_no_query_sees_are_never_used(case, fill):
+    """Between the first tokens and the window, on pages that are held: NaN or Inf in K and V reach no output, over
+    pages and over the contiguous cache."""
+    dtype, H, K, D, page, pasts, T, window, sinks = case
+    g = gen(31)
+    B = len(pasts)
+    cache = Paged(g, [p + T for p in pasts], K, D, page, dtype)
+    cap = max(cache.lens) + 5
+    kc, vc = (torch.full((B, K, cap, D), math.nan, dtype=dtype) for _ in range(2))
+    for b, n in enumerate(cache.lens):
+        hidden = slice(min(sinks, pasts[b]), max(sinks, pasts[b] - window + 1))
+        assert hidden.stop > hidden.start
+        cache.k[b][:, hidden], cache.v[b][:, hidden] = fill, fill
+        kc[b, :, :n], vc[b, :, :n] = cache.k[b], cache.v[b]
+        for j in range(-(-n // page)):
+            lo, hi = j * page, min(n, (j + 1) * page)
+            cache.kp[cache.table[b, j], :, :hi - lo] = cache.k[b][:, lo:hi]
+            cache.vp[cache.table[b, j], :, :hi - lo] = cache.v[b][:, lo:hi]
+    q = torch.randn(B, T, H, D, generator=g).to(dtype).transpose(1, 2)
+    want, bound = cache.want(q, pasts, [T] * B, window, sinks, D ** -0.5)
+    kw = dict(scale=D ** -0.5, window=window, sinks=sinks)
+    assert_close(ops.attn_paged(q.cuda(), cache.kp.cuda(), cache.vp.cuda(), cache.table.cuda(), i32(pasts), **kw), want, bound,
+                 "pages")
+    assert_close(ops.attn_sinks(q.cuda(), kc.cuda(), vc.cuda(), row_pos=i32(pasts), **kw), want, bound, "contiguous")
