@@ -305,6 +305,7 @@ int forge_kv_append_paged(int dtype, int B, int T, int K, int D, const void* k, 
  * FORGE_NORM_QK / FORGE_ROPE). max_kv_len: host upper bound on row_pos[b] + new_lens[b] (at most
  * max_pages * page_size; positions from it on do not exist for the call). Rows t >= new_lens[b], and
  * rows that see no key, come out as zeros.
+ * scale must be positive and finite.
  * workspace: forge_attn_paged_workspace_bytes(...) bytes (256-byte aligned) of fp32 partials, where the
  * keys of a row are split over blocks; NULL: not split. Calls that may overlap need separate ones.
  * ws_flags = FORGE_WS_ZEROED promises that its first FORGE_PAGED_COUNTER_BYTES bytes hold zero: small merges

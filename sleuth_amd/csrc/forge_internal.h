@@ -15,4 +15,12 @@ int check_launch();
 // CUs of the current device (256 where no device answers, e.g. a host-only build check).
 int device_cus();
 
+
+// A softmax scale of the kernels that mask raw scores with -inf and scale them in the exponent's fma: times 0 or a
+// negative number, or a scale that is not finite, the masked ones would come out as NaN or +inf.
+inline bool scale_ok(float scale) {
+  const float c = scale * 1.4426950408889634f;
+  return c >= 1.17549435e-38f && c <= 3.4e38f;
+}
+
 }  // namespace forge

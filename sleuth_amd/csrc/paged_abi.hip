@@ -137,6 +137,7 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   if (p.window < 0 || p.sinks < 0 || p.window > INT_MAX / 2 || p.sinks > INT_MAX / 2)
     return set_error("window and sinks must not be negative");
   if (p.sinks > 0 && p.window == 0) return set_error("sinks need a window (without one every key is visible)");
+  if (!scale_ok(scale)) return set_error("scale must be positive and finite");
   const int64_t es = dtype == FORGE_F32 ? 4 : 2, e16 = 16 / es;
   for (const int64_t st : {p.sqb, p.sqh, p.sqt, p.skp, p.skh, p.sks, p.sob, p.soh, p.sot})
     if (st < 0 || st % e16) return set_error("strides must be multiples of 16 bytes");

@@ -642,8 +642,10 @@ def paged_supported(dtype: torch.dtype, D: int) -> bool:
     return dtype in _DTYPES and (D in (32, 64, 128, 256) or (D == 512 and dtype != torch.float32))
 
 
-def _new_token_args(q, cache, q_weight, eps, norm_q, cos, sin, window, sinks, out):
+def _new_token_args(q, cache, scale, q_weight, eps, norm_q, cos, sin, window, sinks, out):
     """Checks what attn_paged and attn_sinks share; (q, C arguments from dtype to s_cos_t, out)."""
+    if not 1e-37 <= float(scale) <= 1e38:
+        raise ValueError(f"scale must be positive and finite, not {scale}")
     if q.dim() != 4 or q.shape[1] % cache.shape[1] or q.shape[3] != cache.shape[3]:
         raise ValueError(f"q {tuple(q.shape)} does not fit the cache {tuple(cache.shape)}")
     B, H, T, D = q.shape
@@ -697,7 +699,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     max_kv_len = most if max_kv_len is None else min(int(max_kv_len), most)
     if max_kv_len < 1:
         raise ValueError("max_kv_len must be positive")
-    keep, args, out = _new_token_args(q, k_pages, q_weight, eps, norm_q, cos, sin, window, sinks, out)
+    keep, args, out = _new_token_args(q, k_pages, scale, q_weight, eps, norm_q, cos, sin, window, sinks, out)
     with _guard(dev):
         ws = _PagedPartials(dev, lib().forge_attn_paged_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
         st = lib().forge_attn_paged(*args, _ptr(k_pages), _ptr(v_pages), *_strides3(k_pages), k_pages.shape[0], size,
@@ -743,7 +745,7 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
             max_kv_len = 1
         else:
             raise ValueError("max_kv_len must be positive")
-    keep, args, out = _new_token_args(q, k_cache, q_weight, eps, norm_q, cos, sin, window, sinks, out)
+    keep, args, out = _new_token_args(q, k_cache, scale, q_weight, eps, norm_q, cos, sin, window, sinks, out)
     with _guard(dev):
         ws = _PagedPartials(dev, lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
         st = lib().forge_attn_sinks(*args, _ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache), max_len, _ptr(rp), _ptr(pd),

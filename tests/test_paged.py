@@ -896,3 +896,26 @@ def test_keys_that_no_query_sees_are_never_used(case, fill):
     assert_close(ops.attn_paged(q.cuda(), cache.kp.cuda(), cache.vp.cuda(), cache.table.cuda(), i32(pasts), **kw), want, bound,
                  "pages")
     assert_close(ops.attn_sinks(q.cuda(), kc.cuda(), vc.cuda(), row_pos=i32(pasts), **kw), want, bound, "contiguous")
+
+
+# ---------------------------------------------------------------- scales
+BAD_SCALES = [0.0, -0.0, -0.125, math.nan, math.inf, -math.inf, 1e-300, 3e38]
+
+
+@pytest.mark.parametrize("scale", BAD_SCALES)
+def test_c_refuses_scales_that_are_not_positive(scale):
+    """A masked score is -inf before it is scaled: -inf times 0 is NaN, times a negative number +inf."""
+    assert _paged_call(scale=scale) < 0 and "scale" in _lib.lib().forge_last_error().decode()
+    base = [_lib.BF16, 2, 1, 8, 4, 64, _P, 512, 64, 512, None, 1e-6, 0, None, None, 0, 0, _P, _P, 8192, 2048, 64, 32, _P, None,
+            0, 32, 8, 2, scale, _P, 512, 512, 64, None, 0, 0, None]
+    assert _lib.lib().forge_attn_sinks(*base) < 0 and "scale" in _lib.lib().forge_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", BAD_SCALES)
+def test_ops_refuse_scales_that_are_not_positive(scale):
+    q, kp = torch.zeros(2, 8, 1, 64, dtype=BF, device="cuda"), torch.zeros(4, 4, 16, 64, dtype=BF, device="cuda")
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_paged(q, kp, kp, torch.zeros(2, 2, dtype=torch.int32, device="cuda"), i32([0, 0]), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_sinks(q, kp[:2], kp[:2], scale=scale, window=4, sinks=1, pos=0)
