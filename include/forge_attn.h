@@ -194,7 +194,8 @@ size_t forge_attn_decode_workspace_bytes(int dtype, int B, int T, int H, int K, 
  * Queries are at positions offset .. offset+T-1; k/v [B,K,offset+T,D] (normally the
  * cache, already normalised by forge_kv_append) with strides (skb, skh, sks).
  * q is raw when flags has FORGE_NORM_QK / FORGE_ROPE: norm + RoPE run in the Q tile load.
- * Supports D in {64, 128, 256}; returns < 0 for other shapes (use forge_attn_decode).
+ * Supports D in {64, 128, 256}; returns < 0 for other shapes (use forge_attn_decode). scale must be
+ * positive and finite.
  */
 int forge_attn_prefill(int dtype, int B, int T, int H, int K, int D, const void* q,
                        int64_t sqb, int64_t sqh, int64_t sqt, const float* q_weight,

@@ -1556,6 +1556,7 @@ static int prefill_call(int dtype, int B, int T, int H, int K, int D, const void
   int st = prefill_setup(p, 2, B, T, H, K, q, sqb, sqh, sqt, q_weight, eps, flags, cos, sin, s_cos_t, k, v, skb,
                          skh, sks, offset, window, scale, out, sob, sot, soh);
   if (st) return st;
+  if (!scale_ok(scale)) return set_error("forge_attn_prefill: scale must be positive and finite");
   p.doc_lo = doc_lo;
   p.sdb = sdb;
   st = prefill_bind(p, prefill_plan(false, B, T, H, K, D, offset, window, workspace && !doc_lo ? kMaxParts : 1), D,

@@ -171,3 +171,12 @@ def test_positions_whose_end_wraps_are_rejected(at):
         assert st < 0 and b"31 bits" in lib.forge_last_error()
     assert lib.forge_attn_prefill_workspace_bytes(_lib.BF16, 1, 20, 4, 2, 64, at, 0) == 0
     assert lib.forge_attn_prefill_f32_workspace_bytes(1, 20, 4, 2, 64, at, 0) == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf"), 1e-300])
+def test_prefill_refuses_scales_that_are_not_positive(scale):
+    """The 16-bit kernels mask raw scores with -inf before the scale: 0 gave NaN, a negative one +inf."""
+    lib, p = _lib.lib(), 1 << 20
+    args = [_lib.BF16, 1, 20, 4, 2, 64, p, 0, 64, 256, None, 1e-6, 0, None, None, 0, p, p, 0, 64 * 64, 64, 0, 0, scale, p, 0, 256,
+            64, None]
+    assert lib.forge_attn_prefill(*args) < 0 and "scale" in lib.forge_last_error().decode()
