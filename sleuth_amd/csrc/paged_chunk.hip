@@ -201,20 +201,17 @@ void paged_chunk_kernel(PagedParams p) {
   // that a page holds) and the sums take the LDS, bits that every wave looks up itself.
   int flagged[2] = {0, 0};   // what this wave's flag of each stage holds, or the stage's bits
   if (HALVES == 1 && lane < 2) flags[4 * lane + wave] = 0;
-  // first row of the wave's part of tile i, or of the part that stands for it where no query sees its keys
-  auto part_key = [&](int i) {
-    const int key0 = w.tile_key(i, BN);
-    return w.group_from<RW>(key0 + wr0, key0);
-  };
+  int part_key = 0;     // first row of the wave's part of the tile that `page` belongs to, or of what stands for it
   unsigned groups = 0;  // (two halves) bit j: group j of the tile that `page` belongs to has no page
   auto page_at = [&](int i) {
-    if constexpr (HALVES == 1) return p.page_of(b, part_key(i));
     const int key0 = w.tile_key(i, BN), left = w.last - key0;
+    part_key = w.group_from<RW>(key0 + wr0, key0);
+    if constexpr (HALVES == 1) return p.page_of(b, part_key);
     const int p0 = p.page_of(b, key0), p1 = p.page_of(b, key0 + (left >= 16 ? 16 : 0));
     groups = (unsigned)(p0 < 0) | (unsigned)(p1 < 0) << 1;
-    return part_key(i) - key0 < 16 ? p0 : p1;
+    return part_key - key0 < 16 ? p0 : p1;
   };
-  auto issue = [&](int i, int stage, int page) {
+  auto issue = [&](int stage, int page) {
     const unsigned kdst = lds_offset(smem + (2 * stage) * TL::TILEB + wave * TL::LOADS * 1024);
     const unsigned vdst = kdst + TL::TILEB;
     const int miss = page < 0;
@@ -234,9 +231,9 @@ void paged_chunk_kernel(PagedParams p) {
       }
       return;
     }
-    const int key = part_key(i);
+    const int key = part_key;
     const int64_t at = page * pageb + (int64_t)(key & p.page_mask) * rowb;
-    const bool edge = w.last - key < RW - 1 || w.tile_key(i, BN) < w.lo;  // rows of it may stand for others (masked)
+    const bool edge = w.last - key < RW - 1 || (key < w.lo && key + RW > w.se);  // it holds keys that no query sees
     const char* ks = kgb + at;
     const char* vs = vgb + at;
     int lk = ld_k, lv = ld_v;
@@ -264,7 +261,7 @@ void paged_chunk_kernel(PagedParams p) {
     }
   };
   int page = page_at(begin);
-  issue(begin, 0, page);
+  issue(0, page);
   page = page_at(begin + 1 < end ? begin + 1 : begin);
 
   // ---- this lane's query row; the wave's span of positions
@@ -305,7 +302,7 @@ void paged_chunk_kernel(PagedParams p) {
     wait_vm<0>();
     __syncthreads();  // tile `it` is in LDS for every wave; the other stage is free
     if (it + 1 < end) {
-      issue(it + 1, stage ^ 1, page);
+      issue(stage ^ 1, page);
       page = page_at(it + 2 < end ? it + 2 : it + 1);
     }
     const int key0 = w.tile_key(it, BN);
