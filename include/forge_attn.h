@@ -333,7 +333,16 @@ int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q
  * The same attention over a contiguous cache [B, K, max_len, D] for sliding-window layers whose first
  * `sinks` positions stay visible (window > 0; sinks 0: the plain window). Positions as in
  * forge_attn_decode: row_pos, pos_dev or pos0. Any T: prompts, chunks, verify and decode steps.
+ *
+ * flags with FORGE_FIXED_CUT, for steps of T <= 16 tokens: a token's result is the same, bit for bit, in every
+ * such call of one batch size, head layout, max_len, window and sinks, whatever T, max_kv_len and the way the
+ * position is given, so a verify step's rows equal the decodes of its tokens. Its workspace:
+ * forge_attn_sinks_fixed_workspace_bytes (NULL: not split, in all of those calls or in none).
  */
+#define FORGE_FIXED_CUT 8
+#define FORGE_FIXED_CUT_MAX_T 16
+size_t forge_attn_sinks_fixed_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
+                                              int64_t max_len, int window, int sinks);
 size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
                                         int64_t max_kv_len, int window, int sinks);
 int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb,

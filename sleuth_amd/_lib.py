@@ -19,6 +19,7 @@ ABI_VERSION = 3
 F32, BF16, F16 = 0, 1, 2
 NOALLOC_SCRATCH_BYTES = 48 * 1024 * 1024   # FORGE_NOALLOC_SCRATCH_BYTES
 NORM_QK, ROPE, NORM_V = 1, 2, 4
+FIXED_CUT = 8                              # FORGE_FIXED_CUT
 WS_ZEROED = 1                              # FORGE_WS_ZEROED
 
 _p = C.c_void_p
@@ -158,6 +159,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
         _p]),
     "forge_attn_sinks_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
+    "forge_attn_sinks_fixed_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
     "forge_attn_sinks": (_i, [
         _i, _i, _i, _i, _i, _i,              # dtype, B, T, H, K, D
         _p, _i64, _i64, _i64,                # q + strides

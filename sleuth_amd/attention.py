@@ -429,15 +429,15 @@ class Attention(nn.Module):
                 else:
                     pos_kw, max_kv, offset = dict(pos=cache.pos), cache.pos + T, cache.pos
             # from the cache's capacity and T = 1: every step of this layer, decode or verify,
-            # splits its rows at the same keys
-            chunk = ops.decode_chunk(q.dtype, B, 1, H, self.n_kv, hd, cache.max_len, self.window,
+            # splits its rows at the same keys (attn_sinks: fixed_cut)
+            chunk = 0 if self.sinks else ops.decode_chunk(q.dtype, B, 1, H, self.n_kv, hd, cache.max_len, self.window,
                                      uniform="row_pos" not in pos_kw)
 
         if self.sinks:
             ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)
             self.last_path = "hip-sinks"
             return ops.attn_sinks(q, kc, vc, scale=self.scale, window=self.window, sinks=self.sinks, max_kv_len=max_kv,
-                                  **pos_kw, **q_args)
+                                  fixed_cut=cache is not None and T <= DECODE_MAX_T, **pos_kw, **q_args)
         if T > DECODE_MAX_T and offset is not None and ops.prefill_supported(q) and \
                 (q_args["cos"] is None or q_args["cos"].dim() == 2):
             ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)

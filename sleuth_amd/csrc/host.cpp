@@ -532,7 +532,7 @@ PyObject* attn_paged_impl(PyObject* const* a) {
 }
 
 // attn_sinks(table of workspaces, q, k_cache, v_cache, scale, window, sinks, pos | None, pos_dev | None, row_pos | None, max_kv_len | None,
-//            q_weight | None, eps, norm_q, cos | None, sin | None)
+//            q_weight | None, eps, norm_q, cos | None, sin | None, fixed_cut)
 PyObject* attn_sinks_impl(PyObject* const* a) {
   NewTokens n;
   Tensor kc, vc, pos_dev, row_pos;
@@ -562,7 +562,14 @@ PyObject* attn_sinks_impl(PyObject* const* a) {
   max_kv = max_kv < 0 ? max_len : std::min(max_kv, max_len);
   if (max_kv < 1) return nullptr;
   n.set_flags(a[13] == Py_True);
-  n.size(K, max_kv);
+  if (a[16] == Py_True) {
+    if (n.T > FORGE_FIXED_CUT_MAX_T) return nullptr;
+    n.flags |= FORGE_FIXED_CUT;
+    n.need = forge_attn_sinks_fixed_workspace_bytes(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, max_len,
+                                                    (int)n.window, (int)n.sinks);
+  } else {
+    n.size(K, max_kv);
+  }
   const bool kept = n.keep();
   const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
   StreamWorkspace ws(a[0], dev.index(), stream, kept ? n.need : 0);
@@ -605,7 +612,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     FORGE_ENTRY(decode_append, 21), FORGE_ENTRY(kv_append, 11), FORGE_ENTRY(prefill, 11),
     FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), FORGE_ENTRY(kv_append_paged, 13),
-    FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 16), {nullptr, nullptr, 0, nullptr},
+    FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 17), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_forge_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -49,6 +49,9 @@ struct PagedParams {
   // Key split: a row block's tiles go to ceil(tiles / part_tiles) blocks (at most nparts) in equal shares, each
   // writing an fp32 partial that the combine kernel merges in part order. nparts 1: no split.
   int nparts, part_tiles;
+  // Fixed cut: key tile a (of the whole cache) is wave a % 4's of part a / 4 % nparts, so that what a wave adds up
+  // for a query hangs on the query's own position alone, not on the other queries of its block.
+  bool fixed;
   // Planned calls (the chunk kernel, rows of different lengths): block x takes item items[x / K] of KV head
   // x % K; the pairs say where the merge finds a row block's partials. Null: the static split above.
   const PagedItem* items;
@@ -84,6 +87,7 @@ constexpr int step_blocks_per_cu(int esize, int D, int rows) {
 // How the host cuts a call: rows per block, keys per tile, parts.
 struct PagedPlan {
   bool chunk;    // paged_chunk.hip's kernel (rows 128), or paged.hip's
+  bool fixed;    // (paged.hip's) parts and waves by the tile's number in the cache
   bool planned;  // the parts are planned on the device
   int rows, keys;
   int nparts, part_tiles;
@@ -164,6 +168,12 @@ struct BlockWork {
   bool none;  // nothing to do
 };
 
+// The parts of a row block's tiles, where the device does not plan them.
+__device__ __forceinline__ int row_parts(const PagedParams& p, int tiles) {
+  if (p.nparts < 2 || tiles == 0) return 1;
+  return p.fixed ? p.nparts : (tiles + p.part_tiles - 1) / p.part_tiles;
+}
+
 // Grid: x (batch row, KV head), y part, z row block, late ones first (a causal chunk's have the most keys). Blocks
 // start in that order, x first, so where (batch row, KV head) pairs times parts are a multiple of 8 all blocks that
 // read the same keys run on one XCD and meet in its L2.
@@ -190,7 +200,7 @@ template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const 
     w.b = pair / p.K;
     w.kvh = pair - w.b * p.K;
     w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
-    w.parts = p.nparts < 2 ? 1 : (w.span.tiles + p.part_tiles - 1) / p.part_tiles;
+    w.parts = row_parts(p, w.span.tiles);
     w.slot = (pair * nrb + w.rblk) * p.nparts + w.part;
     if (w.part > 0 && w.part >= w.parts) return w;
   }
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   } else {
     const RowSpan w = row_span(p, b, rblk * BM, BM, KT);
     rows = w.rows;
-    parts = (w.tiles + p.part_tiles - 1) / p.part_tiles;
+    parts = row_parts(p, w.tiles);
     slot = ((int64_t)(b * p.K + kvh) * nrb + rblk) * p.nparts;
     stride = 1;
   }

@@ -185,7 +185,7 @@ template <typename T, int D, int RB> struct StepLds {
   static_assert(BLOCKS * BYTES <= 160 * 1024, "LDS");
 };
 
-template <typename T, int D, int RB>
+template <typename T, int D, int RB, bool FIXED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(StepLds<T, D, RB>::BLOCKS >= 2 ? 2 : 1)))
 void paged_step_kernel(PagedParams p) {
   using TL = StepTile<T, D, RB>;
@@ -201,10 +201,16 @@ void paged_step_kernel(PagedParams p) {
   const BlockWork work = block_work<ROWS, KT>(p);
   if (work.none) return;
   const RowSpan w = work.span;
-  const int b = work.b, kvh = work.kvh, rblk = work.rblk, begin = work.begin, end = work.end;
+  const int b = work.b, kvh = work.kvh, rblk = work.rblk;
   const bool whole = work.parts < 2;
 
-  // ---- key tiles of this wave: begin + wave, + 4, ...
+  // ---- key tiles of this wave: begin + wave, + 4, ...; with a fixed cut those whose number in the cache is the wave's
+  // own below 4 nparts, modulo 4 nparts: tiles of the first tokens, then, `hop` behind the first one of the window, those
+  const int own = 4 * work.part + wave, step = FIXED ? 4 * p.nparts : 4;
+  const int sink_end = FIXED ? w.sink_tiles : 0;
+  int hop = FIXED ? (own - w.main_tile) % step : 0;
+  hop += hop < 0 ? step : 0;
+  const auto next = [&](int i) { return FIXED && i < sink_end && i + step >= sink_end ? sink_end + hop : i + step; };
   u32x4 kr[NL], vr[NL];
   const int lrow = lane / TL::NCH, lch = lane % TL::NCH;
   const char* kb0 = static_cast<const char*>(p.k) + kvh * p.skh * (int64_t)sizeof(T);
@@ -251,7 +257,8 @@ void paged_step_kernel(PagedParams p) {
     }
     bad = miss;
   };
-  int i = begin + wave;
+  int i = !FIXED ? work.begin + wave : own < sink_end ? own : sink_end + hop;
+  const int end = FIXED ? w.tiles : work.end;
   if (i < end) load(i);
 
   // ---- query rows, as B operands; rows behind the row's last one stand for that one (never written)
@@ -289,7 +296,7 @@ void paged_step_kernel(PagedParams p) {
   char* kt = smem + wave * LD::WAVE;
   char* vt = kt + TL::TILEB;
 
-  for (; i < end; i += 4) {
+  for (; i < end; i = next(i)) {
     const int key0 = w.tile_key(i, KT);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
@@ -298,7 +305,7 @@ void paged_step_kernel(PagedParams p) {
       *reinterpret_cast<u32x4*>(vt + row * TL::ROWB + ((lch ^ step_swz_v<T, D>(row)) << 4)) = vr[j];
     }
     const unsigned miss = bad;
-    if (i + 4 < end) load(i + 4);
+    if (next(i) < end) load(next(i));
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (this wave's tile: LDS keeps a wave's order)
     __builtin_amdgcn_wave_barrier();
 
@@ -535,13 +542,13 @@ void paged_step_kernel(PagedParams p) {
   }
 }
 
-template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hipStream_t s) {
+template <typename T, int D, int RB, bool FIXED> static int launch_step_rb(PagedParams p, hipStream_t s) {
   using LD = StepLds<T, D, RB>;
   static std::atomic<uint64_t> done{0};
-  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB>), LD::BYTES, done)) return st;
+  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB, FIXED>), LD::BYTES, done)) return st;
   const int nrb = (p.rows + LD::ROWS - 1) / LD::ROWS;
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
-  hipLaunchKernelGGL((paged_step_kernel<T, D, RB>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
+  hipLaunchKernelGGL((paged_step_kernel<T, D, RB, FIXED>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
   int st = check_launch();
   if (st == 0 && p.nparts > 1 && !p.counters) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
   return st;
@@ -549,9 +556,9 @@ template <typename T, int D, int RB> static int launch_step_rb(PagedParams p, hi
 
 template <typename T, int D> static int launch_step(const PagedParams& p, const PagedPlan& plan, hipStream_t s) {
   if constexpr (step_rows_most(sizeof(T), D) >= 32) {
-    if (plan.rows == 32) return launch_step_rb<T, D, 2>(p, s);
+    if (plan.rows == 32) return p.fixed ? launch_step_rb<T, D, 2, true>(p, s) : launch_step_rb<T, D, 2, false>(p, s);
   }
-  if (plan.rows == 16) return launch_step_rb<T, D, 1>(p, s);
+  if (plan.rows == 16) return p.fixed ? launch_step_rb<T, D, 1, true>(p, s) : launch_step_rb<T, D, 1, false>(p, s);
   return set_error("forge_attn_paged: no kernel of this row block");
 }
 

@@ -106,6 +106,31 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   return plan;
 }
 
+// A step whose sums must not hang on how many tokens it has, or on the bound of its keys: everything as for one token
+// of rows that hold all that the cache can (max_len) or the window lets them see. Where a call's query rows are more
+// than a block's, 32 rows a block read the keys half as often, if their tiles are the same. What it costs (us, free /
+// fixed cut, window 1,024): a token of 16 rows, 8 KV heads of 128, 18.4 / 18.5; 5 tokens of 8 rows there 12.1 / 11.8; 4 of 8
+// rows, one KV head of 256 with 8 query heads, 11.5 / 12.9. Verify steps of many rows, which the chunk kernel would take,
+// pay most: 5 tokens of 32 rows, 28 q / 4 KV heads of 128, 23.2 / 32.8; 8 of 16 rows, 16 q / 1 KV head of 512, 35 / 125.
+static PagedPlan fixed_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_len, int window, int sinks, bool split) {
+  PagedPlan plan{};
+  const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
+  plan.fixed = true;
+  plan.keys = step_keys(es, D, 16);
+  plan.rows = G * T > 16 && step_rows_most(es, D) >= 32 && step_keys(es, D, 32) == plan.keys ? 32 : 16;
+  plan.nparts = 1;
+  if (!split) return plan;
+  const int64_t all = (max_len + plan.keys - 1) / plan.keys;
+  const int64_t seen = ((int64_t)window + FORGE_FIXED_CUT_MAX_T + plan.keys - 3) / plan.keys + 1 +
+                       ((int64_t)sinks + plan.keys - 1) / plan.keys;
+  const int64_t tiles = seen < all ? seen : all, units = (int64_t)B * K * ((G + 15) / 16);
+  const int64_t slots = (int64_t)device_cus() * step_blocks_per_cu(es, D, 16);
+  int64_t parts = slots / units, most = tiles / (es * D >= 512 ? 4 : 8);   // (at least as many tiles a part as below)
+  if (parts > most) parts = most;
+  plan.nparts = (int)(parts < 1 ? 1 : parts > 4096 ? 4096 : parts);
+  return plan;
+}
+
 // The workspace: the counters, [items | row blocks' parts] of a planned call, then (m, l) and the output of every
 // slot's rows.
 struct PagedWs {
@@ -152,7 +177,8 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   p.rows = p.G * p.T;
   p.scale_log2 = scale * kLog2e;
   const bool split = workspace != nullptr;
-  const PagedPlan plan = paged_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, p.row_pos != nullptr, split);
+  const PagedPlan plan = p.fixed ? fixed_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, split)
+                                 : paged_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, p.row_pos != nullptr, split);
   p.nparts = plan.nparts;
   p.part_tiles = plan.part_tiles;
   p.slots = plan.slots;
@@ -239,6 +265,14 @@ extern "C" size_t forge_attn_sinks_workspace_bytes(int dtype, int B, int T, int 
   return forge_attn_paged_workspace_bytes(dtype, B, T, H, K, D, max_kv_len, window, sinks);
 }
 
+extern "C" size_t forge_attn_sinks_fixed_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_len,
+                                                         int window, int sinks) {
+  if (B <= 0 || T <= 0 || T > FORGE_FIXED_CUT_MAX_T || H <= 0 || K <= 0 || H % K || !paged_dim_ok(dtype, D) || max_len <= 0 ||
+      window <= 0 || sinks < 0)
+    return 0;
+  return paged_ws(fixed_plan(dtype, B, T, H, K, D, max_len, window, sinks, true), B, T, H, K, D).bytes;
+}
+
 extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
                                 int64_t sqt, const float* q_weight, float eps, int flags, const float* cos,
                                 const float* sin, int64_t s_cos_b, int64_t s_cos_t, const void* k_cache,
@@ -254,7 +288,10 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   if (B == 0 || T == 0) return 0;
   if (!row_pos && !pos_dev && (pos0 < 0 || T < 0 || pos0 > limit - T))
     return set_error("pos + T exceeds max_kv_len or the cache length");
+  const bool fixed = flags & FORGE_FIXED_CUT;
+  if (fixed && T > FORGE_FIXED_CUT_MAX_T) return set_error("FORGE_FIXED_CUT is for steps of at most 16 tokens");
   PagedParams p{};
+  p.fixed = fixed;
   p.q = q; p.sqb = sqb; p.sqh = sqh; p.sqt = sqt;
   p.qw = q_weight; p.eps = eps; p.flags = flags;
   p.cos = cos; p.sin = sin; p.csb = s_cos_b; p.cst = s_cos_t;
@@ -263,5 +300,5 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   p.row_pos = row_pos; p.pos_dev = pos_dev; p.pos0 = pos0;
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
-  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
+  return paged_run(dtype, D, p, fixed ? max_len : max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
 }

@@ -17,7 +17,7 @@ import contextlib
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, F32, NORM_QK, NORM_V, ROPE, WS_ZEROED, check, host, lib
+from ._lib import BF16, F16, F32, FIXED_CUT, NORM_QK, NORM_V, ROPE, WS_ZEROED, check, host, lib
 
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
@@ -716,14 +716,18 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
                row_pos: torch.Tensor | None = None, max_kv_len: int | None = None,
                q_weight: torch.Tensor | None = None, eps: float = 1e-6, norm_q: bool = False,
                cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, fixed_cut: bool = False) -> torch.Tensor:
     """Sliding-window attention whose first `sinks` positions stay visible, over a contiguous cache
     [B,K,max_len,D] that holds the new keys already: query t of row b sits at p = base_b + t (row_pos, pos_dev or
     pos, as attn_decode) and sees keys s <= p with s > p - window or s < sinks. Any T: whole prompts, chunks, verify and
-    decode steps. Returns [B,T,H,D]."""
+    decode steps. Returns [B,T,H,D].
+
+    fixed_cut (T <= 16): a token's result is the same, bit for bit, in every such call on caches of one shape, whatever T,
+    max_kv_len and the way the position is given: a verify step's rows equal the decodes of its tokens."""
+    fixed_cut = bool(fixed_cut)
     if out is None:
         r = host().attn_sinks(_PAGED_WS, q, k_cache, v_cache, float(scale), window, sinks, pos, pos_dev, row_pos, max_kv_len, q_weight,
-                              float(eps), bool(norm_q), cos, sin)
+                              float(eps), bool(norm_q), cos, sin, fixed_cut)
         if r is not None:
             return r if r.__class__ is not int else check(r, "forge_attn_sinks")
     dev = _need_device(q, k_cache, v_cache, pos_dev, row_pos, cos, sin, q_weight if norm_q else None, out)
@@ -734,6 +738,8 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
     if window < 1:
         raise ValueError("attn_sinks needs a window (attn_decode and attn_prefill see every key)")
     B, T, max_len = q.shape[0], q.shape[2], k_cache.shape[2]
+    if fixed_cut and T > DECODE_CHUNK_MAX_T:
+        raise ValueError(f"fixed_cut is for steps of at most {DECODE_CHUNK_MAX_T} tokens")
     rp, pd, p0 = _positions(pos, pos_dev, row_pos, B, dev)
     if rp is None and pd is None:
         if not 0 <= p0 <= max_len - T:
@@ -747,7 +753,11 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
             raise ValueError("max_kv_len must be positive")
     keep, args, out = _new_token_args(q, k_cache, scale, q_weight, eps, norm_q, cos, sin, window, sinks, out)
     with _guard(dev):
-        ws = _PagedPartials(dev, lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
+        need = lib().forge_attn_sinks_fixed_workspace_bytes(*args[:6], max_len, int(window), int(sinks)) if fixed_cut else \
+            lib().forge_attn_sinks_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks))
+        if fixed_cut:
+            args = (*args[:12], args[12] | FIXED_CUT, *args[13:])
+        ws = _PagedPartials(dev, need)
         st = lib().forge_attn_sinks(*args, _ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache), max_len, _ptr(rp), _ptr(pd),
                                     p0, max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
                                     *ws.args(), _stream(dev))

@@ -919,3 +919,67 @@ def test_ops_refuse_scales_that_are_not_positive(scale):
         ops.attn_paged(q, kp, kp, torch.zeros(2, 2, dtype=torch.int32, device="cuda"), i32([0, 0]), scale=scale)
     with pytest.raises(ValueError, match="scale"):
         ops.attn_sinks(q, kp[:2], kp[:2], scale=scale, window=4, sinks=1, pos=0)
+
+
+# ---------------------------------------------------------------- steps whose sums do not hang on T
+FIXED = [(BF, 16, 8, 128, 2, 300, 4), (HF, 12, 4, 64, 1, 1000, 33), (BF, 8, 1, 256, 3, 64, 5), (BF, 16, 1, 512, 1, 200, 3), (SF, 8, 4, 32, 2, 100, 1),
+         (SF, 16, 8, 128, 1, 500, 64), (HF, 28, 4, 128, 1, 129, 0), (BF, 32, 8, 32, 70, 90, 70), (BF, 8, 4, 256, 40, 700, 4), (SF, 8, 1, 256, 1, 333, 9),
+         (HF, 16, 16, 64, 1, 5000, 2)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", FIXED, ids=_id)
+def test_fixed_cut_rows_are_the_decodes_bit_for_bit(case):
+    """A verify step's rows equal the decodes of those tokens, wherever the window starts in a tile, with a host
+    position, one on the device and one for each row, and under any bound."""
+    dtype, H, K, D, B, window, sinks = case
+    g = gen(41)
+    cap, scale = 2100, D ** -0.5
+    kc, vc = ((1.3 * torch.randn(B, K, cap, D, generator=g)).to(dtype).cuda() for _ in range(2))
+    kw = dict(scale=scale, window=window, sinks=sinks, fixed_cut=True)
+    for T, at in ((2, 0), (5, window - 3), (4, window + 29), (3, 62), (16, 1000), (7, 1721), (5, cap - 5), (9, 1500 + sinks)):
+        q = torch.randn(B, T, H, D, generator=g).to(dtype).cuda().transpose(1, 2)
+        at = min(max(at, 0), cap - T)
+        rows = ops.attn_sinks(q, kc, vc, pos=at, **kw)
+        want, bound = _sinks_want(q[:2].cpu(), kc[:2].cpu(), vc[:2].cpu(), [at] * min(B, 2), window, sinks, scale)
+        assert_close(rows[:2], want, bound)
+        for t in range(T):
+            one = ops.attn_sinks(q[:, :, t:t + 1], kc, vc, pos=at + t, **kw)
+            assert torch.equal(one[:, 0], rows[:, t]), (T, at, t)
+        for other in (dict(pos_dev=torch.tensor([at], device="cuda")), dict(row_pos=i32([at] * B)),
+                      dict(row_pos=i32([at] * B), max_kv_len=at + T)):
+            assert torch.equal(ops.attn_sinks(q, kc, vc, **other, **kw), rows)
+        graph = torch.cuda.CUDAGraph()   # (merged by a launch of its own)
+        with torch.cuda.graph(graph):
+            out = ops.attn_sinks(q, kc, vc, pos=at, **kw)
+        graph.replay()
+        assert torch.equal(out, rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+def test_fixed_cut_never_uses_keys_that_no_query_sees(fill):
+    g = gen(42)
+    kc, vc = (torch.randn(1, 8, 800, 128, generator=g).to(BF) for _ in range(2))
+    for c in (kc, vc):
+        c[:, :, 4:637], c[:, :, 703:] = fill, fill
+    q = torch.randn(1, 3, 16, 128, generator=g).to(BF).transpose(1, 2)
+    got = ops.attn_sinks(q.cuda(), kc.cuda(), vc.cuda(), scale=0.1, window=64, sinks=4, pos=700, fixed_cut=True)
+    assert_close(got, *_sinks_want(q, kc, vc, [700], 64, 4, 0.1))
+
+
+def test_fixed_cut_refusals():
+    lib = _lib.lib()
+    base = [_lib.BF16, 2, 17, 8, 4, 64, _P, 512, 64, 512, None, 1e-6, _lib.FIXED_CUT, None, None, 0, 0, _P, _P, 8192, 2048, 64, 32,
+            _P, None, 0, 32, 8, 2, 1.0, _P, 512, 512, 64, None, 0, 0, None]
+    assert lib.forge_attn_sinks(*base) < 0 and "16 tokens" in lib.forge_last_error().decode()
+    f = lib.forge_attn_sinks_fixed_workspace_bytes
+    assert f(_lib.BF16, 1, 17, 16, 8, 128, 9000, 1024, 4) == 0 and f(_lib.BF16, 1, 1, 16, 8, 96, 9000, 1024, 4) == 0
+    assert f(_lib.BF16, 1, 1, 16, 8, 128, 9000, 1024, 4) > 64 * 1024 and f(_lib.BF16, 1, 1, 16, 8, 128, 64, 16, 4) == 0
+
+
+@pytest.mark.gpu
+def test_fixed_cut_refuses_long_calls():
+    c = torch.zeros(1, 4, 64, 64, dtype=BF, device="cuda")
+    with pytest.raises(ValueError, match="fixed_cut"):
+        ops.attn_sinks(torch.zeros(1, 8, 17, 64, dtype=BF, device="cuda"), c, c, scale=1.0, window=4, sinks=1, pos=0, fixed_cut=True)

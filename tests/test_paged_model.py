@@ -378,3 +378,37 @@ def test_gated_attention_refuses_a_paged_cache():
     cache = PagedKVCache([(2, 32)], 1, 32, "cpu", torch.float32)
     with pytest.raises(NotImplementedError, match="paged"):
         m(torch.zeros(1, 1, 16), torch.ones(1, 32), torch.zeros(1, 32), cache)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128])
+@torch.no_grad()
+def test_a_sink_layers_verify_rows_are_its_decodes(hd):
+    """bf16: a verify step over the contiguous cache attends as the single tokens do, bit for bit; so does a recorded
+    step, whose bound is the cache's length."""
+    cfg = config(True, 3, head_size=hd, max_seq_len=512, sliding_window=90)
+    att, x, cos, sin = module_and_inputs(cfg, torch.bfloat16, "cuda", 1, 300, 0)
+    rows = {}
+    for T in (1, 5):
+        cache = KVCache([(2, hd)], 1, 512, "cuda", torch.bfloat16)
+        att(x[:, :200], cos[:200], sin[:200], cache)
+        cache.advance(200)
+        rows[T] = []
+        for at in range(200, 300, T):
+            rows[T].append(att(x[:, at:at + T], cos[at:at + T], sin[at:at + T], cache))
+            cache.advance(T)
+    assert torch.equal(torch.cat(rows[1], 1), torch.cat(rows[5], 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,k", [(64, 4), (128, 3), (32, 8)])
+@torch.no_grad()
+def test_speculative_and_recorded_decoding_with_sinks_equal_plain_greedy(hd, k):
+    from sleuth_amd.generate import speculative_generate
+
+    m = model(config(True, 3, head_size=hd, max_seq_len=256, sliding_window=40), "cuda", torch.bfloat16)
+    prompt = torch.randint(64, (70,), generator=torch.Generator().manual_seed(4)).tolist()
+    plain = generate(m, prompt, 150).new_ids
+    assert generate(m, prompt, 150, cuda_graph=True).new_ids == plain
+    for graph in (False, True):
+        assert speculative_generate(m, prompt, 150, k=k, cuda_graph=graph).new_ids == plain
