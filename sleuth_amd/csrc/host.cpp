@@ -536,7 +536,7 @@ PyObject* attn_paged_impl(PyObject* const* a) {
 PyObject* attn_sinks_impl(PyObject* const* a) {
   NewTokens n;
   Tensor kc, vc, pos_dev, row_pos;
-  int64_t pos = 0, max_kv = -1, sk[3], sv[3];
+  int64_t pos = 0, max_kv = INT64_MAX, sk[3], sv[3];
   if (!take(a[1], n.q) || !take(a[2], kc) || !take(a[3], vc) || !as_float(a[4], n.scale) || !as_int(a[5], n.window) ||
       !as_int(a[6], n.sinks) || (a[7] != Py_None && !as_int(a[7], pos)) || !take_opt(a[8], pos_dev) ||
       !take_opt(a[9], row_pos) || (a[10] != Py_None && !as_int(a[10], max_kv)) || !take_opt(a[11], n.qw) ||
@@ -559,7 +559,7 @@ PyObject* attn_sinks_impl(PyObject* const* a) {
     if (pos < 0 || pos > max_len - n.T) return nullptr;
     max_kv = pos + n.T;
   }
-  max_kv = max_kv < 0 ? max_len : std::min(max_kv, max_len);
+  max_kv = std::min(max_kv, max_len);
   if (max_kv < 1) return nullptr;
   n.set_flags(a[13] == Py_True);
   if (a[16] == Py_True) {

@@ -983,3 +983,13 @@ def test_fixed_cut_refuses_long_calls():
     c = torch.zeros(1, 4, 64, 64, dtype=BF, device="cuda")
     with pytest.raises(ValueError, match="fixed_cut"):
         ops.attn_sinks(torch.zeros(1, 8, 17, 64, dtype=BF, device="cuda"), c, c, scale=1.0, window=4, sinks=1, pos=0, fixed_cut=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bound", [0, -1, -5])
+def test_sinks_bounds_below_one_are_refused(bound):
+    """Where it is the call that gives the bound: positions on the device."""
+    c, q = torch.zeros(2, 4, 32, 64, dtype=BF, device="cuda"), torch.zeros(2, 8, 1, 64, dtype=BF, device="cuda")
+    for where in (dict(row_pos=i32([3, 4])), dict(pos_dev=torch.tensor([3], device="cuda"))):
+        with pytest.raises(ValueError, match="max_kv_len"):
+            ops.attn_sinks(q, c, c, scale=1.0, window=4, sinks=1, max_kv_len=bound, **where)
