@@ -71,7 +71,9 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.slots = cus * (plan.chunk ? (es * D >= 1024 ? 1 : es * D <= 128 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
   const int64_t slots = plan.slots;
   const int64_t blocks = units / K;
-  if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots) {
+  // (the plan adds up tiles in 32 bits)
+  if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots &&
+      blocks * tiles <= INT_MAX / 4) {
     plan.planned = true;
     plan.nitems = (int)(plan.slots / K + blocks);
     return plan;

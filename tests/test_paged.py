@@ -993,3 +993,11 @@ def test_sinks_bounds_below_one_are_refused(bound):
     for where in (dict(row_pos=i32([3, 4])), dict(pos_dev=torch.tensor([3], device="cuda"))):
         with pytest.raises(ValueError, match="max_kv_len"):
             ops.attn_sinks(q, c, c, scale=1.0, window=4, sinks=1, max_kv_len=bound, **where)
+
+
+def test_calls_whose_tiles_pass_32_bits_are_not_planned():
+    """The device's plan adds up the tiles of all row blocks in 32 bits; past that it could hand out more parts than its
+    list holds. 64 row blocks of 2^25 tiles are cut on the host, which needs no plan (nor, here, partials)."""
+    f = _lib.lib().forge_attn_paged_workspace_bytes
+    assert f(_lib.BF16, 2, 2048, 16, 8, 128, 100_000, 0, 0) > 0
+    assert f(_lib.BF16, 2, 2048, 16, 8, 128, 2 ** 31 - 65537, 0, 0) == 0
