@@ -94,9 +94,14 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
     per = n * tile + p * (4 + units) + 192 < tiles * tile ? n : tiles;
   } else {
     // two tiles at least for each wave, one of the long ones from 512 bytes a key on (us, two / one: 32 rows of 1,500 keys
-    // at head dim 256 15.7 / 14.1, 2 rows of 800 at head dim 512 19.2 / 16.3, but one of 8,000 at 128 14.2 / 15.8)
+    // at head dim 256 15.7 / 14.1, 2 rows of 800 at head dim 512 19.2 / 16.3, but one of 8,000 at 128 14.2 / 15.8).
+    // Rows of different lengths end at different times, so long ones are cut though the blocks fill the device already, as
+    // long as those are fewer than eight for each that it holds: us, cut / whole, a step of 128 rows of up to 32,767 keys (8 KV
+    // heads, head dim 128, 2 blocks for each) 1,274 / 1,460, of 512 of up to 16,000 (8) 2,652 / 2,681, of 1,024 of up to 8,000
+    // (16) 2,718 / 2,674; fp32 prompts of 4,096 at head dim 32 behind 15,000 (8) 2,848 / 2,456 and four of them behind 28,000
+    // (32) 21,947 / 18,660, whose partials were 1.1 GB.
     const int64_t least = es * D >= 512 ? 4 : 8, most = (step_blocks_per_cu(es, D, plan.rows) > 1 ? 2048 : 4096) / plan.keys;
-    if (per > most) per = most;
+    if (per > most && units < 8 * slots) per = most;
     if (per < least) per = least;
   }
   int64_t parts = (tiles + per - 1) / per;

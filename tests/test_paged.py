@@ -1001,3 +1001,10 @@ def test_calls_whose_tiles_pass_32_bits_are_not_planned():
     f = _lib.lib().forge_attn_paged_workspace_bytes
     assert f(_lib.BF16, 2, 2048, 16, 8, 128, 100_000, 0, 0) > 0
     assert f(_lib.BF16, 2, 2048, 16, 8, 128, 2 ** 31 - 65537, 0, 0) == 0
+
+
+def test_partials_of_calls_that_fill_the_device_many_times():
+    """Blocks that are many for each that the device holds are not split: their partials would be gigabytes."""
+    f = _lib.lib().forge_attn_paged_workspace_bytes
+    assert f(_lib.F32, 8, 4096, 32, 8, 32, 32768, 0, 0) == 0
+    assert f(_lib.BF16, 64, 1, 16, 8, 128, 32768, 0, 0) > 0 and f(_lib.BF16, 256, 1, 16, 8, 128, 32768, 0, 0) > 0
