@@ -28,7 +28,7 @@ from typing import Callable
 import torch
 
 from .kv_cache import KVCache
-from .paged_cache import PagedKVCache
+from .paged_cache import OutOfPages, PagedKVCache
 
 
 @dataclass
@@ -171,12 +171,16 @@ def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, te
     """generate() for a batch of prompts of any lengths over a paged cache: every pass takes up to `chunk` tokens of
     each prompt that has some left (the batch is padded to the longest), then each running row decodes one token per
     pass. A row's pages come back when it ends, and, where every layer slides, as they leave the windows (the first
-    cfg.sink_tokens positions stay)."""
+    cfg.sink_tokens positions stay). Where the pool is short, OutOfPages is raised with `results`: the finished rows', and
+    the others' so far (stop_reason "out_of_pages")."""
     if not prompts or not all(prompts):
         raise ValueError("every prompt must contain at least one token")
     if chunk < 1:
         raise ValueError("chunk must be positive")
     cfg, dev = model.cfg, next(model.parameters()).device
+    longest = max(map(len, prompts))
+    if longest > cfg.max_seq_len:
+        raise ValueError(f"sequence length {longest} exceeds max_seq_len {cfg.max_seq_len}")
     cache = PagedKVCache.for_model(model, len(prompts), cfg.max_seq_len, cache_dtype, page_size, n_pages)
     gen = torch.Generator(device=dev).manual_seed(seed or 0)
     specs = [cfg.attn_spec(i) for i in range(cfg.n_layers)]
@@ -191,6 +195,13 @@ def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, te
         T = max(new)
         ids = torch.tensor([x[:n] + [0] * (T - n) for x, n in zip(left, new)], device=dev)
         cache.set_new(new)
+        try:
+            cache.reserve(T)
+        except OutOfPages as e:
+            for r, run in zip(results, running):
+                r.stop_reason = "out_of_pages" if run else r.stop_reason
+            e.results = _with_stats(results, cache, passes, most_pages)
+            raise
         logits = model(ids, cache=cache).logits
         passes, most_pages = passes + 1, max(most_pages, cache.n_pages - cache.free_pages)
         last = logits[torch.arange(len(new), device=dev), torch.tensor(new, device=dev).clamp(min=1) - 1]
@@ -214,6 +225,10 @@ def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, te
             cache.release(b)
         if window:
             cache.release_unseen(window, cfg.sink_tokens)
+    return _with_stats(results, cache, passes, most_pages)
+
+
+def _with_stats(results, cache, passes: int, most_pages: int) -> list[GenerationResult]:
     for r in results:
         r.stats = {"kv_cache_mb": round(cache.nbytes() / 1e6, 2), "passes": passes, "most_pages": most_pages}
     return results

@@ -17,6 +17,12 @@ from __future__ import annotations
 import torch
 
 
+class OutOfPages(ValueError):
+    """The pool has fewer free pages than a pass needs. generate_batch adds `results`, what its rows have so far."""
+
+    results: list | None = None
+
+
 class PagedKVCache:
     paged = True
     ragged = True
@@ -102,7 +108,7 @@ class PagedKVCache:
     # ------------------------------------------------------------------ pages
     def reserve(self, T: int) -> None:
         """Pages for the next pass's real tokens (every layer of a pass may call it: the first one acts). Raises
-        ValueError where a row would pass max_len or the pool has no page left; nothing is handed out then."""
+        ValueError where a row would pass max_len, OutOfPages where the pool has no page left; nothing is handed out then."""
         P = self.page_size
         need = []
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
@@ -113,7 +119,7 @@ class PagedKVCache:
         if not need:
             return
         if len(need) > len(self._free):
-            raise ValueError(f"KV cache out of pages ({len(need)} needed, {len(self._free)} of {self.n_pages} free)")
+            raise OutOfPages(f"KV cache out of pages ({len(need)} needed, {len(self._free)} of {self.n_pages} free)")
         for b, j in need:
             self._table[b][j] = self._free.pop()
         self._put_table()

@@ -412,3 +412,28 @@ def test_speculative_and_recorded_decoding_with_sinks_equal_plain_greedy(hd, k):
     assert generate(m, prompt, 150, cuda_graph=True).new_ids == plain
     for graph in (False, True):
         assert speculative_generate(m, prompt, 150, k=k, cuda_graph=graph).new_ids == plain
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_short_pool_keeps_the_rows_results(device):
+    """A row ends, the other two outgrow the pool: what the finished one has is in the error, and what they have so far."""
+    from sleuth_amd.paged_cache import OutOfPages
+
+    m = model(config(), device)
+    prompts = [[1, 2, 3], list(range(40)), [5] * 125]
+    alone = [generate(m, p, 500) for p in prompts]
+    with pytest.raises(OutOfPages, match="out of pages") as e:
+        generate_batch(m, prompts, 500, chunk=125, page_size=16, n_pages=8 + 3 + 2)
+    got = e.value.results
+    assert [r.prompt_ids for r in got] == prompts
+    assert got[2].stop_reason == alone[2].stop_reason == "context_full" and got[2].new_ids == alone[2].new_ids
+    for r, a in zip(got[:2], alone):
+        assert r.stop_reason == "out_of_pages" and len(r.new_ids) > 10 and r.new_ids == a.new_ids[:len(r.new_ids)]
+    assert got[0].stats["passes"] > 0
+
+
+def test_a_prompt_past_the_models_length_is_refused_before_any_pass():
+    m = model(config())
+    m.forward = None   # (no pass)
+    with pytest.raises(ValueError, match="exceeds max_seq_len"):
+        generate_batch(m, [[1], [2] * 129], 4)
