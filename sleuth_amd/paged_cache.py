@@ -4,8 +4,9 @@ The reference's caches (sleuth/forge/infer/kv_cache.py:25-138) hold max_len posi
 K and V are pools [n_pages, K, page_size, hd]; position s of row b is slot s % page_size of page
 page_table[b, s // page_size], the same page of every layer's pools. Pages are handed out as rows grow (reserve), and
 come back when a row ends (release) or when no layer can see them any more (release_unseen: every layer slides, and
-keeps its first tokens). The table and the lengths live on the device in fixed buffers, so recorded graphs see them
-change.
+keeps its first tokens). The table and the lengths live on the device in fixed buffers, so a recorded graph of the
+operators (kv_append_paged, attn_paged, with a max_kv_len for all its replays) sees them change. A whole pass cannot be
+recorded: which pages it needs and how long the rows are is the host's to say, and reserve refuses it.
 
 It speaks the cache protocol of the package's callers (pos, max_len, advance, seq_lens, seq_lens_host, update; `ragged`
 is always true, `static` never) and adds `paged`, page_table, new_lens, reserve, top and row, which the attention module
@@ -109,6 +110,9 @@ class PagedKVCache:
     def reserve(self, T: int) -> None:
         """Pages for the next pass's real tokens (every layer of a pass may call it: the first one acts). Raises
         ValueError where a row would pass max_len, OutOfPages where the pool has no page left; nothing is handed out then."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            # (its max_kv_len would be today's in every replay, and the rows' lengths on the host would stand still)
+            raise RuntimeError("a pass over a paged cache cannot be recorded: record ops.kv_append_paged and attn_paged")
         P = self.page_size
         need = []
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):

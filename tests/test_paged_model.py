@@ -437,3 +437,27 @@ def test_a_prompt_past_the_models_length_is_refused_before_any_pass():
     m.forward = None   # (no pass)
     with pytest.raises(ValueError, match="exceeds max_seq_len"):
         generate_batch(m, [[1], [2] * 129], 4)
+
+
+@pytest.mark.gpu
+@torch.no_grad()
+def test_a_pass_over_a_paged_cache_is_not_recorded():
+    """Its replays would see no key past the lengths of the day it was recorded."""
+    cfg = config()
+    att, x, cos, sin = module_and_inputs(cfg, torch.bfloat16, "cuda", 1, 20, 0)
+    cache = PagedKVCache([(2, 32)], 1, 128, "cuda", torch.bfloat16, 16)
+    at = torch.arange(19, device="cuda")[None]
+    att(x[:, :19], cos[at], sin[at], cache)
+    cache.advance(19)
+    last, n = x[:, 19:], torch.zeros(1, device="cuda")
+    c, s = cos[19:20][None], sin[19:20][None]
+    att(last, c, s, cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        n.add_(1)
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            att(last, c, s, cache)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert n.item() == 1
