@@ -9,8 +9,8 @@ operators (kv_append_paged, attn_paged, with a max_kv_len for all its replays) s
 recorded: which pages it needs and how long the rows are is the host's to say, and reserve refuses it.
 
 It speaks the cache protocol of the package's callers (pos, max_len, advance, seq_lens, seq_lens_host, update; `ragged`
-is always true, `static` never) and adds `paged`, page_table, new_lens, reserve, top and row, which the attention module
-uses (ops.kv_append_paged, ops.attn_paged).
+is always true, `static` never; pos is read only, since rows differ: rewind takes each row's length) and adds `paged`,
+page_table, new_lens, reserve, top and row, which the attention module uses (ops.kv_append_paged, ops.attn_paged).
 """
 
 from __future__ import annotations
@@ -56,6 +56,7 @@ class PagedKVCache:
         self._table = [[-1] * per_row for _ in range(batch)]
         self._free = list(range(n - 1, -1, -1))
         self._rows = [0] * batch
+        self._least = [0] * batch     # rows cannot be rewound below this: pages that it would see were given back
         self._new: list[int] | None = None
 
     @classmethod
@@ -131,8 +132,23 @@ class PagedKVCache:
     def release(self, row: int) -> None:
         """The row ends: its pages come back and its length is 0."""
         self._give_back([(row, j) for j, page in enumerate(self._table[row]) if page >= 0])
-        self._rows[row] = 0
+        self._rows[row] = self._least[row] = 0
         self.seq_lens[row] = 0
+
+    def rewind(self, lengths: list[int]) -> None:
+        """Each row keeps its first lengths[b] tokens (after a verify step: what was accepted); pages behind its new end
+        come back. ValueError, and nothing changed, where a length is not the row's or one before it, or where release_unseen
+        has given back a page that a row of that length would see."""
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != self.batch or any(not 0 <= n <= r for n, r in zip(lengths, self._rows)):
+            raise ValueError(f"rewind needs {self.batch} lengths of at most {self._rows}")
+        for b, (n, r) in enumerate(zip(lengths, self._rows)):
+            if n < r and n < self._least[b]:
+                raise ValueError(f"row {b} cannot go back to {n} tokens: pages that it would see were given back")
+        self._give_back([(b, j) for b, n in enumerate(lengths) for j in range(-(-n // self.page_size), len(self._table[b]))
+                         if self._table[b][j] >= 0])
+        self._rows = lengths
+        self.seq_lens.copy_(torch.tensor(lengths, dtype=torch.int32))
 
     def release_unseen(self, window: int, sinks: int = 0) -> int:
         """Give back the pages that no later query sees where every layer has a window of at most `window` keys and
@@ -143,6 +159,8 @@ class PagedKVCache:
         gone = [(b, j) for b, r in enumerate(self._rows) for j in range(-(-sinks // P), max(0, r - window + 1) // P)
                 if self._table[b][j] >= 0]
         self._give_back(gone)
+        for b, j in gone:
+            self._least[b] = max(self._least[b], (j + 1) * P + window - 1)
         return len(gone)
 
     def _give_back(self, at: list[tuple[int, int]]) -> None:

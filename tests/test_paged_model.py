@@ -461,3 +461,91 @@ def test_a_pass_over_a_paged_cache_is_not_recorded():
     graph.replay()
     torch.cuda.synchronize()
     assert n.item() == 1
+
+
+# ---------------------------------------------------------------- rewinding
+def test_rewind_gives_back_the_pages_behind_the_new_end():
+    c = cache_of()
+    c.set_new([40, 17, 3])
+    c.reserve(40)
+    c.advance(40)
+    assert c.free_pages == 12 - 3 - 2 - 1
+    table = c.page_table.clone()
+    c.rewind([32, 17, 0])
+    assert c.seq_lens_host == [32, 17, 0] == c.seq_lens.tolist() and c.free_pages == 12 - 2 - 2 and c.pos == 32
+    assert torch.equal(c.page_table[0, :2], table[0, :2]) and not (c.page_table[0, 2:] >= 0).any()
+    for bad in ([33, 0, 0], [1, 1], [-1, 0, 0]):
+        with pytest.raises(ValueError, match="rewind"):
+            c.rewind(bad)
+    c.set_new([1, 0, 20])
+    c.reserve(20)
+    c.advance(20)
+    assert c.seq_lens_host == [33, 17, 20] and c.free_pages == 12 - 3 - 2 - 2
+    ids = c.page_table[c.page_table >= 0].tolist()
+    assert len(set(ids)) == len(ids) == 7
+
+
+@pytest.mark.parametrize("window,sinks", [(20, 0), (17, 5), (33, 16)])
+def test_rewind_stops_where_a_page_that_is_gone_would_be_seen(window, sinks):
+    for n in range(60, 100):
+        c = cache_of(batch=1, max_len=200, pages=13)
+        c.set_new([100])
+        c.reserve(100)
+        c.advance(100)
+        c.release_unseen(window, sinks)
+        seen = [s for s in range(n) if s < sinks or s > n - window]   # of the next query, at n
+        whole = all(c.page_table[0, s // 16] >= 0 for s in seen)
+        if whole:
+            c.rewind([n])
+            assert c.seq_lens_host == [n]
+        else:
+            with pytest.raises(ValueError, match="given back"):
+                c.rewind([n])
+            assert c.seq_lens_host == [100] and c.seq_lens.tolist() == [100]
+    c = cache_of(batch=1, max_len=200, pages=13)
+    c.set_new([100])
+    c.reserve(100)
+    c.advance(100)
+    c.release_unseen(window, sinks)
+    c.release(0)
+    assert c.free_pages == 13
+    c.set_new([9])
+    c.reserve(9)
+    c.advance(9)
+    c.rewind([2])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("sliding,sinks", [(False, 0), (True, 3)])
+@torch.no_grad()
+def test_verify_steps_over_pages(device, sliding, sinks):
+    """Guesses, some of them right, verified four tokens at a time for three rows, the rejected ones dropped: each row's
+    tokens are those of generate()."""
+    m = model(config(sliding, sinks), device)
+    prompts, n = PROMPTS[:3], 25
+    alone = [generate(m, p, n).new_ids for p in prompts]
+    cache = PagedKVCache.for_model(m, 3, 128, None, 16, 24)
+    new = [list(p) for p in prompts]
+    cache.set_new([len(p) for p in new])
+    T = max(map(len, new))
+    logits = m(torch.tensor([p + [0] * (T - len(p)) for p in new], device=device), cache=cache).logits
+    out = [[int(logits[b, len(p) - 1].argmax())] for b, p in enumerate(new)]
+    cache.set_new(None)
+    steps = 0
+    while min(map(len, out)) < n:
+        at = cache.seq_lens_host
+        rows = []
+        for b, x in enumerate(out):   # right guesses, but for every third token
+            ahead = [t if (len(x) + i) % 3 else (t + 1) % 64 for i, t in enumerate((alone[b] + [0] * 8)[len(x):len(x) + 3])]
+            rows.append([x[-1]] + (ahead + [0] * 3)[:3])
+        choice = m(torch.tensor(rows, device=device), cache=cache).logits.argmax(-1).tolist()
+        keep = []
+        for b, (row, c) in enumerate(zip(rows, choice)):
+            ok = next((i for i in range(3) if c[i] != row[1 + i]), 3)
+            out[b] += row[1:1 + ok] + [c[ok]]
+            keep.append(at[b] + 1 + ok)
+        cache.rewind(keep)
+        if sliding:
+            cache.release_unseen(20, sinks)
+        steps += 1
+    assert [x[:n] for x in out] == alone and steps < n
