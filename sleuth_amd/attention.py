@@ -517,16 +517,18 @@ class Attention(nn.Module):
 
     def _paged_torch(self, q, cache):
         """Per-row torch attention over a paged cache that holds the new keys: rows past a row's new
-        tokens are zeros, positions without a page are invisible, as in ops.attn_paged."""
+        tokens are zeros, positions without a page are invisible and keys that no query sees unused, as in
+        ops.attn_paged."""
         out = torch.zeros_like(q)
         for b, (L, n) in enumerate(zip(cache.seq_lens_host, cache.new_tokens(q.shape[2]))):
             if not n:
                 continue
             kb, vb, held = cache.row(self.layer_idx, b, L + n)
             rep = self.n_heads // self.n_kv
-            scores = (q[b, :, :n].float() @ kb.repeat_interleave(rep, 0).float().transpose(-2, -1)) * self.scale
             see = self._mask(n, L + n, L, q.device) & held
-            probs = scores.masked_fill(~see, float("-inf")).softmax(-1).nan_to_num(0.0)
+            vb = vb.masked_fill(~see.any(0)[None, :, None], 0)
+            scores = (q[b, :, :n].float() @ kb.repeat_interleave(rep, 0).float().transpose(-2, -1)) * self.scale
+            probs = scores.masked_fill(~see, float("-inf")).softmax(-1).masked_fill(~see.any(-1)[:, None], 0.0)
             if tap_active(self.tap_pattern):
                 probs = self.tap_pattern(probs[None])[0]
             out[b, :, :n] = (probs @ vb.repeat_interleave(rep, 0).float()).to(q.dtype)

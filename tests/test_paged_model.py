@@ -549,3 +549,25 @@ def test_verify_steps_over_pages(device, sliding, sinks):
             cache.release_unseen(20, sinks)
         steps += 1
     assert [x[:n] for x in out] == alone and steps < n
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@torch.no_grad()
+def test_torch_path_over_pages_hides_no_nan_and_takes_none_from_unseen_keys(device, monkeypatch):
+    monkeypatch.setenv("SLEUTH_AMD_NO_HIP", "1")
+    cfg = config(True, 3)
+    att, x, cos, sin = module_and_inputs(cfg, torch.float32, device, 1, 61, 0)
+    want = oracle_layer(att, x, cos, sin, 20, 3)
+    at = torch.arange(61, device=device)[None]
+
+    def last(poison):
+        c = PagedKVCache([(2, 32)], 1, 128, device, torch.float32, 16)
+        att(x[:, :60], cos[at[:, :60]], sin[at[:, :60]], c)
+        c.advance(60)
+        for pos in poison:
+            for pool in (c.k[0], c.v[0]):
+                pool[c.page_table[0, pos // 16], :, pos % 16] = math.nan
+        return att(x[:, 60:], cos[at[:, 60:]], sin[at[:, 60:]], c)
+
+    assert rel(last([3, 20, 40]), want[:, 60:]) < REL[torch.float32]   # between the first tokens and the window
+    assert last([41]).isnan().all() and last([2]).isnan().all()
