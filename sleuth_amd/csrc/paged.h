@@ -84,6 +84,10 @@ constexpr int step_blocks_per_cu(int esize, int D, int rows) {
   return esize * D <= 128 && rows == 16 ? 4 : esize * D <= 256 ? 2 : 1;
 }
 
+// The chunk kernel's: its launch bounds hold the compiler to the registers, its LDS is asserted. (Three at 128 bytes a
+// key: a 512-token chunk at 15,360, 12 q / 4 KV heads of 64, 53 -> 45 us.)
+constexpr int chunk_blocks_per_cu(int esize, int D) { return esize * D >= 1024 ? 1 : esize * D <= 128 ? 3 : 2; }
+
 // How the host cuts a call: rows per block, keys per tile, parts.
 struct PagedPlan {
   bool chunk;    // paged_chunk.hip's kernel (rows 128), or paged.hip's

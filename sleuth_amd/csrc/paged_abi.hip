@@ -67,8 +67,7 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   plan.nparts = 1;
   if (!split) return plan;
   const int64_t tiles = tiles_of(), units = units_of();
-  // (three chunk blocks per CU at head dim 64: a 512-token chunk at 15,360, 12 q / 4 KV heads, 53 -> 45 us)
-  plan.slots = cus * (plan.chunk ? (es * D >= 1024 ? 1 : es * D <= 128 ? 3 : 2) : step_blocks_per_cu(es, D, plan.rows));
+  plan.slots = cus * (plan.chunk ? chunk_blocks_per_cu(es, D) : step_blocks_per_cu(es, D, plan.rows));
   const int64_t slots = plan.slots;
   const int64_t blocks = units / K;
   // (the plan adds up tiles in 32 bits)

@@ -38,7 +38,7 @@ template <typename T, int D> struct ChunkTile {
   static constexpr int LOADS = TILEB / (WAVES * 1024);   // 16-byte loads per lane per tile
   static constexpr int LDS_BYTES = STAGES * 2 * TILEB + (HALVES == 2 ? WAVES * 4096 : 64);  // and sums, or flags
   static constexpr int QS = D / HALVES * (int)sizeof(T) / 32;  // 16-byte pieces of a lane's share of a query row
-  static constexpr int BLOCKS = ROWB >= 1024 ? 1 : 2;    // per CU
+  static constexpr int BLOCKS = chunk_blocks_per_cu(sizeof(T), D);
   static_assert(BLOCKS * LDS_BYTES <= 160 * 1024, "LDS");
 };
 // Chunk swizzles by key row: as prefill_tile.h's in 16 bits; in fp32 a V read is 32 channels of two rows 4 apart.
