@@ -424,7 +424,11 @@ void paged_chunk_kernel(PagedParams p) {
       }
     if constexpr (ES == 4) l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
 
-    // O^T += V^T . P^T (16-bit weights are rounded to the type: the matrix cores take nothing wider beside V)
+    // O^T += V^T . P^T. In 16 bits the weights are rounded to the type once, as the prefill kernels' are: as two numbers
+    // of it, like the split kernel's, they would cost a second product, and products are half of this kernel's time. us,
+    // once / as two, and the outputs' 2-norm error against 64 bits: 512 tokens behind 15,360 80 / 109, 0.0023 / 0.0017 (the
+    // last is the output's own rounding); a ragged batch of chunks 225 / 293; fp16 prompts of 4,093 43 / 59, 0.00026 /
+    // 0.00021; 8,192 tokens with a window of 2,048 144 / 201, 0.0022 / 0.0017.
     if constexpr (ES == 4) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)

@@ -1008,3 +1008,60 @@ def test_partials_of_calls_that_fill_the_device_many_times():
     f = _lib.lib().forge_attn_paged_workspace_bytes
     assert f(_lib.F32, 8, 4096, 32, 8, 32, 32768, 0, 0) == 0
     assert f(_lib.BF16, 64, 1, 16, 8, 128, 32768, 0, 0) > 0 and f(_lib.BF16, 256, 1, 16, 8, 128, 32768, 0, 0) > 0
+
+
+# ---------------------------------------------------------------- the split kernel's weights
+def _pairs(g, dtype, H, K, D, pairs):
+    """Keys in pairs whose scores differ a little and whose values are opposite: a row is a small difference of large
+    terms, so that half a step on a weight shows beside half a step on the output. Small queries: the bound's part for the
+    scores' own roundings, which grows with sum |q k|, is small too."""
+    k = torch.randn(K, 2 * pairs, D, generator=g)
+    k[:, 1::2] = k[:, ::2] * 1.01
+    v = 3 * torch.randn(K, 2 * pairs, D, generator=g)
+    v[:, 1::2] = -v[:, ::2].to(dtype).float()
+    return k.to(dtype), v.to(dtype), (0.1 * torch.randn(H, 1, D, generator=g)).to(dtype)
+
+
+def _two_number_bound(q, k, v, see, scale):
+    """attend64's bound with weights of two numbers of the type: what the second leaves out is half a step of half a step
+    (h * h in place of h)."""
+    want, bound = attend64(q, k, v, see, scale)
+    h = torch.finfo(q.dtype).eps / 2
+    vmax = v.double().abs().masked_fill(~see.any(0)[None, :, None], 0).amax((1, 2))          # [K]
+    return want, bound - (vmax * (h - h * h)).repeat_interleave(q.shape[0] // k.shape[0])[None, :, None]
+
+
+SPLIT = [(BF, 16, 8, 128), (HF, 12, 4, 64), (BF, 8, 1, 256), (BF, 16, 1, 512), (HF, 8, 4, 32)]
+
+
+@pytest.mark.parametrize("dtype,H,K,D", SPLIT)
+def test_the_two_number_bound_tells_weights_rounded_once(dtype, H, K, D):
+    """The oracle's own output with weights rounded once lies outside the bound."""
+    k, v, q = _pairs(gen(51), dtype, H, K, D, 3)
+    see = torch.ones(1, 6, dtype=torch.bool)
+    want, bound = _two_number_bound(q, k, v, see, D ** -0.5)
+    rep = H // K
+    s = (q.double() @ k.double().repeat_interleave(rep, 0).transpose(1, 2)) * D ** -0.5
+    w = (s - s.amax(-1, keepdim=True)).exp()
+    once = ((w.to(dtype).double() @ v.double().repeat_interleave(rep, 0)) / w.sum(-1, keepdim=True)).transpose(0, 1)
+    with pytest.raises(AssertionError, match="outside"):
+        assert_close(once.to(dtype), want, bound)
+    exact = ((w @ v.double().repeat_interleave(rep, 0)) / w.sum(-1, keepdim=True)).transpose(0, 1)
+    assert_close(exact.to(dtype), want, bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,H,K,D", SPLIT)
+@pytest.mark.parametrize("pairs", [1, 3, 40, 700])
+def test_split_weights_are_not_rounded_to_the_type(dtype, H, K, D, pairs):
+    g = gen(52)
+    k, v, q = _pairs(g, dtype, H, K, D, pairs)
+    n = 2 * pairs
+    want, bound = _two_number_bound(q, k, v, torch.ones(1, n, dtype=torch.bool), D ** -0.5)
+    kc, vc = (torch.nn.functional.pad(x, (0, 0, 0, -n % 16))[None].cuda() for x in (k, v))
+    for fixed in (False, True):
+        got = ops.attn_sinks(q[None].cuda(), kc, vc, scale=D ** -0.5, window=4096, sinks=2, pos=n - 1, fixed_cut=fixed)
+        assert_close(got[0], want, bound)
+    kp, vp = (x.view(K, -1, 16, D).transpose(0, 1).contiguous() for x in (kc[0], vc[0]))
+    table = torch.arange(kp.shape[0], dtype=torch.int32, device="cuda")[None]
+    assert_close(ops.attn_paged(q[None].cuda(), kp, vp, table, i32([n - 1]), scale=D ** -0.5)[0], want, bound)
