@@ -172,6 +172,7 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   const int64_t es = dtype == FORGE_F32 ? 4 : 2, e16 = 16 / es;
   for (const int64_t st : {p.sqb, p.sqh, p.sqt, p.skp, p.skh, p.sks, p.sob, p.soh, p.sot})
     if (st < 0 || st % e16) return set_error("strides must be multiples of 16 bytes");
+  if ((p.B > 1 && p.sob == 0) || (p.T > 1 && p.sot == 0) || (p.H > 1 && p.soh == 0)) return set_error("out's rows overlap");
   if (unaligned(p.q) || unaligned(p.k) || unaligned(p.v) || unaligned(p.out))
     return set_error("q, k, v and out must be 16-byte aligned");
   if (p.sks < D || p.sks > INT_MAX / 16 / 64) return set_error("cache positions must be head dim to 2^21 elements apart");
@@ -246,6 +247,7 @@ extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, co
   clear_error();
   if (page_size < 16 || (page_size & (page_size - 1))) return set_error("the page size must be a power of two of at least 16");
   if (n_pages <= 0 || max_pages <= 0 || s_table < 0) return set_error("bad page table sizes");
+  if (flags & FORGE_FIXED_CUT) return set_error("FORGE_FIXED_CUT is for forge_attn_sinks");
   if (max_kv_len <= 0) return set_error("max_kv_len must be positive");
   if (B == 0 || T == 0) return 0;  // (torch's empty tensors have no address)
   if (!page_table || !row_pos) return set_error("null page table or row positions");

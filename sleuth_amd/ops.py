@@ -662,7 +662,8 @@ def _new_token_args(q, cache, scale, q_weight, eps, norm_q, cos, sin, window, si
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty(B, T, H, D, dtype=q.dtype, device=dev)
-    elif out.shape != (B, T, H, D) or out.dtype != q.dtype or out.device != dev or not _aligned(out):
+    elif out.shape != (B, T, H, D) or out.dtype != q.dtype or out.device != dev or not _aligned(out) or \
+            any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
         raise ValueError(f"out must be a 16-byte aligned [B,T,H,D] = {(B, T, H, D)} {q.dtype} on {dev}")
     c, s, s_b, s_t = _rope_tables(cos, sin, B, T, D)
     w = _weight(q_weight, D) if norm_q else None
@@ -691,6 +692,8 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
         if r is not None:
             return r if r.__class__ is not int else check(r, "forge_attn_paged")
     dev = _need_device(q, k_pages, v_pages, page_table, row_pos, new_lens, cos, sin, q_weight if norm_q else None, out)
+    if q.dim() != 4:
+        raise ValueError(f"q {tuple(q.shape)} must be [B, H, T, D]")
     B, T = q.shape[0], q.shape[2]
     table = _pages(k_pages, v_pages, page_table, B, dev)
     rp, nl = _int32_rows(row_pos, B, dev, "row_pos"), _int32_rows(new_lens, B, dev, "new_lens")
@@ -731,7 +734,8 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
         if r is not None:
             return r if r.__class__ is not int else check(r, "forge_attn_sinks")
     dev = _need_device(q, k_cache, v_cache, pos_dev, row_pos, cos, sin, q_weight if norm_q else None, out)
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.dtype != v_cache.dtype or q.shape[0] != k_cache.shape[0]:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.dtype != v_cache.dtype or \
+            q.dim() != 4 or q.shape[0] != k_cache.shape[0]:
         raise ValueError(f"q {tuple(q.shape)} does not fit caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if _strides3(k_cache) != _strides3(v_cache) or not _aligned(k_cache) or not _aligned(v_cache):
         raise ValueError("k and v caches must have the same strides, the last dimension contiguous, 16-byte aligned")

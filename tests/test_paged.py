@@ -1065,3 +1065,24 @@ def test_split_weights_are_not_rounded_to_the_type(dtype, H, K, D, pairs):
     kp, vp = (x.view(K, -1, 16, D).transpose(0, 1).contiguous() for x in (kc[0], vc[0]))
     table = torch.arange(kp.shape[0], dtype=torch.int32, device="cuda")[None]
     assert_close(ops.attn_paged(q[None].cuda(), kp, vp, table, i32([n - 1]), scale=D ** -0.5)[0], want, bound)
+
+
+def test_c_refuses_overlapping_outputs_and_stray_flags():
+    for over in (dict(sob=0), dict(sot=0, T=2, sqt=512), dict(soh=0)):
+        assert _paged_call(**over) < 0 and "overlap" in _lib.lib().forge_last_error().decode()
+    assert _paged_call(flags=_lib.FIXED_CUT) < 0 and "forge_attn_sinks" in _lib.lib().forge_last_error().decode()
+
+
+@pytest.mark.gpu
+def test_ops_refuse_overlapping_outputs_and_q_of_other_ranks():
+    z = lambda *s, dtype=BF: torch.zeros(*s, dtype=dtype, device="cuda")   # noqa: E731
+    q, kp, table, rp, c = z(2, 8, 1, 64), z(4, 4, 16, 64), z(2, 2, dtype=torch.int32), z(2, dtype=torch.int32), z(2, 4, 32, 64)
+    with pytest.raises(ValueError, match="out must"):
+        ops.attn_paged(q, kp, kp, table, rp, scale=1.0, out=z(1, 1, 8, 64).expand(2, 1, 8, 64))
+    with pytest.raises(ValueError, match="out must"):
+        ops.attn_sinks(q, c, c, scale=1.0, window=4, sinks=1, pos=0, out=z(2, 1, 1, 64).expand(2, 1, 8, 64))
+    for bad in (z(8, 64), z(2, 8, 64)):
+        with pytest.raises(ValueError, match="q "):
+            ops.attn_paged(bad, kp, kp, table, rp, scale=1.0)
+        with pytest.raises(ValueError, match="q "):
+            ops.attn_sinks(bad, c, c, scale=1.0, window=4, sinks=1, pos=0)
