@@ -131,7 +131,9 @@ static PagedPlan fixed_plan(int dtype, int B, int T, int H, int K, int D, int64_
                        ((int64_t)sinks + plan.keys - 1) / plan.keys;
   const int64_t tiles = seen < all ? seen : all, units = (int64_t)B * K * ((G + 15) / 16);
   const int64_t slots = (int64_t)device_cus() * step_blocks_per_cu(es, D, 16);
-  int64_t parts = slots / units, most = tiles / (es * D >= 512 ? 4 : 8);   // (at least as many tiles a part as below)
+  // Two tiles at most for each wave, one of the long ones, where the device has room for that many blocks.
+  const int64_t least = es * D >= 512 ? 4 : 8, most = (tiles + least - 1) / least;
+  int64_t parts = slots / units;
   if (parts > most) parts = most;
   plan.nparts = (int)(parts < 1 ? 1 : parts > 4096 ? 4096 : parts);
   return plan;
