@@ -405,7 +405,7 @@ class Attention(nn.Module):
             kp, vp = cache.k[self.layer_idx], cache.v[self.layer_idx]
             ops.kv_append_paged(k, v, kp, vp, *where, new_lens=cache.new_lens, norm_v=norm_v, **k_args)
             self.last_path = "hip-paged"
-            return ops.attn_paged(q, kp, vp, *where, scale=self.scale, new_lens=cache.new_lens, max_kv_len=cache.top(T),
+            return ops.attn_paged(q, kp, vp, *where, scale=self.scale, new_lens=cache.new_lens, max_kv_len=cache.bound(T),
                                   window=self.window, sinks=self.sinks, **q_args)
 
         if cache is None:

@@ -5,8 +5,8 @@ K and V are pools [n_pages, K, page_size, hd]; position s of row b is slot s % p
 page_table[b, s // page_size], the same page of every layer's pools. Pages are handed out as rows grow (reserve), and
 come back when a row ends (release) or when no layer can see them any more (release_unseen: every layer slides, and
 keeps its first tokens). The table and the lengths live on the device in fixed buffers, so a recorded graph of the
-operators (kv_append_paged, attn_paged, with a max_kv_len for all its replays) sees them change. A whole pass cannot be
-recorded: which pages it needs and how long the rows are is the host's to say, and reserve refuses it.
+operators or of the layers sees them change. What is the host's to say stays outside of it: reserve before a replay,
+advance after it (both refuse to be recorded).
 
 It speaks the cache protocol of the package's callers (pos, max_len, advance, seq_lens, seq_lens_host, update; `ragged`
 is always true, `static` never; pos is read only, since rows differ: rewind takes each row's length) and adds `paged`,
@@ -107,13 +107,18 @@ class PagedKVCache:
         """The longest row once a pass of T tokens is in."""
         return max(1, max(r + n for r, n in zip(self._rows, self.new_tokens(T))))
 
+    def bound(self, T: int) -> int:
+        """max_kv_len of a pass of T tokens: top(T), or, for a graph that is being recorded, all that the cache holds: its
+        replays see longer rows."""
+        return self.max_len if self._recording() else self.top(T)
+
+    def _recording(self) -> bool:
+        return self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
     # ------------------------------------------------------------------ pages
     def reserve(self, T: int) -> None:
         """Pages for the next pass's real tokens (every layer of a pass may call it: the first one acts). Raises
         ValueError where a row would pass max_len, OutOfPages where the pool has no page left; nothing is handed out then."""
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            # (its max_kv_len would be today's in every replay, and the rows' lengths on the host would stand still)
-            raise RuntimeError("a pass over a paged cache cannot be recorded: record ops.kv_append_paged and attn_paged")
         P = self.page_size
         need = []
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
@@ -123,6 +128,8 @@ class PagedKVCache:
                 need += [(b, j) for j in range(r // P, (r + n - 1) // P + 1) if self._table[b][j] < 0]
         if not need:
             return
+        if self._recording():
+            raise RuntimeError("reserve a paged cache's pages before recording a graph")
         if len(need) > len(self._free):
             raise OutOfPages(f"KV cache out of pages ({len(need)} needed, {len(self._free)} of {self.n_pages} free)")
         for b, j in need:
@@ -205,6 +212,8 @@ class PagedKVCache:
 
     def advance(self, n: int) -> None:
         """All layers have stored this pass's tokens."""
+        if self._recording():
+            raise RuntimeError("advance a paged cache outside of a recorded graph: its lengths are the host's too")
         new = self.new_tokens(n)
         self._rows = [r + x for r, x in zip(self._rows, new)]
         if self._new is None:

@@ -440,27 +440,57 @@ def test_a_prompt_past_the_models_length_is_refused_before_any_pass():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sliding,sinks", [(False, 0), (True, 3)])
 @torch.no_grad()
-def test_a_pass_over_a_paged_cache_is_not_recorded():
-    """Its replays would see no key past the lengths of the day it was recorded."""
-    cfg = config()
-    att, x, cos, sin = module_and_inputs(cfg, torch.bfloat16, "cuda", 1, 20, 0)
-    cache = PagedKVCache([(2, 32)], 1, 128, "cuda", torch.bfloat16, 16)
+def test_a_recorded_layer_over_pages_sees_the_rows_grow(sliding, sinks):
+    """Recorded at 19 and 5 tokens, replayed up to 100: reserve before each replay, advance after it."""
+    cfg = config(sliding, sinks, head_size=64)
+    att, x, cos, sin = module_and_inputs(cfg, torch.bfloat16, "cuda", 2, 100, 0)
+    want = oracle_layer(att, x, cos, sin, cfg.sliding_window, sinks)
+    cache = PagedKVCache([(2, 64)], 2, 128, "cuda", torch.bfloat16, 16)
+    cache.set_new([19, 5])
     at = torch.arange(19, device="cuda")[None]
     att(x[:, :19], cos[at], sin[at], cache)
     cache.advance(19)
-    last, n = x[:, 19:], torch.zeros(1, device="cuda")
-    c, s = cos[19:20][None], sin[19:20][None]
-    att(last, c, s, cache)
+    cache.set_new(None)
+    step, c, s = x[:, 19:20].clone(), cos[:1].repeat(2, 1, 1), sin[:1].repeat(2, 1, 1)
+    cache.reserve(1)
+    att(step, c, s, cache)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        n.add_(1)
-        with pytest.raises(RuntimeError, match="cannot be recorded"):
-            att(last, c, s, cache)
-    graph.replay()
+        y = att(step, c, s, cache)
+        with pytest.raises(RuntimeError, match="advance"):
+            cache.advance(1)
+        with pytest.raises(RuntimeError, match="reserve"):
+            cache.reserve(60)
+    assert cache.seq_lens_host == [19, 5] == cache.seq_lens.tolist()
+    for _ in range(81):
+        rows = cache.seq_lens_host
+        cache.reserve(1)
+        step.copy_(torch.stack([x[b, n:n + 1] for b, n in enumerate(rows)]))
+        c.copy_(cos[rows][:, None])
+        s.copy_(sin[rows][:, None])
+        graph.replay()
+        cache.advance(1)
+        for b, n in enumerate(rows):
+            assert rel(y[b], want[b, n:n + 1]) < REL[torch.bfloat16], (rows, b)
+
+
+@pytest.mark.gpu
+@torch.no_grad()
+def test_a_whole_models_pass_over_pages_is_not_recorded():
+    m = model(config(), "cuda", torch.bfloat16)
+    cache = PagedKVCache.for_model(m, 1, 128, None, 16)
+    ids = torch.tensor([[3]], device="cuda")
+    m(ids, cache=cache)
     torch.cuda.synchronize()
-    assert n.item() == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="advance"):
+            m(ids, cache=cache)
+    torch.cuda.synchronize()
+    assert cache.seq_lens_host == [1] == cache.seq_lens.tolist()
 
 
 # ---------------------------------------------------------------- rewinding
