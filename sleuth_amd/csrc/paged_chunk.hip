@@ -7,7 +7,7 @@
 // two LDS stages, as the causal prefill kernel does: direct loads into LDS in swizzled chunk order, S^T = K . Q^T
 // with Q^T in registers, one lane per query row (two lanes share a row's keys), P^T fed to O^T = V^T . P^T straight
 // from the score registers. Bound by the matrix units and the softmax's VALU work, which take turns on a SIMD: 512 tokens
-// behind 15,360 at head dim 128 78 us (832 TFLOP/s, 0.72 of a large library product; 0.47 of the cycles MFMA, 0.41 VALU),
+// behind 15,360 at head dim 128 80 us (817 TFLOP/s, 0.59 of a large library product; 0.48 of the cycles MFMA, 0.41 VALU),
 // two prompts of 8,192 506 us at head dim 256 (1,086 TFLOP/s), 562 at 128, 317 at 64.
 // See prefill.hip for the operand layouts; what differs here:
 //   * A wave loads RW (BN / 4, or / 8) consecutive key rows of a tile, which never straddle pages (pages are multiples of 16
