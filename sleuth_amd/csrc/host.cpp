@@ -578,6 +578,7 @@ PyObject* attn_sinks_impl(PyObject* const* a) {
   {
     NoGil unlocked;
     n.allocate(kept);
+    if ((n.flags & FORGE_FIXED_CUT) && n.need && !kept && !n.ws.defined()) return nullptr;   // (raised the Python way)
     st = forge_attn_sinks(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w,
                           n.eps, n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kc), ptr(vc), sk[0], sk[1],
                           max_len > 1 ? sk[2] : n.D, max_len, static_cast<const int32_t*>(ptr(row_pos)),

@@ -762,6 +762,8 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
         if fixed_cut:
             args = (*args[:12], args[12] | FIXED_CUT, *args[13:])
         ws = _PagedPartials(dev, need)
+        if fixed_cut and need and ws.ws is None:   # (unsplit, its bits would be others)
+            raise torch.cuda.OutOfMemoryError(f"attn_sinks: no memory for {need} bytes of partials, which fixed_cut needs")
         st = lib().forge_attn_sinks(*args, _ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache), max_len, _ptr(rp), _ptr(pd),
                                     p0, max_kv_len, int(window), int(sinks), float(scale), _ptr(out), *_strides3(out),
                                     *ws.args(), _stream(dev))

@@ -1086,3 +1086,18 @@ def test_ops_refuse_overlapping_outputs_and_q_of_other_ranks():
             ops.attn_paged(bad, kp, kp, table, rp, scale=1.0)
         with pytest.raises(ValueError, match="q "):
             ops.attn_sinks(bad, c, c, scale=1.0, window=4, sinks=1, pos=0)
+
+
+@pytest.mark.gpu
+def test_fixed_cut_without_memory_for_its_partials_raises(monkeypatch):
+    """Unsplit, the call's bits would be others."""
+    from types import SimpleNamespace
+
+    c, q = torch.zeros(1, 8, 2000, 128, dtype=BF, device="cuda"), torch.zeros(1, 16, 1, 128, dtype=BF, device="cuda")
+    kw = dict(scale=1.0, window=1024, sinks=4, pos=1500)
+    monkeypatch.setattr(ops, "host", lambda: SimpleNamespace(attn_sinks=lambda *a: None))
+    monkeypatch.setattr(ops, "_PAGED_WS_KEPT", 0)
+    monkeypatch.setattr(ops, "_partials", lambda need, dev: None)
+    ops.attn_sinks(q, c, c, **kw)   # (not split)
+    with pytest.raises(torch.cuda.OutOfMemoryError, match="fixed_cut"):
+        ops.attn_sinks(q, c, c, fixed_cut=True, **kw)
