@@ -10,7 +10,7 @@ advance after it (both refuse to be recorded).
 
 It speaks the cache protocol of the package's callers (pos, max_len, advance, seq_lens, seq_lens_host, update; `ragged`
 is always true, `static` never; pos is read only, since rows differ: rewind takes each row's length) and adds `paged`,
-page_table, new_lens, reserve, top and row, which the attention module uses (ops.kv_append_paged, ops.attn_paged).
+page_table, new_lens, reserve, top, bound and row, which the attention module uses (ops.kv_append_paged, ops.attn_paged).
 """
 
 from __future__ import annotations
