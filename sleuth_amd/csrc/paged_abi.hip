@@ -115,9 +115,10 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
 // A step whose sums must not hang on how many tokens it has, or on the bound of its keys: everything as for one token
 // of rows that hold all that the cache can (max_len) or the window lets them see. Where a call's query rows are more
 // than a block's, 32 rows a block read the keys half as often, if their tiles are the same. What it costs (us, free /
-// fixed cut, window 1,024): a token of 16 rows, 8 KV heads of 128, 18.4 / 18.5; 5 tokens of 8 rows there 12.1 / 11.8; 4 of 8
-// rows, one KV head of 256 with 8 query heads, 11.5 / 12.9. Verify steps of many rows, which the chunk kernel would take,
-// pay most: 5 tokens of 32 rows, 28 q / 4 KV heads of 128, 23.2 / 32.8; 8 of 16 rows, 16 q / 1 KV head of 512, 35 / 125.
+// fixed cut, window 1,024): a token of 16 rows, 8 KV heads of 128, 17.2 / 18.1, of one row 9.0 / 9.0; 5 tokens of 8 rows there
+// 13.1 / 13.6; 4 of 8 rows, one KV head of 256 with 8 query heads, 12.2 / 13.9. Verify steps of many rows, which the chunk
+// kernel would take, pay most: 5 tokens of 32 rows, 28 q / 4 KV heads of 128, 24.3 / 33.3; 8 of 16 rows, 16 q / 1 KV head of
+// 512, 36 / 124.
 static PagedPlan fixed_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_len, int window, int sinks, bool split) {
   PagedPlan plan{};
   const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K;
