@@ -354,6 +354,99 @@ int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, const void* q
                      void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
                      size_t workspace_bytes, int ws_flags, void* stream);
 
+/*
+ * ---- Trees of drafted tokens (no counterpart in the reference, whose speculative decoder verifies one chain,
+ * speculative.py:83-277). A step's T new tokens of a row are the nodes of a tree: token t was drafted behind
+ * an earlier one, parents[t], whose keys and its ancestors' it sees beside the cache. New tokens take the slots
+ * base .. base + T - 1 in their own order; their positions are base + depth.
+ *
+ * forge_tree_mask: parents [B, T] int32 (row stride s_parents_b; 0: one tree for all rows) -> mask
+ * [B, T, ceil(T / 64)], bit j % 64 of word j / 64 set where token t sees new token j (itself and its ancestors),
+ * and depth [B, T], how many ancestors it has. A parent outside [0, t) is none: the token hangs on the cache
+ * alone. Rows' nodes from new_lens[b] on (NULL: none) get no bit and depth 0. At most FORGE_TREE_MAX_TOKENS.
+ */
+#define FORGE_TREE_MAX_TOKENS 1024
+int forge_tree_mask(int B, int T, const int32_t* parents, int64_t s_parents_b,
+                    const int32_t* new_lens, int64_t* mask, int32_t* depth, void* stream);
+
+/*
+ * Attention of a drafted tree's T new tokens per row over a cache that holds them already, paged as in
+ * forge_attn_paged (page_table not NULL, row_pos required) or contiguous as in forge_attn_sinks (page_table NULL:
+ * n_pages and max_pages unused, page_size the rows' length, skp the batch stride, and row_pos, pos_dev or pos0).
+ * Query t of row b sees the keys before the row's first new token, base, and the new tokens j whose bit is
+ * set in mask[b][t] (any mask: also of later tokens, or none), padding (j >= new_lens[b]) never. With a window > 0
+ * positions count, s for a key of the cache, base + depth[j] for new token j: a key is seen within the window,
+ * position > base + depth[t] - window, or where its position is below `sinks`. depth: [B, T] int32 (row stride
+ * s_depth_b), taken into [0, new_lens[b]); only read with a window. mask and depth strides may be 0 (one tree for
+ * all rows). Rows that see nothing, and padding, come out as zeros. Everything else as forge_attn_paged;
+ * max_kv_len bounds base + new_lens.
+ * No key that a query does not see reaches it, whatever its bits: a branch with an infinity or a NaN among its
+ * values leaves the others alone.
+ */
+size_t forge_attn_tree_workspace_bytes(int dtype, int B, int T, int H, int K, int D,
+                                       int64_t max_kv_len, int window, int sinks);
+int forge_attn_tree(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb,
+                    int64_t sqh, int64_t sqt, const float* q_weight, float eps, int flags,
+                    const float* cos, const float* sin, int64_t s_cos_b, int64_t s_cos_t,
+                    const void* k_cache, const void* v_cache, int64_t skp, int64_t skh,
+                    int64_t sks, int n_pages, int64_t page_size, const int32_t* page_table,
+                    int64_t s_table, int max_pages, const int32_t* row_pos,
+                    const int64_t* pos_dev, int64_t pos0, const int32_t* new_lens,
+                    int64_t max_kv_len, int window, int sinks, float scale, const int64_t* mask,
+                    int64_t s_mask_b, int64_t s_mask_t, const int32_t* depth, int64_t s_depth_b,
+                    void* out, int64_t sob, int64_t sot, int64_t soh, void* workspace,
+                    size_t workspace_bytes, int ws_flags, void* stream);
+
+/*
+ * Verification of drafted tokens against the target's logits [B, T, V] (strides s_logits_b, s_logits_t; the last
+ * dimension contiguous): logits[b][t] is what the target says behind node t. Node 0 is the row's last token that
+ * stands; tokens [B, T] int64 (token 0 is not read), parents [B, T] int32 (NULL: a chain, t - 1). From node 0 on
+ * the children of a node, in order, are accepted or rejected as samples of the target at temperature
+ * temperatures[b] (NULL: `temperature`), with uniform[b][t] in [0, 1) deciding on node t and uniform[b][0] drawing the
+ * token behind the last accepted one from what the rejections leave of the target's probabilities: accepted
+ * children and that token are distributed as the target's samples. Temperature 0 (in `temperatures` also what is
+ * negative or no number): the argmax decides, the lowest index of equal ones; uniform may be NULL if all rows are so.
+ * draft_probs [B, >= T - 1, V] (probs_dtype: fp32, or the logits' type): what the drafter's children of node t were
+ * drawn from, independently; NULL: drafted tokens were not drawn (a search, a drafter's likeliest), siblings differ
+ * (a token that an earlier sibling has already is never accepted). A logit of -inf has probability 0, as a NaN;
+ * +inf logits share it all. Where rejections leave nothing, the token is the target's argmax. Tokens outside [0, V)
+ * and nodes whose parent is not before them are passed over, nodes from new_lens[b] on do not exist.
+ * Out: count[b] how many nodes stand, node 0 included (0 for a row without nodes); path [B, T] int32 those nodes in
+ * order; out [B, T] int64 the row's count[b] new tokens (the accepted ones', then the drawn one); -1 behind them.
+ * All sums in 64 bits. workspace: forge_verify_drafts_workspace_bytes(...) bytes, 256-byte aligned, separate for calls
+ * that may overlap. V at most 2^22 - 8.
+ */
+size_t forge_verify_drafts_workspace_bytes(int B, int T, int V, int draft_probs);
+int forge_verify_drafts(int dtype, int B, int T, int V, const void* logits, int64_t s_logits_b,
+                        int64_t s_logits_t, const int64_t* tokens, int64_t s_tokens_b,
+                        const int32_t* parents, int64_t s_parents_b, const float* uniform,
+                        int64_t s_uniform_b, const float* temperatures, double temperature,
+                        int probs_dtype, const void* draft_probs, int64_t s_probs_b,
+                        int64_t s_probs_t, const int32_t* new_lens, int64_t* out, int32_t* path,
+                        int32_t* count, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Moves within the caches of `layers` layers of one shape (k, v: host arrays of device pointers, read during the
+ * call; esize 2 or 4 bytes an element, D * esize a multiple of 16, 16-byte aligned tensors and strides).
+ *
+ * forge_kv_compact: an accepted branch closes up. Slot base + i of row b takes the key and value of slot base +
+ * path[b][i], for i < counts[b]; path as forge_verify_drafts leaves it (rising; an entry below its place i, or beyond the
+ * cache, moves nothing, nor do positions without a page). Cache arguments as in forge_attn_tree. Rows must not share the
+ * pages that are written.
+ * forge_copy_pages: page dst[i] takes what page src[i] holds, i < n, in K and V of every layer (pools as in
+ * forge_attn_paged). Numbers outside the pool copy nothing. No page may be named in dst twice, or in both src and dst of
+ * different i.
+ */
+int forge_kv_compact(int esize, int layers, int B, int K, int D, const void* const* k,
+                     const void* const* v, int64_t skp, int64_t skh, int64_t sks, int n_pages,
+                     int64_t page_size, const int32_t* page_table, int64_t s_table, int max_pages,
+                     const int32_t* row_pos, const int64_t* pos_dev, int64_t pos0,
+                     const int32_t* path, int64_t s_path, int T, const int32_t* counts,
+                     void* stream);
+int forge_copy_pages(int esize, int layers, int K, int D, const void* const* k,
+                     const void* const* v, int64_t skp, int64_t skh, int64_t sks, int n_pages,
+                     int page_size, int n, const int32_t* src, const int32_t* dst, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

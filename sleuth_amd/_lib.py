@@ -171,6 +171,43 @@ SIGNATURES: dict[str, tuple] = {
         _p, _i64, _i64, _i64,                # out + strides (b, t, h)
         _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
         _p]),
+    "forge_tree_mask": (_i, [_i, _i, _p, _i64, _p, _p, _p, _p]),   # B, T, parents, stride, new_lens, mask, depth
+    "forge_attn_tree_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i, _i, _i, _i64, _i, _i]),
+    "forge_attn_tree": (_i, [
+        _i, _i, _i, _i, _i, _i,              # dtype, B, T, H, K, D
+        _p, _i64, _i64, _i64,                # q + strides
+        _p, _f, _i,                          # q_weight, eps, flags
+        _p, _p, _i64, _i64,                  # cos, sin, s_cos_b, s_cos_t
+        _p, _p, _i64, _i64, _i64,            # k_cache, v_cache, skp, skh, sks
+        _i, _i64, _p, _i64, _i,              # n_pages, page_size, page_table, s_table, max_pages
+        _p, _p, _i64, _p, _i64,              # row_pos, pos_dev, pos0, new_lens, max_kv_len
+        _i, _i, _f,                          # window, sinks, scale
+        _p, _i64, _i64, _p, _i64,            # mask + strides (b, t), depth, its row stride
+        _p, _i64, _i64, _i64,                # out + strides (b, t, h)
+        _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
+        _p]),
+    "forge_verify_drafts_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i]),
+    "forge_verify_drafts": (_i, [
+        _i, _i, _i, _i,                      # dtype, B, T, V
+        _p, _i64, _i64,                      # logits + strides (b, t)
+        _p, _i64, _p, _i64, _p, _i64,        # tokens, parents, uniform, each with its row stride
+        _p, C.c_double,                      # temperatures or None, temperature
+        _i, _p, _i64, _i64,                  # dtype of draft_probs, draft_probs or None + strides (b, t)
+        _p, _p, _p, _p,                      # new_lens, out, path, count
+        _p, C.c_size_t,                      # workspace, bytes
+        _p]),
+    "forge_kv_compact": (_i, [
+        _i, _i, _i, _i, _i,                  # element size, layers, B, K, D
+        _p, _p, _i64, _i64, _i64,            # host arrays of K's and V's pointers, strides
+        _i, _i64, _p, _i64, _i,              # n_pages, page_size, page_table, s_table, max_pages
+        _p, _p, _i64,                        # row_pos, pos_dev, pos0
+        _p, _i64, _i, _p,                    # path, row stride, T, counts
+        _p]),
+    "forge_copy_pages": (_i, [
+        _i, _i, _i, _i,                      # element size, layers, K, D
+        _p, _p, _i64, _i64, _i64,            # host arrays of K's and V's pointers, strides
+        _i, _i, _i, _p, _p,                  # n_pages, page_size, n, src, dst
+        _p]),
 }
 
 _lock = threading.Lock()

@@ -22,8 +22,8 @@ LIB_NAME = "libforge_attn.so"
 HOST_NAME = "_forge_host.so"
 # (source, defines, object name); decode.hip's and the paged kernels are built per dtype, side by side
 SOURCES = [("abi.hip", [], "abi"), ("prep.hip", [], "prep"), ("prefill.hip", [], "prefill"), ("linear.hip", [], "linear"),
-           ("paged_abi.hip", [], "paged_abi"),
-           *((f"{k}.hip", [f"-DFORGE_PAGED_PART={n}"], f"{k}{n}") for k in ("paged", "paged_chunk") for n in range(1, 4)),
+           ("paged_abi.hip", [], "paged_abi"), ("tree.hip", [], "tree"), ("verify.hip", [], "verify"),
+           *((f"{k}.hip", [f"-DFORGE_PAGED_PART={n}"], f"{k}{n}") for k in ("paged", "paged_chunk") for n in range(1, 7)),
            *(("decode.hip", [f"-DFORGE_DECODE_PART={n}"], f"decode{n}") for n in range(4))]
 ARCH = "gfx950"
 

@@ -468,8 +468,9 @@ struct NewTokens {
     if (!rope_ok(cos, sin, B, T, D, dev, r) || !gain_ok(qw, D, dev) || (uintptr_t)ptr(qw) % 16) return false;
     return true;
   }
-  void size(int64_t K, int64_t max_kv) {
-    need = forge_attn_paged_workspace_bytes(dt, (int)B, (int)T, (int)H, (int)K, (int)D, max_kv, (int)window, (int)sinks);
+  void size(int64_t K, int64_t max_kv, bool tree = false) {
+    need = (tree ? forge_attn_tree_workspace_bytes : forge_attn_paged_workspace_bytes)(
+        dt, (int)B, (int)T, (int)H, (int)K, (int)D, max_kv, (int)window, (int)sinks);
   }
   // Calls of few partials outside graph capture use their stream's workspace (ops._PagedPartials)
   bool keep() const { return need && need <= ((size_t)32 << 20) && !capturing(); }
@@ -591,6 +592,322 @@ PyObject* attn_sinks_impl(PyObject* const* a) {
   return st < 0 ? nullptr : result(st, n.out);
 }
 
+// A tree's bits [B, T, words] or [T, words] and depths [B, T] or [T] (ops._tree_args)
+struct Tree {
+  Tensor mask, depth, news;
+  int64_t mb = 0, mt = 0, db = 0;
+  bool ok(int64_t B, int64_t T, int64_t window, c10::Device dev) {
+    const int64_t words = (T + 63) / 64, d = mask.dim();
+    if (T > FORGE_TREE_MAX_TOKENS || mask.scalar_type() != at::kLong || mask.device() != dev || (d != 2 && d != 3) ||
+        mask.size(d - 1) != words || mask.size(d - 2) != T || (d == 3 && mask.size(0) != B) ||
+        (words > 1 && mask.stride(d - 1) != 1) || (window && !depth.defined()))
+      return false;
+    mt = T > 1 ? mask.stride(d - 2) : 0;
+    mb = d == 3 && B > 1 ? mask.stride(0) : 0;
+    if (mt < 0 || mb < 0) return false;
+    if (depth.defined()) {
+      const int64_t e = depth.dim();
+      if (depth.scalar_type() != at::kInt || depth.device() != dev || (e != 1 && e != 2) || depth.size(e - 1) != T ||
+          (e == 2 && depth.size(0) != B) || (T > 1 && depth.stride(e - 1) != 1))
+        return false;
+      db = e == 2 && B > 1 ? depth.stride(0) : 0;
+    }
+    return !news.defined() || rows_ok(news, B, dev);
+  }
+};
+
+// What attn_tree and attn_tree_paged share once their caches are checked.
+PyObject* launch_tree(PyObject* table, NewTokens& n, Tree& t, const Tensor& kc, const Tensor& vc, const int64_t (&sk)[3],
+                      int64_t sks, int n_pages, int64_t page_size, const Tensor& pages, int64_t s_table, int64_t max_pages,
+                      const Tensor& row_pos, const Tensor& pos_dev, int64_t pos, int64_t max_kv, bool norm_q) {
+  const c10::Device dev = n.q.device();
+  const int64_t K = kc.size(1);
+  n.set_flags(norm_q);
+  n.size(K, max_kv, true);
+  const bool kept = n.keep();
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  StreamWorkspace ws(table, dev.index(), stream, kept ? n.need : 0);
+  if (kept && !ws.ptr) return nullptr;   // (made the Python way)
+  int st;
+  {
+    NoGil unlocked;
+    n.allocate(kept);
+    st = forge_attn_tree(n.dt, (int)n.B, (int)n.T, (int)n.H, (int)K, (int)n.D, ptr(n.q), n.sq[0], n.sq[1], n.sq[2], n.w, n.eps,
+                         n.flags, n.r.cos, n.r.sin, n.r.sb, n.r.st, ptr(kc), ptr(vc), sk[0], sk[1], sks, n_pages, page_size,
+                         static_cast<const int32_t*>(ptr(pages)), s_table, (int)max_pages,
+                         static_cast<const int32_t*>(ptr(row_pos)), static_cast<const int64_t*>(ptr(pos_dev)), pos,
+                         static_cast<const int32_t*>(ptr(t.news)), max_kv, (int)n.window, (int)n.sinks, n.scale,
+                         static_cast<const int64_t*>(ptr(t.mask)), t.mb, t.mt, static_cast<const int32_t*>(ptr(t.depth)), t.db,
+                         n.out.data_ptr(), n.out.stride(0), n.out.stride(1), n.out.stride(2),
+                         kept ? ws.ptr : n.ws.defined() ? n.ws.data_ptr() : nullptr, kept ? ws.bytes : n.need,
+                         kept ? FORGE_WS_ZEROED : 0, stream);
+  }
+  if (st == 0) ws.put_back();
+  return st < 0 ? nullptr : result(st, n.out);
+}
+
+// attn_tree(table of workspaces, q, k_cache, v_cache, mask, scale, pos | None, pos_dev | None, row_pos | None, depth | None,
+//           new_lens | None, max_kv_len | None, window, sinks, q_weight | None, eps, norm_q, cos | None, sin | None)
+PyObject* attn_tree_impl(PyObject* const* a) {
+  NewTokens n;
+  Tree t;
+  Tensor kc, vc, pos_dev, row_pos;
+  int64_t pos = 0, max_kv = INT64_MAX, sk[3], sv[3];
+  if (!take(a[1], n.q) || !take(a[2], kc) || !take(a[3], vc) || !take(a[4], t.mask) || !as_float(a[5], n.scale) ||
+      (a[6] != Py_None && !as_int(a[6], pos)) || !take_opt(a[7], pos_dev) || !take_opt(a[8], row_pos) ||
+      !take_opt(a[9], t.depth) || !take_opt(a[10], t.news) || (a[11] != Py_None && !as_int(a[11], max_kv)) ||
+      !as_int(a[12], n.window) || !as_int(a[13], n.sinks) || !take_opt(a[14], n.qw) || !as_float(a[15], n.eps) ||
+      !take_opt(a[17], n.cos) || !take_opt(a[18], n.sin))
+    return nullptr;
+  if (!n.take_args(kc) || (a[6] != Py_None) + pos_dev.defined() + row_pos.defined() > 1) return nullptr;
+  const c10::Device dev = n.q.device();
+  if (kc.sizes() != vc.sizes() || kc.scalar_type() != vc.scalar_type() || kc.device() != dev || vc.device() != dev ||
+      kc.size(0) != n.B || !strides16(kc, sk) || !strides16(vc, sv) || !std::equal(sk, sk + 3, sv) ||
+      !t.ok(n.B, n.T, n.window, dev))
+    return nullptr;
+  const int64_t max_len = kc.size(2);
+  if (row_pos.defined()) {
+    if (!rows_ok(row_pos, n.B, dev)) return nullptr;
+  } else if (pos_dev.defined()) {
+    if (pos_dev.scalar_type() != at::kLong || pos_dev.numel() < 1 || pos_dev.device() != dev) return nullptr;
+  } else {
+    if (pos < 0 || pos > max_len - n.T) return nullptr;
+    max_kv = pos + n.T;
+  }
+  max_kv = std::min(max_kv, max_len);
+  if (max_kv < 1) return nullptr;
+  return launch_tree(a[0], n, t, kc, vc, sk, max_len > 1 ? sk[2] : n.D, 1, max_len, Tensor(), 0, 0, row_pos, pos_dev, pos, max_kv,
+                     a[16] == Py_True);
+}
+
+// attn_tree_paged(table of workspaces, q, k_pages, v_pages, table, row_pos, mask, scale, depth | None, new_lens | None,
+//                 max_kv_len | None, window, sinks, q_weight | None, eps, norm_q, cos | None, sin | None)
+PyObject* attn_tree_paged_impl(PyObject* const* a) {
+  NewTokens n;
+  Tree t;
+  Tensor kp, vp, table, row_pos;
+  int64_t max_kv = INT64_MAX;
+  if (!take(a[1], n.q) || !take(a[2], kp) || !take(a[3], vp) || !take(a[4], table) || !take(a[5], row_pos) ||
+      !take(a[6], t.mask) || !as_float(a[7], n.scale) || !take_opt(a[8], t.depth) || !take_opt(a[9], t.news) ||
+      (a[10] != Py_None && !as_int(a[10], max_kv)) || !as_int(a[11], n.window) || !as_int(a[12], n.sinks) ||
+      !take_opt(a[13], n.qw) || !as_float(a[14], n.eps) || !take_opt(a[16], n.cos) || !take_opt(a[17], n.sin))
+    return nullptr;
+  if (!n.take_args(kp)) return nullptr;
+  const c10::Device dev = n.q.device();
+  Pages p;
+  if (!pages_ok(kp, vp, table, n.B, dev, p) || !rows_ok(row_pos, n.B, dev) || !t.ok(n.B, n.T, n.window, dev)) return nullptr;
+  max_kv = std::min(max_kv, p.max * p.size);
+  if (max_kv < 1) return nullptr;
+  return launch_tree(a[0], n, t, kp, vp, p.s, p.s[2], p.n, p.size, table, p.stride, p.max, row_pos, Tensor(), 0, max_kv,
+                     a[15] == Py_True);
+}
+
+PyObject* tuple_of(std::initializer_list<Tensor> ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  Py_ssize_t i = 0;
+  for (const Tensor& t : ts)
+    if (r) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t));
+  return r;
+}
+
+// tree_mask(parents, new_lens | None)
+PyObject* tree_mask_impl(PyObject* const* a) {
+  Tensor parents, news;
+  if (!take(a[0], parents) || !take_opt(a[1], news)) return nullptr;
+  const c10::Device dev = parents.device();
+  if (parents.scalar_type() != at::kInt || parents.dim() != 2 || c10::hip::current_device() != dev.index()) return nullptr;
+  const int64_t B = parents.size(0), T = parents.size(1);
+  if (B < 1 || B > INT_MAX || T < 1 || T > FORGE_TREE_MAX_TOKENS || (T > 1 && parents.stride(1) != 1) ||
+      (news.defined() && !rows_ok(news, B, dev)))
+    return nullptr;
+  Tensor mask, depth;
+  int st;
+  {
+    NoGil unlocked;
+    mask = at::empty({B, T, (T + 63) / 64}, parents.options().dtype(at::kLong));
+    depth = at::empty({B, T}, parents.options());
+    st = forge_tree_mask((int)B, (int)T, static_cast<const int32_t*>(ptr(parents)), B > 1 ? parents.stride(0) : 0,
+                         static_cast<const int32_t*>(ptr(news)), static_cast<int64_t*>(mask.data_ptr()),
+                         static_cast<int32_t*>(depth.data_ptr()), c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  if (st) return st < 0 ? nullptr : PyLong_FromLong(st);
+  return tuple_of({mask, depth});
+}
+
+// [B, T] of a type on dev with its rows contiguous, or undefined
+bool rows2_ok(const Tensor& t, at::ScalarType type, int64_t B, int64_t T, c10::Device dev, int64_t& stride) {
+  stride = 0;
+  if (!t.defined()) return true;
+  if (t.scalar_type() != type || t.dim() != 2 || t.size(0) != B || t.size(1) != T || t.device() != dev ||
+      (T > 1 && t.stride(1) != 1))
+    return false;
+  if (B > 1) stride = t.stride(0);
+  return true;
+}
+
+// verify_drafts(logits, tokens, parents | None, uniform | None, temperature, draft_probs | None, new_lens | None)
+PyObject* verify_drafts_impl(PyObject* const* a) {
+  Tensor logits, tokens, parents, uniform, temps, probs, news;
+  if (!take(a[0], logits) || !take(a[1], tokens) || !take_opt(a[2], parents) || !take_opt(a[3], uniform) ||
+      !take_opt(a[5], probs) || !take_opt(a[6], news))
+    return nullptr;
+  double heat = 0.0;
+  if (PyFloat_CheckExact(a[4])) heat = PyFloat_AS_DOUBLE(a[4]);
+  else if (!take(a[4], temps)) return nullptr;
+  const c10::Device dev = logits.device();
+  const int dt = dtype_of(logits);
+  if (dt < 0 || logits.dim() != 3 || c10::hip::current_device() != dev.index()) return nullptr;
+  const int64_t B = logits.size(0), T = logits.size(1), V = logits.size(2);
+  int64_t st_, sp, su;
+  if (B < 1 || B > INT_MAX || T < 1 || T > FORGE_TREE_MAX_TOKENS || V < 1 || V > INT_MAX || (V > 1 && logits.stride(2) != 1) ||
+      !rows2_ok(tokens, at::kLong, B, T, dev, st_) || !rows2_ok(parents, at::kInt, B, T, dev, sp) ||
+      !rows2_ok(uniform, at::kFloat, B, T, dev, su) || (news.defined() && !rows_ok(news, B, dev)))
+    return nullptr;
+  if (temps.defined() && (temps.scalar_type() != at::kFloat || temps.dim() != 1 || temps.size(0) != B ||
+                          !temps.is_contiguous() || temps.device() != dev))
+    return nullptr;
+  if ((temps.defined() || heat != 0.0) && !uniform.defined()) return nullptr;
+  if (T == 1) probs.reset();
+  int pdt = 0;
+  if (probs.defined()) {
+    pdt = dtype_of(probs);
+    if ((pdt != FORGE_F32 && pdt != dt) || probs.dim() != 3 || probs.size(0) != B ||
+        (probs.size(1) != T && probs.size(1) != T - 1) || probs.size(2) != V || (V > 1 && probs.stride(2) != 1) ||
+        probs.device() != dev)
+      return nullptr;
+  }
+  Tensor out, path, count, ws;
+  int st;
+  {
+    NoGil unlocked;
+    const size_t need = forge_verify_drafts_workspace_bytes((int)B, (int)T, (int)V, probs.defined());
+    if (!need) return nullptr;
+    out = at::empty({B, T}, tokens.options());
+    path = at::empty({B, T}, tokens.options().dtype(at::kInt));
+    count = at::empty({B}, tokens.options().dtype(at::kInt));
+    ws = at::empty({(int64_t)need}, tokens.options().dtype(at::kByte));
+    st = forge_verify_drafts(dt, (int)B, (int)T, (int)V, ptr(logits), logits.stride(0), logits.stride(1),
+                             static_cast<const int64_t*>(ptr(tokens)), st_, static_cast<const int32_t*>(ptr(parents)), sp,
+                             static_cast<const float*>(ptr(uniform)), su, static_cast<const float*>(ptr(temps)), heat, pdt,
+                             ptr(probs), probs.defined() ? probs.stride(0) : 0, probs.defined() ? probs.stride(1) : 0,
+                             static_cast<const int32_t*>(ptr(news)), static_cast<int64_t*>(out.data_ptr()),
+                             static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()), ws.data_ptr(), need,
+                             c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  if (st) return st < 0 ? nullptr : PyLong_FromLong(st);
+  return tuple_of({out, path, count});
+}
+
+// The K and V caches of layers of one shape and layout (ops._layer_groups takes the others)
+struct Layers {
+  std::vector<const void*> k, v;
+  Tensor first;
+  int64_t s[3];
+  bool take_lists(PyObject* ks, PyObject* vs) {
+    const auto sequence = [](PyObject* o) { return PyList_CheckExact(o) || PyTuple_CheckExact(o); };
+    if (!sequence(ks) || !sequence(vs)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(ks);
+    if (n < 1 || PySequence_Fast_GET_SIZE(vs) != n) return false;
+    k.reserve(n);
+    v.reserve(n);
+    for (Py_ssize_t i = 0; i < 2 * n; ++i) {
+      Tensor t;
+      if (!take(PySequence_Fast_GET_ITEM(i < n ? ks : vs, i % n), t)) return false;
+      if (i == 0) {
+        first = t;
+        if (t.dim() != 4 || dtype_of(t) < 0 || t.size(3) * t.element_size() % 16 || !strides16(t, s) ||
+            c10::hip::current_device() != t.device().index())
+          return false;
+        for (int d = 0; d < 4; ++d)
+          if (t.stride(d) == 0 && t.size(d) > 1) return false;
+      } else {
+        if (t.sizes() != first.sizes() || t.strides() != first.strides() || t.scalar_type() != first.scalar_type() ||
+            t.device() != first.device() || (uintptr_t)t.const_data_ptr() % 16)
+          return false;
+      }
+      (i < n ? k : v).push_back(t.const_data_ptr());
+    }
+    return true;
+  }
+};
+
+PyObject* status(int st) { return st < 0 ? nullptr : PyLong_FromLong(st); }
+
+// kv_compact(k_caches, v_caches, path, count, pos | None, pos_dev | None, row_pos | None)
+PyObject* kv_compact_impl(PyObject* const* a) {
+  Layers l;
+  Tensor path, count, pos_dev, row_pos;
+  int64_t pos = 0, sp;
+  if (!take(a[2], path) || !take(a[3], count) || (a[4] != Py_None && !as_int(a[4], pos)) || !take_opt(a[5], pos_dev) ||
+      !take_opt(a[6], row_pos) || !l.take_lists(a[0], a[1]))
+    return nullptr;
+  const c10::Device dev = l.first.device();
+  const int64_t B = l.first.size(0), max_len = l.first.size(2);
+  if (path.dim() != 2 || B < 1 || max_len < 1 || path.size(1) < 1 || path.size(1) > INT_MAX || pos < 0 ||
+      !rows2_ok(path, at::kInt, B, path.size(1), dev, sp) || !rows_ok(count, B, dev) ||
+      (row_pos.defined() && !rows_ok(row_pos, B, dev)) ||
+      (pos_dev.defined() && (pos_dev.scalar_type() != at::kLong || pos_dev.numel() < 1 || pos_dev.device() != dev)) ||
+      (a[4] != Py_None) + pos_dev.defined() + row_pos.defined() > 1)
+    return nullptr;
+  int st;
+  {
+    NoGil unlocked;
+    st = forge_kv_compact((int)l.first.element_size(), (int)l.k.size(), (int)B, (int)l.first.size(1), (int)l.first.size(3),
+                          l.k.data(), l.v.data(), l.s[0], l.s[1], l.s[2], (int)B, max_len, nullptr, 0, 0,
+                          static_cast<const int32_t*>(ptr(row_pos)), static_cast<const int64_t*>(ptr(pos_dev)), pos,
+                          static_cast<const int32_t*>(ptr(path)), sp, (int)path.size(1),
+                          static_cast<const int32_t*>(ptr(count)), c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return status(st);
+}
+
+// kv_compact_paged(k_pools, v_pools, table, row_pos, path, count)
+PyObject* kv_compact_paged_impl(PyObject* const* a) {
+  Layers l;
+  Tensor table, row_pos, path, count;
+  int64_t sp;
+  if (!take(a[2], table) || !take(a[3], row_pos) || !take(a[4], path) || !take(a[5], count) || !l.take_lists(a[0], a[1]))
+    return nullptr;
+  const c10::Device dev = l.first.device();
+  if (path.dim() != 2) return nullptr;
+  const int64_t B = path.size(0), T = path.size(1);
+  Pages p;
+  if (B < 1 || T < 1 || T > INT_MAX || !rows2_ok(path, at::kInt, B, T, dev, sp) || !rows_ok(count, B, dev) ||
+      !rows_ok(row_pos, B, dev) || !pages_ok(l.first, l.first, table, B, dev, p))
+    return nullptr;
+  int st;
+  {
+    NoGil unlocked;
+    st = forge_kv_compact((int)l.first.element_size(), (int)l.k.size(), (int)B, (int)l.first.size(1), (int)l.first.size(3),
+                          l.k.data(), l.v.data(), l.s[0], l.s[1], l.s[2], p.n, p.size,
+                          static_cast<const int32_t*>(ptr(table)), p.stride, (int)p.max,
+                          static_cast<const int32_t*>(ptr(row_pos)), nullptr, 0, static_cast<const int32_t*>(ptr(path)), sp,
+                          (int)T, static_cast<const int32_t*>(ptr(count)), c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return status(st);
+}
+
+// copy_pages(k_pools, v_pools, src, dst), the page numbers as tensors
+PyObject* copy_pages_impl(PyObject* const* a) {
+  Layers l;
+  Tensor src, dst;
+  if (!take(a[2], src) || !take(a[3], dst) || !l.take_lists(a[0], a[1])) return nullptr;
+  const c10::Device dev = l.first.device();
+  const int64_t n = src.numel(), size = l.first.size(2);
+  if (src.dim() != 1 || n < 1 || n > INT_MAX || !rows_ok(src, n, dev) || !rows_ok(dst, n, dev) || size > INT_MAX ||
+      l.first.size(0) < 1 || l.first.size(0) > INT_MAX)
+    return nullptr;
+  int st;
+  {
+    NoGil unlocked;
+    st = forge_copy_pages((int)l.first.element_size(), (int)l.k.size(), (int)l.first.size(1), (int)l.first.size(3), l.k.data(),
+                          l.v.data(), l.s[0], l.s[1], l.s[2], (int)l.first.size(0), (int)size, (int)n,
+                          static_cast<const int32_t*>(ptr(src)), static_cast<const int32_t*>(ptr(dst)),
+                          c10::hip::getCurrentHIPStream(dev.index()).stream());
+  }
+  return status(st);
+}
+
 // An exception on the way (out of memory, for one) goes the Python way too, which raises it there.
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -613,7 +930,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     FORGE_ENTRY(decode_append, 21), FORGE_ENTRY(kv_append, 11), FORGE_ENTRY(prefill, 11),
     FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), FORGE_ENTRY(kv_append_paged, 13),
-    FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 17), {nullptr, nullptr, 0, nullptr},
+    FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 17), FORGE_ENTRY(tree_mask, 2),
+    FORGE_ENTRY(attn_tree, 19),     FORGE_ENTRY(attn_tree_paged, 18), FORGE_ENTRY(verify_drafts, 7),
+    FORGE_ENTRY(kv_compact, 7),     FORGE_ENTRY(kv_compact_paged, 6), FORGE_ENTRY(copy_pages, 4), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_forge_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -62,6 +62,13 @@ struct PagedParams {
   // Arrival counters [row block of a (batch row, KV head)], all zero between calls: the last part of a row block
   // merges it. Null: the combine kernel does, launched behind.
   unsigned* counters;
+  // Trees of drafted tokens (template parameter TREE): bit j of row (b, t) says that new token t sees new token j, whatever
+  // their slots' order. Depths say how far past the row's first new position a token sits: read where there is a window.
+  const uint32_t* tree;  // [B][T][words]
+  int64_t tsb, tst;
+  int words;             // of 32 bits
+  const int32_t* depth;  // [B][T], or null without a window
+  int64_t dsb;
 
   // Token of query row r (r / G).
   __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((unsigned)r, g_inv); }
@@ -138,6 +145,9 @@ struct RowSpan {
   }
 };
 
+// A tree's queries all see the cache up to the row's first new token, and any of its new tokens: `first` is then the last key
+// that all of them see, `last` the last new token, which no query's position passes.
+template <bool TREE = false>
 __device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int rows, int row0, int nrows, int KT) {
   RowSpan w;
   w.base = base;
@@ -146,9 +156,10 @@ __device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int
   w.first = w.last = w.lo = w.se = 0;
   if (row0 >= rows) return w;
   const int row1 = (row0 + nrows < rows ? row0 + nrows : rows) - 1;
-  w.first = base + p.token(row0);
-  w.last = base + p.token(row1);
-  w.lo = p.window > 0 && w.first >= p.window ? w.first - p.window + 1 : 0;
+  w.first = TREE ? base - 1 : base + p.token(row0);
+  w.last = base + p.token(TREE ? rows - 1 : row1);
+  const int from = TREE ? base : w.first;   // the lowest position of a query
+  w.lo = p.window > 0 && from >= p.window ? from - p.window + 1 : 0;
   w.main_tile = w.lo / KT;
   w.se = p.sinks < w.lo ? p.sinks : w.lo;
   const int st = (w.se + KT - 1) / KT;
@@ -158,10 +169,11 @@ __device__ __forceinline__ RowSpan make_span(const PagedParams& p, int base, int
 }
 
 // The same for batch row b of a block (uniform: scalar registers).
+template <bool TREE = false>
 __device__ __forceinline__ RowSpan row_span(const PagedParams& p, int b, int row0, int nrows, int KT) {
   int base, rows;
   row_extent(p, b, base, rows);
-  return make_span(p, __builtin_amdgcn_readfirstlane(base), __builtin_amdgcn_readfirstlane(rows), row0, nrows, KT);
+  return make_span<TREE>(p, __builtin_amdgcn_readfirstlane(base), __builtin_amdgcn_readfirstlane(rows), row0, nrows, KT);
 }
 
 // What a block does: part `part` of `parts` (0 or 1: the whole) of row block rblk of (b, kvh); its tiles, and the
@@ -181,7 +193,7 @@ __device__ __forceinline__ int row_parts(const PagedParams& p, int tiles) {
 // Grid: x (batch row, KV head), y part, z row block, late ones first (a causal chunk's have the most keys). Blocks
 // start in that order, x first, so where (batch row, KV head) pairs times parts are a multiple of 8 all blocks that
 // read the same keys run on one XCD and meet in its L2.
-template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const PagedParams& p) {
+template <int BM, int KT, bool TREE = false> __device__ __forceinline__ BlockWork block_work(const PagedParams& p) {
   BlockWork w;
   const int nrb = (p.rows + BM - 1) / BM;
   w.none = true;
@@ -196,14 +208,14 @@ template <int BM, int KT> __device__ __forceinline__ BlockWork block_work(const 
     w.b = it[0] / nrb;
     w.rblk = it[0] % nrb;
     if (w.parts < 0) return w;  // behind the last item
-    w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
+    w.span = row_span<TREE>(p, w.b, w.rblk * BM, BM, KT);
   } else {
     const int pair = blockIdx.x;
     w.part = blockIdx.y;
     w.rblk = nrb - 1 - (int)blockIdx.z;
     w.b = pair / p.K;
     w.kvh = pair - w.b * p.K;
-    w.span = row_span(p, w.b, w.rblk * BM, BM, KT);
+    w.span = row_span<TREE>(p, w.b, w.rblk * BM, BM, KT);
     w.parts = row_parts(p, w.span.tiles);
     w.slot = (pair * nrb + w.rblk) * p.nparts + w.part;
     if (w.part > 0 && w.part >= w.parts) return w;
@@ -226,6 +238,68 @@ __device__ __forceinline__ unsigned low_bits(int n) {
 __device__ __forceinline__ float masked(float s, unsigned see, int bit) {
   const int keep = (int)__builtin_amdgcn_sbfe((int)see, bit, 1);
   return __int_as_float((__float_as_int(s) & keep) | (__float_as_int(kNegInf) & ~keep));
+}
+
+// The position of new token t of batch row b in a tree, whose row has n real ones.
+__device__ __forceinline__ int tree_position(const PagedParams& p, int b, int base, int n, int t) {
+  if (!p.depth) return base;   // (no window: nothing hangs on it)
+  const int d = p.depth[b * p.dsb + t];
+  return base + (d < 0 ? 0 : d < n ? d : n - 1);
+}
+// What new token t, at position qpos, sees of the 32 keys from `key` on (bit i: key + i): the cache's, whose slots are
+// their positions, and the row's n new tokens, whose bits say it, within the window by their own depths.
+__device__ __forceinline__ unsigned tree_sees(const PagedParams& p, int b, int base, int n, int t, int qpos, int key) {
+  const int before = base - key;   // keys of the cache from `key` on
+  unsigned see = low_bits(before);
+  if (p.window > 0) see &= ~low_bits(qpos - p.window + 1 - key) | low_bits(p.sinks - key);
+  if (before >= 32) return see;
+  const int off = -before, i = off >> 5;   // the first bit's new token (negative: bits of the cache before it)
+  const uint32_t* row = p.tree + b * p.tsb + t * p.tst;
+  const unsigned lo = i >= 0 && i < p.words ? row[i] : 0, hi = i + 1 >= 0 && i + 1 < p.words ? row[i + 1] : 0;
+  unsigned bits = __builtin_amdgcn_alignbit(hi, lo, (unsigned)off & 31) & low_bits(n - off) & ~low_bits(before);
+  if (p.window > 0 && p.window < n) {      // (else no two tokens of the tree are a window apart)
+    for (unsigned rest = bits; rest; rest &= rest - 1) {
+      const int j = __builtin_ctz(rest), at = tree_position(p, b, base, n, off + j);
+      if (at <= qpos - p.window && at >= p.sinks) bits &= ~(1u << j);
+    }
+  }
+  return see | bits;
+}
+
+// A branch of a tree must not see what is in another's values: 0 * NaN of an unseen key would be NaN. So where some
+// query sees a tile in part, values that are no finite numbers are taken out of it before the products, and what they
+// are to the queries that do see them is added at the end, to every output whose key is seen: an infinity or a NaN, whatever
+// the key's weight.
+template <typename T> __device__ __forceinline__ bool not_finite(T x) {
+  if constexpr (sizeof(T) == 4) return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u;
+  else {
+    constexpr unsigned e = __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+    return (__builtin_bit_cast(unsigned short, x) & e) == e;
+  }
+}
+// Whether `bytes` of LDS hold such a value (the whole wave looks, and knows).
+template <typename T> __device__ __forceinline__ bool tile_not_finite(const char* tile, int bytes) {
+  bool bad = false;
+#pragma unroll 1
+  for (int x = (threadIdx.x % kWave) * 16; x < bytes; x += kWave * 16) {
+    const uint4 u = load16(tile + x);
+    T v[16 / sizeof(T)];
+    *reinterpret_cast<uint4*>(v) = u;
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); ++e) bad |= not_finite(v[e]);
+  }
+  return __any(bad);
+}
+// Takes them out; thread `at` of `of`.
+template <typename T> __device__ __forceinline__ void make_finite(char* tile, int bytes, int at, int of) {
+#pragma unroll 1
+  for (int x = at * 4; x < bytes; x += of * 4) {
+    T v[4 / sizeof(T)];
+    *reinterpret_cast<unsigned*>(v) = *reinterpret_cast<const unsigned*>(tile + x);
+#pragma unroll
+    for (int e = 0; e < 4 / (int)sizeof(T); ++e) v[e] = not_finite(v[e]) ? (T)0.0f : v[e];
+    *reinterpret_cast<unsigned*>(tile + x) = *reinterpret_cast<const unsigned*>(v);
+  }
 }
 
 // Four output channels of query row `flat` of (b, kvh).
@@ -284,7 +358,8 @@ __device__ __forceinline__ float merge_parts(const float2* ml, const float* po, 
     M = top;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float a = i0 + u < parts ? rescale(e[u].x, M) : 0.0f;
+      if (i0 + u >= parts) continue;   // (0 * Inf of the last part, read again, would be NaN)
+      const float a = rescale(e[u].x, M);
       L += a * e[u].y;
       O.x += a * o[u].x;
       O.y += a * o[u].y;
@@ -301,7 +376,7 @@ constexpr int combine_rows(int D, int BM) { return 1024 / D < BM ? 1024 / D : BM
 // Merges the parts of the rows whose tiles were split: D / 4 lanes per row, four channels each, the
 // parts in order, eight at a time; four in planned calls, whose many rows of few parts want the registers for more
 // waves.
-template <typename T, int D, int BM, int KT, bool PLANNED>
+template <typename T, int D, int BM, int KT, bool PLANNED, bool TREE>
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   constexpr int LPR = D / 4, RPB = combine_rows(D, BM);
   const int nrb = (p.rows + BM - 1) / BM;
@@ -319,7 +394,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
     rows = e[2];
     stride = p.K;
   } else {
-    const RowSpan w = row_span(p, b, rblk * BM, BM, KT);
+    const RowSpan w = row_span<TREE>(p, b, rblk * BM, BM, KT);
     rows = w.rows;
     parts = row_parts(p, w.tiles);
     slot = ((int64_t)(b * p.K + kvh) * nrb + rblk) * p.nparts;
@@ -333,12 +408,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedParams p) {
   store_row<T>(p, b, kvh, flat, x, O, L > 0.0f ? 1.0f / L : 0.0f);
 }
 
-template <typename T, int D, int BM, int KT, bool PLANNED = false> static int launch_paged_combine(const PagedParams& p, hipStream_t s) {
+template <typename T, int D, int BM, int KT, bool PLANNED = false, bool TREE = false> static int launch_paged_combine(const PagedParams& p, hipStream_t s) {
   constexpr int RPB = combine_rows(D, BM);
   const int64_t nrb = (p.rows + BM - 1) / BM;
   const int subs = p.rows < BM ? (p.rows + RPB - 1) / RPB : BM / RPB;  // (blocks of a row block)
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
-  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT, PLANNED>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
+  hipLaunchKernelGGL((paged_combine_kernel<T, D, BM, KT, PLANNED, TREE>), dim3((unsigned)(p.B * p.K), subs, (unsigned)nrb), dim3(RPB * (D / 4)),
                      0, s, p);
   return check_launch();
 }
@@ -356,7 +431,7 @@ inline int reserve_lds(const void* kernel, int bytes, std::atomic<uint64_t>& don
   return 0;
 }
 
-template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
-template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
+template <typename T, bool TREE> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
+template <typename T, bool TREE> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s);
 
 }  // namespace forge

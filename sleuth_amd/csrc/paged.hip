@@ -185,20 +185,24 @@ template <typename T, int D, int RB> struct StepLds {
   static_assert(BLOCKS * BYTES <= 160 * 1024, "LDS");
 };
 
-template <typename T, int D, int RB, bool FIXED>
+// How a call's keys are cut and seen: freely, at places fixed in the cache, or freely by the rows of a tree.
+enum StepMode { kFree, kFixed, kTree };
+
+template <typename T, int D, int RB, StepMode MODE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(StepLds<T, D, RB>::BLOCKS >= 2 ? 2 : 1)))
 void paged_step_kernel(PagedParams p) {
   using TL = StepTile<T, D, RB>;
   using LD = StepLds<T, D, RB>;
   constexpr int KT = TL::KT, KB = TL::KB, NL = TL::NL, S = TL::NCH / 4, DB = D / 16, ROWS = LD::ROWS;
   constexpr int GROUPS = KT / 16;
+  constexpr bool FIXED = MODE == kFixed, TREE = MODE == kTree;
 
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = threadIdx.x % kWave;
   const int n = lane & 15, g = lane >> 4;
 
-  const BlockWork work = block_work<ROWS, KT>(p);
+  const BlockWork work = block_work<ROWS, KT, TREE>(p);
   if (work.none) return;
   const RowSpan w = work.span;
   const int b = work.b, kvh = work.kvh, rblk = work.rblk;
@@ -263,13 +267,18 @@ void paged_step_kernel(PagedParams p) {
 
   // ---- query rows, as B operands; rows behind the row's last one stand for that one (never written)
   u32x4 q[LD::Q_LDS ? 1 : RB][S];
-  int qpos[RB];
+  int qpos[RB], qtok[TREE ? RB : 1];
+  const int ntok = TREE ? w.last - w.base + 1 : 0;   // the tree's real tokens
   char* ql = smem + LD::Q_OFF;  // [ROWS][chunks turned with the row]
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int row = rblk * ROWS + 16 * r + n;
     const int at = row < w.rows ? row : w.rows - 1;
     qpos[r] = w.base + p.token(at);
+    if constexpr (TREE) {
+      qtok[r] = p.token(at);
+      qpos[r] = w.rows > 0 ? tree_position(p, b, w.base, ntok, qtok[r]) : w.base;
+    }
     if constexpr (LD::Q_LDS) {
       if (r % 4 == wave && w.rows > 0) {
         step_load_q<T, D>(p, b, kvh, at, g, q[0]);
@@ -296,6 +305,7 @@ void paged_step_kernel(PagedParams p) {
   char* kt = smem + wave * LD::WAVE;
   char* vt = kt + TL::TILEB;
 
+  int odd_from = -1, odd_to = -2;   // (trees) the wave's tiles among which are those with values taken out
   for (; i < end; i = next(i)) {
     const int key0 = w.tile_key(i, KT);
 #pragma unroll
@@ -341,6 +351,7 @@ void paged_step_kernel(PagedParams p) {
         const int lo = (p.window > 0 ? qpos[r] - p.window + 1 : 0) - base;
         const int first = p.sinks - base < top ? p.sinks - base : top;
         unsigned see = (low_bits(top) & ~low_bits(lo)) | low_bits(first);
+        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, qtok[r], qpos[r], base);
         if (miss & 1) see &= ~0xffffu;
         if (miss & 2) see &= 0xffffu;
 #pragma unroll
@@ -376,6 +387,16 @@ void paged_step_kernel(PagedParams p) {
           s[r][kb][j] = w8;
           l[r] += w8;
         }
+    }
+
+    if constexpr (TREE) {
+      if (!full && tile_not_finite<T>(vt, TL::TILEB)) {   // (paged.h)
+        make_finite<T>(vt, TL::TILEB, lane, kWave);
+        odd_from = odd_from < 0 ? i : odd_from;
+        odd_to = i;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
     }
 
     // O^T += V^T . P^T; the k-slots of a lane are the keys whose weights it holds
@@ -441,6 +462,30 @@ void paged_step_kernel(PagedParams p) {
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  }
+
+  if constexpr (TREE) {
+#pragma unroll 1
+    for (int y = odd_from; y >= 0 && y <= odd_to; y += 4) {   // the values that were taken out, for the rows that see them
+      const int key0 = w.tile_key(y, KT);
+#pragma unroll 1
+      for (int key = key0; key < key0 + KT && key <= w.last; ++key) {
+        const int page = p.page_of(b, key);
+        if (page < 0) continue;
+        const char* src = vb0 + page * pageb + (int64_t)(key & p.page_mask) * rowb;
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          if (!(tree_sees(p, b, w.base, ntok, qtok[r], qpos[r], key) & 1)) continue;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const T v = reinterpret_cast<const T*>(src)[16 * d + 4 * g + j];
+              if (not_finite(v)) o[r][d][j] += to_f32<T>(v);
+            }
+        }
+      }
+    }
   }
 
   // ---- the four waves' rows meet: each scales its own to the common maximum and puts it into its LDS
@@ -542,44 +587,56 @@ void paged_step_kernel(PagedParams p) {
   }
 }
 
-template <typename T, int D, int RB, bool FIXED> static int launch_step_rb(PagedParams p, hipStream_t s) {
+template <typename T, int D, int RB, StepMode MODE> static int launch_step_rb(PagedParams p, hipStream_t s) {
   using LD = StepLds<T, D, RB>;
   static std::atomic<uint64_t> done{0};
-  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB, FIXED>), LD::BYTES, done)) return st;
+  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_step_kernel<T, D, RB, MODE>), LD::BYTES, done)) return st;
   const int nrb = (p.rows + LD::ROWS - 1) / LD::ROWS;
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
-  hipLaunchKernelGGL((paged_step_kernel<T, D, RB, FIXED>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
+  hipLaunchKernelGGL((paged_step_kernel<T, D, RB, MODE>), dim3((unsigned)(p.B * p.K), p.nparts, nrb), dim3(256), LD::BYTES, s, p);
   int st = check_launch();
-  if (st == 0 && p.nparts > 1 && !p.counters) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT>(p, s);
+  if (st == 0 && p.nparts > 1 && !p.counters) st = launch_paged_combine<T, D, LD::ROWS, StepTile<T, D, RB>::KT, false, MODE == kTree>(p, s);
   return st;
 }
 
-template <typename T, int D> static int launch_step(const PagedParams& p, const PagedPlan& plan, hipStream_t s) {
+template <typename T, int D, int RB, bool TREE> static int launch_step_rows(const PagedParams& p, hipStream_t s) {
+  if constexpr (TREE) return launch_step_rb<T, D, RB, kTree>(p, s);
+  else return p.fixed ? launch_step_rb<T, D, RB, kFixed>(p, s) : launch_step_rb<T, D, RB, kFree>(p, s);
+}
+
+template <typename T, int D, bool TREE> static int launch_step(const PagedParams& p, const PagedPlan& plan, hipStream_t s) {
   if constexpr (step_rows_most(sizeof(T), D) >= 32) {
-    if (plan.rows == 32) return p.fixed ? launch_step_rb<T, D, 2, true>(p, s) : launch_step_rb<T, D, 2, false>(p, s);
+    if (plan.rows == 32) return launch_step_rows<T, D, 2, TREE>(p, s);
   }
-  if (plan.rows == 16) return p.fixed ? launch_step_rb<T, D, 1, true>(p, s) : launch_step_rb<T, D, 1, false>(p, s);
+  if (plan.rows == 16) return launch_step_rows<T, D, 1, TREE>(p, s);
   return set_error("forge_attn_paged: no kernel of this row block");
 }
 
-template <typename T> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
+template <typename T, bool TREE> int launch_paged(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
   switch (D) {
-    case 32: return launch_step<T, 32>(p, plan, s);
-    case 64: return launch_step<T, 64>(p, plan, s);
-    case 128: return launch_step<T, 128>(p, plan, s);
-    case 256: return launch_step<T, 256>(p, plan, s);
+    case 32: return launch_step<T, 32, TREE>(p, plan, s);
+    case 64: return launch_step<T, 64, TREE>(p, plan, s);
+    case 128: return launch_step<T, 128, TREE>(p, plan, s);
+    case 256: return launch_step<T, 256, TREE>(p, plan, s);
     case 512:
-      if constexpr (sizeof(T) == 2) return launch_step<T, 512>(p, plan, s);
+      if constexpr (sizeof(T) == 2) return launch_step<T, 512, TREE>(p, plan, s);
     default: return set_error("forge_attn_paged: unsupported head dim");
   }
 }
 
+// (one type a translation unit, trees apart: they build side by side)
 #if FORGE_PAGED_PART == 1
-template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged<bf16, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #elif FORGE_PAGED_PART == 2
-template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged<f16, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #elif FORGE_PAGED_PART == 3
-template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged<float, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 4
+template int launch_paged<bf16, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 5
+template int launch_paged<f16, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 6
+template int launch_paged<float, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #endif
 
 }  // namespace forge

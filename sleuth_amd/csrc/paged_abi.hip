@@ -7,28 +7,36 @@
 
 namespace forge {
 
-extern template int launch_paged<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged_chunk<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
-extern template int launch_paged<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#define FORGE_EXTERN(T)                                                                            \
+  extern template int launch_paged<T, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);       \
+  extern template int launch_paged<T, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);        \
+  extern template int launch_paged_chunk<T, false>(const PagedParams&, const PagedPlan&, int, hipStream_t); \
+  extern template int launch_paged_chunk<T, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+FORGE_EXTERN(bf16)
+FORGE_EXTERN(f16)
+FORGE_EXTERN(float)
+#undef FORGE_EXTERN
+
+template <typename T> static int launch_any(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
+  if (p.tree) return plan.chunk ? launch_paged_chunk<T, true>(p, plan, D, s) : launch_paged<T, true>(p, plan, D, s);
+  return plan.chunk ? launch_paged_chunk<T, false>(p, plan, D, s) : launch_paged<T, false>(p, plan, D, s);
+}
 
 static bool paged_dim_ok(int dtype, int D) {
   return D == 32 || D == 64 || D == 128 || D == 256 || (D == 512 && dtype != FORGE_F32);
 }
 
 // Rows per block, keys per tile and the key split of a call whose rows hold at most max_kv keys.
-// ragged: the rows may have different lengths (row_pos).
+// ragged: the rows may have different lengths (row_pos). tree: every block sees all of the row's new tokens.
 static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_t max_kv, int window, int sinks,
-                            bool ragged, bool split) {
+                            bool ragged, bool split, bool tree = false) {
   PagedPlan plan{};
   const int es = dtype == FORGE_F32 ? 4 : 2, G = H / K, cus = device_cus();
   const int64_t rows = (int64_t)G * T;
   // tiles that a block can have: its queries' window and the first tokens (whose ends may lie inside tiles), or
   // the whole row; and the call's blocks
   const auto tiles_of = [&] {
-    const int64_t tokens = rows < plan.rows ? T : (plan.rows - 1) / G + 2;
+    const int64_t tokens = tree || rows < plan.rows ? T : (plan.rows - 1) / G + 2;
     const int64_t all = (max_kv + plan.keys - 1) / plan.keys;
     if (window <= 0) return all;
     const int64_t seen = (window + tokens + plan.keys - 3) / plan.keys + 1 + (sinks + plan.keys - 1) / plan.keys;
@@ -188,7 +196,7 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
   p.scale_log2 = scale * kLog2e;
   const bool split = workspace != nullptr;
   const PagedPlan plan = p.fixed ? fixed_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, split)
-                                 : paged_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, p.row_pos != nullptr, split);
+                                 : paged_plan(dtype, p.B, p.T, p.H, p.K, D, max_kv, p.window, p.sinks, p.row_pos != nullptr, split, p.tree != nullptr);
   p.nparts = plan.nparts;
   p.part_tiles = plan.part_tiles;
   p.slots = plan.slots;
@@ -212,9 +220,9 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
       p.counters = reinterpret_cast<unsigned*>(at);
   }
   switch (dtype) {
-    case FORGE_F32: return plan.chunk ? launch_paged_chunk<float>(p, plan, D, s) : launch_paged<float>(p, plan, D, s);
-    case FORGE_BF16: return plan.chunk ? launch_paged_chunk<bf16>(p, plan, D, s) : launch_paged<bf16>(p, plan, D, s);
-    default: return plan.chunk ? launch_paged_chunk<f16>(p, plan, D, s) : launch_paged<f16>(p, plan, D, s);
+    case FORGE_F32: return launch_any<float>(p, plan, D, s);
+    case FORGE_BF16: return launch_any<bf16>(p, plan, D, s);
+    default: return launch_any<f16>(p, plan, D, s);
   }
 }
 
@@ -222,13 +230,13 @@ static int paged_run(int dtype, int D, PagedParams p, int64_t max_kv, float scal
 
 using namespace forge;
 
-extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
-                                                   int window, int sinks) {
+static size_t workspace_bytes_of(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len, int window, int sinks,
+                                 bool tree) {
   if (B <= 0 || T <= 0 || H <= 0 || K <= 0 || H % K || !paged_dim_ok(dtype, D) || max_kv_len <= 0 || window < 0 ||
       sinks < 0 || max_kv_len > INT_MAX)
     return 0;
   const auto bytes = [&](bool ragged, bool* planned) {
-    const PagedPlan plan = paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, ragged, true);
+    const PagedPlan plan = paged_plan(dtype, B, T, H, K, D, max_kv_len, window, sinks, ragged, true, tree);
     *planned = plan.planned;
     return paged_ws(plan, B, T, H, K, D).bytes;
   };
@@ -237,6 +245,16 @@ extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int 
   if (!planned) return a;
   const size_t b = bytes(false, &planned);  // (without row positions nothing is planned: what either needs)
   return a > b ? a : b;
+}
+
+extern "C" size_t forge_attn_paged_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
+                                                   int window, int sinks) {
+  return workspace_bytes_of(dtype, B, T, H, K, D, max_kv_len, window, sinks, false);
+}
+
+extern "C" size_t forge_attn_tree_workspace_bytes(int dtype, int B, int T, int H, int K, int D, int64_t max_kv_len,
+                                                  int window, int sinks) {
+  return workspace_bytes_of(dtype, B, T, H, K, D, max_kv_len, window, sinks, true);
 }
 
 extern "C" int forge_attn_paged(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
@@ -312,4 +330,50 @@ extern "C" int forge_attn_sinks(int dtype, int B, int T, int H, int K, int D, co
   p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
   p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
   return paged_run(dtype, D, p, fixed ? max_len : max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
+}
+
+extern "C" int forge_attn_tree(int dtype, int B, int T, int H, int K, int D, const void* q, int64_t sqb, int64_t sqh,
+                               int64_t sqt, const float* q_weight, float eps, int flags, const float* cos,
+                               const float* sin, int64_t s_cos_b, int64_t s_cos_t, const void* k_cache,
+                               const void* v_cache, int64_t skp, int64_t skh, int64_t sks, int n_pages, int64_t page_size,
+                               const int32_t* page_table, int64_t s_table, int max_pages, const int32_t* row_pos,
+                               const int64_t* pos_dev, int64_t pos0, const int32_t* new_lens, int64_t max_kv_len,
+                               int window, int sinks, float scale, const int64_t* mask, int64_t s_mask_b,
+                               int64_t s_mask_t, const int32_t* depth, int64_t s_depth_b, void* out, int64_t sob,
+                               int64_t sot, int64_t soh, void* workspace, size_t workspace_bytes, int ws_flags,
+                               void* stream) {
+  clear_error();
+  if (flags & FORGE_FIXED_CUT) return set_error("FORGE_FIXED_CUT is for forge_attn_sinks");
+  if (max_kv_len <= 0 || page_size <= 0) return set_error("max_kv_len and the cache's length must be positive");
+  if (page_table && (page_size < 16 || (page_size & (page_size - 1)) || page_size > INT_MAX))
+    return set_error("the page size must be a power of two of at least 16");
+  if (page_table && (n_pages <= 0 || max_pages <= 0 || s_table < 0)) return set_error("bad page table sizes");
+  if (B == 0 || T == 0) return 0;  // (torch's empty tensors have no address)
+  if (T > FORGE_TREE_MAX_TOKENS) return set_error("a tree has at most 1024 tokens");
+  if (!mask || (uintptr_t)mask % 8 || s_mask_b < 0 || s_mask_t < 0) return set_error("bad mask");
+  if (window > 0 && (!depth || s_depth_b < 0)) return set_error("a window needs the tokens' depths");
+  if (page_table && !row_pos) return set_error("a paged cache needs row positions");
+  int64_t limit = page_table ? max_pages * page_size : page_size;
+  if (max_kv_len < limit) limit = max_kv_len;
+  if (limit > INT_MAX - 65536) return set_error("rows are limited to 2^31 - 65536 keys");
+  if (max_kv_len > limit) max_kv_len = limit;
+  if (!row_pos && !pos_dev && (pos0 < 0 || T < 0 || pos0 > limit - T))
+    return set_error("pos + T exceeds max_kv_len or the cache length");
+  PagedParams p{};
+  p.q = q; p.sqb = sqb; p.sqh = sqh; p.sqt = sqt;
+  p.qw = q_weight; p.eps = eps; p.flags = flags;
+  p.cos = cos; p.sin = sin; p.csb = s_cos_b; p.cst = s_cos_t;
+  p.k = k_cache; p.v = v_cache; p.skp = skp; p.skh = skh; p.sks = sks;
+  if (page_table) {
+    p.table = page_table; p.spt = s_table; p.npages = n_pages;
+    p.page_shift = __builtin_ctz((unsigned)page_size); p.page_mask = (int)page_size - 1;
+  } else {
+    p.page_shift = 31; p.page_mask = 0x7fffffff; p.npages = B;
+  }
+  p.row_pos = row_pos; p.pos_dev = pos_dev; p.pos0 = pos0; p.new_lens = new_lens;
+  p.B = B; p.T = T; p.H = H; p.K = K; p.limit = (int)limit; p.window = window; p.sinks = sinks;
+  p.tree = reinterpret_cast<const uint32_t*>(mask); p.tsb = 2 * s_mask_b; p.tst = 2 * s_mask_t; p.words = 2 * ((T + 63) / 64);
+  p.depth = window > 0 ? depth : nullptr; p.dsb = s_depth_b;
+  p.out = out; p.sob = sob; p.sot = sot; p.soh = soh;
+  return paged_run(dtype, D, p, max_kv_len, scale, workspace, workspace_bytes, ws_flags, (hipStream_t)stream);
 }

@@ -140,7 +140,7 @@ template <typename T, typename V> __device__ __forceinline__ float pair_sum(V a,
   else return __builtin_amdgcn_fdot2(a, V{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE>
 __global__ __launch_bounds__(256 * chunk_halves(D))
 __attribute__((amdgpu_waves_per_eu(ChunkTile<T, D>::BLOCKS * chunk_halves(D))))
 void paged_chunk_kernel(PagedParams p) {
@@ -161,7 +161,7 @@ void paged_chunk_kernel(PagedParams p) {
   const int n = lane & 31, hi = lane >> 5;
   const int half = HALVES == 2 ? wave >> 2 : 0;
 
-  const BlockWork work = block_work<BM, BN>(p);
+  const BlockWork work = block_work<BM, BN, TREE>(p);
   if (work.none) return;
   const RowSpan w = work.span;
   const int b = work.b, kvh = work.kvh, rblk = work.rblk, part = work.part, begin = work.begin, end = work.end;
@@ -270,9 +270,11 @@ void paged_chunk_kernel(PagedParams p) {
   const int flat = w_row + n;
   const bool valid = flat < w.rows;
   const int t = p.token(valid ? flat : w.rows - 1), h = kvh * p.G + (valid ? flat : w.rows - 1) - t * p.G;
-  const int qpos = w.base + t;
-  const int wq_lo = w.base + p.token(w_row);
-  const int wq_hi = w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
+  const int ntok = TREE ? w.last - w.base + 1 : 0;   // the tree's real tokens
+  const int qpos = TREE ? tree_position(p, b, w.base, ntok, t) : w.base + t;
+  // positions between which the wave's queries lie; keys up to wq_all that all of them see
+  const int wq_lo = TREE ? w.base : w.base + p.token(w_row), wq_all = TREE ? w.first : wq_lo;
+  const int wq_hi = TREE ? w.last : w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
   uint4 qreg[KSTEPS];
   chunk_load_q<T, D>(p, b, h, t, hi, half, qreg);
 
@@ -297,6 +299,7 @@ void paged_chunk_kernel(PagedParams p) {
   float m_run = kNegInf, l_run = 0.0f;
   const float c = p.scale_log2;
 
+  int odd_from = -1, odd_to = -2;   // (trees) the tiles among which are those with values taken out
   for (int it = begin; it < end; ++it) {
     const int stage = (it - begin) & 1;
     wait_vm<0>();
@@ -306,13 +309,24 @@ void paged_chunk_kernel(PagedParams p) {
       page = page_at(it + 2 < end ? it + 2 : it + 1);
     }
     const int key0 = w.tile_key(it, BN);
+    if constexpr (TREE) {   // (paged.h; every wave finds the same)
+      const bool part = !(key0 + BN - 1 <= w.first && (p.window <= 0 || w.last - key0 < p.window || key0 + BN <= p.sinks));
+      char* vtile = smem + (2 * stage + 1) * TL::TILEB;
+      if (part && tile_not_finite<T>(vtile, TL::TILEB)) {
+        __syncthreads();
+        make_finite<T>(vtile, TL::TILEB, threadIdx.x, TL::THREADS);
+        odd_from = odd_from < 0 ? it : odd_from;
+        odd_to = it;
+        __syncthreads();
+      }
+    }
     const bool needed = wave_any && key0 <= wq_hi &&
                         (p.window <= 0 || key0 + BN - 1 > wq_lo - p.window || key0 < p.sinks);
     if (HALVES == 1 && !needed) continue;
     unsigned bad = 0;
     if constexpr (HALVES == 2) bad = (unsigned)(stage ? flagged[1] : flagged[0]);
     else if (p.table) bad = (unsigned)__ballot(flags[4 * stage + (lane & 3)] != 0) & 15u;
-    const bool full = bad == 0 && key0 + BN - 1 <= wq_lo &&
+    const bool full = bad == 0 && key0 + BN - 1 <= wq_all &&
                       (p.window <= 0 || wq_hi - key0 < p.window || key0 + BN <= p.sinks);
 
     const unsigned kl = lds0 + (2 * stage) * TL::TILEB + k_rd + 256 * half;
@@ -386,6 +400,7 @@ void paged_chunk_kernel(PagedParams p) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         unsigned see = (low_bits(top - 32 * kb) & ~low_bits(lo - 32 * kb)) | low_bits(first - 32 * kb);
+        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, t, qpos, base + 32 * kb);
         if (bad) {
 #pragma unroll
           for (int x = 0; x < 16; x += 4)
@@ -470,6 +485,25 @@ void paged_chunk_kernel(PagedParams p) {
 
   l_run += __shfl_xor(l_run, 32, kWave);
   if (!valid) return;
+  if constexpr (TREE) {
+#pragma unroll 1
+    for (int y = odd_from; y >= 0 && y <= odd_to; ++y) {   // the values that were taken out, for the rows that see them
+      const int key0 = w.tile_key(y, BN);
+#pragma unroll 1
+      for (int key = key0; key < key0 + BN && key <= w.last; ++key) {
+        const int page = p.page_of(b, key);
+        if (page < 0 || !(tree_sees(p, b, w.base, ntok, t, qpos, key) & 1)) continue;
+        const T* src = reinterpret_cast<const T*>(vgb + page * pageb + (int64_t)(key & p.page_mask) * rowb);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const T v = src[half * (D / 2) + d * 32 + 8 * (x >> 2) + 4 * hi + (x & 3)];
+            if (not_finite(v)) oacc[d][x] += to_f32<T>(v);
+          }
+      }
+    }
+  }
   if (!whole) {
     const int64_t slot = (int64_t)work.slot * BM + (wave & 3) * 32 + n;
     float* po = p.ws_o + slot * D + half * (D / 2) + 4 * hi;
@@ -496,7 +530,7 @@ void paged_chunk_kernel(PagedParams p) {
 // (wave w tries one, over the row blocks in turn) with which all parts are resident at once; the parts go out
 // longest first (64 classes of length), so that a CU that got a long one gets a short one beside it.
 constexpr int kPlanThreads = 1024;
-template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedParams p, PagedItem* items,
+template <int BM, int KT, bool TREE> __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedParams p, PagedItem* items,
                                                                                         int4* pairs, int nitems) {
   __shared__ int tiles[kPlanPairs];
   __shared__ int wave_of[16], wave_tot[16], cls[64], pick;
@@ -507,7 +541,7 @@ template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_
   for (int i = threadIdx.x; i < n; i += kPlanThreads) {
     int base, rows;
     row_extent(p, i / nrb, base, rows);
-    tiles[i] = make_span(p, base, rows, i % nrb * BM, BM, KT).tiles;
+    tiles[i] = make_span<TREE>(p, base, rows, i % nrb * BM, BM, KT).tiles;
     sum += tiles[i];
   }
   for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d, kWave);
@@ -580,46 +614,52 @@ template <int BM, int KT> __global__ __launch_bounds__(kPlanThreads) void paged_
   for (int i = pick + threadIdx.x; i < nitems; i += kPlanThreads) items[i] = PagedItem{0, 0, -1, 0};
 }
 
-template <typename T, int D> static int launch_chunk_d(PagedParams p, const PagedPlan& plan, hipStream_t s) {
+template <typename T, int D, bool TREE> static int launch_chunk_d(PagedParams p, const PagedPlan& plan, hipStream_t s) {
   using TL = ChunkTile<T, D>;
   static std::atomic<uint64_t> done{0};
-  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D>), TL::LDS_BYTES, done)) return st;
+  if (const int st = reserve_lds(reinterpret_cast<const void*>(&paged_chunk_kernel<T, D, TREE>), TL::LDS_BYTES, done)) return st;
   const int nrb = (p.rows + TL::BM - 1) / TL::BM;
   if (nrb > 65535) return set_error("forge_attn_paged: too many query rows");
   dim3 grid((unsigned)(p.B * p.K), p.nparts, nrb);
   if (plan.planned) {
     grid = dim3((unsigned)(plan.nitems * p.K));
-    hipLaunchKernelGGL((paged_plan_kernel<TL::BM, TL::BN>), dim3(1), dim3(kPlanThreads), 0, s, p,
+    hipLaunchKernelGGL((paged_plan_kernel<TL::BM, TL::BN, TREE>), dim3(1), dim3(kPlanThreads), 0, s, p,
                        const_cast<PagedItem*>(p.items), const_cast<int4*>(p.pairs), plan.nitems);
     const int st = check_launch();
     if (st) return st;
   }
-  hipLaunchKernelGGL((paged_chunk_kernel<T, D>), grid, dim3(TL::THREADS), TL::LDS_BYTES, s, p);
+  hipLaunchKernelGGL((paged_chunk_kernel<T, D, TREE>), grid, dim3(TL::THREADS), TL::LDS_BYTES, s, p);
   const int st = check_launch();
   if (st) return st;
-  if (plan.planned) return launch_paged_combine<T, D, TL::BM, TL::BN, true>(p, s);
-  return p.nparts > 1 ? launch_paged_combine<T, D, TL::BM, TL::BN>(p, s) : 0;
+  if (plan.planned) return launch_paged_combine<T, D, TL::BM, TL::BN, true, TREE>(p, s);
+  return p.nparts > 1 ? launch_paged_combine<T, D, TL::BM, TL::BN, false, TREE>(p, s) : 0;
 }
 
-template <typename T> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
+template <typename T, bool TREE> int launch_paged_chunk(const PagedParams& p, const PagedPlan& plan, int D, hipStream_t s) {
   switch (D) {
     case 32:
-      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 32>(p, plan, s);
+      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 32, TREE>(p, plan, s);
       break;
-    case 64: return launch_chunk_d<T, 64>(p, plan, s);
-    case 128: return launch_chunk_d<T, 128>(p, plan, s);
-    case 256: return launch_chunk_d<T, 256>(p, plan, s);
+    case 64: return launch_chunk_d<T, 64, TREE>(p, plan, s);
+    case 128: return launch_chunk_d<T, 128, TREE>(p, plan, s);
+    case 256: return launch_chunk_d<T, 256, TREE>(p, plan, s);
     case 512:
-      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 512>(p, plan, s);
+      if constexpr (sizeof(T) == 2) return launch_chunk_d<T, 512, TREE>(p, plan, s);
   }
   return set_error("forge_attn_paged: unsupported head dim");
 }
 #if FORGE_PAGED_PART == 1
-template int launch_paged_chunk<bf16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged_chunk<bf16, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #elif FORGE_PAGED_PART == 2
-template int launch_paged_chunk<f16>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged_chunk<f16, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #elif FORGE_PAGED_PART == 3
-template int launch_paged_chunk<float>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+template int launch_paged_chunk<float, false>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 4
+template int launch_paged_chunk<bf16, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 5
+template int launch_paged_chunk<f16, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
+#elif FORGE_PAGED_PART == 6
+template int launch_paged_chunk<float, true>(const PagedParams&, const PagedPlan&, int, hipStream_t);
 #endif
 
 }  // namespace forge

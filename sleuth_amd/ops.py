@@ -772,6 +772,359 @@ def attn_sinks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
     return out
 
 
+# ---------------------------------------------------------------- trees of drafted tokens
+TREE_MAX_TOKENS = 1024   # FORGE_TREE_MAX_TOKENS
+
+
+def _no_positions(pos, pos_dev, row_pos) -> None:
+    if (pos is not None) + (pos_dev is not None) + (row_pos is not None) > 1:
+        raise ValueError("give one of pos, pos_dev and row_pos")
+
+
+def tree_mask(parents: torch.Tensor, new_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drafted trees as attn_tree takes them: parents [B, T] or [T] (one tree for every row) int32, token t drafted behind
+    token parents[t] < t (anything else: behind the cache alone). Returns mask int64 [B, T, ceil(T / 64)], bit j % 64 of
+    word j // 64 set where token t sees new token j (itself and its ancestors), and depth int32 [B, T], how many
+    ancestors it has (its position is the row's first new one plus that); [T, ..] and [T] for one tree. Tokens from
+    new_lens[b] on get no bit and depth 0. T at most 1,024."""
+    r = host().tree_mask(parents, new_lens)
+    if r is not None:
+        return r if r.__class__ is not int else check(r, "forge_tree_mask")
+    dev = _need_device(parents, new_lens)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2):
+        raise ValueError("parents must be int32, [B, T] or [T]")
+    if parents.shape[-1] > TREE_MAX_TOKENS:
+        raise ValueError(f"a tree has at most {TREE_MAX_TOKENS} tokens")
+    rows = parents[None] if parents.dim() == 1 else parents
+    B, T = rows.shape
+    if T > 1 and rows.stride(1) != 1 or B > 1 and rows.stride(0) < 0:
+        rows = rows.contiguous()
+    nl = _int32_rows(new_lens, B, dev, "new_lens")
+    mask = torch.empty(B, T, -(-T // 64), dtype=torch.int64, device=dev)
+    depth = torch.empty(B, T, dtype=torch.int32, device=dev)
+    with _guard(dev):
+        st = lib().forge_tree_mask(B, T, _ptr(rows), rows.stride(0) if B > 1 else 0, _ptr(nl), _ptr(mask), _ptr(depth), _stream(dev))
+    check(st, "forge_tree_mask")
+    return (mask[0], depth[0]) if parents.dim() == 1 else (mask, depth)
+
+
+def _tree_args(mask, depth, new_lens, B: int, T: int, window: int, dev: torch.device):
+    """Checks a tree's bits and depths; what keeps them alive, and (mask, its strides, depth, its stride)."""
+    words = -(-T // 64)
+    if T > TREE_MAX_TOKENS:
+        raise ValueError(f"a tree has at most {TREE_MAX_TOKENS} tokens")
+    if mask.dtype != torch.int64 or mask.device != dev or tuple(mask.shape) not in ((B, T, words), (T, words)):
+        raise ValueError(f"mask must be int64 [B, T, ceil(T / 64)] = {(B, T, words)}, or {(T, words)} for all rows, on {dev}")
+    if words > 1 and mask.stride(-1) != 1 or any(st < 0 for st in mask.stride()):
+        mask = mask.contiguous()
+    if window and depth is None:
+        raise ValueError("a window needs the tokens' depths")
+    if depth is not None:
+        if depth.dtype != torch.int32 or depth.device != dev or tuple(depth.shape) not in ((B, T), (T,)):
+            raise ValueError(f"depth must be int32 [B, T] = {(B, T)}, or {(T,)} for all rows, on {dev}")
+        if T > 1 and depth.stride(-1) != 1 or any(st < 0 for st in depth.stride()):
+            depth = depth.contiguous()
+    shared = mask.dim() == 2 or B == 1
+    return (mask, depth), (_ptr(mask), 0 if shared else mask.stride(0), mask.stride(-2) if T > 1 else 0,
+                           _ptr(depth), 0 if depth is None or depth.dim() == 1 or B == 1 else depth.stride(0))
+
+
+def _tree_launch(q, cache, mask, depth, new_lens, max_kv_len, scale, window, sinks, q_weight, eps, norm_q, cos, sin, out, dev,
+                 where_args, pools):
+    """The launch that attn_tree and attn_tree_paged share. where_args: n_pages, page_size .. pos0 as in forge_attn_tree."""
+    B, T = q.shape[0], q.shape[2]
+    nl = _int32_rows(new_lens, B, dev, "new_lens")
+    alive, tree = _tree_args(mask, depth, new_lens, B, T, window, dev)
+    keep, args, out = _new_token_args(q, cache, scale, q_weight, eps, norm_q, cos, sin, window, sinks, out)
+    if B == 0 or T == 0:
+        return out
+    with _guard(dev):
+        ws = _PagedPartials(dev, lib().forge_attn_tree_workspace_bytes(*args[:6], max_kv_len, int(window), int(sinks)))
+        st = lib().forge_attn_tree(*args, *pools, *where_args, _ptr(nl), max_kv_len, int(window), int(sinks), float(scale),
+                                   *tree, _ptr(out), *_strides3(out), *ws.args(), _stream(dev))
+    check(st, "forge_attn_tree")
+    ws.launched()
+    return out
+
+
+def attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, mask: torch.Tensor, *, scale: float,
+              pos: int | None = None, pos_dev: torch.Tensor | None = None, row_pos: torch.Tensor | None = None,
+              depth: torch.Tensor | None = None, new_lens: torch.Tensor | None = None, max_kv_len: int | None = None,
+              window: int = 0, sinks: int = 0, q_weight: torch.Tensor | None = None, eps: float = 1e-6,
+              norm_q: bool = False, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a drafted tree's tokens q [B,H,T,D] over a contiguous cache [B,K,max_len,D] that holds their keys at
+    slots base_b + t already (row_pos, pos_dev or pos, as attn_decode): token t sees the cache before base_b and the new
+    tokens whose bit mask [B, T, ceil(T / 64)] (or [T, ..]: one tree for all rows; tree_mask) has set, never padding (tokens
+    from new_lens[b] on). A window counts positions, base_b + depth for new tokens (depth [B, T] or [T], needed then), and
+    the first `sinks` positions stay visible. RoPE rows (cos, sin) are the caller's: those of the positions. Returns
+    [B,T,H,D]; padding, and rows that see nothing, are zeros. What a token does not see cannot reach it: a branch with an
+    infinity or a NaN in it leaves the others alone. T at most 1,024."""
+    if out is None:
+        r = host().attn_tree(_PAGED_WS, q, k_cache, v_cache, mask, float(scale), pos, pos_dev, row_pos, depth, new_lens,
+                             max_kv_len, window, sinks, q_weight, float(eps), bool(norm_q), cos, sin)
+        if r is not None:
+            return r if r.__class__ is not int else check(r, "forge_attn_tree")
+    dev = _need_device(q, k_cache, v_cache, mask, pos_dev, row_pos, depth, new_lens, cos, sin, q_weight if norm_q else None, out)
+    _no_positions(pos, pos_dev, row_pos)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.dtype != v_cache.dtype or \
+            q.dim() != 4 or q.shape[0] != k_cache.shape[0]:
+        raise ValueError(f"q {tuple(q.shape)} does not fit caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if _strides3(k_cache) != _strides3(v_cache) or not _aligned(k_cache) or not _aligned(v_cache):
+        raise ValueError("k and v caches must have the same strides, the last dimension contiguous, 16-byte aligned")
+    B, T, max_len = q.shape[0], q.shape[2], k_cache.shape[2]
+    rp, pd, p0 = _positions(pos, pos_dev, row_pos, B, dev)
+    if rp is None and pd is None:
+        if not 0 <= p0 <= max_len - T:
+            raise ValueError(f"pos {p0} + {T} tokens do not fit a cache of {max_len}")
+        max_kv_len = p0 + T
+    max_kv_len = max_len if max_kv_len is None else min(int(max_kv_len), max_len)
+    if max_kv_len < 1 and B and T:
+        raise ValueError("max_kv_len must be positive")
+    return _tree_launch(q, k_cache, mask, depth, new_lens, max_kv_len, scale, window, sinks, q_weight, eps, norm_q, cos, sin, out,
+                        dev, (1, max_len, None, 0, 0, _ptr(rp), _ptr(pd), p0),
+                        (_ptr(k_cache), _ptr(v_cache), *_cache_strides(k_cache)))
+
+
+def attn_tree_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    row_pos: torch.Tensor, mask: torch.Tensor, *, scale: float, depth: torch.Tensor | None = None,
+                    new_lens: torch.Tensor | None = None, max_kv_len: int | None = None, window: int = 0, sinks: int = 0,
+                    q_weight: torch.Tensor | None = None, eps: float = 1e-6, norm_q: bool = False,
+                    cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """attn_tree over the paged cache (pools, table and max_kv_len as in attn_paged), which holds the tree's keys at
+    positions row_pos[b] + t already (kv_append_paged)."""
+    if out is None:
+        r = host().attn_tree_paged(_PAGED_WS, q, k_pages, v_pages, page_table, row_pos, mask, float(scale), depth, new_lens,
+                                   max_kv_len, window, sinks, q_weight, float(eps), bool(norm_q), cos, sin)
+        if r is not None:
+            return r if r.__class__ is not int else check(r, "forge_attn_tree")
+    dev = _need_device(q, k_pages, v_pages, page_table, row_pos, mask, depth, new_lens, cos, sin, q_weight if norm_q else None, out)
+    if q.dim() != 4:
+        raise ValueError(f"q {tuple(q.shape)} must be [B, H, T, D]")
+    B = q.shape[0]
+    table = _pages(k_pages, v_pages, page_table, B, dev)
+    rp = _int32_rows(row_pos, B, dev, "row_pos")
+    size = k_pages.shape[2]
+    most = table.shape[1] * size
+    max_kv_len = most if max_kv_len is None else min(int(max_kv_len), most)
+    if max_kv_len < 1:
+        raise ValueError("max_kv_len must be positive")
+    return _tree_launch(q, k_pages, mask, depth, new_lens, max_kv_len, scale, window, sinks, q_weight, eps, norm_q, cos, sin, out,
+                        dev, (k_pages.shape[0], size, _ptr(table), table.stride(0) if B > 1 else 0, table.shape[1], _ptr(rp),
+                              None, 0), (_ptr(k_pages), _ptr(v_pages), *_strides3(k_pages)))
+
+
+def _rows2(t: torch.Tensor | None, dtype: torch.dtype, B: int, T: int, dev: torch.device, name: str):
+    """A [B, T] tensor (or None) with its rows contiguous, and its row stride."""
+    if t is None:
+        return None, 0
+    if t.dtype != dtype or tuple(t.shape) != (B, T) or t.device != dev:
+        raise ValueError(f"{name} must be {dtype} [B, T] = {(B, T)} on {dev}")
+    if T > 1 and t.stride(1) != 1 or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, t.stride(0) if B > 1 else 0
+
+
+def _rows3(t: torch.Tensor) -> torch.Tensor:
+    return t if (t.shape[-1] == 1 or t.stride(-1) == 1) and min(t.stride()) >= 0 else t.contiguous()
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, *, parents: torch.Tensor | None = None,
+                  uniform: torch.Tensor | None = None, temperature: float | torch.Tensor = 0.0,
+                  draft_probs: torch.Tensor | None = None, new_lens: torch.Tensor | None = None
+                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token behind them: logits [B, T, V] are what the target says behind each node of
+    the row's tree, node 0 the last token that stands; tokens int64 [B, T]; parents int32 [B, T] or [T] (None: a chain).
+
+    At a temperature (a number, or fp32 [B] on the GPU; 0: the argmax decides) the drafted tokens are accepted so that they
+    and the next token are distributed as the target's samples: a node's children in order, by uniform[b, t] (fp32 [B, T],
+    in [0, 1)) each, and uniform[b, 0] for the next token, which is drawn from what the rejections left. draft_probs
+    [B, T or T - 1, V] (fp32 or the logits' type): the probabilities that each node's children were drawn from, independently;
+    None: they were not drawn (a search, the drafter's likeliest tokens), and a rejected one is out as it is.
+
+    Returns (tokens int64 [B, T], path int32 [B, T], count int32 [B]): the row's count[b] new tokens (the accepted ones,
+    then the next one), the count[b] nodes that stand (node 0 first: what kv_compact takes), -1 behind both; a row without
+    nodes (new_lens[b] == 0) has none. Sums are held in 64 bits. No gradient."""
+    r = host().verify_drafts(logits, tokens, parents, uniform, temperature, draft_probs, new_lens)
+    if r is not None:
+        return r if r.__class__ is not int else check(r, "forge_verify_drafts")
+    dev = _need_device(logits, tokens, parents, uniform, draft_probs, new_lens)
+    if logits.dim() != 3 or 0 in logits.shape[1:]:
+        raise ValueError(f"logits {tuple(logits.shape)} must be [B, T, V]")
+    B, T, V = logits.shape
+    if T > TREE_MAX_TOKENS:
+        raise ValueError(f"a tree has at most {TREE_MAX_TOKENS} tokens")
+    dt = dtype_code(logits)
+    logits = _rows3(logits.detach())
+    tokens, s_tokens = _rows2(tokens, torch.int64, B, T, dev, "tokens")
+    if parents is not None and parents.dim() == 1:
+        parents = parents.expand(B, -1)
+    parents, s_parents = _rows2(parents, torch.int32, B, T, dev, "parents")
+    uniform, s_uniform = _rows2(uniform, torch.float32, B, T, dev, "uniform")
+    temps, heat = None, 0.0
+    if isinstance(temperature, torch.Tensor):
+        temps = temperature
+        if temps.dtype != torch.float32 or tuple(temps.shape) != (B,) or temps.device != dev:
+            raise ValueError(f"temperature must be a number or a float32 [B] tensor on {dev}")
+        temps = temps.contiguous()
+    else:
+        heat = float(temperature)
+        if heat != 0.0 and not 1e-30 <= heat <= 1e30:
+            raise ValueError(f"temperature must be 0, or positive and finite, not {temperature}")
+    if (temps is not None or heat) and uniform is None:
+        raise ValueError("a temperature needs uniform, the random numbers")
+    sq_b = sq_t = pdt = 0
+    if draft_probs is not None:
+        if draft_probs.dim() != 3 or draft_probs.shape[0] != B or draft_probs.shape[1] not in (T, T - 1) or draft_probs.shape[2] != V:
+            raise ValueError(f"draft_probs {tuple(draft_probs.shape)} must be [B, T or T - 1, V] = {(B, T, V)}")
+        if draft_probs.dtype not in (torch.float32, logits.dtype):
+            raise ValueError("draft_probs must be float32 or of the logits' type")
+        if T == 1:
+            draft_probs = None   # (no child: nothing to accept)
+        else:
+            draft_probs = _rows3(draft_probs.detach())
+            pdt, sq_b, sq_t = dtype_code(draft_probs), draft_probs.stride(0), draft_probs.stride(1)
+    nl = _int32_rows(new_lens, B, dev, "new_lens")
+    out = torch.empty(B, T, dtype=torch.int64, device=dev)
+    path = torch.empty(B, T, dtype=torch.int32, device=dev)
+    count = torch.empty(B, dtype=torch.int32, device=dev)
+    if B == 0:
+        return out, path, count
+    with _guard(dev):
+        need = lib().forge_verify_drafts_workspace_bytes(B, T, V, int(draft_probs is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        st = lib().forge_verify_drafts(dt, B, T, V, _ptr(logits), logits.stride(0), logits.stride(1), _ptr(tokens), s_tokens,
+                                       _ptr(parents), s_parents, _ptr(uniform), s_uniform, _ptr(temps), heat, pdt,
+                                       _ptr(draft_probs), sq_b, sq_t, _ptr(nl), _ptr(out), _ptr(path), _ptr(count), _ptr(ws),
+                                       need, _stream(dev))
+    check(st, "forge_verify_drafts")
+    return out, path, count
+
+
+def _layer_groups(ks, vs, dims: str):
+    """Caches of several layers, grouped by shape and layout (each group is one launch): the device, and [(K of the first
+    layer, K pointers, V pointers)]. All must be alike in their outer sizes."""
+    ks, vs = list(ks), list(vs)
+    if len(ks) != len(vs):
+        raise ValueError(f"{len(ks)} K and {len(vs)} V caches")
+    if not ks:
+        return None, []
+    dev = _need_device(*ks, *vs)
+    groups: dict = {}
+    for k, v in zip(ks, vs):
+        if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _DTYPES:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be {dims} of one float type")
+        if _strides3(k) != _strides3(v) or not _aligned(k) or not _aligned(v) or k.shape[3] * k.element_size() % 16:
+            raise ValueError("k and v must have the same strides, the last dimension contiguous, 16-byte aligned")
+        if any(st == 0 and n > 1 for st, n in zip(k.stride(), k.shape)):
+            raise ValueError("a cache's positions must not overlap")
+        groups.setdefault((k.shape, k.element_size(), _strides3(k)), []).append((k, v))
+    if len({(k.shape[0], k.shape[2]) for k in ks}) > 1:
+        raise ValueError("the layers' caches must have the same rows or pages, and positions")
+    return dev, [(g[0][0], [k.data_ptr() for k, _ in g], [v.data_ptr() for _, v in g]) for g in groups.values()]
+
+
+def _pointers(ptrs: list[int]):
+    return (_lib.C.c_void_p * len(ptrs))(*ptrs)
+
+
+def _compact(groups, dev, B, where, path, counts, s_path, T) -> None:
+    with _guard(dev):
+        for k, kp, vp in groups:
+            st = lib().forge_kv_compact(k.element_size(), len(kp), B, k.shape[1], k.shape[3], _pointers(kp), _pointers(vp),
+                                        *_strides3(k), *where, _ptr(path), s_path, T, _ptr(counts), _stream(dev))
+            check(st, "forge_kv_compact")
+
+
+def _path_args(path, count, B: int, dev):
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != B or path.device != dev:
+        raise ValueError(f"path must be int32 [B, T] with B={B} on {dev}")
+    count = _int32_rows(count, B, dev, "count")
+    path, s_path = _rows2(path, torch.int32, B, path.shape[1], dev, "path")
+    return path, s_path, count
+
+
+def kv_compact(k_caches, v_caches, path: torch.Tensor, count: torch.Tensor, *, pos: int | None = None,
+               pos_dev: torch.Tensor | None = None, row_pos: torch.Tensor | None = None) -> None:
+    """The accepted branch of a verified tree closes up, in every layer: slot base_b + i of the contiguous caches
+    [B,K,max_len,D] (lists of the layers' tensors) takes the key and value of slot base_b + path[b, i], for i < count[b]
+    (verify_drafts' path and count). What an entry below its own place i, or beyond the cache, names moves nothing. One launch
+    for all layers of a shape."""
+    st = host().kv_compact(k_caches, v_caches, path, count, pos, pos_dev, row_pos)
+    if st is not None:
+        return check(st, "forge_kv_compact")
+    _no_positions(pos, pos_dev, row_pos)
+    dev, groups = _layer_groups(k_caches, v_caches, "[B, K, max_len, D]")
+    if not groups:
+        return
+    B, max_len = groups[0][0].shape[0], groups[0][0].shape[2]
+    path, s_path, count = _path_args(path, count, B, dev)
+    rp, pd, p0 = _positions(pos, pos_dev, row_pos, B, dev)
+    if rp is None and pd is None and p0 < 0:
+        raise ValueError("pos must not be negative")
+    if max_len and path.shape[1]:
+        _compact(groups, dev, B, (B, max_len, None, 0, 0, _ptr(rp), _ptr(pd), p0), path, count, s_path, path.shape[1])
+
+
+def kv_compact_paged(k_pools, v_pools, page_table: torch.Tensor, row_pos: torch.Tensor, path: torch.Tensor,
+                     count: torch.Tensor) -> None:
+    """kv_compact over paged caches (lists of the layers' pools [n_pages,K,page_size,D] behind one table). Positions without a
+    page move nothing; rows must not share the pages that hold their new tokens."""
+    st = host().kv_compact_paged(k_pools, v_pools, page_table, row_pos, path, count)
+    if st is not None:
+        return check(st, "forge_kv_compact")
+    dev, groups = _layer_groups(k_pools, v_pools, "[n_pages, K, page_size, D]")
+    if not groups:
+        return
+    B = path.shape[0]
+    path, s_path, count = _path_args(path, count, B, dev)
+    table = _pages(groups[0][0], groups[0][0], page_table, B, dev)
+    rp = _int32_rows(row_pos, B, dev, "row_pos")
+    n, size = groups[0][0].shape[0], groups[0][0].shape[2]
+    if path.shape[1]:
+        _compact(groups, dev, B, (n, size, _ptr(table), table.stride(0) if B > 1 else 0, table.shape[1], _ptr(rp), None, 0), path,
+                 count, s_path, path.shape[1])
+
+
+def copy_pages(k_pools, v_pools, src, dst) -> None:
+    """Page dst[i] takes what page src[i] holds, in K and V of every layer (lists of pools [n_pages,K,page_size,D]): rows that
+    fork, or write to a page they share. src and dst are lists of page numbers, which are checked (in the pool, none written
+    twice, none both read and written), or int32 tensors on the GPU, which are not: numbers outside the pool copy nothing there,
+    and the rest is the caller's to keep."""
+    st = host().copy_pages(k_pools, v_pools, src, dst)
+    if st is not None:
+        return check(st, "forge_copy_pages")
+    dev, groups = _layer_groups(k_pools, v_pools, "[n_pages, K, page_size, D]")
+    if not groups:
+        return
+    n_pages, size = groups[0][0].shape[0], groups[0][0].shape[2]
+    if size < 16 or size & (size - 1) or n_pages < 1:
+        raise ValueError(f"pages hold a power of two of at least 16 positions, not {size}")
+    if isinstance(src, torch.Tensor) != isinstance(dst, torch.Tensor):
+        raise ValueError("src and dst must both be lists or both be tensors")
+    if isinstance(src, torch.Tensor):
+        if src.dtype != torch.int32 or src.dim() != 1 or src.shape != dst.shape or dst.dtype != torch.int32 or \
+                src.device != dev or dst.device != dev:
+            raise ValueError(f"src and dst must be int32 [n] tensors on {dev}")
+        src, dst = src.contiguous(), dst.contiguous()
+    else:
+        src, dst = [int(x) for x in src], [int(x) for x in dst]
+        if len(src) != len(dst) or any(not 0 <= x < n_pages for x in src + dst):
+            raise ValueError(f"src and dst must be page numbers of a pool of {n_pages}, as many of one as of the other")
+        if len(set(dst)) < len(dst) or any(x in set(src) for x in dst):
+            raise ValueError("a page may be written once, and not be read as well")
+        both = torch.tensor([src, dst], dtype=torch.int32).to(dev)
+        src, dst = both[0], both[1]
+    if not len(src):
+        return
+    with _guard(dev):
+        for k, kp, vp in groups:
+            st = lib().forge_copy_pages(k.element_size(), len(kp), k.shape[1], k.shape[3], _pointers(kp), _pointers(vp),
+                                        *_strides3(k), n_pages, size, len(src), _ptr(src), _ptr(dst), _stream(dev))
+            check(st, "forge_copy_pages")
+
+
 def _cache_strides(t: torch.Tensor) -> tuple[int, int, int]:
     """_strides3 with a positions' stride the kernels accept where there is one position."""
     b, h, s = _strides3(t)
@@ -780,4 +1133,5 @@ def _cache_strides(t: torch.Tensor) -> tuple[int, int, int]:
 
 __all__ = ["head_norm_rope", "kv_append", "attn_decode", "attn_decode_append", "attn_decode_noalloc", "attn_prefill", "attn_prefill_f32", "decode_chunk",
            "decode_workspace_bytes", "attn_drafter", "prefill_supported", "kv_append_paged",
-           "attn_paged", "attn_sinks", "paged_supported", "dtype_code", "_lib"]
+           "attn_paged", "attn_sinks", "paged_supported", "tree_mask", "attn_tree", "attn_tree_paged", "verify_drafts",
+           "kv_compact", "kv_compact_paged", "copy_pages", "dtype_code", "_lib"]
