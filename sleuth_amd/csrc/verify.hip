@@ -14,8 +14,8 @@
 //
 // Every node's logits are read once, whichever the walk needs, by one launch over chunks of all nodes (each chunk's
 // maximum and sum); a block per row then walks, and draws within the one chunk that its number falls into. What a
-// rejected child's probabilities leave has to be summed over a whole row of the vocabulary: two launches more, whose blocks
-// end at once for the rows that need none.
+// rejected child's probabilities leave has to be summed over a whole row of the vocabulary: a launch more, whose blocks
+// end at once for the rows that need none, and whose last one draws.
 #include <limits.h>
 
 #include "common.h"
@@ -23,9 +23,8 @@
 
 namespace forge {
 
-constexpr int kVerifyThreads = 256;
 constexpr int kVerifyChunk = 4096;  // elements of a row that a block takes
-constexpr int kPer = kVerifyChunk / kVerifyThreads;
+constexpr int kScanThreads = 256, kWalkThreads = 512;
 
 struct VerifyParams {
   const void* logits;
@@ -49,6 +48,7 @@ struct VerifyParams {
   double* part_z;  // [B][T][C]
   float* part_m;
   int32_t* part_i;
+  double scale_hi, scale_lo;  // of `temperature`
   struct State* state;  // [B]
   double* rest;         // [B][C]
 
@@ -68,27 +68,28 @@ struct State {
   int node, at;  // where; which of the row's outputs the token is
   int left;      // 0: drawn already
   int arg;       // the argmax, for a row without anything left
+  unsigned done;  // blocks that have summed their chunk
 };
 
 // log2(e) / temperature in two parts.
 struct Scale {
   double hi, lo;
 };
-__device__ __forceinline__ Scale scale_of(double temperature) {
+__host__ __device__ inline Scale scale_of(double temperature) {
   constexpr double l_hi = 0x1.71547652b82fep+0, l_lo = 0x1.777d0ffda0d24p-56;
   Scale s;
   s.hi = l_hi / temperature;
   s.lo = (fma(-s.hi, temperature, l_hi) + l_lo) / temperature;
   return s;
 }
+__device__ __forceinline__ Scale row_scale(const VerifyParams& p, int b) {
+  if (!p.temps) return Scale{p.scale_hi, p.scale_lo};
+  const double heat = p.heat(b);
+  return scale_of(heat > 0.0 ? heat : 1.0);
+}
 
-// exp((x - m) / temperature) to about 1e-15, exactly 1 at x = m: 2^t with t = k + f, |f| <= 1/2, and 2^f - 1 = f P(f),
-// P of degree 9 from (2^f - 1) / f at Chebyshev's points (6e-16 at most). k comes out of the low bits of t + 1.5 2^52.
-__device__ __forceinline__ double weight(float x, float m, Scale c) {
-  if (m == -kNegInf) return x == m ? 1.0 : 0.0;   // infinite logits share the mass
-  const double d = (double)x - (double)m;
-  const double t = d * c.hi, lo = fma(d, c.lo, fma(d, c.hi, -t));
-  const double big = t + 0x1.8p52, f = (t - (big - 0x1.8p52)) + lo;
+// 2^f = 1 + f P(f), |f| <= 1/2: P interpolates (2^f - 1) / f at ten Chebyshev points (off by 6e-16 at most).
+__device__ __forceinline__ double exp2_part(double f) {
   double p = 0x1.e5e83cccccccdp-28;
   p = fma(p, f, 0x1.b657203333333p-24);
   p = fma(p, f, 0x1.62bfe55000000p-20);
@@ -99,18 +100,27 @@ __device__ __forceinline__ double weight(float x, float m, Scale c) {
   p = fma(p, f, 0x1.c6b08d7044115p-5);
   p = fma(p, f, 0x1.ebfbdff82c590p-3);
   p = fma(p, f, 0x1.62e42fefa39f7p-1);
-  p = fma(p, f, 1.0);
-  return t > -1100.0 ? ldexp(p, __double2loint(big)) : 0.0;   // (NaN: 0)
+  return fma(p, f, 1.0);
+}
+// exp((x - m) / temperature) to about 1e-15, exactly 1 at x = m, 0 for -inf: 2^t with t = k + f, k from the low bits of
+// t + 1.5 2^52.
+__device__ __forceinline__ double weight(float x, float m, Scale c) {
+  if (m == -kNegInf) return x == m ? 1.0 : 0.0;   // infinite logits share the mass
+  const double d = (double)x - (double)m;
+  const double t = d * c.hi, lo = fma(d, c.lo, fma(d, c.hi, -t));
+  const double big = t + 0x1.8p52, f = (t - (big - 0x1.8p52)) + lo;
+  return t > -1100.0 ? ldexp(exp2_part(f), __double2loint(big)) : 0.0;   // (NaN: 0)
 }
 
 // Sum over the block, in one fixed order; every thread receives it. `lds`: one double a wave.
-__device__ __forceinline__ double block_sum(double x, double* lds) {
+template <int THREADS> __device__ __forceinline__ double block_sum(double x, double* lds) {
   for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, kWave);
   __syncthreads();   // (the last call's readers)
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
   __syncthreads();
   double s = 0.0;
-  for (int w = 0; w < kVerifyThreads / kWave; ++w) s += lds[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) s += lds[w];
   return s;
 }
 
@@ -141,52 +151,81 @@ template <typename T> __device__ __forceinline__ Row<T> logits_row(const VerifyP
 }
 
 // Chunk c of node t of row b: its maximum, the first element that holds it, the sum of its weights against it.
-template <typename T> __global__ __launch_bounds__(kVerifyThreads) void verify_scan_kernel(VerifyParams p) {
+//
+// In a sum next to a 1 a weight needs no more than 1e-13 of itself, and none below 2^-1000 counts: the scan's own form
+// of it has the temperature's scale in one part, a polynomial through nine points (4e-14), the exponent added as a whole number:
+// 18 instructions a logit. They are what it waits for: a vocabulary's bf16 logits come from memory twice as fast.
+template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
   const int c = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
   if (t >= p.nodes(b)) return;
-  constexpr int E = Row<T>::E, U = kPer / E;
+  constexpr int E = Row<T>::E, U = kVerifyChunk / kScanThreads / E, WAVES = kScanThreads / kWave;
   const Row<T> row = logits_row<T>(p, b, t);
   const int first = c * kVerifyChunk - row.shift;
   float x[U][E];
 #pragma unroll
-  for (int u = 0; u < U; ++u) row.piece(first + (u * kVerifyThreads + (int)threadIdx.x) * E, x[u]);
+  for (int u = 0; u < U; ++u) row.piece(first + (u * kScanThreads + (int)threadIdx.x) * E, x[u]);
   float m = kNegInf;
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < E; ++e) m = fmaxf(m, x[u][e]);
-  __shared__ float wm[kVerifyThreads / kWave];
-  __shared__ int wi[kVerifyThreads / kWave];
-  __shared__ double wz[kVerifyThreads / kWave];
+  __shared__ float wm[WAVES];
+  __shared__ int wi[WAVES];
+  __shared__ double wz[WAVES];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   m = group_max<64>(m);
   if (lane == 0) wm[wave] = m;
   __syncthreads();
-  for (int w = 0; w < kVerifyThreads / kWave; ++w) m = fmaxf(m, wm[w]);
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, wm[w]);
   int i = p.V;
 #pragma unroll
   for (int u = U - 1; u >= 0; --u)
 #pragma unroll
     for (int e = E - 1; e >= 0; --e)
-      if (x[u][e] == m) i = first + (u * kVerifyThreads + (int)threadIdx.x) * E + e;
+      if (x[u][e] == m) i = first + (u * kScanThreads + (int)threadIdx.x) * E + e;
   if (i < 0) i = 0;   // (-inf before the row's first element)
   for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d, kWave));
-  if (lane == 0) wi[wave] = i;
   const double heat = p.heat(b);
   double z = 0.0;
   if (heat > 0.0 && m > kNegInf) {
-    const Scale s = scale_of(heat);
+    const Scale s = row_scale(p, b);
+    if (m == -kNegInf) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) z += weight(x[u][e], m, s);
+        for (int e = 0; e < E; ++e) z += x[u][e] == m ? 1.0 : 0.0;
+    } else {
+      const double md = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const double t2 = fmax(((double)x[u][e] - md) * s.hi, -1000.0);
+          const double big = t2 + 0x1.8p52, f = t2 - (big - 0x1.8p52);
+          double q = 0x1.b6387fc000000p-24;
+          q = fma(q, f, 0x1.63d1362f8e38ep-20);
+          q = fma(q, f, 0x1.ffcb951640000p-17);
+          q = fma(q, f, 0x1.4308ac85afeabp-13);
+          q = fma(q, f, 0x1.5d87fe86fe75cp-10);
+          q = fma(q, f, 0x1.3b2ab7181b731p-7);
+          q = fma(q, f, 0x1.c6b08d7047e52p-5);
+          q = fma(q, f, 0x1.ebfbdff823cedp-3);
+          q = fma(q, f, 0x1.62e42fefa39efp-1);
+          q = fma(q, f, 1.0);
+          z += __hiloint2double(__double2hiint(q) + (int)((unsigned)__double2loint(big) << 20), __double2loint(q));
+        }
+    }
+    for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d, kWave);
   }
-  z = block_sum(z, wz);
+  if (lane == 0) wi[wave] = i, wz[wave] = z;
+  __syncthreads();
   if (threadIdx.x == 0) {
     const int64_t at = ((int64_t)b * p.T + t) * p.C + c;
-    for (int w = 1; w < kVerifyThreads / kWave; ++w) wi[0] = min(wi[0], wi[w]);
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) i = min(i, wi[w]), z += wz[w];
     p.part_m[at] = m;
-    p.part_i[at] = wi[0];
+    p.part_i[at] = i;
     p.part_z[at] = z;
   }
 }
@@ -227,30 +266,18 @@ template <typename F> __device__ __forceinline__ Found find_chunk(int C, double 
   return found;
 }
 
-// A thread's 16 elements of a chunk that starts at `first`, as weights, without those whose bit is set in `cut`.
-template <typename T>
-__device__ __forceinline__ void chunk_weights(const Row<T>& row, int i0, float m, Scale s, unsigned cut, double (&r)[kPer]) {
-  constexpr int E = Row<T>::E;
-#pragma unroll
-  for (int u = 0; u < kPer / E; ++u) {
-    float x[E];
-    row.piece(i0 + u * E, x);
-#pragma unroll
-    for (int e = 0; e < E; ++e) r[u * E + e] = cut >> (u * E + e) & 1 ? 0.0 : weight(x[e], m, s);
-  }
-}
-
-// The first element of a chunk at which the running sum of what the threads hold (16 elements each, r) passes the target,
+// The first element of a chunk at which the running sum of what the threads hold (PER elements each, r) passes the target,
 // or the last that has any.
-__device__ __forceinline__ int find_element(int first, double target, const double (&r)[kPer]) {
-  __shared__ double sums[kVerifyThreads / kWave];
+template <int THREADS, int PER = kVerifyChunk / THREADS>
+__device__ __forceinline__ int find_element(int first, double target, const double (&r)[PER]) {
+  __shared__ double sums[THREADS / kWave];
   __shared__ int hit, most;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int i0 = first + (int)threadIdx.x * kPer;
+  const int i0 = first + (int)threadIdx.x * PER;
   if (threadIdx.x == 0) hit = INT_MAX, most = -1;
   double own = 0.0;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) own += r[e];
+  for (int e = 0; e < PER; ++e) own += r[e];
   double upto = own;
   for (int d = 1; d < kWave; d <<= 1) {
     const double y = __shfl_up(upto, d, kWave);
@@ -258,15 +285,13 @@ __device__ __forceinline__ int find_element(int first, double target, const doub
   }
   if (lane == kWave - 1) sums[wave] = upto;
   __syncthreads();
-  double sum = upto - own;
-  {
-    double before = 0.0;
-    for (int w = 0; w < wave; ++w) before += sums[w];
-    sum += before;
-  }
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / kWave; ++w) sum += w < wave ? sums[w] : 0.0;
+  sum += upto - own;
   int at = INT_MAX, last = -1;
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
+  for (int e = 0; e < PER; ++e) {
     sum += r[e];
     if (r[e] > 0.0) {
       last = i0 + e;
@@ -279,68 +304,135 @@ __device__ __forceinline__ int find_element(int first, double target, const doub
   return hit < INT_MAX ? hit : most < 0 ? 0 : most;
 }
 
-constexpr int kVerifyNodes = FORGE_TREE_MAX_TOKENS;
+// max(e - a q, 0) over a row whose next token is drawn from there.
+template <typename T, typename Q> struct Rest {
+  Row<T> row;
+  const Q* q;
+  double taken;
+  float most;
+  Scale s;
+  __device__ __forceinline__ Rest(const VerifyParams& p, int b, int node, double taken, float most, Scale s)
+      : row(logits_row<T>(p, b, node)), q(static_cast<const Q*>(p.probs) + b * p.sqb + node * p.sqt), taken(taken), most(most),
+        s(s) {}
+  __device__ __forceinline__ double of(float x, double q) const { return fmax(weight(x, most, s) - taken * q, 0.0); }
+  __device__ __forceinline__ double one(int v) const { return of(row.one(v), (double)to_f32<Q>(q[v])); }
+  // the 8 elements from i0 on, a piece's first; 0 where there are none
+  __device__ __forceinline__ void eight(int i0, double (&r)[8]) const {
+    constexpr int E = Row<T>::E;
+    float x[8], y[8];
+#pragma unroll
+    for (int u = 0; u < 8 / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
+    if (i0 >= 0 && i0 + 8 <= row.V && (uintptr_t)(q + i0) % 16 == 0) {
+#pragma unroll
+      for (int u = 0; u < 8 * (int)sizeof(Q) / 16; ++u) unpack16<Q>(load16(q + i0 + u * (16 / (int)sizeof(Q))), y + u * (16 / (int)sizeof(Q)));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = i0 + e >= 0 && i0 + e < row.V ? to_f32<Q>(q[i0 + e]) : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = of(x[e], (double)y[e]);
+  }
+};
 
-template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyParams p) {
+constexpr int kVerifyNodes = FORGE_TREE_MAX_TOKENS;
+static_assert(kVerifyChunk / kWalkThreads == 8, "a thread of the walk's draw holds eight elements");
+
+// One block per row: from the chunks' numbers to its new tokens. Latency: the nodes' numbers, their tokens' logits and the one
+// chunk that the draw falls into are read one after the other.
+template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
   __shared__ float most[kVerifyNodes], us[kVerifyNodes];
   __shared__ double zs[kVerifyNodes], es[kVerifyNodes];
   __shared__ int args[kVerifyNodes], tok[kVerifyNodes], par[kVerifyNodes], child[kVerifyNodes], sib[kVerifyNodes];
   __shared__ bool yes[kVerifyNodes];
-  __shared__ double lds[kVerifyThreads / kWave];
+  __shared__ double lds[kWalkThreads / kWave];
   const int b = blockIdx.x, n = p.nodes(b), tid = threadIdx.x;
-  const int lane = tid % kWave, wave = tid / kWave;
   int64_t* out = p.out + (int64_t)b * p.T;
   int32_t* path = p.path + (int64_t)b * p.T;
-  for (int t = tid; t < p.T; t += kVerifyThreads) {
-    out[t] = -1;
-    path[t] = t == 0 && n > 0 ? 0 : -1;
+  const double heat = p.heat(b);
+  const bool warm = heat > 0.0;
+  const Scale s = row_scale(p, b);
+  const Q* probs = static_cast<const Q*>(p.probs);
+  const auto q_of = [&](int node, int v) { return (double)to_f32<Q>(probs[b * p.sqb + node * p.sqt + v]); };
+
+  // each drafted token, its parent and the logit it is judged by (the loads go out before the chunks' numbers are met)
+  constexpr int MINE = kVerifyNodes / kWalkThreads;
+  float logit[MINE];
+#pragma unroll
+  for (int y = 0; y < MINE; ++y) {
+    const int t = tid + y * kWalkThreads;
+    logit[y] = kNegInf;
+    if (t < p.T) {
+      out[t] = -1;
+      path[t] = t == 0 && n > 0 ? 0 : -1;
+    }
+    if (t >= n) continue;
+    const int64_t x = p.tokens[b * p.stb + t];
+    const int up = t == 0 ? -1 : p.parents ? p.parents[b * p.spb + t] : t - 1;
+    const bool real = x >= 0 && x < p.V && up >= 0 && up < t;   // (others are passed over)
+    tok[t] = real ? (int)x : -1;
+    par[t] = real ? up : -1;
+    us[t] = warm ? p.uniform[b * p.sub + t] : 0.0f;
+    child[t] = p.T;
+    if (real && warm) logit[y] = logits_row<T>(p, b, up).one((int)x);
   }
-  if (p.probs && tid == 0) p.state[b].left = 0;
+  if (probs && tid == 0) {
+    p.state[b].left = 0;
+    p.state[b].done = 0;
+  }
   if (n == 0) {
     if (tid == 0) p.count[b] = 0;
     return;
   }
-  const double heat = p.heat(b);
-  const bool warm = heat > 0.0;
-  const Scale s = scale_of(warm ? heat : 1.0);
 
-  // each node's maximum, argmax and sum
-  for (int t = wave; t < n; t += kVerifyThreads / kWave) {
+  // each node's maximum, argmax and sum: 16 lanes a node
+  for (int t = tid / 16; t < n; t += kWalkThreads / 16) {
     const int64_t at = ((int64_t)b * p.T + t) * p.C;
+    const int l = tid % 16;
     float m = kNegInf;
-    for (int c = lane; c < p.C; c += kWave) m = fmaxf(m, p.part_m[at + c]);
-    m = group_max<64>(m);
     int i = p.V;
     double z = 0.0;
-    for (int c = lane; c < p.C; c += kWave) {
+    for (int c = l; c < p.C; c += 16) {   // (the running sum against the running maximum)
       const float mc = p.part_m[at + c];
-      if (mc == m) i = min(i, p.part_i[at + c]);
-      if (warm && mc > kNegInf) z += p.part_z[at + c] * weight(mc, m, s);
+      const int ic = p.part_i[at + c];
+      const double zc = p.part_z[at + c];
+      if (mc > m) {
+        z = warm ? zc + (m > kNegInf ? z * weight(m, mc, s) : 0.0) : 0.0;
+        m = mc;
+        i = ic;
+      } else if (mc == m) {   // (in rising order: the first stays)
+        z += zc;
+        i = min(i, ic);
+      } else if (warm && mc > kNegInf) {
+        z += zc * weight(mc, m, s);
+      }
     }
-    for (int d = 32; d; d >>= 1) {
+    const float top = group_max<16>(m);
+    if (m < top) i = p.V;
+    if (warm) z = m > kNegInf ? z * weight(m, top, s) : 0.0;
+    for (int d = 8; d; d >>= 1) {
       i = min(i, __shfl_xor(i, d, kWave));
       z += __shfl_xor(z, d, kWave);
     }
-    if (lane == 0) most[t] = m, args[t] = i, zs[t] = z;
-  }
-  for (int t = tid; t < n; t += kVerifyThreads) {
-    const int64_t x = p.tokens[b * p.stb + t];
-    tok[t] = x >= 0 && x < p.V ? (int)x : -1;
-    const int up = t == 0 ? -1 : p.parents ? p.parents[b * p.spb + t] : t - 1;
-    par[t] = up >= 0 && up < t && tok[t] >= 0 ? up : -1;   // (tokens that are none are passed over)
-    us[t] = warm ? p.uniform[b * p.sub + t] : 0.0f;
-    child[t] = p.T;
+    if (l == 0) most[t] = top, args[t] = i, zs[t] = z;
   }
   __syncthreads();
-  for (int t = tid; t < n; t += kVerifyThreads)
-    es[t] = warm && par[t] >= 0 && most[par[t]] > kNegInf ? weight(logits_row<T>(p, b, par[t]).one(tok[t]), most[par[t]], s) : 0.0;
+#pragma unroll
+  for (int y = 0; y < MINE; ++y) {
+    const int t = tid + y * kWalkThreads;
+    if (t >= n) continue;
+    const int up = par[t];
+    es[t] = warm && up >= 0 && most[up] > kNegInf ? weight(logit[y], most[up], s) : 0.0;
+    if (!warm || probs || up < 0) continue;
+    bool twice = false;   // an earlier sibling has the token
+#pragma unroll 4
+    for (int j = up + 1; j < t; ++j) twice |= par[j] == up && tok[j] == tok[t];
+    yes[t] = !twice;
+  }
   __syncthreads();
 
   // Who would be accepted if the walk came to its parent. With the drafter's probabilities that is known for first
   // children only: child[] are a node's first children, sib[] their next siblings. Else child[] are the accepted ones.
-  const Q* probs = static_cast<const Q*>(p.probs);
-  const auto q_of = [&](int node, int v) { return (double)to_f32<Q>(probs[b * p.sqb + node * p.sqt + v]); };
-  for (int t = tid; t < n; t += kVerifyThreads) {
+  for (int t = tid; t < n; t += kWalkThreads) {
     const int up = par[t];
     if (up < 0) continue;
     if (!warm) {
@@ -349,19 +441,14 @@ template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) v
       yes[t] = us[t] * q_of(up, tok[t]) * zs[up] < es[t];
       atomicMin(&child[up], t);
       int next = p.T;
+#pragma unroll 4
       for (int j = n - 1; j > t; --j) next = par[j] == up ? j : next;
       sib[t] = next;
-    } else {
+    } else if (yes[t]) {
       double left = zs[up];
-      bool twice = false;
-      for (int j = up + 1; j < t; ++j) {
-        if (par[j] != up) continue;
-        twice |= tok[j] == tok[t];
-        bool counted = false;   // (its token is out already)
-        for (int k = up + 1; k < j; ++k) counted |= par[k] == up && tok[k] == tok[j];
-        if (!counted) left -= es[j];
-      }
-      if (!twice && us[t] * fmax(left, 0.0) < es[t]) atomicMin(&child[up], t);
+#pragma unroll 4
+      for (int j = up + 1; j < t; ++j) left -= par[j] == up && yes[j] ? es[j] : 0.0;
+      if (us[t] * fmax(left, 0.0) < es[t]) atomicMin(&child[up], t);
     }
   }
   __syncthreads();
@@ -374,11 +461,17 @@ template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) v
     if (t >= p.T) break;
     if (warm && probs && !yes[t]) {
       taken = zs[at];
-      const Row<T> row = logits_row<T>(p, b, at);
       for (t = sib[t]; t < p.T; t = sib[t]) {
+        const Rest<T, Q> rest(p, b, at, taken, most[at], s);
         double w = 0.0;
-        for (int v = tid; v < p.V; v += kVerifyThreads) w += fmax(weight(row.one(v), most[at], s) - taken * q_of(at, v), 0.0);
-        w = block_sum(w, lds);
+#pragma unroll 2
+        for (int i = tid * 8 - rest.row.shift; i < p.V; i += kWalkThreads * 8) {
+          double x[8];
+          rest.eight(i, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w += x[e];
+        }
+        w = block_sum<kWalkThreads>(w, lds);
         const double q = q_of(at, tok[t]);
         if (us[t] * q * w < es[t] - taken * q) break;
         taken += w;
@@ -396,62 +489,75 @@ template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) v
 
   int token = args[at];
   if (warm && most[at] > kNegInf && taken > 0.0) {   // what the drafter's probabilities left is drawn from below
-    if (tid == 0) p.state[b] = State{taken, most[at], at, count - 1, 1, token};
+    if (tid == 0) p.state[b] = State{taken, most[at], at, count - 1, 1, token, 0};
     token = -1;
   } else if (warm && most[at] > kNegInf) {
     const Row<T> row = logits_row<T>(p, b, at);
     const int64_t base = ((int64_t)b * p.T + at) * p.C;
+    const float top = most[at];
     double* masses = zs;   // (the nodes' are done with: [chunk])
+    double* whole = es;    // a chunk's, before tokens were taken out
     int* gone = child;     // the rejected children's tokens, and the chunks they are in
     int* again = sib;
     __shared__ int ngone, nagain;
     __syncthreads();
     if (tid == 0) ngone = nagain = 0;
-    for (int c = tid; c < p.C; c += kVerifyThreads) {
+    for (int c = tid; c < p.C; c += kWalkThreads) {
       const float mc = p.part_m[base + c];
-      masses[c] = mc > kNegInf ? p.part_z[base + c] * weight(mc, most[at], s) : 0.0;
-      args[c] = 0;
+      masses[c] = mc > kNegInf ? p.part_z[base + c] * weight(mc, top, s) : 0.0;
     }
     __syncthreads();
     if (!probs) {
-      for (int j = at + 1 + tid; j < n; j += kVerifyThreads) {
-        if (par[j] != at) continue;
-        gone[atomicAdd(&ngone, 1)] = tok[j];
-        const int c = (tok[j] + row.shift) / kVerifyChunk;
-        if (atomicExch(&args[c], 1) == 0) again[atomicAdd(&nagain, 1)] = c;
+      for (int j = at + 1 + tid; j < n; j += kWalkThreads)
+        if (par[j] == at && yes[j]) gone[atomicAdd(&ngone, 1)] = tok[j];
+      __syncthreads();
+      // a chunk that loses all but a thousandth of its sum is summed again: the difference could leave what is not there
+      for (int g = tid; g < ngone; g += kWalkThreads) {
+        const int c = (gone[g] + row.shift) / kVerifyChunk;
+        double out_of = 0.0;
+        bool first = true;
+        for (int h = 0; h < ngone; ++h) {
+          if ((gone[h] + row.shift) / kVerifyChunk != c) continue;
+          first &= h >= g;
+          out_of += weight(row.one(gone[h]), top, s);
+        }
+        if (!first) continue;
+        const double left = masses[c] - out_of;
+        if (left < masses[c] * 0x1p-10) again[atomicAdd(&nagain, 1)] = c;
+        else masses[c] = left;
       }
     }
     __syncthreads();
-    const auto cut_of = [&](int i0) {   // which of the 16 elements from i0 on were rejected
+    const auto eight = [&](int i0, double (&r)[8]) {   // the weights of the 8 elements from i0 on, without rejected ones
+      constexpr int E = Row<T>::E;
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8 / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
       unsigned cut = 0;
       for (int g = 0; g < ngone; ++g)
-        if ((unsigned)(gone[g] - i0) < kPer) cut |= 1u << (gone[g] - i0);
-      return cut;
-    };
-    // those chunks are summed again without them, a wave each: a difference could leave what is not there
-    for (int g = wave; g < nagain; g += kVerifyThreads / kWave) {
-      const int c = again[g];
-      double w = 0.0;
-      for (int i = lane * kPer; i < kVerifyChunk; i += kWave * kPer) {
-        const int i0 = c * kVerifyChunk - row.shift + i;
-        double x[kPer];
-        chunk_weights<T>(row, i0, most[at], s, cut_of(i0), x);
+        if ((unsigned)(gone[g] - i0) < 8) cut |= 1u << (gone[g] - i0);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) w += x[e];
-      }
-      for (int d = 32; d; d >>= 1) w += __shfl_xor(w, d, kWave);
-      if (lane == 0) masses[c] = w;
+      for (int e = 0; e < 8; ++e) r[e] = cut >> e & 1 ? 0.0 : weight(x[e], top, s);
+    };
+    double x[8];
+    for (int g = 0; g < nagain; ++g) {
+      const int c = again[g];
+      eight(c * kVerifyChunk - row.shift + tid * 8, x);
+      double w = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w += x[e];
+      w = block_sum<kWalkThreads>(w, lds);
+      if (tid == 0) masses[c] = w;
     }
     __syncthreads();
     double total = 0.0;
-    for (int c = tid; c < p.C; c += kVerifyThreads) total += masses[c];
-    total = block_sum(total, lds);
+    for (int c = tid; c < p.C; c += kWalkThreads) total += masses[c];
+    total = block_sum<kWalkThreads>(total, lds);
     if (total > 0.0) {
       const Found f = find_chunk(p.C, us[0] * total, [&](int c) { return masses[c]; });
-      const int first = f.c * kVerifyChunk - row.shift, i0 = first + tid * kPer;
-      double x[kPer];
-      chunk_weights<T>(row, i0, most[at], s, cut_of(i0), x);
-      token = find_element(first, f.target, x);
+      const int first = f.c * kVerifyChunk - row.shift;
+      eight(first + tid * 8, x);
+      token = find_element<kWalkThreads>(first, f.target, x);
     }
   }
   if (tid == 0) {
@@ -460,51 +566,45 @@ template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) v
   }
 }
 
-// max(e - a q, 0) summed over chunk c of a row whose next token comes from there, and the draw.
-template <typename T, typename Q> struct Rest {
-  Row<T> row;
-  const Q* q;
-  State st;
-  Scale s;
-  __device__ __forceinline__ Rest(const VerifyParams& p, int b, State st)
-      : row(logits_row<T>(p, b, st.node)), q(static_cast<const Q*>(p.probs) + b * p.sqb + st.node * p.sqt), st(st),
-        s(scale_of(p.heat(b))) {}
-  __device__ __forceinline__ double operator()(int v) const {
-    return fmax(weight(row.one(v), st.most, s) - st.taken * (double)to_f32<Q>(q[v]), 0.0);
-  }
-};
-template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) void verify_rest_kernel(VerifyParams p) {
-  __shared__ double lds[kVerifyThreads / kWave];
+// Sums over blocks on several XCDs, whose caches are their own: written past them, counted, and read by the block that
+// counts last.
+__device__ __forceinline__ void store_agent(double* p, double x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double load_agent(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// What the drafter's probabilities left of a row, chunk by chunk; a row's last block draws from it.
+template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_rest_kernel(VerifyParams p) {
+  __shared__ double lds[kWalkThreads / kWave];
+  __shared__ bool last;
   const int c = blockIdx.x, b = blockIdx.y;
   const State st = p.state[b];
   if (!st.left) return;
-  const Rest<T, Q> rest(p, b, st);
-  const int first = c * kVerifyChunk - rest.row.shift;
-  double w = 0.0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < kVerifyChunk; i += kVerifyThreads)
-    if (first + i >= 0 && first + i < p.V) w += rest(first + i);
-  w = block_sum(w, lds);
-  if (threadIdx.x == 0) p.rest[(int64_t)b * p.C + c] = w;
-}
-template <typename T, typename Q> __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyParams p) {
-  __shared__ double lds[kVerifyThreads / kWave];
-  const int b = blockIdx.x;
-  const State st = p.state[b];
-  if (!st.left) return;
-  const double* sums = p.rest + (int64_t)b * p.C;
+  const Rest<T, Q> rest(p, b, st.node, st.taken, st.most, row_scale(p, b));
+  double* sums = p.rest + (int64_t)b * p.C;
+  double x[8], w = 0.0;
+  rest.eight(c * kVerifyChunk - rest.row.shift + (int)threadIdx.x * 8, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w += x[e];
+  w = block_sum<kWalkThreads>(w, lds);
+  if (threadIdx.x == 0) {
+    store_agent(sums + c, w);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = atomicAdd(&p.state[b].done, 1u) == (unsigned)p.C - 1;
+  }
+  __syncthreads();
+  if (!last) return;
   double total = 0.0;
-  for (int c = threadIdx.x; c < p.C; c += kVerifyThreads) total += sums[c];
-  total = block_sum(total, lds);
+  for (int i = threadIdx.x; i < p.C; i += kWalkThreads) total += load_agent(sums + i);
+  total = block_sum<kWalkThreads>(total, lds);
   int token = st.arg;
   if (total > 0.0) {
-    const Rest<T, Q> rest(p, b, st);
-    const Found f = find_chunk(p.C, (double)p.uniform[b * p.sub] * total, [&](int c) { return sums[c]; });
-    const int first = f.c * kVerifyChunk - rest.row.shift, i0 = first + (int)threadIdx.x * kPer;
-    double x[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = i0 + e >= 0 && i0 + e < p.V ? rest(i0 + e) : 0.0;
-    token = find_element(first, f.target, x);
+    const Found f = find_chunk(p.C, (double)p.uniform[b * p.sub] * total, [&](int i) { return load_agent(sums + i); });
+    const int first = f.c * kVerifyChunk - rest.row.shift;
+    rest.eight(first + (int)threadIdx.x * 8, x);
+    token = find_element<kWalkThreads>(first, f.target, x);
   }
   if (threadIdx.x == 0) p.out[(int64_t)b * p.T + st.at] = token;
 }
@@ -526,16 +626,13 @@ static VerifyWs verify_ws(int B, int T, int V, bool probs) {
 }
 
 template <typename T, typename Q> static int launch_verify(const VerifyParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((verify_scan_kernel<T>), dim3(p.C, p.T, p.B), dim3(kVerifyThreads), 0, s, p);
+  hipLaunchKernelGGL((verify_scan_kernel<T>), dim3(p.C, p.T, p.B), dim3(kScanThreads), 0, s, p);
   int st = check_launch();
   if (st) return st;
-  hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kVerifyThreads), 0, s, p);
+  hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kWalkThreads), 0, s, p);
   st = check_launch();
   if (st || !p.probs) return st;
-  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kVerifyThreads), 0, s, p);
-  st = check_launch();
-  if (st) return st;
-  hipLaunchKernelGGL((verify_draw_kernel<T, Q>), dim3(p.B), dim3(kVerifyThreads), 0, s, p);
+  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kWalkThreads), 0, s, p);
   return check_launch();
 }
 
@@ -582,6 +679,10 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
   p.tokens = tokens; p.stb = s_tokens_b; p.parents = parents; p.spb = s_parents_b;
   p.uniform = uniform; p.sub = s_uniform_b; p.temps = temperatures; p.temperature = temperature;
   p.probs = draft_probs; p.sqb = s_probs_b; p.sqt = s_probs_t;
+  if (!temperatures) {
+    const Scale scale = scale_of(temperature > 0.0 ? temperature : 1.0);
+    p.scale_hi = scale.hi; p.scale_lo = scale.lo;
+  }
   p.new_lens = new_lens;
   p.B = B; p.T = T; p.V = V; p.C = verify_chunks(V);
   p.out = out; p.path = path; p.count = count;
