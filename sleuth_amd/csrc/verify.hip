@@ -67,7 +67,6 @@ struct State {
   float most;    // max l
   int node, at;  // where; which of the row's outputs the token is
   int left;      // 0: drawn already
-  int arg;       // the argmax, for a row without anything left
   unsigned done;  // blocks that have summed their chunk
 };
 
@@ -139,7 +138,7 @@ template <typename T> struct Row {
       for (int e = 0; e < E; ++e) x[e] = i + e >= 0 && i + e < V ? to_f32<T>(at[i + e]) : kNegInf;
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] == x[e] ? x[e] : kNegInf;
+    for (int e = 0; e < E; ++e) x[e] = fmaxf(x[e], kNegInf);   // (of a NaN and a number the number)
   }
   __device__ __forceinline__ float one(int i) const {
     const float x = to_f32<T>(at[i]);
@@ -152,9 +151,11 @@ template <typename T> __device__ __forceinline__ Row<T> logits_row(const VerifyP
 
 // Chunk c of node t of row b: its maximum, the first element that holds it, the sum of its weights against it.
 //
-// In a sum next to a 1 a weight needs no more than 1e-13 of itself, and none below 2^-1000 counts: the scan's own form
-// of it has the temperature's scale in one part, a polynomial through nine points (4e-14), the exponent added as a whole number:
-// 18 instructions a logit. They are what it waits for: a vocabulary's bf16 logits come from memory twice as fast.
+// The draw takes a chunk's elements apart with weights of 1e-15, so what a sum here may be off by moves a few chunks' ends
+// and a threshold, not every element's: 1e-10 of itself turns one answer in 10^8. So the scan has its own form of a weight,
+// with the temperature's scale in one part and a polynomial through seven points (1.2e-10), the exponent added as a whole
+// number, and nothing below 2^-1000: 19 instructions a logit, which are what it waits for (a bf16 logit comes from memory
+// in half that time). The argmax is looked for where it decides, at temperature 0.
 template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
   const int c = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
   if (t >= p.nodes(b)) return;
@@ -178,17 +179,19 @@ template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_sca
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) m = fmaxf(m, wm[w]);
-  int i = p.V;
-#pragma unroll
-  for (int u = U - 1; u >= 0; --u)
-#pragma unroll
-    for (int e = E - 1; e >= 0; --e)
-      if (x[u][e] == m) i = first + (u * kScanThreads + (int)threadIdx.x) * E + e;
-  if (i < 0) i = 0;   // (-inf before the row's first element)
-  for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d, kWave));
   const double heat = p.heat(b);
   double z = 0.0;
-  if (heat > 0.0 && m > kNegInf) {
+  int i = 0;
+  if (!(heat > 0.0)) {
+    i = p.V;
+#pragma unroll
+    for (int u = U - 1; u >= 0; --u)
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (x[u][e] == m) i = first + (u * kScanThreads + (int)threadIdx.x) * E + e;
+    if (i < 0) i = 0;   // (-inf before the row's first element)
+    for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d, kWave));
+  } else if (m > kNegInf) {
     const Scale s = row_scale(p, b);
     if (m == -kNegInf) {
 #pragma unroll
@@ -196,21 +199,19 @@ template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_sca
 #pragma unroll
         for (int e = 0; e < E; ++e) z += x[u][e] == m ? 1.0 : 0.0;
     } else {
-      const double md = m;
+      const double md = m, least = -1000.0 / s.hi;
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const double t2 = fmax(((double)x[u][e] - md) * s.hi, -1000.0);
-          const double big = t2 + 0x1.8p52, f = t2 - (big - 0x1.8p52);
-          double q = 0x1.b6387fc000000p-24;
-          q = fma(q, f, 0x1.63d1362f8e38ep-20);
-          q = fma(q, f, 0x1.ffcb951640000p-17);
-          q = fma(q, f, 0x1.4308ac85afeabp-13);
-          q = fma(q, f, 0x1.5d87fe86fe75cp-10);
-          q = fma(q, f, 0x1.3b2ab7181b731p-7);
-          q = fma(q, f, 0x1.c6b08d7047e52p-5);
-          q = fma(q, f, 0x1.ebfbdff823cedp-3);
+          const double d = fmax((double)x[u][e] - md, least), big = fma(d, s.hi, 0x1.8p52);
+          const double f = fma(d, s.hi, -(big - 0x1.8p52));
+          double q = 0x1.00a581599a492p-16;
+          q = fma(q, f, 0x1.443fffc90e1b7p-13);
+          q = fma(q, f, 0x1.5d879ead062cep-10);
+          q = fma(q, f, 0x1.3b2a1b7152be9p-7);
+          q = fma(q, f, 0x1.c6b08d883dca7p-5);
+          q = fma(q, f, 0x1.ebfbe045f4d3cp-3);
           q = fma(q, f, 0x1.62e42fefa39efp-1);
           q = fma(q, f, 1.0);
           z += __hiloint2double(__double2hiint(q) + (int)((unsigned)__double2loint(big) << 20), __double2loint(q));
@@ -302,6 +303,18 @@ __device__ __forceinline__ int find_element(int first, double target, const doub
   if (last >= 0) atomicMax(&most, last);
   __syncthreads();
   return hit < INT_MAX ? hit : most < 0 ? 0 : most;
+}
+
+// The first element that holds the row's maximum (where rejections left nothing: once in a blue moon).
+template <typename T> __device__ __forceinline__ int argmax_of(Row<T> row, float top) {
+  __shared__ int first;
+  if (threadIdx.x == 0) first = INT_MAX;
+  __syncthreads();
+  int i = threadIdx.x;
+  while (i < row.V && row.one(i) != top) i += kWalkThreads;
+  if (i < row.V) atomicMin(&first, i);
+  __syncthreads();
+  return first < INT_MAX ? first : 0;
 }
 
 // max(e - a q, 0) over a row whose next token is drawn from there.
@@ -487,9 +500,9 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
     ++count;
   }
 
-  int token = args[at];
+  int token = warm ? 0 : args[at];
   if (warm && most[at] > kNegInf && taken > 0.0) {   // what the drafter's probabilities left is drawn from below
-    if (tid == 0) p.state[b] = State{taken, most[at], at, count - 1, 1, token, 0};
+    if (tid == 0) p.state[b] = State{taken, most[at], at, count - 1, 1, 0};
     token = -1;
   } else if (warm && most[at] > kNegInf) {
     const Row<T> row = logits_row<T>(p, b, at);
@@ -558,6 +571,8 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
       const int first = f.c * kVerifyChunk - row.shift;
       eight(first + tid * 8, x);
       token = find_element<kWalkThreads>(first, f.target, x);
+    } else {
+      token = argmax_of(row, top);
     }
   }
   if (tid == 0) {
@@ -599,12 +614,14 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
   double total = 0.0;
   for (int i = threadIdx.x; i < p.C; i += kWalkThreads) total += load_agent(sums + i);
   total = block_sum<kWalkThreads>(total, lds);
-  int token = st.arg;
+  int token;
   if (total > 0.0) {
     const Found f = find_chunk(p.C, (double)p.uniform[b * p.sub] * total, [&](int i) { return load_agent(sums + i); });
     const int first = f.c * kVerifyChunk - rest.row.shift;
     rest.eight(first + (int)threadIdx.x * 8, x);
     token = find_element<kWalkThreads>(first, f.target, x);
+  } else {
+    token = argmax_of(rest.row, st.most);
   }
   if (threadIdx.x == 0) p.out[(int64_t)b * p.T + st.at] = token;
 }
