@@ -194,7 +194,7 @@ SIGNATURES: dict[str, tuple] = {
         _p, C.c_double,                      # temperatures or None, temperature
         _i, _p, _i64, _i64,                  # dtype of draft_probs, draft_probs or None + strides (b, t)
         _p, _p, _p, _p,                      # new_lens, out, path, count
-        _p, C.c_size_t,                      # workspace, bytes
+        _p, C.c_size_t, _i,                  # workspace, bytes, ws_flags
         _p]),
     "forge_kv_compact": (_i, [
         _i, _i, _i, _i, _i,                  # element size, layers, B, K, D

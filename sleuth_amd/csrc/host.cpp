@@ -745,15 +745,15 @@ bool rows2_ok(const Tensor& t, at::ScalarType type, int64_t B, int64_t T, c10::D
   return true;
 }
 
-// verify_drafts(logits, tokens, parents | None, uniform | None, temperature, draft_probs | None, new_lens | None)
+// verify_drafts(table of workspaces, logits, tokens, parents | None, uniform | None, temperature, draft_probs | None, new_lens | None)
 PyObject* verify_drafts_impl(PyObject* const* a) {
   Tensor logits, tokens, parents, uniform, temps, probs, news;
-  if (!take(a[0], logits) || !take(a[1], tokens) || !take_opt(a[2], parents) || !take_opt(a[3], uniform) ||
-      !take_opt(a[5], probs) || !take_opt(a[6], news))
+  if (!take(a[1], logits) || !take(a[2], tokens) || !take_opt(a[3], parents) || !take_opt(a[4], uniform) ||
+      !take_opt(a[6], probs) || !take_opt(a[7], news))
     return nullptr;
   double heat = 0.0;
-  if (PyFloat_CheckExact(a[4])) heat = PyFloat_AS_DOUBLE(a[4]);
-  else if (!take(a[4], temps)) return nullptr;
+  if (PyFloat_CheckExact(a[5])) heat = PyFloat_AS_DOUBLE(a[5]);
+  else if (!take(a[5], temps)) return nullptr;
   const c10::Device dev = logits.device();
   const int dt = dtype_of(logits);
   if (dt < 0 || logits.dim() != 3 || c10::hip::current_device() != dev.index()) return nullptr;
@@ -776,24 +776,29 @@ PyObject* verify_drafts_impl(PyObject* const* a) {
         probs.device() != dev)
       return nullptr;
   }
+  const size_t need = forge_verify_drafts_workspace_bytes((int)B, (int)T, (int)V, probs.defined());
+  if (!need) return nullptr;
+  const bool kept = need <= ((size_t)32 << 20) && !capturing();
+  const hipStream_t stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
+  StreamWorkspace sw(a[0], dev.index(), stream, kept ? need : 0);
+  if (kept && !sw.ptr) return nullptr;   // (made the Python way)
   Tensor out, path, count, ws;
   int st;
   {
     NoGil unlocked;
-    const size_t need = forge_verify_drafts_workspace_bytes((int)B, (int)T, (int)V, probs.defined());
-    if (!need) return nullptr;
     out = at::empty({B, T}, tokens.options());
     path = at::empty({B, T}, tokens.options().dtype(at::kInt));
     count = at::empty({B}, tokens.options().dtype(at::kInt));
-    ws = at::empty({(int64_t)need}, tokens.options().dtype(at::kByte));
+    if (!kept) ws = at::empty({(int64_t)need}, tokens.options().dtype(at::kByte));
     st = forge_verify_drafts(dt, (int)B, (int)T, (int)V, ptr(logits), logits.stride(0), logits.stride(1),
                              static_cast<const int64_t*>(ptr(tokens)), st_, static_cast<const int32_t*>(ptr(parents)), sp,
                              static_cast<const float*>(ptr(uniform)), su, static_cast<const float*>(ptr(temps)), heat, pdt,
                              ptr(probs), probs.defined() ? probs.stride(0) : 0, probs.defined() ? probs.stride(1) : 0,
                              static_cast<const int32_t*>(ptr(news)), static_cast<int64_t*>(out.data_ptr()),
-                             static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()), ws.data_ptr(), need,
-                             c10::hip::getCurrentHIPStream(dev.index()).stream());
+                             static_cast<int32_t*>(path.data_ptr()), static_cast<int32_t*>(count.data_ptr()),
+                             kept ? sw.ptr : ws.data_ptr(), kept ? sw.bytes : need, kept ? FORGE_WS_ZEROED : 0, stream);
   }
+  if (st == 0) sw.put_back();
   if (st) return st < 0 ? nullptr : PyLong_FromLong(st);
   return tuple_of({out, path, count});
 }
@@ -931,7 +936,7 @@ PyMethodDef methods[] = {
     FORGE_ENTRY(decode_append, 21), FORGE_ENTRY(kv_append, 11), FORGE_ENTRY(prefill, 11),
     FORGE_ENTRY(linear_small, 8),   FORGE_ENTRY(tensors_are, 4), FORGE_ENTRY(kv_append_paged, 13),
     FORGE_ENTRY(attn_paged, 16),    FORGE_ENTRY(attn_sinks, 17), FORGE_ENTRY(tree_mask, 2),
-    FORGE_ENTRY(attn_tree, 19),     FORGE_ENTRY(attn_tree_paged, 18), FORGE_ENTRY(verify_drafts, 7),
+    FORGE_ENTRY(attn_tree, 19),     FORGE_ENTRY(attn_tree_paged, 18), FORGE_ENTRY(verify_drafts, 8),
     FORGE_ENTRY(kv_compact, 7),     FORGE_ENTRY(kv_compact_paged, 6), FORGE_ENTRY(copy_pages, 4), {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_forge_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -25,6 +25,7 @@ namespace forge {
 
 constexpr int kVerifyChunk = 4096;  // elements of a row that a block takes
 constexpr int kScanThreads = 256, kWalkThreads = 512;
+constexpr int kVerifyNodes = FORGE_TREE_MAX_TOKENS;
 
 struct VerifyParams {
   const void* logits;
@@ -44,10 +45,9 @@ struct VerifyParams {
   int64_t* out;    // [B][T]
   int32_t* path;
   int32_t* count;
-  // workspace: each chunk's maximum, its first place, its sum; a row's state between launches; the sums of what is left
-  double* part_z;  // [B][T][C]
-  float* part_m;
-  int32_t* part_i;
+  // workspace: each chunk's sum, maximum and its first place; a row's state between launches; the sums of what is left
+  struct Part* parts;  // [B][T][C]
+  unsigned* counters;  // [B], zero between calls: the block that scans a row's last chunk walks. Null: a launch of its own does
   double scale_hi, scale_lo;  // of `temperature`
   struct State* state;  // [B]
   double* rest;         // [B][C]
@@ -59,6 +59,12 @@ struct VerifyParams {
   __device__ __forceinline__ double heat(int b) const {
     return !temps ? temperature : temps[b] > 1e30f ? 1e30 : (double)temps[b];
   }
+};
+
+struct Part {
+  double z;
+  float m;
+  int i;
 };
 
 // Where a row's walk ended, if its next token is drawn from what the drafter's probabilities left.
@@ -101,7 +107,7 @@ __device__ __forceinline__ double exp2_part(double f) {
   p = fma(p, f, 0x1.62e42fefa39f7p-1);
   return fma(p, f, 1.0);
 }
-// exp((x - m) / temperature) to about 1e-15, exactly 1 at x = m, 0 for -inf: 2^t with t = k + f, k from the low bits of
+// exp((x - m) / temperature) to about 1e-15, exactly 1 at x = m, 0 for -inf and for a NaN (which no maximum takes): 2^t with t = k + f, k from the low bits of
 // t + 1.5 2^52.
 __device__ __forceinline__ double weight(float x, float m, Scale c) {
   if (m == -kNegInf) return x == m ? 1.0 : 0.0;   // infinite logits share the mass
@@ -123,13 +129,30 @@ template <int THREADS> __device__ __forceinline__ double block_sum(double x, dou
   return s;
 }
 
+// Numbers of blocks on several XCDs, whose caches are their own, are written past those, counted, and read by the block that
+// counts last.
+__device__ __forceinline__ void store_agent(double* p, double x) {
+  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ double load_agent(const double* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_part(Part* p, Part x) {
+  store_agent(&p->z, x.z);
+  store_agent(reinterpret_cast<double*>(&p->m), __hiloint2double(x.i, __float_as_int(x.m)));
+}
+__device__ __forceinline__ Part load_part(const Part* p) {
+  const double z = load_agent(&p->z), mi = load_agent(reinterpret_cast<const double*>(&p->m));
+  return Part{z, __int_as_float(__double2loint(mi)), __double2hiint(mi)};
+}
+
 // A row of logits, whose 16-byte pieces start `shift` elements before it; chunk c is elements c * 4096 - shift on.
 template <typename T> struct Row {
   static constexpr int E = 16 / sizeof(T);
   const T* at;
   int V, shift;
   __device__ __forceinline__ Row(const T* p, int V) : at(p), V(V), shift((int)((uintptr_t)p % 16 / sizeof(T))) {}
-  // the E elements from i on (a piece's first), -inf where there are none; a NaN counts as -inf
+  // the E elements from i on (a piece's first), -inf where there are none
   __device__ __forceinline__ void piece(int i, float (&x)[E]) const {
     if (i >= 0 && i + E <= V) {
       unpack16<T>(load16(at + i), x);
@@ -137,13 +160,8 @@ template <typename T> struct Row {
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = i + e >= 0 && i + e < V ? to_f32<T>(at[i + e]) : kNegInf;
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = fmaxf(x[e], kNegInf);   // (of a NaN and a number the number)
   }
-  __device__ __forceinline__ float one(int i) const {
-    const float x = to_f32<T>(at[i]);
-    return x == x ? x : kNegInf;
-  }
+  __device__ __forceinline__ float one(int i) const { return to_f32<T>(at[i]); }
 };
 template <typename T> __device__ __forceinline__ Row<T> logits_row(const VerifyParams& p, int b, int t) {
   return Row<T>(static_cast<const T*>(p.logits) + b * p.slb + t * p.slt, p.V);
@@ -156,9 +174,7 @@ template <typename T> __device__ __forceinline__ Row<T> logits_row(const VerifyP
 // with the temperature's scale in one part and a polynomial through seven points (1.2e-10), the exponent added as a whole
 // number, and nothing below 2^-1000: 19 instructions a logit, which are what it waits for (a bf16 logit comes from memory
 // in half that time). The argmax is looked for where it decides, at temperature 0.
-template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
-  const int c = blockIdx.x, t = blockIdx.y, b = blockIdx.z;
-  if (t >= p.nodes(b)) return;
+template <typename T> __device__ __forceinline__ Part scan_chunk(const VerifyParams& p, int b, int t, int c) {
   constexpr int E = Row<T>::E, U = kVerifyChunk / kScanThreads / E, WAVES = kScanThreads / kWave;
   const Row<T> row = logits_row<T>(p, b, t);
   const int first = c * kVerifyChunk - row.shift;
@@ -189,7 +205,6 @@ template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_sca
 #pragma unroll
       for (int e = E - 1; e >= 0; --e)
         if (x[u][e] == m) i = first + (u * kScanThreads + (int)threadIdx.x) * E + e;
-    if (i < 0) i = 0;   // (-inf before the row's first element)
     for (int d = 32; d; d >>= 1) i = min(i, __shfl_xor(i, d, kWave));
   } else if (m > kNegInf) {
     const Scale s = row_scale(p, b);
@@ -221,14 +236,9 @@ template <typename T> __global__ __launch_bounds__(kScanThreads) void verify_sca
   }
   if (lane == 0) wi[wave] = i, wz[wave] = z;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    const int64_t at = ((int64_t)b * p.T + t) * p.C + c;
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) i = min(i, wi[w]), z += wz[w];
-    p.part_m[at] = m;
-    p.part_i[at] = i;
-    p.part_z[at] = z;
-  }
+  for (int w = 0; w < WAVES; ++w) i = w == 0 ? wi[0] : min(i, wi[w]), z = w == 0 ? wz[0] : z + wz[w];
+  return Part{z, m, i};
 }
 
 // The chunk that `target` falls into by the sums mass(0), mass(1), ..: the first c with mass(0) + .. + mass(c) > target, and
@@ -306,12 +316,12 @@ __device__ __forceinline__ int find_element(int first, double target, const doub
 }
 
 // The first element that holds the row's maximum (where rejections left nothing: once in a blue moon).
-template <typename T> __device__ __forceinline__ int argmax_of(Row<T> row, float top) {
+template <int THREADS, typename T> __device__ __forceinline__ int argmax_of(Row<T> row, float top) {
   __shared__ int first;
   if (threadIdx.x == 0) first = INT_MAX;
   __syncthreads();
   int i = threadIdx.x;
-  while (i < row.V && row.one(i) != top) i += kWalkThreads;
+  while (i < row.V && row.one(i) != top) i += THREADS;
   if (i < row.V) atomicMin(&first, i);
   __syncthreads();
   return first < INT_MAX ? first : 0;
@@ -329,64 +339,92 @@ template <typename T, typename Q> struct Rest {
         s(s) {}
   __device__ __forceinline__ double of(float x, double q) const { return fmax(weight(x, most, s) - taken * q, 0.0); }
   __device__ __forceinline__ double one(int v) const { return of(row.one(v), (double)to_f32<Q>(q[v])); }
-  // the 8 elements from i0 on, a piece's first; 0 where there are none
-  __device__ __forceinline__ void eight(int i0, double (&r)[8]) const {
-    constexpr int E = Row<T>::E;
-    float x[8], y[8];
+  // the 8 N elements from i0 on, a piece's first; 0 where there are none
+  template <int N> __device__ __forceinline__ void eights(int i0, double (&r)[8 * N]) const {
+    constexpr int E = Row<T>::E, F = 16 / (int)sizeof(Q);
+    float x[8 * N], y[8 * N];
 #pragma unroll
-    for (int u = 0; u < 8 / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
-    if (i0 >= 0 && i0 + 8 <= row.V && (uintptr_t)(q + i0) % 16 == 0) {
+    for (int u = 0; u < 8 * N / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
+    if (i0 >= 0 && i0 + 8 * N <= row.V && (uintptr_t)(q + i0) % 16 == 0) {
 #pragma unroll
-      for (int u = 0; u < 8 * (int)sizeof(Q) / 16; ++u) unpack16<Q>(load16(q + i0 + u * (16 / (int)sizeof(Q))), y + u * (16 / (int)sizeof(Q)));
+      for (int u = 0; u < 8 * N / F; ++u) unpack16<Q>(load16(q + i0 + u * F), y + u * F);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = i0 + e >= 0 && i0 + e < row.V ? to_f32<Q>(q[i0 + e]) : 0.0f;
+      for (int e = 0; e < 8 * N; ++e) y[e] = i0 + e >= 0 && i0 + e < row.V ? to_f32<Q>(q[i0 + e]) : 0.0f;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = of(x[e], (double)y[e]);
+    for (int e = 0; e < 8 * N; ++e) r[e] = of(x[e], (double)y[e]);
   }
 };
 
-constexpr int kVerifyNodes = FORGE_TREE_MAX_TOKENS;
-static_assert(kVerifyChunk / kWalkThreads == 8, "a thread of the walk's draw holds eight elements");
+// The walk's shared memory: a few numbers a node, a sum a chunk, and all chunks' numbers where they are few.
+struct WalkLds {
+  static constexpr int KEPT = 1024;   // chunks of all nodes
+  double *zs, *es, *masses, *sums;
+  Part* parts;
+  float *most, *us, *qs;
+  int *args, *tok, *par, *child, *sib;
+  bool* yes;
+  __host__ __device__ static bool keeps(int T, int C) { return T <= 512 && T * C <= KEPT; }   // (all of it below 64 KB)
+  __host__ __device__ static size_t bytes(int T, int C) {
+    return 8 * (2 * (size_t)T + C + 16) + (keeps(T, C) ? sizeof(Part) * T * C : 0) + 33 * (size_t)T;
+  }
+  __device__ __forceinline__ WalkLds(char* at, int T, int C) {
+    const auto take = [&](auto*& p, size_t n) {
+      p = reinterpret_cast<decltype(p + 0)>(at);
+      at += n * sizeof(*p);
+    };
+    take(parts, keeps(T, C) ? T * C : 0);
+    take(zs, T);
+    take(es, T);
+    take(masses, C);
+    take(sums, 16);
+    take(most, T);
+    take(us, T);
+    take(qs, T);
+    take(args, T);
+    take(tok, T);
+    take(par, T);
+    take(child, T);
+    take(sib, T);
+    take(yes, T);
+  }
+};
 
-// One block per row: from the chunks' numbers to its new tokens. Latency: the nodes' numbers, their tokens' logits and the one
-// chunk that the draw falls into are read one after the other.
-template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
-  __shared__ float most[kVerifyNodes], us[kVerifyNodes];
-  __shared__ double zs[kVerifyNodes], es[kVerifyNodes];
-  __shared__ int args[kVerifyNodes], tok[kVerifyNodes], par[kVerifyNodes], child[kVerifyNodes], sib[kVerifyNodes];
-  __shared__ bool yes[kVerifyNodes];
-  __shared__ double lds[kWalkThreads / kWave];
-  const int b = blockIdx.x, n = p.nodes(b), tid = threadIdx.x;
+// A row's walk, by one block: from the chunks' numbers to its new tokens. Latency: what is read hangs on what was read
+// before, the tokens, their logits, the chunks' numbers, the one chunk that the draw falls into.
+template <typename T, typename Q, int THREADS> __device__ __forceinline__ void walk_row(const VerifyParams& p, int b, char* smem) {
+  constexpr int PER = kVerifyChunk / THREADS, WAVES = THREADS / kWave;
+  const WalkLds l(smem, p.T, p.C);
+  const int n = p.nodes(b), tid = threadIdx.x, lane = tid % kWave;
   int64_t* out = p.out + (int64_t)b * p.T;
   int32_t* path = p.path + (int64_t)b * p.T;
   const double heat = p.heat(b);
   const bool warm = heat > 0.0;
   const Scale s = row_scale(p, b);
   const Q* probs = static_cast<const Q*>(p.probs);
-  const auto q_of = [&](int node, int v) { return (double)to_f32<Q>(probs[b * p.sqb + node * p.sqt + v]); };
 
-  // each drafted token, its parent and the logit it is judged by (the loads go out before the chunks' numbers are met)
-  constexpr int MINE = kVerifyNodes / kWalkThreads;
-  float logit[MINE];
-#pragma unroll
-  for (int y = 0; y < MINE; ++y) {
-    const int t = tid + y * kWalkThreads;
-    logit[y] = kNegInf;
-    if (t < p.T) {
-      out[t] = -1;
-      path[t] = t == 0 && n > 0 ? 0 : -1;
-    }
-    if (t >= n) continue;
-    const int64_t x = p.tokens[b * p.stb + t];
+  // Each drafted token, its parent, and the logit and probability it is judged by; the first two rounds' stay in registers
+  // while the chunks' numbers are on their way.
+  constexpr int MINE = 2;
+  float logit[MINE], prob[MINE];
+  const auto judged = [&](int t, float& x, float& q) {
+    const int64_t token = p.tokens[b * p.stb + t];
     const int up = t == 0 ? -1 : p.parents ? p.parents[b * p.spb + t] : t - 1;
-    const bool real = x >= 0 && x < p.V && up >= 0 && up < t;   // (others are passed over)
-    tok[t] = real ? (int)x : -1;
-    par[t] = real ? up : -1;
-    us[t] = warm ? p.uniform[b * p.sub + t] : 0.0f;
-    child[t] = p.T;
-    if (real && warm) logit[y] = logits_row<T>(p, b, up).one((int)x);
+    const bool real = token >= 0 && token < p.V && up >= 0 && up < t;   // (others are passed over)
+    l.tok[t] = real ? (int)token : -1;
+    l.par[t] = real ? up : -1;
+    l.us[t] = warm ? p.uniform[b * p.sub + t] : 0.0f;
+    l.child[t] = p.T;
+    x = real && warm ? logits_row<T>(p, b, up).one((int)token) : kNegInf;
+    q = real && warm && probs ? to_f32<Q>(probs[b * p.sqb + up * p.sqt + token]) : 0.0f;
+  };
+#pragma unroll
+  for (int y = 0; y < MINE; ++y)
+    if (tid + y * THREADS < n) judged(tid + y * THREADS, logit[y], prob[y]);
+  for (int t = tid; t < p.T; t += THREADS) {
+    out[t] = -1;
+    path[t] = t == 0 && n > 0 ? 0 : -1;
   }
   if (probs && tid == 0) {
     p.state[b].left = 0;
@@ -397,71 +435,89 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
     return;
   }
 
-  // each node's maximum, argmax and sum: 16 lanes a node
-  for (int t = tid / 16; t < n; t += kWalkThreads / 16) {
-    const int64_t at = ((int64_t)b * p.T + t) * p.C;
-    const int l = tid % 16;
+  // each node's maximum, argmax and sum: 16 lanes a node, or a wave where that is enough
+  const bool keep = WalkLds::keeps(p.T, p.C);
+  const Part* parts = p.parts + (int64_t)b * p.T * p.C;
+  const int wide = n <= WAVES ? 64 : 16, mine = tid & (wide - 1);
+  for (int t = tid / wide; t < n; t += THREADS / wide) {
     float m = kNegInf;
     int i = p.V;
     double z = 0.0;
-    for (int c = l; c < p.C; c += 16) {   // (the running sum against the running maximum)
-      const float mc = p.part_m[at + c];
-      const int ic = p.part_i[at + c];
-      const double zc = p.part_z[at + c];
-      if (mc > m) {
-        z = warm ? zc + (m > kNegInf ? z * weight(m, mc, s) : 0.0) : 0.0;
-        m = mc;
-        i = ic;
-      } else if (mc == m) {   // (in rising order: the first stays)
-        z += zc;
-        i = min(i, ic);
-      } else if (warm && mc > kNegInf) {
-        z += zc * weight(mc, m, s);
+    for (int c0 = 0; c0 < p.C; c0 += 2 * wide) {
+      Part x[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int c = c0 + y * wide + mine;
+        x[y] = c < p.C ? load_part(parts + t * p.C + c) : Part{0.0, kNegInf, p.V};
+        if (keep && c < p.C) l.parts[t * p.C + c] = x[y];
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {   // (the running sum against the running maximum)
+        if (x[y].m > m) {
+          z = warm ? x[y].z + (m > kNegInf ? z * weight(m, x[y].m, s) : 0.0) : 0.0;
+          m = x[y].m;
+          i = x[y].i;
+        } else if (x[y].m == m) {
+          z += x[y].z;
+          i = min(i, x[y].i);
+        } else if (warm && x[y].m > kNegInf) {
+          z += x[y].z * weight(x[y].m, m, s);
+        }
       }
     }
-    const float top = group_max<16>(m);
+    float top = group_max<16>(m);
+    if (wide == 64) top = fmaxf(top, __shfl_xor(top, 16, kWave)), top = fmaxf(top, __shfl_xor(top, 32, kWave));
     if (m < top) i = p.V;
     if (warm) z = m > kNegInf ? z * weight(m, top, s) : 0.0;
-    for (int d = 8; d; d >>= 1) {
+    for (int d = wide / 2; d; d >>= 1) {
       i = min(i, __shfl_xor(i, d, kWave));
       z += __shfl_xor(z, d, kWave);
     }
-    if (l == 0) most[t] = top, args[t] = i, zs[t] = z;
+    if (mine == 0) l.most[t] = top, l.args[t] = top > kNegInf ? i : 0, l.zs[t] = z;   // (nothing: the first)
   }
   __syncthreads();
-#pragma unroll
-  for (int y = 0; y < MINE; ++y) {
-    const int t = tid + y * kWalkThreads;
-    if (t >= n) continue;
-    const int up = par[t];
-    es[t] = warm && up >= 0 && most[up] > kNegInf ? weight(logit[y], most[up], s) : 0.0;
-    if (!warm || probs || up < 0) continue;
+  const auto weigh = [&](int t, float x, float q) {
+    const int up = l.par[t];
+    l.es[t] = warm && up >= 0 && l.most[up] > kNegInf ? weight(x, l.most[up], s) : 0.0;
+    l.qs[t] = q;
+    if (!warm || probs || up < 0) return;
     bool twice = false;   // an earlier sibling has the token
 #pragma unroll 4
-    for (int j = up + 1; j < t; ++j) twice |= par[j] == up && tok[j] == tok[t];
-    yes[t] = !twice;
+    for (int j = up + 1; j < t; ++j) twice |= l.par[j] == up && l.tok[j] == l.tok[t];
+    l.yes[t] = !twice;
+  };
+#pragma unroll
+  for (int y = 0; y < MINE; ++y)
+    if (tid + y * THREADS < n) weigh(tid + y * THREADS, logit[y], prob[y]);
+  if (n > MINE * THREADS) {   // (a large tree's others)
+    for (int t = MINE * THREADS + tid; t < n; t += THREADS) judged(t, logit[0], prob[0]);
+    __syncthreads();
+    for (int t = MINE * THREADS + tid; t < n; t += THREADS) {
+      judged(t, logit[0], prob[0]);
+      weigh(t, logit[0], prob[0]);
+    }
   }
   __syncthreads();
 
   // Who would be accepted if the walk came to its parent. With the drafter's probabilities that is known for first
   // children only: child[] are a node's first children, sib[] their next siblings. Else child[] are the accepted ones.
-  for (int t = tid; t < n; t += kWalkThreads) {
-    const int up = par[t];
+  for (int t = tid; t < n; t += THREADS) {
+    const int up = l.par[t];
     if (up < 0) continue;
     if (!warm) {
-      if (tok[t] == args[up]) atomicMin(&child[up], t);
+      if (l.tok[t] == l.args[up]) atomicMin(&l.child[up], t);
     } else if (probs) {
-      yes[t] = us[t] * q_of(up, tok[t]) * zs[up] < es[t];
-      atomicMin(&child[up], t);
+      l.yes[t] = l.us[t] * (double)l.qs[t] * l.zs[up] < l.es[t];
+      atomicMin(&l.child[up], t);
       int next = p.T;
 #pragma unroll 4
-      for (int j = n - 1; j > t; --j) next = par[j] == up ? j : next;
-      sib[t] = next;
-    } else if (yes[t]) {
-      double left = zs[up];
+      for (int j = n - 1; j > t; --j) next = l.par[j] == up ? j : next;
+      l.sib[t] = next;
+    } else if (l.yes[t]) {
+      double left = l.zs[up];
 #pragma unroll 4
-      for (int j = up + 1; j < t; ++j) left -= par[j] == up && yes[j] ? es[j] : 0.0;
-      if (us[t] * fmax(left, 0.0) < es[t]) atomicMin(&child[up], t);
+      for (int j = up + 1; j < t; ++j) left -= l.par[j] == up && l.yes[j] ? l.es[j] : 0.0;
+      if (l.us[t] * fmax(left, 0.0) < l.es[t]) atomicMin(&l.child[up], t);
     }
   }
   __syncthreads();
@@ -470,69 +526,67 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
   int at = 0, count = 1;
   double taken = 0.0;
   while (true) {
-    int t = child[at];
+    int t = l.child[at];
     if (t >= p.T) break;
-    if (warm && probs && !yes[t]) {
-      taken = zs[at];
-      for (t = sib[t]; t < p.T; t = sib[t]) {
-        const Rest<T, Q> rest(p, b, at, taken, most[at], s);
+    if (warm && probs && !l.yes[t]) {
+      taken = l.zs[at];
+      for (t = l.sib[t]; t < p.T; t = l.sib[t]) {
+        const Rest<T, Q> rest(p, b, at, taken, l.most[at], s);
         double w = 0.0;
 #pragma unroll 2
-        for (int i = tid * 8 - rest.row.shift; i < p.V; i += kWalkThreads * 8) {
+        for (int i = tid * 8 - rest.row.shift; i < p.V; i += THREADS * 8) {
           double x[8];
-          rest.eight(i, x);
+          rest.template eights<1>(i, x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) w += x[e];
         }
-        w = block_sum<kWalkThreads>(w, lds);
-        const double q = q_of(at, tok[t]);
-        if (us[t] * q * w < es[t] - taken * q) break;
+        w = block_sum<THREADS>(w, l.sums);
+        const double q = l.qs[t];
+        if (l.us[t] * q * w < l.es[t] - taken * q) break;
         taken += w;
       }
       if (t >= p.T) break;
       taken = 0.0;
     }
     if (tid == 0) {
-      out[count - 1] = tok[t];
+      out[count - 1] = l.tok[t];
       path[count] = t;
     }
     at = t;
     ++count;
   }
 
-  int token = warm ? 0 : args[at];
-  if (warm && most[at] > kNegInf && taken > 0.0) {   // what the drafter's probabilities left is drawn from below
-    if (tid == 0) p.state[b] = State{taken, most[at], at, count - 1, 1, 0};
+  int token = warm ? 0 : l.args[at];
+  if (warm && l.most[at] > kNegInf && taken > 0.0) {   // what the drafter's probabilities left is drawn from below
+    if (tid == 0) p.state[b] = State{taken, l.most[at], at, count - 1, 1, 0};
     token = -1;
-  } else if (warm && most[at] > kNegInf) {
+  } else if (warm && l.most[at] > kNegInf) {
     const Row<T> row = logits_row<T>(p, b, at);
-    const int64_t base = ((int64_t)b * p.T + at) * p.C;
-    const float top = most[at];
-    double* masses = zs;   // (the nodes' are done with: [chunk])
-    double* whole = es;    // a chunk's, before tokens were taken out
-    int* gone = child;     // the rejected children's tokens, and the chunks they are in
-    int* again = sib;
+    const float top = l.most[at];
+    double* masses = l.masses;
+    int* gone = l.child;     // the rejected children's tokens, and the chunks they are in
+    int* again = l.sib;
     __shared__ int ngone, nagain;
     __syncthreads();
     if (tid == 0) ngone = nagain = 0;
-    for (int c = tid; c < p.C; c += kWalkThreads) {
-      const float mc = p.part_m[base + c];
-      masses[c] = mc > kNegInf ? p.part_z[base + c] * weight(mc, top, s) : 0.0;
+    for (int c = tid; c < p.C; c += THREADS) {
+      const Part x = keep ? l.parts[at * p.C + c] : load_part(parts + at * p.C + c);
+      masses[c] = x.m > kNegInf ? x.z * weight(x.m, top, s) : 0.0;
     }
     __syncthreads();
     if (!probs) {
-      for (int j = at + 1 + tid; j < n; j += kWalkThreads)
-        if (par[j] == at && yes[j]) gone[atomicAdd(&ngone, 1)] = tok[j];
+      for (int j = at + 1 + tid; j < n; j += THREADS)
+        if (l.par[j] == at && l.yes[j]) gone[atomicAdd(&ngone, 1)] = j;
       __syncthreads();
       // a chunk that loses all but a thousandth of its sum is summed again: the difference could leave what is not there
-      for (int g = tid; g < ngone; g += kWalkThreads) {
-        const int c = (gone[g] + row.shift) / kVerifyChunk;
+      for (int g = tid; g < ngone; g += THREADS) {
+        const int c = (l.tok[gone[g]] + row.shift) / kVerifyChunk;
         double out_of = 0.0;
         bool first = true;
         for (int h = 0; h < ngone; ++h) {
-          if ((gone[h] + row.shift) / kVerifyChunk != c) continue;
+          if ((l.tok[gone[h]] + row.shift) / kVerifyChunk != c) continue;
           first &= h >= g;
-          out_of += weight(row.one(gone[h]), top, s);
+          out_of += l.es[gone[h]];
         }
         if (!first) continue;
         const double left = masses[c] - out_of;
@@ -541,38 +595,39 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
       }
     }
     __syncthreads();
-    const auto eight = [&](int i0, double (&r)[8]) {   // the weights of the 8 elements from i0 on, without rejected ones
+    const auto piece = [&](int c, double (&r)[PER]) {   // the thread's weights of chunk c, without rejected tokens
       constexpr int E = Row<T>::E;
-      float x[8];
+      const int i0 = c * kVerifyChunk - row.shift + tid * PER;
+      float x[PER];
 #pragma unroll
-      for (int u = 0; u < 8 / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
+      for (int u = 0; u < PER / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
       unsigned cut = 0;
-      for (int g = 0; g < ngone; ++g)
-        if ((unsigned)(gone[g] - i0) < 8) cut |= 1u << (gone[g] - i0);
+      for (int g = 0; g < ngone; ++g) {
+        const int d = l.tok[gone[g]] - i0;
+        if ((unsigned)d < PER) cut |= 1u << d;
+      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = cut >> e & 1 ? 0.0 : weight(x[e], top, s);
+      for (int e = 0; e < PER; ++e) r[e] = cut >> e & 1 ? 0.0 : weight(x[e], top, s);
     };
-    double x[8];
+    double x[PER];
     for (int g = 0; g < nagain; ++g) {
-      const int c = again[g];
-      eight(c * kVerifyChunk - row.shift + tid * 8, x);
+      piece(again[g], x);
       double w = 0.0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w += x[e];
-      w = block_sum<kWalkThreads>(w, lds);
-      if (tid == 0) masses[c] = w;
+      for (int e = 0; e < PER; ++e) w += x[e];
+      w = block_sum<THREADS>(w, l.sums);
+      if (tid == 0) masses[again[g]] = w;
     }
-    __syncthreads();
-    double total = 0.0;
-    for (int c = tid; c < p.C; c += kWalkThreads) total += masses[c];
-    total = block_sum<kWalkThreads>(total, lds);
+    if (nagain) __syncthreads();
+    double total = 0.0;   // (each wave for itself)
+    for (int c = lane; c < p.C; c += kWave) total += masses[c];
+    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, kWave);
     if (total > 0.0) {
-      const Found f = find_chunk(p.C, us[0] * total, [&](int c) { return masses[c]; });
-      const int first = f.c * kVerifyChunk - row.shift;
-      eight(first + tid * 8, x);
-      token = find_element<kWalkThreads>(first, f.target, x);
+      const Found f = find_chunk(p.C, l.us[0] * total, [&](int c) { return masses[c]; });
+      piece(f.c, x);
+      token = find_element<THREADS>(f.c * kVerifyChunk - row.shift, f.target, x);
     } else {
-      token = argmax_of(row, top);
+      token = argmax_of<THREADS>(row, top);
     }
   }
   if (tid == 0) {
@@ -581,29 +636,56 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
   }
 }
 
-// Sums over blocks on several XCDs, whose caches are their own: written past them, counted, and read by the block that
-// counts last.
-__device__ __forceinline__ void store_agent(double* p, double x) {
-  __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// The scan, a block a chunk. FUSED: the block that ends a row's scan walks it too, where blocks are few and a second launch
+// would cost more than the walk's registers take from the scan's occupancy.
+template <typename T, typename Q, bool FUSED>
+__global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int c = blockIdx.x, t = blockIdx.y, b = blockIdx.z, n = p.nodes(b);
+  if (t < n) {
+    const Part x = scan_chunk<T>(p, b, t, c);
+    Part* to = p.parts + ((int64_t)b * p.T + t) * p.C + c;
+    if constexpr (!FUSED) {
+      if (threadIdx.x == 0) *to = x;
+      return;
+    } else {
+      __shared__ bool last;
+      if (threadIdx.x == 0) {
+        store_part(to, x);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const unsigned all = (unsigned)(n * p.C);   // (the counter wraps to zero for the next call)
+        last = atomicInc(p.counters + b, all - 1) == all - 1;
+      }
+      __syncthreads();
+      if (!last) return;
+    }
+  } else if (!FUSED || n > 0 || t > 0 || c > 0) {
+    return;
+  }
+  if constexpr (FUSED) walk_row<T, Q, kScanThreads>(p, b, smem);
 }
-__device__ __forceinline__ double load_agent(const double* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  walk_row<T, Q, kWalkThreads>(p, blockIdx.x, smem);
 }
 
 // What the drafter's probabilities left of a row, chunk by chunk; a row's last block draws from it.
-template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_rest_kernel(VerifyParams p) {
-  __shared__ double lds[kWalkThreads / kWave];
+template <typename T, typename Q> __global__ __launch_bounds__(kScanThreads) void verify_rest_kernel(VerifyParams p) {
+  constexpr int PER = kVerifyChunk / kScanThreads;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  double* all = reinterpret_cast<double*>(smem);   // [C]
+  __shared__ double lds[kScanThreads / kWave];
   __shared__ bool last;
   const int c = blockIdx.x, b = blockIdx.y;
   const State st = p.state[b];
   if (!st.left) return;
   const Rest<T, Q> rest(p, b, st.node, st.taken, st.most, row_scale(p, b));
   double* sums = p.rest + (int64_t)b * p.C;
-  double x[8], w = 0.0;
-  rest.eight(c * kVerifyChunk - rest.row.shift + (int)threadIdx.x * 8, x);
+  double x[PER], w = 0.0;
+  rest.template eights<PER / 8>(c * kVerifyChunk - rest.row.shift + (int)threadIdx.x * PER, x);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w += x[e];
-  w = block_sum<kWalkThreads>(w, lds);
+  for (int e = 0; e < PER; ++e) w += x[e];
+  w = block_sum<kScanThreads>(w, lds);
   if (threadIdx.x == 0) {
     store_agent(sums + c, w);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -611,45 +693,51 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
   }
   __syncthreads();
   if (!last) return;
-  double total = 0.0;
-  for (int i = threadIdx.x; i < p.C; i += kWalkThreads) total += load_agent(sums + i);
-  total = block_sum<kWalkThreads>(total, lds);
+  const float u = p.uniform[b * p.sub];
+  for (int i = threadIdx.x; i < p.C; i += kScanThreads) all[i] = load_agent(sums + i);
+  __syncthreads();
+  double total = 0.0;   // (each wave for itself)
+  for (int i = threadIdx.x % kWave; i < p.C; i += kWave) total += all[i];
+  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, kWave);
   int token;
   if (total > 0.0) {
-    const Found f = find_chunk(p.C, (double)p.uniform[b * p.sub] * total, [&](int i) { return load_agent(sums + i); });
+    const Found f = find_chunk(p.C, u * total, [&](int i) { return all[i]; });
     const int first = f.c * kVerifyChunk - rest.row.shift;
-    rest.eight(first + (int)threadIdx.x * 8, x);
-    token = find_element<kWalkThreads>(first, f.target, x);
+    rest.template eights<PER / 8>(first + (int)threadIdx.x * PER, x);
+    token = find_element<kScanThreads>(first, f.target, x);
   } else {
-    token = argmax_of(rest.row, st.most);
+    token = argmax_of<kScanThreads>(rest.row, st.most);
   }
   if (threadIdx.x == 0) p.out[(int64_t)b * p.T + st.at] = token;
 }
 
 struct VerifyWs {
-  size_t z, m, i, state, rest, bytes;
+  size_t parts, state, rest, bytes;
 };
 static int verify_chunks(int V) { return (V + 7 + kVerifyChunk - 1) / kVerifyChunk; }   // (a row may start inside a piece)
 static VerifyWs verify_ws(int B, int T, int V, bool probs) {
   const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  const size_t n = (size_t)B * T * verify_chunks(V);
+  const size_t C = verify_chunks(V);
   VerifyWs w{};
-  w.m = up(n * sizeof(double));
-  w.i = w.m + up(n * sizeof(float));
-  w.state = w.i + up(n * sizeof(int32_t));
+  w.parts = FORGE_PAGED_COUNTER_BYTES;
+  w.state = w.parts + up((size_t)B * T * C * sizeof(Part));
   w.rest = w.state + (probs ? up((size_t)B * sizeof(State)) : 0);
-  w.bytes = w.rest + (probs ? up((size_t)B * verify_chunks(V) * sizeof(double)) : 0);
+  w.bytes = w.rest + (probs ? up((size_t)B * C * sizeof(double)) : 0);
   return w;
 }
 
 template <typename T, typename Q> static int launch_verify(const VerifyParams& p, hipStream_t s) {
-  hipLaunchKernelGGL((verify_scan_kernel<T>), dim3(p.C, p.T, p.B), dim3(kScanThreads), 0, s, p);
-  int st = check_launch();
-  if (st) return st;
-  hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kWalkThreads), 0, s, p);
-  st = check_launch();
-  if (st || !p.probs) return st;
-  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kWalkThreads), 0, s, p);
+  const size_t lds = WalkLds::bytes(p.T, p.C);
+  const dim3 scan(p.C, p.T, p.B);
+  if (p.counters) {
+    hipLaunchKernelGGL((verify_scan_kernel<T, Q, true>), scan, dim3(kScanThreads), lds, s, p);
+  } else {
+    hipLaunchKernelGGL((verify_scan_kernel<T, float, false>), scan, dim3(kScanThreads), 0, s, p);
+    if (const int st = check_launch()) return st;
+    hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kWalkThreads), lds, s, p);
+  }
+  if (const int st = check_launch(); st || !p.probs) return st;
+  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kScanThreads), p.C * sizeof(double), s, p);
   return check_launch();
 }
 
@@ -671,7 +759,7 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
                                    int64_t s_parents_b, const float* uniform, int64_t s_uniform_b, const float* temperatures,
                                    double temperature, int probs_dtype, const void* draft_probs, int64_t s_probs_b,
                                    int64_t s_probs_t, const int32_t* new_lens, int64_t* out, int32_t* path, int32_t* count,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+                                   void* workspace, size_t workspace_bytes, int ws_flags, void* stream) {
   clear_error();
   if (dtype != FORGE_F32 && dtype != FORGE_BF16 && dtype != FORGE_F16) return set_error("unknown dtype code");
   if (B < 0 || T <= 0 || V <= 0) return set_error("bad sizes");
@@ -703,9 +791,8 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
   p.new_lens = new_lens;
   p.B = B; p.T = T; p.V = V; p.C = verify_chunks(V);
   p.out = out; p.path = path; p.count = count;
-  p.part_z = reinterpret_cast<double*>(at);
-  p.part_m = reinterpret_cast<float*>(at + ws.m);
-  p.part_i = reinterpret_cast<int32_t*>(at + ws.i);
+  p.parts = reinterpret_cast<Part*>(at + ws.parts);
+  if ((ws_flags & FORGE_WS_ZEROED) && (int64_t)p.C * T * B <= 2 * device_cus()) p.counters = reinterpret_cast<unsigned*>(at);
   p.state = reinterpret_cast<State*>(at + ws.state);
   p.rest = reinterpret_cast<double*>(at + ws.rest);
   const hipStream_t s = (hipStream_t)stream;

@@ -244,7 +244,7 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *
 
 
 _STREAM_WS: dict = {}
-_PAGED_WS: dict = {}      # the same for attn_paged and attn_sinks, whose workspaces begin with other counters
+_PAGED_WS: dict = {}      # the same for attn_paged, attn_sinks, attn_tree and verify_drafts: they begin with other counters
 _STREAM_WS_MAX = 16   # streams whose workspace is kept (the oldest is dropped beyond that)
 
 
@@ -946,7 +946,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, *, parents: torch.
     Returns (tokens int64 [B, T], path int32 [B, T], count int32 [B]): the row's count[b] new tokens (the accepted ones,
     then the next one), the count[b] nodes that stand (node 0 first: what kv_compact takes), -1 behind both; a row without
     nodes (new_lens[b] == 0) has none. Sums are held in 64 bits. No gradient."""
-    r = host().verify_drafts(logits, tokens, parents, uniform, temperature, draft_probs, new_lens)
+    r = host().verify_drafts(_PAGED_WS, logits, tokens, parents, uniform, temperature, draft_probs, new_lens)
     if r is not None:
         return r if r.__class__ is not int else check(r, "forge_verify_drafts")
     dev = _need_device(logits, tokens, parents, uniform, draft_probs, new_lens)
@@ -993,12 +993,17 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, *, parents: torch.
         return out, path, count
     with _guard(dev):
         need = lib().forge_verify_drafts_workspace_bytes(B, T, V, int(draft_probs is not None))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        if not need:
+            raise ValueError(f"verify_drafts takes up to 65,535 rows and 2^22 - 8 tokens, not {tuple(logits.shape)}")
+        ws = _PagedPartials(dev, need)
+        if ws.ws is None:
+            raise torch.cuda.OutOfMemoryError(f"verify_drafts: no memory for {need} bytes")
         st = lib().forge_verify_drafts(dt, B, T, V, _ptr(logits), logits.stride(0), logits.stride(1), _ptr(tokens), s_tokens,
                                        _ptr(parents), s_parents, _ptr(uniform), s_uniform, _ptr(temps), heat, pdt,
-                                       _ptr(draft_probs), sq_b, sq_t, _ptr(nl), _ptr(out), _ptr(path), _ptr(count), _ptr(ws),
-                                       need, _stream(dev))
+                                       _ptr(draft_probs), sq_b, sq_t, _ptr(nl), _ptr(out), _ptr(path), _ptr(count),
+                                       *ws.args(), _stream(dev))
     check(st, "forge_verify_drafts")
+    ws.launched()
     return out, path, count
 
 

@@ -84,7 +84,7 @@ def test_attn_tree_of_nothing():
 def _verify_call(**kw):
     a = dict(dtype=_lib.BF16, B=2, T=4, V=100, logits=FAKE, slb=400, slt=100, tokens=FAKE, stb=4, parents=None, spb=0, uniform=FAKE,
              sub=4, temps=None, heat=1.0, pdt=0, probs=None, sqb=0, sqt=0, news=None, out=FAKE, path=FAKE, count=FAKE, ws=FAKE,
-             wsb=1 << 20, stream=None)
+             wsb=1 << 20, wsf=0, stream=None)
     assert not set(kw) - set(a)
     a.update(kw)
     return _lib.lib().forge_verify_drafts(*a.values())
