@@ -110,8 +110,7 @@ __device__ __forceinline__ double exp2_part(double f) {
 // exp((x - m) / temperature) to about 1e-15, exactly 1 at x = m, 0 for -inf and for a NaN (which no maximum takes): 2^t with t = k + f, k from the low bits of
 // t + 1.5 2^52.
 __device__ __forceinline__ double weight(float x, float m, Scale c) {
-  if (m == -kNegInf) return x == m ? 1.0 : 0.0;   // infinite logits share the mass
-  const double d = (double)x - (double)m;
+  const double d = x == m ? 0.0 : (double)x - (double)m;   // (infinite logits share the mass)
   const double t = d * c.hi, lo = fma(d, c.lo, fma(d, c.hi, -t));
   const double big = t + 0x1.8p52, f = (t - (big - 0x1.8p52)) + lo;
   return t > -1100.0 ? ldexp(exp2_part(f), __double2loint(big)) : 0.0;   // (NaN: 0)
@@ -141,7 +140,8 @@ __device__ __forceinline__ void store_part(Part* p, Part x) {
   store_agent(&p->z, x.z);
   store_agent(reinterpret_cast<double*>(&p->m), __hiloint2double(x.i, __float_as_int(x.m)));
 }
-__device__ __forceinline__ Part load_part(const Part* p) {
+template <bool FUSED> __device__ __forceinline__ Part load_part(const Part* p) {   // (of another launch: as any memory)
+  if constexpr (!FUSED) return *p;
   const double z = load_agent(&p->z), mi = load_agent(reinterpret_cast<const double*>(&p->m));
   return Part{z, __int_as_float(__double2loint(mi)), __double2hiint(mi)};
 }
@@ -360,40 +360,42 @@ template <typename T, typename Q> struct Rest {
 // The walk's shared memory: a few numbers a node, a sum a chunk, and all chunks' numbers where they are few.
 struct WalkLds {
   static constexpr int KEPT = 1024;   // chunks of all nodes
-  double *zs, *es, *masses, *sums;
+  double *zs, *es, *masses, *sums;   // (es, par and tok are read four nodes at a time)
   Part* parts;
   float *most, *us, *qs;
   int *args, *tok, *par, *child, *sib;
   bool* yes;
   __host__ __device__ static bool keeps(int T, int C) { return T <= 512 && T * C <= KEPT; }   // (all of it below 64 KB)
   __host__ __device__ static size_t bytes(int T, int C) {
-    return 8 * (2 * (size_t)T + C + 16) + (keeps(T, C) ? sizeof(Part) * T * C : 0) + 33 * (size_t)T;
+    const size_t nodes = (T + 3) / 4 * 4;
+    return 8 * (2 * nodes + C + C % 2 + 16) + (keeps(T, C) ? sizeof(Part) * T * C : 0) + 33 * nodes;
   }
   __device__ __forceinline__ WalkLds(char* at, int T, int C) {
     const auto take = [&](auto*& p, size_t n) {
       p = reinterpret_cast<decltype(p + 0)>(at);
       at += n * sizeof(*p);
     };
+    const int nodes = (T + 3) / 4 * 4;
     take(parts, keeps(T, C) ? T * C : 0);
-    take(zs, T);
-    take(es, T);
-    take(masses, C);
+    take(zs, nodes);
+    take(es, nodes);
+    take(masses, C + C % 2);
     take(sums, 16);
-    take(most, T);
-    take(us, T);
-    take(qs, T);
-    take(args, T);
-    take(tok, T);
-    take(par, T);
-    take(child, T);
-    take(sib, T);
-    take(yes, T);
+    take(most, nodes);
+    take(us, nodes);
+    take(qs, nodes);
+    take(args, nodes);
+    take(tok, nodes);
+    take(par, nodes);
+    take(child, nodes);
+    take(sib, nodes);
+    take(yes, nodes);
   }
 };
 
 // A row's walk, by one block: from the chunks' numbers to its new tokens. Latency: what is read hangs on what was read
 // before, the tokens, their logits, the chunks' numbers, the one chunk that the draw falls into.
-template <typename T, typename Q, int THREADS> __device__ __forceinline__ void walk_row(const VerifyParams& p, int b, char* smem) {
+template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinline__ void walk_row(const VerifyParams& p, int b, char* smem) {
   constexpr int PER = kVerifyChunk / THREADS, WAVES = THREADS / kWave;
   const WalkLds l(smem, p.T, p.C);
   const int n = p.nodes(b), tid = threadIdx.x, lane = tid % kWave;
@@ -404,24 +406,47 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
   const Scale s = row_scale(p, b);
   const Q* probs = static_cast<const Q*>(p.probs);
 
-  // Each drafted token, its parent, and the logit and probability it is judged by; the first two rounds' stay in registers
-  // while the chunks' numbers are on their way.
+  // Each drafted token, its parent, and the logit and probability it is judged by; the first chunks' numbers are on their
+  // way meanwhile.
   constexpr int MINE = 2;
-  float logit[MINE], prob[MINE];
-  const auto judged = [&](int t, float& x, float& q) {
-    const int64_t token = p.tokens[b * p.stb + t];
-    const int up = t == 0 ? -1 : p.parents ? p.parents[b * p.spb + t] : t - 1;
-    const bool real = token >= 0 && token < p.V && up >= 0 && up < t;   // (others are passed over)
-    l.tok[t] = real ? (int)token : -1;
-    l.par[t] = real ? up : -1;
-    l.us[t] = warm ? p.uniform[b * p.sub + t] : 0.0f;
-    l.child[t] = p.T;
-    x = real && warm ? logits_row<T>(p, b, up).one((int)token) : kNegInf;
-    q = real && warm && probs ? to_f32<Q>(probs[b * p.sqb + up * p.sqt + token]) : 0.0f;
+  struct Drafted {
+    int64_t token;
+    int up;
+    float u;
   };
+  const auto drafted = [&](int t) {
+    return Drafted{p.tokens[b * p.stb + t], t == 0 ? -1 : p.parents ? p.parents[b * p.spb + t] : t - 1,
+                   warm ? p.uniform[b * p.sub + t] : 0.0f};
+  };
+  const auto judged = [&](int t, Drafted d, float& x, float& q) {
+    const bool real = d.token >= 0 && d.token < p.V && d.up >= 0 && d.up < t;   // (others are passed over)
+    l.tok[t] = real ? (int)d.token : -1;
+    l.par[t] = real ? d.up : -1;
+    l.us[t] = d.u;
+    l.child[t] = p.T;
+    x = real && warm ? logits_row<T>(p, b, d.up).one((int)d.token) : kNegInf;
+    q = real && warm && probs ? to_f32<Q>(probs[b * p.sqb + d.up * p.sqt + d.token]) : 0.0f;
+  };
+  float logit[MINE], prob[MINE];
+  Drafted d[MINE];
 #pragma unroll
   for (int y = 0; y < MINE; ++y)
-    if (tid + y * THREADS < n) judged(tid + y * THREADS, logit[y], prob[y]);
+    if (tid + y * THREADS < n) d[y] = drafted(tid + y * THREADS);
+  const bool keep = WalkLds::keeps(p.T, p.C);
+  const Part* parts = p.parts + (int64_t)b * p.T * p.C;
+  const int wide = n <= THREADS / kWave ? 64 : 16, mine = tid & (wide - 1);   // lanes a node: a wave where those are enough
+  const auto two = [&](int t, int c0, Part (&x)[2]) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const int c = c0 + y * wide + mine;
+      x[y] = t < n && c < p.C ? load_part<FUSED>(parts + t * p.C + c) : Part{0.0, kNegInf, p.V};
+    }
+  };
+  Part early[2];
+  two(tid / wide, 0, early);
+#pragma unroll
+  for (int y = 0; y < MINE; ++y)
+    if (tid + y * THREADS < n) judged(tid + y * THREADS, d[y], logit[y], prob[y]);
   for (int t = tid; t < p.T; t += THREADS) {
     out[t] = -1;
     path[t] = t == 0 && n > 0 ? 0 : -1;
@@ -435,21 +460,18 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
     return;
   }
 
-  // each node's maximum, argmax and sum: 16 lanes a node, or a wave where that is enough
-  const bool keep = WalkLds::keeps(p.T, p.C);
-  const Part* parts = p.parts + (int64_t)b * p.T * p.C;
-  const int wide = n <= WAVES ? 64 : 16, mine = tid & (wide - 1);
+  // each node's maximum, argmax and sum
   for (int t = tid / wide; t < n; t += THREADS / wide) {
     float m = kNegInf;
     int i = p.V;
     double z = 0.0;
     for (int c0 = 0; c0 < p.C; c0 += 2 * wide) {
-      Part x[2];
+      Part x[2] = {early[0], early[1]};
+      if (t >= THREADS / wide || c0 > 0) two(t, c0, x);
+      if (keep) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int c = c0 + y * wide + mine;
-        x[y] = c < p.C ? load_part(parts + t * p.C + c) : Part{0.0, kNegInf, p.V};
-        if (keep && c < p.C) l.parts[t * p.C + c] = x[y];
+        for (int y = 0; y < 2; ++y)
+          if (c0 + y * wide + mine < p.C) l.parts[t * p.C + c0 + y * wide + mine] = x[y];
       }
 #pragma unroll
       for (int y = 0; y < 2; ++y) {   // (the running sum against the running maximum)
@@ -478,22 +500,31 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
   __syncthreads();
   const auto weigh = [&](int t, float x, float q) {
     const int up = l.par[t];
-    l.es[t] = warm && up >= 0 && l.most[up] > kNegInf ? weight(x, l.most[up], s) : 0.0;
+    double e = warm && up >= 0 && l.most[up] > kNegInf ? weight(x, l.most[up], s) : 0.0;
     l.qs[t] = q;
-    if (!warm || probs || up < 0) return;
-    bool twice = false;   // an earlier sibling has the token
-#pragma unroll 4
-    for (int j = up + 1; j < t; ++j) twice |= l.par[j] == up && l.tok[j] == l.tok[t];
-    l.yes[t] = !twice;
+    if (warm && !probs && up >= 0) {   // a token that an earlier sibling has is out already
+      const int mine = l.tok[t];
+      bool twice = false;
+#pragma unroll 2
+      for (int j = (up + 1) & ~3; j < t; j += 4) {
+        const int4 a = *reinterpret_cast<const int4*>(l.par + j), k = *reinterpret_cast<const int4*>(l.tok + j);
+        twice |= a.x == up && k.x == mine;
+        twice |= a.y == up && k.y == mine && j + 1 < t;
+        twice |= a.z == up && k.z == mine && j + 2 < t;
+        twice |= a.w == up && k.w == mine && j + 3 < t;
+      }
+      if (twice) e = 0.0;
+    }
+    l.es[t] = e;
   };
 #pragma unroll
   for (int y = 0; y < MINE; ++y)
     if (tid + y * THREADS < n) weigh(tid + y * THREADS, logit[y], prob[y]);
   if (n > MINE * THREADS) {   // (a large tree's others)
-    for (int t = MINE * THREADS + tid; t < n; t += THREADS) judged(t, logit[0], prob[0]);
+    for (int t = MINE * THREADS + tid; t < n; t += THREADS) judged(t, drafted(t), logit[0], prob[0]);
     __syncthreads();
     for (int t = MINE * THREADS + tid; t < n; t += THREADS) {
-      judged(t, logit[0], prob[0]);
+      judged(t, drafted(t), logit[0], prob[0]);
       weigh(t, logit[0], prob[0]);
     }
   }
@@ -510,13 +541,26 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
       l.yes[t] = l.us[t] * (double)l.qs[t] * l.zs[up] < l.es[t];
       atomicMin(&l.child[up], t);
       int next = p.T;
-#pragma unroll 4
-      for (int j = n - 1; j > t; --j) next = l.par[j] == up ? j : next;
+#pragma unroll 2
+      for (int j = (n - 1) & ~3; j + 3 > t; j -= 4) {
+        const int4 a = *reinterpret_cast<const int4*>(l.par + j);
+        next = a.w == up && j + 3 < n ? j + 3 : next;
+        next = a.z == up && j + 2 < n && j + 2 > t ? j + 2 : next;
+        next = a.y == up && j + 1 < n && j + 1 > t ? j + 1 : next;
+        next = a.x == up && j > t ? j : next;
+      }
       l.sib[t] = next;
-    } else if (l.yes[t]) {
+    } else {
       double left = l.zs[up];
-#pragma unroll 4
-      for (int j = up + 1; j < t; ++j) left -= l.par[j] == up && l.yes[j] ? l.es[j] : 0.0;
+#pragma unroll 2
+      for (int j = (up + 1) & ~3; j < t; j += 4) {
+        const int4 a = *reinterpret_cast<const int4*>(l.par + j);
+        const double2 e0 = *reinterpret_cast<const double2*>(l.es + j), e1 = *reinterpret_cast<const double2*>(l.es + j + 2);
+        left -= a.x == up ? e0.x : 0.0;
+        left -= a.y == up && j + 1 < t ? e0.y : 0.0;
+        left -= a.z == up && j + 2 < t ? e1.x : 0.0;
+        left -= a.w == up && j + 3 < t ? e1.y : 0.0;
+      }
       if (l.us[t] * fmax(left, 0.0) < l.es[t]) atomicMin(&l.child[up], t);
     }
   }
@@ -564,29 +608,36 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
     const Row<T> row = logits_row<T>(p, b, at);
     const float top = l.most[at];
     double* masses = l.masses;
-    int* gone = l.child;     // the rejected children's tokens, and the chunks they are in
+    int* gone = l.child;     // the rejected children's tokens and weights, and chunks that are summed again
+    double* weights = l.zs;
     int* again = l.sib;
     __shared__ int ngone, nagain;
     __syncthreads();
     if (tid == 0) ngone = nagain = 0;
     for (int c = tid; c < p.C; c += THREADS) {
-      const Part x = keep ? l.parts[at * p.C + c] : load_part(parts + at * p.C + c);
+      const Part x = keep ? l.parts[at * p.C + c] : load_part<FUSED>(parts + at * p.C + c);
       masses[c] = x.m > kNegInf ? x.z * weight(x.m, top, s) : 0.0;
     }
     __syncthreads();
     if (!probs) {
       for (int j = at + 1 + tid; j < n; j += THREADS)
-        if (l.par[j] == at && l.yes[j]) gone[atomicAdd(&ngone, 1)] = j;
+        if (l.par[j] == at && l.es[j] > 0.0) {
+          const int g = atomicAdd(&ngone, 1);
+          gone[g] = l.tok[j];
+          weights[g] = l.es[j];
+        }
       __syncthreads();
       // a chunk that loses all but a thousandth of its sum is summed again: the difference could leave what is not there
-      for (int g = tid; g < ngone; g += THREADS) {
-        const int c = (l.tok[gone[g]] + row.shift) / kVerifyChunk;
+      const int most_gone = ngone;
+      for (int g = tid; g < most_gone; g += THREADS) {
+        const int c = (gone[g] + row.shift) / kVerifyChunk;
         double out_of = 0.0;
         bool first = true;
-        for (int h = 0; h < ngone; ++h) {
-          if ((l.tok[gone[h]] + row.shift) / kVerifyChunk != c) continue;
-          first &= h >= g;
-          out_of += l.es[gone[h]];
+#pragma unroll 4
+        for (int h = 0; h < most_gone; ++h) {
+          const bool here = (gone[h] + row.shift) / kVerifyChunk == c;
+          first &= !here || h >= g;
+          out_of += here ? weights[h] : 0.0;
         }
         if (!first) continue;
         const double left = masses[c] - out_of;
@@ -602,9 +653,11 @@ template <typename T, typename Q, int THREADS> __device__ __forceinline__ void w
 #pragma unroll
       for (int u = 0; u < PER / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
       unsigned cut = 0;
-      for (int g = 0; g < ngone; ++g) {
-        const int d = l.tok[gone[g]] - i0;
-        if ((unsigned)d < PER) cut |= 1u << d;
+      const int most_gone = ngone;
+#pragma unroll 4
+      for (int g = 0; g < most_gone; ++g) {
+        const int d = gone[g] - i0;
+        cut |= (unsigned)d < PER ? 1u << (d & 31) : 0u;
       }
 #pragma unroll
       for (int e = 0; e < PER; ++e) r[e] = cut >> e & 1 ? 0.0 : weight(x[e], top, s);
@@ -662,11 +715,11 @@ __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams 
   } else if (!FUSED || n > 0 || t > 0 || c > 0) {
     return;
   }
-  if constexpr (FUSED) walk_row<T, Q, kScanThreads>(p, b, smem);
+  if constexpr (FUSED) walk_row<T, Q, kScanThreads, true>(p, b, smem);
 }
 template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  walk_row<T, Q, kWalkThreads>(p, blockIdx.x, smem);
+  walk_row<T, Q, kWalkThreads, false>(p, blockIdx.x, smem);
 }
 
 // What the drafter's probabilities left of a row, chunk by chunk; a row's last block draws from it.
