@@ -116,9 +116,42 @@ __device__ __forceinline__ double weight(float x, float m, Scale c) {
   return t > -1100.0 ? ldexp(exp2_part(f), __double2loint(big)) : 0.0;   // (NaN: 0)
 }
 
+// 64-bit numbers across lanes without a way through LDS (the walk is one chain of such steps).
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ double dpp64(double x) {   // 0 where a lane has no partner
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, ROWS, 0xF, true),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, ROWS, 0xF, true));
+}
+// Sum over aligned groups of 16 or 64 lanes: every lane receives it.
+template <int W> __device__ __forceinline__ double lanes_sum(double x) {
+  x += dpp64<kDppQuadXor1>(x);
+  x += dpp64<kDppQuadXor2>(x);
+  x += dpp64<kDppRowHalfMirror>(x);
+  x += dpp64<kDppRowMirror>(x);
+  if constexpr (W == 64) {
+    const auto halves = [](double y, auto swap) {   // both halves of each pair, added in one order
+      const auto lo = swap((unsigned)__double2loint(y)), hi = swap((unsigned)__double2hiint(y));
+      const unsigned l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+      return __hiloint2double((int)h0, (int)l0) + __hiloint2double((int)h1, (int)l1);
+    };
+    x = halves(x, [](unsigned u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    x = halves(x, [](unsigned u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
+  }
+  return x;
+}
+// Sum of the lanes up to one's own.
+__device__ __forceinline__ double lanes_upto(double x) {
+  x += dpp64<0x111>(x);         // row_shr 1, 2, 4, 8: within rows of 16
+  x += dpp64<0x112>(x);
+  x += dpp64<0x114>(x);
+  x += dpp64<0x118>(x);
+  x += dpp64<0x142, 0xA>(x);    // a row's last lane to the next row
+  x += dpp64<0x143, 0xC>(x);    // lane 31 to the upper half
+  return x;
+}
+
 // Sum over the block, in one fixed order; every thread receives it. `lds`: one double a wave.
 template <int THREADS> __device__ __forceinline__ double block_sum(double x, double* lds) {
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, kWave);
+  x = lanes_sum<64>(x);
   __syncthreads();   // (the last call's readers)
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = x;
   __syncthreads();
@@ -256,11 +289,7 @@ template <typename F> __device__ __forceinline__ Found find_chunk(int C, double 
     int last = 0;
     for (int c0 = 0; c0 < C && f.c < 0; c0 += kWave) {
       const double own = c0 + lane < C ? mass(c0 + lane) : 0.0;
-      double upto = own;
-      for (int d = 1; d < kWave; d <<= 1) {
-        const double y = __shfl_up(upto, d, kWave);
-        if (lane >= d) upto += y;
-      }
+      const double upto = lanes_upto(own);
       const uint64_t over = __ballot(before + upto > target && own > 0.0), some = __ballot(own > 0.0);
       if (some) last = c0 + 63 - __builtin_clzll(some);
       if (over) {
@@ -289,11 +318,7 @@ __device__ __forceinline__ int find_element(int first, double target, const doub
   double own = 0.0;
 #pragma unroll
   for (int e = 0; e < PER; ++e) own += r[e];
-  double upto = own;
-  for (int d = 1; d < kWave; d <<= 1) {
-    const double y = __shfl_up(upto, d, kWave);
-    if (lane >= d) upto += y;
-  }
+  const double upto = lanes_upto(own);
   if (lane == kWave - 1) sums[wave] = upto;
   __syncthreads();
   double sum = 0.0;
@@ -491,10 +516,9 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
     if (wide == 64) top = fmaxf(top, __shfl_xor(top, 16, kWave)), top = fmaxf(top, __shfl_xor(top, 32, kWave));
     if (m < top) i = p.V;
     if (warm) z = m > kNegInf ? z * weight(m, top, s) : 0.0;
-    for (int d = wide / 2; d; d >>= 1) {
-      i = min(i, __shfl_xor(i, d, kWave));
-      z += __shfl_xor(z, d, kWave);
-    }
+    z = wide == 64 ? lanes_sum<64>(z) : lanes_sum<16>(z);
+    if (!warm)
+      for (int d = wide / 2; d; d >>= 1) i = min(i, __shfl_xor(i, d, kWave));
     if (mine == 0) l.most[t] = top, l.args[t] = top > kNegInf ? i : 0, l.zs[t] = z;   // (nothing: the first)
   }
   __syncthreads();
@@ -674,7 +698,7 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
     if (nagain) __syncthreads();
     double total = 0.0;   // (each wave for itself)
     for (int c = lane; c < p.C; c += kWave) total += masses[c];
-    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, kWave);
+    total = lanes_sum<64>(total);
     if (total > 0.0) {
       const Found f = find_chunk(p.C, l.us[0] * total, [&](int c) { return masses[c]; });
       piece(f.c, x);
@@ -723,11 +747,11 @@ template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) voi
 }
 
 // What the drafter's probabilities left of a row, chunk by chunk; a row's last block draws from it.
-template <typename T, typename Q> __global__ __launch_bounds__(kScanThreads) void verify_rest_kernel(VerifyParams p) {
-  constexpr int PER = kVerifyChunk / kScanThreads;
+template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_rest_kernel(VerifyParams p) {
+  constexpr int PER = kVerifyChunk / kWalkThreads;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   double* all = reinterpret_cast<double*>(smem);   // [C]
-  __shared__ double lds[kScanThreads / kWave];
+  __shared__ double lds[kWalkThreads / kWave];
   __shared__ bool last;
   const int c = blockIdx.x, b = blockIdx.y;
   const State st = p.state[b];
@@ -738,7 +762,7 @@ template <typename T, typename Q> __global__ __launch_bounds__(kScanThreads) voi
   rest.template eights<PER / 8>(c * kVerifyChunk - rest.row.shift + (int)threadIdx.x * PER, x);
 #pragma unroll
   for (int e = 0; e < PER; ++e) w += x[e];
-  w = block_sum<kScanThreads>(w, lds);
+  w = block_sum<kWalkThreads>(w, lds);
   if (threadIdx.x == 0) {
     store_agent(sums + c, w);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -747,19 +771,19 @@ template <typename T, typename Q> __global__ __launch_bounds__(kScanThreads) voi
   __syncthreads();
   if (!last) return;
   const float u = p.uniform[b * p.sub];
-  for (int i = threadIdx.x; i < p.C; i += kScanThreads) all[i] = load_agent(sums + i);
+  for (int i = threadIdx.x; i < p.C; i += kWalkThreads) all[i] = load_agent(sums + i);
   __syncthreads();
   double total = 0.0;   // (each wave for itself)
   for (int i = threadIdx.x % kWave; i < p.C; i += kWave) total += all[i];
-  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d, kWave);
+  total = lanes_sum<64>(total);
   int token;
   if (total > 0.0) {
     const Found f = find_chunk(p.C, u * total, [&](int i) { return all[i]; });
     const int first = f.c * kVerifyChunk - rest.row.shift;
     rest.template eights<PER / 8>(first + (int)threadIdx.x * PER, x);
-    token = find_element<kScanThreads>(first, f.target, x);
+    token = find_element<kWalkThreads>(first, f.target, x);
   } else {
-    token = argmax_of<kScanThreads>(rest.row, st.most);
+    token = argmax_of<kWalkThreads>(rest.row, st.most);
   }
   if (threadIdx.x == 0) p.out[(int64_t)b * p.T + st.at] = token;
 }
@@ -790,7 +814,7 @@ template <typename T, typename Q> static int launch_verify(const VerifyParams& p
     hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kWalkThreads), lds, s, p);
   }
   if (const int st = check_launch(); st || !p.probs) return st;
-  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kScanThreads), p.C * sizeof(double), s, p);
+  hipLaunchKernelGGL((verify_rest_kernel<T, Q>), dim3(p.C, p.B), dim3(kWalkThreads), p.C * sizeof(double), s, p);
   return check_launch();
 }
 
