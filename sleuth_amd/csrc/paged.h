@@ -246,17 +246,35 @@ __device__ __forceinline__ int tree_position(const PagedParams& p, int b, int ba
   const int d = p.depth[b * p.dsb + t];
   return base + (d < 0 ? 0 : d < n ? d : n - 1);
 }
-// What new token t, at position qpos, sees of the 32 keys from `key` on (bit i: key + i): the cache's, whose slots are
-// their positions, and the row's n new tokens, whose bits say it, within the window by their own depths.
-__device__ __forceinline__ unsigned tree_sees(const PagedParams& p, int b, int base, int n, int t, int qpos, int key) {
+// A token's row of the mask: its bits, in registers where they are 64 at most (a load then would be waited for in the
+// tree's own tiles, at the end of the row).
+struct TreeRow {
+  const uint32_t* row;
+  unsigned lo, hi;
+};
+__device__ __forceinline__ TreeRow tree_row(const PagedParams& p, int b, int t) {
+  TreeRow r{p.tree + b * p.tsb + t * p.tst, 0, 0};
+  if (p.words <= 2) r.lo = r.row[0], r.hi = r.row[1];
+  return r;
+}
+// What a new token of mask row r, at position qpos, sees of the 32 keys from `key` on (bit i: key + i): the cache's, whose
+// slots are their positions, and the row's n new tokens, whose bits say it, within the window by their own depths.
+__device__ __forceinline__ unsigned tree_sees(const PagedParams& p, int b, int base, int n, const TreeRow& r, int qpos, int key) {
   const int before = base - key;   // keys of the cache from `key` on
   unsigned see = low_bits(before);
   if (p.window > 0) see &= ~low_bits(qpos - p.window + 1 - key) | low_bits(p.sinks - key);
   if (before >= 32) return see;
-  const int off = -before, i = off >> 5;   // the first bit's new token (negative: bits of the cache before it)
-  const uint32_t* row = p.tree + b * p.tsb + t * p.tst;
-  const unsigned lo = i >= 0 && i < p.words ? row[i] : 0, hi = i + 1 >= 0 && i + 1 < p.words ? row[i + 1] : 0;
-  unsigned bits = __builtin_amdgcn_alignbit(hi, lo, (unsigned)off & 31) & low_bits(n - off) & ~low_bits(before);
+  const int off = -before;         // the first bit's new token (negative: bits of the cache before it)
+  unsigned bits;
+  if (p.words <= 2) {
+    const uint64_t all = r.lo | (uint64_t)r.hi << 32;
+    bits = (unsigned)(off >= 0 ? off < 64 ? all >> off : 0 : all << -off);
+  } else {
+    const int i = off >> 5;
+    const unsigned lo = i >= 0 && i < p.words ? r.row[i] : 0, hi = i + 1 >= 0 && i + 1 < p.words ? r.row[i + 1] : 0;
+    bits = __builtin_amdgcn_alignbit(hi, lo, (unsigned)off & 31);
+  }
+  bits &= low_bits(n - off) & ~low_bits(before);
   if (p.window > 0 && p.window < n) {      // (else no two tokens of the tree are a window apart)
     for (unsigned rest = bits; rest; rest &= rest - 1) {
       const int j = __builtin_ctz(rest), at = tree_position(p, b, base, n, off + j);
@@ -277,29 +295,28 @@ template <typename T> __device__ __forceinline__ bool not_finite(T x) {
     return (__builtin_bit_cast(unsigned short, x) & e) == e;
   }
 }
-// Whether `bytes` of LDS hold such a value (the whole wave looks, and knows).
-template <typename T> __device__ __forceinline__ bool tile_not_finite(const char* tile, int bytes) {
-  bool bad = false;
-#pragma unroll 1
-  for (int x = (threadIdx.x % kWave) * 16; x < bytes; x += kWave * 16) {
-    const uint4 u = load16(tile + x);
-    T v[16 / sizeof(T)];
-    *reinterpret_cast<uint4*>(v) = u;
-#pragma unroll
-    for (int e = 0; e < 16 / (int)sizeof(T); ++e) bad |= not_finite(v[e]);
+// The dwords of a lane's 16-byte pieces: add() each, then bad() says whether one holds such a value.
+template <typename T> struct OddValues {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  unsigned top = 0;   // the largest magnitude, as a number; of each half in 16 bits
+  __device__ __forceinline__ void add(unsigned x) {
+    if constexpr (sizeof(T) == 4) top = max(top, x & 0x7fffffffu);
+    else top = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
   }
-  return __any(bad);
-}
-// Takes them out; thread `at` of `of`.
-template <typename T> __device__ __forceinline__ void make_finite(char* tile, int bytes, int at, int of) {
-#pragma unroll 1
-  for (int x = at * 4; x < bytes; x += of * 4) {
-    T v[4 / sizeof(T)];
-    *reinterpret_cast<unsigned*>(v) = *reinterpret_cast<const unsigned*>(tile + x);
-#pragma unroll
-    for (int e = 0; e < 4 / (int)sizeof(T); ++e) v[e] = not_finite(v[e]) ? (T)0.0f : v[e];
-    *reinterpret_cast<unsigned*>(tile + x) = *reinterpret_cast<const unsigned*>(v);
+  __device__ __forceinline__ bool bad() const {
+    if constexpr (sizeof(T) == 4) return top >= 0x7f800000u;
+    else {
+      constexpr unsigned e = __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+      return (top & 0xffff) >= e || top >> 16 >= e;
+    }
   }
+};
+template <typename T> __device__ __forceinline__ unsigned finite_dword(unsigned x) {
+  T v[4 / sizeof(T)];
+  *reinterpret_cast<unsigned*>(v) = x;
+#pragma unroll
+  for (int e = 0; e < 4 / (int)sizeof(T); ++e) v[e] = not_finite(v[e]) ? (T)0.0f : v[e];
+  return *reinterpret_cast<const unsigned*>(v);
 }
 
 // Four output channels of query row `flat` of (b, kvh).

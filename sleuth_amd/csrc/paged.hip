@@ -267,7 +267,8 @@ void paged_step_kernel(PagedParams p) {
 
   // ---- query rows, as B operands; rows behind the row's last one stand for that one (never written)
   u32x4 q[LD::Q_LDS ? 1 : RB][S];
-  int qpos[RB], qtok[TREE ? RB : 1];
+  int qpos[RB];
+  TreeRow qtree[TREE ? RB : 1];
   const int ntok = TREE ? w.last - w.base + 1 : 0;   // the tree's real tokens
   char* ql = smem + LD::Q_OFF;  // [ROWS][chunks turned with the row]
 #pragma unroll
@@ -276,8 +277,8 @@ void paged_step_kernel(PagedParams p) {
     const int at = row < w.rows ? row : w.rows - 1;
     qpos[r] = w.base + p.token(at);
     if constexpr (TREE) {
-      qtok[r] = p.token(at);
-      qpos[r] = w.rows > 0 ? tree_position(p, b, w.base, ntok, qtok[r]) : w.base;
+      qtree[r] = tree_row(p, b, w.rows > 0 ? p.token(at) : 0);
+      qpos[r] = w.rows > 0 ? tree_position(p, b, w.base, ntok, p.token(at)) : w.base;
     }
     if constexpr (LD::Q_LDS) {
       if (r % 4 == wave && w.rows > 0) {
@@ -308,6 +309,25 @@ void paged_step_kernel(PagedParams p) {
   int odd_from = -1, odd_to = -2;   // (trees) the wave's tiles among which are those with values taken out
   for (; i < end; i = next(i)) {
     const int key0 = w.tile_key(i, KT);
+    // whether every row of the block sees the tile whole
+    const bool whole_tile = key0 + KT - 1 <= w.first && (p.window <= 0 || key0 > w.last - p.window || key0 + KT <= p.sinks);
+    if constexpr (TREE) {
+      if (!whole_tile) {   // (paged.h)
+        OddValues<T> odd;
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd.add(vr[j][e]);
+        if (__any(odd.bad())) {
+          odd_from = odd_from < 0 ? i : odd_from;
+          odd_to = i;
+#pragma unroll
+          for (int j = 0; j < NL; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vr[j][e] = finite_dword<T>(vr[j][e]);
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int row = j * TL::RPI + lrow;
@@ -339,10 +359,8 @@ void paged_step_kernel(PagedParams p) {
         }
       }
 
-    // a tile that every row of the block sees whole needs no mask
-    const bool full = miss == 0 && key0 + KT - 1 <= w.first &&
-                      (p.window <= 0 || key0 > w.last - p.window || key0 + KT <= p.sinks);
-    if (!full) {
+    // a tile that every row sees whole, in pages that are there, needs no mask
+    if (miss || !whole_tile) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
         // bits of the keys from key0 + 4g on: the window up to the query, and the first tokens up to it
@@ -351,7 +369,7 @@ void paged_step_kernel(PagedParams p) {
         const int lo = (p.window > 0 ? qpos[r] - p.window + 1 : 0) - base;
         const int first = p.sinks - base < top ? p.sinks - base : top;
         unsigned see = (low_bits(top) & ~low_bits(lo)) | low_bits(first);
-        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, qtok[r], qpos[r], base);
+        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, qtree[r], qpos[r], base);
         if (miss & 1) see &= ~0xffffu;
         if (miss & 2) see &= 0xffffu;
 #pragma unroll
@@ -387,16 +405,6 @@ void paged_step_kernel(PagedParams p) {
           s[r][kb][j] = w8;
           l[r] += w8;
         }
-    }
-
-    if constexpr (TREE) {
-      if (!full && tile_not_finite<T>(vt, TL::TILEB)) {   // (paged.h)
-        make_finite<T>(vt, TL::TILEB, lane, kWave);
-        odd_from = odd_from < 0 ? i : odd_from;
-        odd_to = i;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
     }
 
     // O^T += V^T . P^T; the k-slots of a lane are the keys whose weights it holds
@@ -475,7 +483,7 @@ void paged_step_kernel(PagedParams p) {
         const char* src = vb0 + page * pageb + (int64_t)(key & p.page_mask) * rowb;
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
-          if (!(tree_sees(p, b, w.base, ntok, qtok[r], qpos[r], key) & 1)) continue;
+          if (!(tree_sees(p, b, w.base, ntok, qtree[r], qpos[r], key) & 1)) continue;
 #pragma unroll
           for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -272,6 +272,8 @@ void paged_chunk_kernel(PagedParams p) {
   const int t = p.token(valid ? flat : w.rows - 1), h = kvh * p.G + (valid ? flat : w.rows - 1) - t * p.G;
   const int ntok = TREE ? w.last - w.base + 1 : 0;   // the tree's real tokens
   const int qpos = TREE ? tree_position(p, b, w.base, ntok, t) : w.base + t;
+  TreeRow qtree{};
+  if constexpr (TREE) qtree = tree_row(p, b, t);
   // positions between which the wave's queries lie; keys up to wq_all that all of them see
   const int wq_lo = TREE ? w.base : w.base + p.token(w_row), wq_all = TREE ? w.first : wq_lo;
   const int wq_hi = TREE ? w.last : w.base + p.token(w_row + 31 < w.rows ? w_row + 31 : w.rows - 1);
@@ -299,27 +301,38 @@ void paged_chunk_kernel(PagedParams p) {
   float m_run = kNegInf, l_run = 0.0f;
   const float c = p.scale_log2;
 
-  int odd_from = -1, odd_to = -2;   // (trees) the tiles among which are those with values taken out
+  int odd = 0;   // (trees) values were taken out of the wave's rows of a tile
+  const auto whole_tile = [&](int key0) {
+    return key0 + BN - 1 <= w.first && (p.window <= 0 || w.last - key0 < p.window || key0 + BN <= p.sinks);
+  };
   for (int it = begin; it < end; ++it) {
     const int stage = (it - begin) & 1;
     wait_vm<0>();
+    if constexpr (TREE) {   // (paged.h; each wave looks at the rows that it loaded, before the others read them)
+      if (!whole_tile(w.tile_key(it, BN))) {
+        char* mine = smem + (2 * stage + 1) * TL::TILEB + wave * TL::LOADS * 1024 + lane * 16;
+        OddValues<T> values;
+#pragma unroll
+        for (int x = 0; x < TL::LOADS; ++x) {
+          const uint4 v = load16(mine + x * 1024);
+          values.add(v.x), values.add(v.y), values.add(v.z), values.add(v.w);
+        }
+        if (__any(values.bad())) {
+          odd = 1;
+#pragma unroll 1
+          for (int x = 0; x < 4 * TL::LOADS; ++x) {
+            unsigned* at = reinterpret_cast<unsigned*>(mine + (x >> 2) * 1024) + (x & 3);
+            *at = finite_dword<T>(*at);
+          }
+        }
+      }
+    }
     __syncthreads();  // tile `it` is in LDS for every wave; the other stage is free
     if (it + 1 < end) {
       issue(stage ^ 1, page);
       page = page_at(it + 2 < end ? it + 2 : it + 1);
     }
     const int key0 = w.tile_key(it, BN);
-    if constexpr (TREE) {   // (paged.h; every wave finds the same)
-      const bool part = !(key0 + BN - 1 <= w.first && (p.window <= 0 || w.last - key0 < p.window || key0 + BN <= p.sinks));
-      char* vtile = smem + (2 * stage + 1) * TL::TILEB;
-      if (part && tile_not_finite<T>(vtile, TL::TILEB)) {
-        __syncthreads();
-        make_finite<T>(vtile, TL::TILEB, threadIdx.x, TL::THREADS);
-        odd_from = odd_from < 0 ? it : odd_from;
-        odd_to = it;
-        __syncthreads();
-      }
-    }
     const bool needed = wave_any && key0 <= wq_hi &&
                         (p.window <= 0 || key0 + BN - 1 > wq_lo - p.window || key0 < p.sinks);
     if (HALVES == 1 && !needed) continue;
@@ -400,7 +413,7 @@ void paged_chunk_kernel(PagedParams p) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
         unsigned see = (low_bits(top - 32 * kb) & ~low_bits(lo - 32 * kb)) | low_bits(first - 32 * kb);
-        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, t, qpos, base + 32 * kb);
+        if constexpr (TREE) see = tree_sees(p, b, w.base, ntok, qtree, qpos, base + 32 * kb);
         if (bad) {
 #pragma unroll
           for (int x = 0; x < 16; x += 4)
@@ -484,15 +497,25 @@ void paged_chunk_kernel(PagedParams p) {
   }
 
   l_run += __shfl_xor(l_run, 32, kWave);
+  if constexpr (TREE) {   // whether any wave took values out (the tiles' LDS is free)
+    int* all = reinterpret_cast<int*>(smem);
+    __syncthreads();
+    if (lane == 0) all[wave] = odd;
+    __syncthreads();
+    odd = 0;
+#pragma unroll
+    for (int y = 0; y < TL::WAVES; ++y) odd |= all[y];
+  }
   if (!valid) return;
   if constexpr (TREE) {
 #pragma unroll 1
-    for (int y = odd_from; y >= 0 && y <= odd_to; ++y) {   // the values that were taken out, for the rows that see them
+    for (int y = begin; odd && y < end; ++y) {   // those, for the rows that see them
       const int key0 = w.tile_key(y, BN);
+      if (whole_tile(key0)) continue;
 #pragma unroll 1
       for (int key = key0; key < key0 + BN && key <= w.last; ++key) {
         const int page = p.page_of(b, key);
-        if (page < 0 || !(tree_sees(p, b, w.base, ntok, t, qpos, key) & 1)) continue;
+        if (page < 0 || !(tree_sees(p, b, w.base, ntok, qtree, qpos, key) & 1)) continue;
         const T* src = reinterpret_cast<const T*>(vgb + page * pageb + (int64_t)(key & p.page_mask) * rowb);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
