@@ -142,6 +142,18 @@ __device__ __forceinline__ void lds_dma16(const void* gbase, unsigned voff, unsi
       : "v"(voff), "s"(gbase), "s"(lds)
       : "memory");
 }
+// The same for bytes that no other block reads: they are not kept in the caches.
+__device__ __forceinline__ void lds_dma16_once(const void* gbase, unsigned voff, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "global_load_lds_dwordx4 %1, %2 nt\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(voff), "s"(gbase), "s"(lds)
+      : "memory");
+}
 
 // max over lanes l and l ^ 32 with gfx950's v_permlane32_swap (VALU, no LDS round trip):
 // swapping x with itself returns the lower half's and the upper half's value of the pair.

@@ -82,7 +82,7 @@ static PagedPlan paged_plan(int dtype, int B, int T, int H, int K, int D, int64_
   if (plan.chunk && ragged && B > 1 && K <= 64 && units < 2 * slots && blocks <= kPlanPairs && units * tiles > 16 * slots &&
       blocks * tiles <= INT_MAX / 4) {
     plan.planned = true;
-    plan.nitems = (int)(plan.slots / K + blocks);
+    plan.nitems = (int)((tree ? 2 : 1) * (plan.slots / K) + blocks);
     return plan;
   }
   // Parts that are on the device together: one more would wait for a whole part of the others (us, with parts rounded

@@ -238,7 +238,15 @@ void paged_chunk_kernel(PagedParams p) {
     const char* vs = vgb + at;
     int lk = ld_k, lv = ld_v;
     if constexpr (!KEEP) asm volatile("" : "+v"(lk), "+v"(lv));  // (not kept over the loop)
-    if (!edge) {
+    if (TREE && KEEP && !edge && p.rows <= BM) {
+      // A tree of one row block has its keys to itself (32 rows of up to 16,383 keys, 64 tokens, 16 q / 8 KV heads of 128:
+      // 256 -> 238 us)
+#pragma unroll
+      for (int x = 0; x < (KEEP ? TL::LOADS : 0); ++x) {
+        lds_dma16_once(ks, (unsigned)kept_k[x], kdst + x * 1024);
+        lds_dma16_once(vs, (unsigned)kept_v[x], vdst + x * 1024);
+      }
+    } else if (!edge) {
 #pragma unroll
       for (int x = 0; x < TL::LOADS; ++x) {
         if constexpr (KEEP) {
@@ -576,21 +584,47 @@ template <int BM, int KT, bool TREE> __global__ __launch_bounds__(kPlanThreads) 
   const int room = p.slots / p.K;
   const int least = max(8, (total + room - 1) / room);
   auto per_of = [&](int w) { return w == 15 ? 1 << 30 : least + (int)((int64_t)least * w / 10); };
-  {
-    const int per = per_of(wave);
+  int per;
+  if constexpr (!TREE) {
+    const int tried = per_of(wave);
     int parts = 0;
-    for (int i = lane; i < n; i += kWave) parts += (tiles[i] + per - 1) / per;
+    for (int i = lane; i < n; i += kWave) parts += (tiles[i] + tried - 1) / tried;
     for (int d = 1; d < kWave; d <<= 1) parts += __shfl_xor(parts, d, kWave);
     if (lane == 0) wave_of[wave] = parts;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int w = 0;
+      while (w < 15 && wave_of[w] > room) ++w;
+      pick = w;
+    }
+    __syncthreads();
+    per = per_of(pick);
+  } else {
+    // Few rows of different lengths leave much of one round empty (32 of up to 16,383 keys: 62 parts, the longest 93 tiles
+    // where 69 would be an equal share), and two rounds of half as long parts less: for each the least of 32 steps of 5 %
+    // that fits, and the one whose longest parts take less time, with what a part costs by itself, three tiles' time
+    // (there 238 us in one round, 216 in two, 232 in three).
+    const int half = max(8, (total + 2 * room - 1) / (2 * room));
+    __shared__ int best[2];
+    if (threadIdx.x < 2) best[threadIdx.x] = 1 << 30;
+    __syncthreads();
+    const int from = wave < 8 ? least : half, fits = (wave < 8 ? 1 : 2) * room;   // (a wave tries four)
+    int tried[4], parts[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) tried[x] = from + (int)((int64_t)from * (4 * (wave & 7) + x) / 20);
+    for (int i = lane; i < n; i += kWave)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) parts[x] += (tiles[i] + tried[x] - 1) / tried[x];
+    for (int d = 1; d < kWave; d <<= 1)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) parts[x] += __shfl_xor(parts[x], d, kWave);
+    if (lane == 0)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (parts[x] <= fits) atomicMin(&best[wave >> 3], tried[x]);
+    __syncthreads();
+    per = best[1] < 1 << 30 && 2 * (int64_t)best[1] + 6 < best[0] + 3 ? best[1] : best[0];
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int w = 0;
-    while (w < 15 && wave_of[w] > room) ++w;
-    pick = w;
-  }
-  __syncthreads();
-  const int per = per_of(pick);
   // lengths relative to the longest part: class 0 is the longest; a row block without a real query is one part
   // of no tiles, which writes its zeros
   auto parts_of = [&](int i) { return tiles[i] > 0 ? (tiles[i] + per - 1) / per : 1; };
