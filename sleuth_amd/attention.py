@@ -19,6 +19,8 @@ of head_norm_rope + cache.update + SDPA):
       a paged cache (PagedKVCache):           forge_kv_append_paged, then forge_attn_paged;
       a window with first tokens that stay visible (spec.sinks): forge_kv_append, then
                         forge_attn_sinks;
+      a cache with a tree set (cache.set_tree): the new tokens are drafted branches: forge_kv_append(_paged),
+                        then forge_attn_tree;
       otherwise         forge_attn_decode_append: the cache write and the split-K
                         attention (decode, verify, static steps, other head sizes)
                         in one launch, the q norm + RoPE fused into the q load.
@@ -49,6 +51,7 @@ from .config import ModelConfig
 from .norm import RMSNorm
 from .rope import apply_rope
 from .taps import make_tap, tap_active
+from .tree import tree_mask
 
 DECODE_MAX_T = 16
 _HIP_HEAD_DIMS = (32, 64, 128, 256, 512)   # 512 (Gemma 4's full layers) in bf16/fp16 only
@@ -404,6 +407,12 @@ class Attention(nn.Module):
             where = (cache.page_table, cache.seq_lens)
             kp, vp = cache.k[self.layer_idx], cache.v[self.layer_idx]
             ops.kv_append_paged(k, v, kp, vp, *where, new_lens=cache.new_lens, norm_v=norm_v, **k_args)
+            tree = cache.tree
+            if tree is not None:
+                self.last_path = "hip-paged-tree"
+                return ops.attn_tree_paged(q, kp, vp, *where, tree.mask, depth=tree.depth if self.window else None,
+                                           scale=self.scale, new_lens=cache.new_lens, max_kv_len=cache.bound(T),
+                                           window=self.window, sinks=self.sinks, **q_args)
             self.last_path = "hip-paged"
             return ops.attn_paged(q, kp, vp, *where, scale=self.scale, new_lens=cache.new_lens, max_kv_len=cache.bound(T),
                                   window=self.window, sinks=self.sinks, **q_args)
@@ -433,6 +442,12 @@ class Attention(nn.Module):
             chunk = 0 if self.sinks else ops.decode_chunk(q.dtype, B, 1, H, self.n_kv, hd, cache.max_len, self.window,
                                      uniform="row_pos" not in pos_kw)
 
+        tree = getattr(cache, "tree", None)
+        if tree is not None:
+            ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)
+            self.last_path = "hip-tree"
+            return ops.attn_tree(q, kc, vc, tree.mask, scale=self.scale, depth=tree.depth if self.window else None,
+                                 max_kv_len=max_kv, window=self.window, sinks=self.sinks, **pos_kw, **q_args)
         if self.sinks:
             ops.kv_append(k, v, kc, vc, norm_v=norm_v, **pos_kw, **k_args)
             self.last_path = "hip-sinks"
@@ -469,6 +484,11 @@ class Attention(nn.Module):
         if self.use_rope:
             q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         q, k = self.tap_q(q), self.tap_k(k)
+        if getattr(cache, "tree", None) is not None:
+            if same_doc is not None:
+                raise NotImplementedError("document masks are for whole windows: no drafted trees")
+            cache.update(self.layer_idx, k, v)
+            return self._rows_torch(q, cache, cache.tree)
         if cache is not None and getattr(cache, "ragged", False) and not getattr(cache, "static", False):
             if _is_block_mask(same_doc):
                 raise NotImplementedError(_FLEX_LIMITS)
@@ -505,7 +525,7 @@ class Attention(nn.Module):
             if same_doc is not None:
                 raise NotImplementedError("document masks are for whole windows: no paged cache")
             cache.update(self.layer_idx, k, v)
-            return self._paged_torch(q, cache)
+            return self._rows_torch(q, cache)
         cache.update(self.layer_idx, k, v)
         out = []
         for b, L in enumerate(lens):
@@ -515,17 +535,26 @@ class Attention(nn.Module):
             out.append(fn(q[b:b + 1], kb, vb, L, same_doc))
         return torch.cat(out, 0)
 
-    def _paged_torch(self, q, cache):
-        """Per-row torch attention over a paged cache that holds the new keys: rows past a row's new
-        tokens are zeros, positions without a page are invisible and keys that no query sees unused, as in
-        ops.attn_paged."""
+    def _rows_torch(self, q, cache, tree=None):
+        """Per-row torch attention over a paged cache (or of a drafted tree over any) that holds the new keys: rows past a
+        row's new tokens are zeros, positions without a page are invisible and keys that no query sees unused, as in
+        ops.attn_paged and attn_tree."""
         out = torch.zeros_like(q)
-        for b, (L, n) in enumerate(zip(cache.seq_lens_host, cache.new_tokens(q.shape[2]))):
+        paged = getattr(cache, "paged", False)
+        T = q.shape[2]
+        lens = [int(cache.pos_t)] * q.shape[0] if getattr(cache, "static", False) else cache.seq_lens_host
+        for b, (L, n) in enumerate(zip(lens, cache.new_tokens(T) if paged else [T] * q.shape[0])):
             if not n:
                 continue
-            kb, vb, held = cache.row(self.layer_idx, b, L + n)
+            if paged:
+                kb, vb, held = cache.row(self.layer_idx, b, L + n)
+            else:
+                kb, vb, held = cache.k[self.layer_idx][b, :, :L + n], cache.v[self.layer_idx][b, :, :L + n], True
             rep = self.n_heads // self.n_kv
-            see = self._mask(n, L + n, L, q.device) & held
+            if tree is not None:
+                see = tree_mask(tree, b, L, n, self.window, self.sinks, q.device) & held
+            else:
+                see = self._mask(n, L + n, L, q.device) & held
             vb = vb.masked_fill(~see.any(0)[None, :, None], 0)
             scores = (q[b, :, :n].float() @ kb.repeat_interleave(rep, 0).float().transpose(-2, -1)) * self.scale
             probs = scores.masked_fill(~see, float("-inf")).softmax(-1).masked_fill(~see.any(-1)[:, None], 0.0)

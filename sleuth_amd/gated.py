@@ -47,6 +47,8 @@ class GatedAttention(nn.Module):
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache=None) -> torch.Tensor:
         if getattr(cache, "paged", False):
             raise NotImplementedError("gated attention has no path over a paged cache")
+        if getattr(cache, "tree", None) is not None:
+            raise NotImplementedError("gated attention has no path for drafted trees")
         c = self.cfg
         B, T, _ = x.shape
         qg = self.q_proj(x).view(B, T, c.n_heads, 2 * c.head_dim)

@@ -4,12 +4,14 @@ draft-then-verify, and graph-replayed decode steps.
 generate()             the decode loop of sleuth/forge/infer/generate.py:49-136: the prompt's
                        prefill, then one token per step through the cache (greedy or
                        temperature sampling)
-speculative_generate() greedy draft-then-verify as in speculative.py:83-277: [pending] + k
-                       guesses in one forward at offset cache.pos, the agreeing prefix kept by
-                       moving pos back (the rewind the reference's keep() does)
+speculative_generate() draft-then-verify as in speculative.py:83-277: [pending] + k guesses in one
+                       forward at offset cache.pos, the agreeing prefix kept by moving pos back (the
+                       rewind the reference's keep() does); beyond the reference, drafts may be trees
+                       (their accepted branch closes up in the cache) and a temperature's samples
 generate_batch()       several prompts of different lengths at once over a paged cache: their chunks
                        of new tokens padded to one batch, then one token per step for the rows
-                       still running; pages come back as rows end or leave every layer's sight
+                       still running; pages come back as rows end or leave every layer's sight;
+                       several continuations of a prompt share its pages (PagedKVCache.fork)
 GraphDecoder           decode/verify steps replayed from a HIP graph (the role of
                        cuda_graph.py:67-144), built for kernels that read the live length on
                        the device: the attention reads only the keys below pos_t + T, whatever
@@ -29,6 +31,7 @@ import torch
 
 from .kv_cache import KVCache
 from .paged_cache import OutOfPages, PagedKVCache
+from .tree import Drafts, verify
 
 
 @dataclass
@@ -62,6 +65,7 @@ class GraphDecoder:
         self._ids = torch.zeros(1, tokens_per_step, dtype=torch.long, device=p.device)
         self._graph: torch.cuda.CUDAGraph | None = None
         self._logits: torch.Tensor | None = None
+        self._trees = False
         self.replays = 0
 
     @property
@@ -105,28 +109,34 @@ class GraphDecoder:
     def step(self, token: torch.Tensor) -> torch.Tensor:
         """Logits [1, vocab] of `token` at position cache.pos; the cache moves on by one.
         The result is the graph's output buffer: read it before the next replay."""
-        if self.T != 1:
+        if self.T != 1 or self._trees:
             raise ValueError("step() is for one token at a time; use verify()")
         logits = self._launch(token)
         self.cache.pos += 1
         return logits
 
-    def verify(self, tokens: torch.Tensor) -> torch.Tensor:
+    def verify(self, tokens: torch.Tensor, parents: list[int] | None = None) -> torch.Tensor:
         """Logits [T, vocab] of T tokens at positions cache.pos, ...; cache.pos stays (the
-        caller sets it to what it keeps)."""
+        caller sets it to what it keeps). parents: the tokens are the nodes of a drafted tree, for which
+        this decoder then records (cache.keep says which nodes stand)."""
+        if self._graph is not None and (parents is not None) != self._trees:
+            raise ValueError("this decoder was recorded for " + ("trees" if self._trees else "chains"))
+        self._trees = parents is not None
+        self.cache.set_tree(parents)
         return self._launch(tokens)
 
 
 _decoders: "weakref.WeakKeyDictionary[torch.nn.Module, dict]" = weakref.WeakKeyDictionary()
 
 
-def decoder_for(model, max_len: int, dtype: torch.dtype, tokens_per_step: int = 1) -> GraphDecoder:
-    """The model's graph decoder for this context and step size, kept across calls (the
-    graph is recorded once per model); its cache is rewound for the new prompt."""
+def decoder_for(model, max_len: int, dtype: torch.dtype, tokens_per_step: int = 1, trees: bool = False) -> GraphDecoder:
+    """The model's graph decoder for this context and step size (and for chains or trees), kept across
+    calls (the graph is recorded once per model); its cache is rewound for the new prompt."""
     per_model = _decoders.setdefault(model, {})
-    dec = per_model.get((max_len, tokens_per_step, dtype))
+    key = (max_len, tokens_per_step, dtype, trees)
+    dec = per_model.get(key)
     if dec is None:
-        dec = per_model[(max_len, tokens_per_step, dtype)] = GraphDecoder(model, max_len, dtype, tokens_per_step)
+        dec = per_model[key] = GraphDecoder(model, max_len, dtype, tokens_per_step)
     dec.cache.reset()
     return dec
 
@@ -167,26 +177,30 @@ def generate(model, prompt_ids: list[int], max_new_tokens: int = 32, temperature
 @torch.no_grad()
 def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, temperature: float = 0.0,
                    stop_ids: set[int] | None = None, seed: int | None = None, chunk: int = 512, page_size: int = 64,
-                   n_pages: int | None = None, cache_dtype: torch.dtype | None = None) -> list[GenerationResult]:
+                   n_pages: int | None = None, cache_dtype: torch.dtype | None = None, samples: int = 1) -> list[GenerationResult]:
     """generate() for a batch of prompts of any lengths over a paged cache: every pass takes up to `chunk` tokens of
     each prompt that has some left (the batch is padded to the longest), then each running row decodes one token per
     pass. A row's pages come back when it ends, and, where every layer slides, as they leave the windows (the first
     cfg.sink_tokens positions stay). Where the pool is short, OutOfPages is raised with `results`: the finished rows', and
-    the others' so far (stop_reason "out_of_pages")."""
+    the others' so far (stop_reason "out_of_pages").
+    samples: continuations of each prompt (results in the prompts' order, a prompt's together): the prompt runs once, and its
+    rows share its pages."""
     if not prompts or not all(prompts):
         raise ValueError("every prompt must contain at least one token")
-    if chunk < 1:
-        raise ValueError("chunk must be positive")
+    if chunk < 1 or samples < 1:
+        raise ValueError("chunk and samples must be positive")
     cfg, dev = model.cfg, next(model.parameters()).device
     longest = max(map(len, prompts))
     if longest > cfg.max_seq_len:
         raise ValueError(f"sequence length {longest} exceeds max_seq_len {cfg.max_seq_len}")
+    prompts = [p for p in prompts for _ in range(samples)]
     cache = PagedKVCache.for_model(model, len(prompts), cfg.max_seq_len, cache_dtype, page_size, n_pages)
     gen = torch.Generator(device=dev).manual_seed(seed or 0)
     specs = [cfg.attn_spec(i) for i in range(cfg.n_layers)]
     window = max(s.window for s in specs) if all(s.window for s in specs) else 0
     model.eval()
-    left = [list(p) for p in prompts]                 # tokens that no pass has taken yet
+    # tokens that no pass has taken yet; a prompt's other rows wait for its first one
+    left = [list(p) if b % samples == 0 else [] for b, p in enumerate(prompts)]
     results = [GenerationResult(list(p), [], "max_new_tokens") for p in prompts]
     running = [max_new_tokens > 0] * len(prompts)
     passes, most_pages = 0, 0
@@ -204,11 +218,17 @@ def generate_batch(model, prompts: list[list[int]], max_new_tokens: int = 32, te
             raise
         logits = model(ids, cache=cache).logits
         passes, most_pages = passes + 1, max(most_pages, cache.n_pages - cache.free_pages)
-        last = logits[torch.arange(len(new), device=dev), torch.tensor(new, device=dev).clamp(min=1) - 1]
-        tokens = _pick(last, temperature, gen).tolist()
+        first = list(range(len(new)))                 # the row whose logits a row draws from
         for b, n in enumerate(new):
             left[b] = left[b][n:]
-            if not n or left[b]:
+            if samples > 1 and b % samples == 0 and n and not left[b] and not results[b].new_ids:
+                for other in range(b + 1, b + samples):   # the prompt is in
+                    cache.fork(b, other)
+                    first[other] = b
+        last = logits[torch.arange(len(new), device=dev), torch.tensor(new, device=dev).clamp(min=1) - 1]
+        tokens = _pick(last if samples == 1 else last[torch.tensor(first, device=dev)], temperature, gen).tolist()
+        for b, n in enumerate(new):
+            if not (n or first[b] != b) or left[b]:
                 continue                              # not running, or more of its prompt to come
             r = results[b]
             r.new_ids.append(tokens[b])
@@ -247,41 +267,94 @@ def ngram_draft(max_ngram: int = 3) -> Callable[[list[int], int], list[int]]:
     return draft
 
 
+def ngram_tree_draft(max_ngram: int = 3, branches: int = 3) -> Callable[[list[int], int], Drafts]:
+    """ngram_draft with what followed several earlier occurrences: up to `branches` of them, the latest first, as one tree of at
+    most k tokens (what they begin with alike is drafted once)."""
+    def draft(ids: list[int], k: int) -> Drafts:
+        for n in range(min(max_ngram, len(ids) - 1), 0, -1):
+            tail = ids[-n:]
+            found = [s + n for s in range(len(ids) - n - 1, -1, -1) if ids[s:s + n] == tail][:min(branches, k)]
+            if not found:
+                continue
+            tokens, parents, known = [], [], {}
+            for left, start in zip(range(len(found) - 1, -1, -1), found):
+                most, at = k - left * (k // len(found)), -1      # the others' shares stay
+                for t in ids[start:start + k]:
+                    if (at, t) not in known:
+                        if len(tokens) >= most:
+                            break
+                        known[at, t] = len(tokens)
+                        tokens.append(t)
+                        parents.append(at)
+                    at = known[at, t]
+            return Drafts(tokens, parents)
+        return Drafts([])
+    return draft
+
+
 @torch.no_grad()
 def speculative_generate(model, prompt_ids: list[int], max_new_tokens: int = 32, k: int = 4,
-                         draft: Callable[[list[int], int], list[int]] | None = None,
-                         cuda_graph: bool = False, cache_dtype: torch.dtype | None = None) -> GenerationResult:
-    """Greedy draft-then-verify: each round runs [pending] + guesses in one forward at
-    offset cache.pos (T = 1 + k), keeps the longest agreeing prefix and rewinds pos."""
+                         draft: Callable[[list[int], int], list[int] | Drafts] | None = None,
+                         cuda_graph: bool = False, cache_dtype: torch.dtype | None = None, temperature: float = 0.0,
+                         seed: int | None = None, trees: bool = False) -> GenerationResult:
+    """Draft-then-verify: each round runs [pending] + guesses in one forward at offset cache.pos (T = 1 + k) and keeps
+    what stands: greedily the longest agreeing prefix (pos is rewound), at a temperature what the target would have sampled
+    (tree.verify; the drafts count as not drawn). draft(ids, k) gives a list, a chain of guesses, or Drafts, a tree of them,
+    whose accepted branch closes up in the cache. trees: with cuda_graph, record the passes for trees (a chain is one); a graph
+    for chains leaves a tree's round to an eager pass. A tree's nodes see other slots than a decode's tokens would, so its sums have
+    another order: its logits are a decode's to rounding, not bit for bit."""
     draft = draft or ngram_draft()
     p = next(model.parameters())
     max_len = model.cfg.max_seq_len
     dtype = cache_dtype or p.dtype
-    dec = decoder_for(model, max_len, dtype, tokens_per_step=k + 1) if cuda_graph else None
+    dec = decoder_for(model, max_len, dtype, tokens_per_step=k + 1, trees=trees) if cuda_graph else None
     cache = dec.cache if dec is not None else KVCache.for_model(model, 1, max_len, dtype)
+    gen = torch.Generator(device=p.device).manual_seed(seed or 0)
     model.eval()
     logits = model(torch.tensor([prompt_ids], device=p.device), cache=cache).logits[0, -1]
-    ids = list(prompt_ids) + [int(logits.argmax())]
+    ids = list(prompt_ids) + [int(_pick(logits[None], temperature, gen))]
     new = ids[len(prompt_ids):]
     stats = {"forwards": 0, "drafted": 0, "accepted": 0}
     while len(new) < max_new_tokens:
         room = min(k, max_new_tokens - len(new), max_len - cache.pos - 1)
         if room < 0:
             break
-        guess = draft(ids, room)[:room] if room > 0 else []
-        start = cache.pos
-        if dec is not None and start + k + 1 <= max_len:
-            row = [new[-1]] + guess + [new[-1]] * (k - len(guess))   # fixed T: pad the guesses
-            out = dec.verify(torch.tensor(row, device=p.device))
+        drafts = draft(ids, room) if room > 0 else []
+        if not isinstance(drafts, Drafts):
+            drafts = Drafts(list(drafts))
+        if len(drafts.tokens) > room:
+            drafts = Drafts(drafts.tokens[:room], None if drafts.parents is None else drafts.parents[:room])
+        guess, start = drafts.tokens, cache.pos
+        graph = dec is not None and start + k + 1 <= max_len and (trees or drafts.chain)
+        tree = trees if graph else not drafts.chain
+        pad = k - len(guess) if graph else 0                    # fixed T: pad the guesses (with nodes that nothing reaches)
+        row = torch.tensor([[new[-1]] + guess + [new[-1]] * pad], device=p.device)
+        parents = drafts.nodes() + [-1] * pad
+        if graph:
+            out = dec.verify(row[0], parents if tree else None)
         else:
-            out = model(torch.tensor([[new[-1]] + guess], device=p.device), cache=cache).logits[0]
-        choice = out[:len(guess) + 1].argmax(-1).tolist()
-        n_ok = next((i for i, (c, g) in enumerate(zip(choice, guess)) if c != g), len(guess))
+            cache.set_tree(parents if tree else None)
+            out = model(row, cache=cache).logits[0]
+        if tree or temperature > 0:
+            news, path, count = verify(out[None], row, parents=torch.tensor([parents], dtype=torch.int32, device=p.device),
+                                       uniform=torch.rand(1, row.shape[1], generator=gen, device=p.device) if temperature > 0 else None,
+                                       temperature=temperature)
+            n_ok = int(count) - 1
+            stands = news[0, :n_ok + 1].tolist()
+            if tree:
+                cache.keep(path, count)
+                cache.set_tree(None)
+            else:
+                cache.pos = start + 1 + n_ok
+        else:
+            choice = out[:len(guess) + 1].argmax(-1).tolist()
+            n_ok = next((i for i, (c, g) in enumerate(zip(choice, guess)) if c != g), len(guess))
+            stands = guess[:n_ok] + [choice[n_ok]]
+            cache.pos = start + 1 + n_ok          # keep the pending token and the accepted guesses
         stats["forwards"] += 1
         stats["drafted"] += len(guess)
         stats["accepted"] += n_ok
-        cache.pos = start + 1 + n_ok          # keep the pending token and the accepted guesses
-        for t in (guess[:n_ok] + [choice[n_ok]])[:max_new_tokens - len(new)]:
+        for t in stands[:max_new_tokens - len(new)]:
             ids.append(t)
             new.append(t)
     res = GenerationResult(list(prompt_ids), new, "max_new_tokens", {"speculative": stats})

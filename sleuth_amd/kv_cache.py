@@ -14,6 +14,9 @@ decoder, the benchmark); it speaks the same protocol and adds what the kernels c
              (pos_t + 0 .. tokens_per_step-1) is computed into a fixed buffer, so a
              captured graph recomputes it on every replay.
 
+  trees  set_tree makes the next passes' tokens the nodes of drafted trees: a pass stores them behind the rows,
+             whose lengths stay until keep says which nodes stand.
+
 Protocol members: k, v, pos, max_len, update, advance, reset, nbytes, token_history,
 for_model; static, pos_t, length, tokens_per_step, positions, attn_mask, new_step.
 """
@@ -21,6 +24,22 @@ for_model; static, pos_t, length, tokens_per_step, positions, attn_mask, new_ste
 from __future__ import annotations
 
 import torch
+
+from .tree import TokenTree
+
+
+def _set_tree(cache, parents) -> None:
+    """KVCache.set_tree and PagedKVCache.set_tree: the buffers of trees of one size are kept (recorded graphs read them)."""
+    if parents is None:
+        cache.tree = None
+        return
+    rows = TokenTree._rows(parents, cache.batch)
+    tree = cache._trees.get(len(rows[0]))
+    if tree is None:
+        tree = cache._trees[len(rows[0])] = TokenTree(rows, cache.batch, cache.device)
+    else:
+        tree.set(rows)
+    cache.tree = tree
 
 
 class KVCache:
@@ -42,6 +61,8 @@ class KVCache:
         self._rows = [0] * batch
         self._rows_dev: torch.Tensor | None = None   # device mirror, made when rows differ
         self._history: torch.Tensor | None = None
+        self.tree: TokenTree | None = None
+        self._trees: dict[int, TokenTree] = {}
         # static (graph) mode
         self.static = False
         self.length = max_len
@@ -123,16 +144,43 @@ class KVCache:
 
     def advance(self, n: int) -> None:
         """All layers have stored n more tokens per row. In static mode the caller owns
-        the position (pos and pos_t), so nothing moves here."""
-        if self.static:
+        the position (pos and pos_t), so nothing moves here; nor with a tree, whose nodes stand once keep says so."""
+        if self.static or self.tree is not None:
             return
         self._rows = [r + n for r in self._rows]
         if self._rows_dev is not None:
             self._rows_dev.add_(n)
 
+    # ------------------------------------------------------------------ trees
+    def set_tree(self, parents) -> None:
+        """The next passes' T tokens of each row are the nodes of a tree: parents [T] or [B, T], node 0 the row's last token,
+        node t drafted behind node parents[t] < t (anything else: behind the row's tokens alone). None: tokens in a row again."""
+        _set_tree(self, parents)
+
+    def keep(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
+        """Of the last pass's nodes, path[b, :count[b]] stand (tree.verify): their keys and values close up behind the row, which
+        grows by count[b]. Returns the counts."""
+        n = [int(x) for x in count.tolist()]
+        if len(n) != self.batch or min(n) < 0 or max(n) > path.shape[1] or any(r + x > self.max_len for r, x in zip(self._rows, n)):
+            raise ValueError(f"keep needs paths and counts of {self.batch} rows that fit the cache")
+        if self.k[0].is_cuda:
+            from . import ops
+
+            where = dict(row_pos=self.seq_lens) if self.ragged else dict(pos=self.pos)
+            ops.kv_compact(self.k, self.v, path, count, **where)
+        else:
+            for b, (r, x) in enumerate(zip(self._rows, n)):
+                at = r + path[b, :x].long()
+                for c in (*self.k, *self.v):
+                    c[b, :, r:r + x] = c[b, :, at]
+        self._rows = [r + x for r, x in zip(self._rows, n)]
+        self._rows_dev = None
+        return n
+
     def reset(self) -> None:
         self.pos = 0
         self.static = False
+        self.tree = None
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()

@@ -141,7 +141,13 @@ class Transformer(nn.Module):
 
     def rope_rows(self, offset, T, cache=None):
         """cos/sin per layer kind for this pass: index_select(pos) in static mode, a slice
-        at offset otherwise, per-row rows [B, T, hd] for a ragged cache."""
+        at offset otherwise, per-row rows [B, T, hd] for a ragged cache; with a drafted tree those of its nodes' depths."""
+        tree = getattr(cache, "tree", None)
+        if tree is not None:
+            base = cache.pos_t if getattr(cache, "static", False) else cache.seq_lens.long()[:, None]
+            idx = (base + tree.depth).clamp(max=self.cfg.max_seq_len - 1)   # (the padding of a padded batch)
+            return {k: (getattr(self, f"rope_cos_{k}")[idx], getattr(self, f"rope_sin_{k}")[idx])
+                    for k in self._rope_kinds()}
         if getattr(cache, "static", False):
             pos = cache.positions
             return {k: (getattr(self, f"rope_cos_{k}").index_select(0, pos),
@@ -161,6 +167,9 @@ class Transformer(nn.Module):
         longest = cache.top(T) if getattr(cache, "paged", False) else offset + T
         if longest > self.cfg.max_seq_len:
             raise ValueError(f"sequence length {longest} exceeds max_seq_len {self.cfg.max_seq_len}")
+        tree = getattr(cache, "tree", None)
+        if tree is not None and (tree.batch, tree.T) != (B, T):
+            raise ValueError(f"the cache's trees have {(tree.batch, tree.T)} nodes, the pass {(B, T)}")
         if getattr(cache, "static", False):
             cache.new_step()
         # (fp32 rows of 16-bit tables, made once per pass: a model cast to bf16 holds its tables in bf16,

@@ -4,18 +4,22 @@ The reference's caches (sleuth/forge/infer/kv_cache.py:25-138) hold max_len posi
 K and V are pools [n_pages, K, page_size, hd]; position s of row b is slot s % page_size of page
 page_table[b, s // page_size], the same page of every layer's pools. Pages are handed out as rows grow (reserve), and
 come back when a row ends (release) or when no layer can see them any more (release_unseen: every layer slides, and
-keeps its first tokens). The table and the lengths live on the device in fixed buffers, so a recorded graph of the
+keeps its first tokens). A row may fork (fork): the new one shares its pages, and whoever writes to a shared page first gets a
+copy of its own (reserve). The table and the lengths live on the device in fixed buffers, so a recorded graph of the
 operators or of the layers sees them change. What is the host's to say stays outside of it: reserve before a replay,
 advance after it (both refuse to be recorded).
 
 It speaks the cache protocol of the package's callers (pos, max_len, advance, seq_lens, seq_lens_host, update; `ragged`
 is always true, `static` never; pos is read only, since rows differ: rewind takes each row's length) and adds `paged`,
-page_table, new_lens, reserve, top, bound and row, which the attention module uses (ops.kv_append_paged, ops.attn_paged).
+page_table, new_lens, reserve, top, bound, row, set_tree and keep (KVCache's), which the attention module uses (ops.kv_append_paged, ops.attn_paged).
 """
 
 from __future__ import annotations
 
 import torch
+
+from .kv_cache import _set_tree
+from .tree import TokenTree
 
 
 class OutOfPages(ValueError):
@@ -55,6 +59,9 @@ class PagedKVCache:
         self._new_buf = torch.zeros(batch, dtype=torch.int32, device=dev)
         self._table = [[-1] * per_row for _ in range(batch)]
         self._free = list(range(n - 1, -1, -1))
+        self._users = [0] * n         # rows that hold a page
+        self.tree: TokenTree | None = None
+        self._trees: dict[int, TokenTree] = {}
         self._rows = [0] * batch
         self._least = [0] * batch     # rows cannot be rewound below this: pages that it would see were given back
         self._new: list[int] | None = None
@@ -117,23 +124,67 @@ class PagedKVCache:
 
     # ------------------------------------------------------------------ pages
     def reserve(self, T: int) -> None:
-        """Pages for the next pass's real tokens (every layer of a pass may call it: the first one acts). Raises
-        ValueError where a row would pass max_len, OutOfPages where the pool has no page left; nothing is handed out then."""
+        """Pages for the next pass's real tokens (every layer of a pass may call it: the first one acts); one that other rows
+        hold too is copied first, in every layer. Raises ValueError where a row would pass max_len, OutOfPages where the pool
+        has no page left; nothing is handed out then."""
         P = self.page_size
         need = []
+        users = {}
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
             if r + n > self.max_len:
                 raise ValueError(f"KV cache full ({self.max_len} tokens)")
             if n:
-                need += [(b, j) for j in range(r // P, (r + n - 1) // P + 1) if self._table[b][j] < 0]
+                for j in range(r // P, (r + n - 1) // P + 1):
+                    page = self._table[b][j]
+                    if page < 0:
+                        need.append((b, j))
+                    elif self._users[page] > 1:   # (the last of the rows that write to it keeps it)
+                        left = users.get(page, self._users[page])
+                        if left > 1:
+                            need.append((b, j))
+                            users[page] = left - 1
         if not need:
             return
         if self._recording():
             raise RuntimeError("reserve a paged cache's pages before recording a graph")
         if len(need) > len(self._free):
             raise OutOfPages(f"KV cache out of pages ({len(need)} needed, {len(self._free)} of {self.n_pages} free)")
+        copies = []
         for b, j in need:
-            self._table[b][j] = self._free.pop()
+            old, page = self._table[b][j], self._free.pop()
+            self._table[b][j] = page
+            self._users[page] = 1
+            if old >= 0:
+                self._users[old] -= 1
+                copies.append((old, page))
+        self._copy(copies)
+        self._put_table()
+
+    def _copy(self, pages: list[tuple[int, int]]) -> None:
+        if not pages:
+            return
+        src, dst = [a for a, _ in pages], [b for _, b in pages]
+        if self.device.type == "cuda":
+            from . import ops
+
+            ops.copy_pages(self.k, self.v, src, dst)
+        else:
+            for pool in (*self.k, *self.v):
+                pool[dst] = pool[src]
+
+    def fork(self, row: int, into: int) -> None:
+        """Row `into`, which must be empty, goes on from where `row` stands: it shares its pages (no copy until either writes
+        to one)."""
+        if row == into or self._rows[into] or any(page >= 0 for page in self._table[into]):
+            raise ValueError(f"row {into} must be empty, and another than {row}")
+        if self._recording():
+            raise RuntimeError("fork a paged cache's rows outside of a recorded graph")
+        self._table[into] = list(self._table[row])
+        for page in self._table[into]:
+            if page >= 0:
+                self._users[page] += 1
+        self._rows[into], self._least[into] = self._rows[row], self._least[row]
+        self.seq_lens[into] = self._rows[row]
         self._put_table()
 
     def release(self, row: int) -> None:
@@ -172,7 +223,10 @@ class PagedKVCache:
 
     def _give_back(self, at: list[tuple[int, int]]) -> None:
         for b, j in at:
-            self._free.append(self._table[b][j])
+            page = self._table[b][j]
+            self._users[page] -= 1
+            if not self._users[page]:
+                self._free.append(page)
             self._table[b][j] = -1
         if at:
             self._put_table()
@@ -212,6 +266,8 @@ class PagedKVCache:
 
     def advance(self, n: int) -> None:
         """All layers have stored this pass's tokens."""
+        if self.tree is not None:
+            return   # (its nodes stand once keep says so)
         if self._recording():
             raise RuntimeError("advance a paged cache outside of a recorded graph: its lengths are the host's too")
         new = self.new_tokens(n)
@@ -221,10 +277,39 @@ class PagedKVCache:
         else:
             self.seq_lens.add_(self._new_buf.clamp(max=n))
 
+    # ------------------------------------------------------------------ trees
+    def set_tree(self, parents) -> None:
+        """KVCache.set_tree: the next passes' tokens are the nodes of drafted trees (rows with fewer: set_new)."""
+        _set_tree(self, parents)
+
+    def keep(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
+        """KVCache.keep: path[b, :count[b]] of the last pass's nodes stand and close up; pages behind the rows' new ends come
+        back. Returns the counts."""
+        n = [int(x) for x in count.tolist()]
+        if len(n) != self.batch or min(n) < 0 or max(n) > path.shape[1] or any(r + x > self.max_len for r, x in zip(self._rows, n)):
+            raise ValueError(f"keep needs paths and counts of {self.batch} rows that fit the cache")
+        if self.device.type == "cuda":
+            from . import ops
+
+            ops.kv_compact_paged(self.k, self.v, self.page_table, self.seq_lens, path, count)
+        else:
+            P = self.page_size
+            for b, (r, x) in enumerate(zip(self._rows, n)):
+                of, to = r + path[b, :x].long(), r + torch.arange(x)
+                pages = self.page_table[b].long()
+                for pool in (*self.k, *self.v):
+                    pool[pages[to // P], :, to % P] = pool[pages[of // P], :, of % P]
+        self._rows = [r + x for r, x in zip(self._rows, n)]
+        self.seq_lens.add_(torch.tensor(n, dtype=torch.int32).to(self.device))
+        self._give_back([(b, j) for b, r in enumerate(self._rows) for j in range(-(-r // self.page_size), len(self._table[b]))
+                         if self._table[b][j] >= 0])
+        return n
+
     def reset(self) -> None:
         for b in range(self.batch):
             self.release(b)
         self._new = None
+        self.tree = None
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()
