@@ -816,21 +816,27 @@ struct Layers {
     k.reserve(n);
     v.reserve(n);
     for (Py_ssize_t i = 0; i < 2 * n; ++i) {
-      Tensor t;
-      if (!take(PySequence_Fast_GET_ITEM(i < n ? ks : vs, i % n), t)) return false;
+      PyObject* o = PySequence_Fast_GET_ITEM(i < n ? ks : vs, i % n);
       if (i == 0) {
-        first = t;
-        if (t.dim() != 4 || dtype_of(t) < 0 || t.size(3) * t.element_size() % 16 || !strides16(t, s) ||
-            c10::hip::current_device() != t.device().index())
+        if (!take(o, first) || first.dim() != 4 || dtype_of(first) < 0 || first.size(3) * first.element_size() % 16 ||
+            !strides16(first, s) || c10::hip::current_device() != first.device().index())
           return false;
         for (int d = 0; d < 4; ++d)
-          if (t.stride(d) == 0 && t.size(d) > 1) return false;
-      } else {
-        if (t.sizes() != first.sizes() || t.strides() != first.strides() || t.scalar_type() != first.scalar_type() ||
-            t.device() != first.device() || (uintptr_t)t.const_data_ptr() % 16)
-          return false;
+          if (first.stride(d) == 0 && first.size(d) > 1) return false;
+        k.push_back(first.const_data_ptr());
+        continue;
       }
-      (i < n ? k : v).push_back(t.const_data_ptr());
+      // (the others are plain tensors if they are what the first is; of 56 the full look takes longer than the launch)
+      if (!THPVariable_CheckExact(o)) return false;
+      const Tensor& t = THPVariable_Unpack(o);
+      const c10::TensorImpl *x = t.unsafeGetTensorImpl(), *y = first.unsafeGetTensorImpl();
+      if (!t.defined() || x->key_set() != y->key_set() || x->is_python_dispatch() || !x->has_storage() ||
+          x->dtype() != y->dtype() || x->device() != y->device() || x->sizes() != y->sizes() || x->strides() != y->strides() ||
+          t._fw_grad(0).defined())
+        return false;
+      const void* at = t.const_data_ptr();
+      if ((uintptr_t)at % 16) return false;
+      (i < n ? k : v).push_back(at);
     }
     return true;
   }
