@@ -9,7 +9,8 @@ namespace forge {
 
 // ---------------------------------------------------------------- who sees whom
 // vis(t) = {t} and vis(parent of t). Doubling: after k rounds a node has its 2^k nearest ancestors, itself among them, and
-// knows the one after those, whose set it takes next; a chain of 1,024 takes ten rounds, a usual tree three.
+// knows the one after those, whose set it takes next; a chain of 1,024 takes ten rounds, a usual tree three. One block a
+// row. Bound by its start and the rounds' barriers: 1.9 us for a row of 12 nodes, 5.2 for 64 rows of 256.
 template <int W> __global__ __launch_bounds__(1024) void tree_mask_kernel(const int32_t* parents, int64_t spb,
                                                                         const int32_t* new_lens, int T, uint64_t* mask,
                                                                         int32_t* depth) {
@@ -89,7 +90,9 @@ struct MoveParams {
 // The accepted branch closes up: slot base + i takes what slot base + path[i] holds, for i below the row's count. Entries
 // with path[i] < i or beyond the cache move nothing; all others lie at or behind their place, so that in rising order,
 // eight at a time, each is read before anything is written to it. A thread owns one 16-byte chunk of one head of one
-// layer's K or V, for the whole path.
+// layer's K or V, for the whole path. Latency, position, entry, pages, chunk: 3.4 us for one row of 28 layers, 8.3 for 64
+// rows' 19 MB over pages (12.4 with all sixteen pages of a batch looked up at once, 10.7 by scalar loads: most entries of
+// a path are not there).
 __global__ __launch_bounds__(256) void kv_compact_kernel(MoveParams p) {
   const int b = blockIdx.z, unit = blockIdx.x * 256 + threadIdx.x;
   const int head = unit / p.chunks, chunk = unit - head * p.chunks;
@@ -128,7 +131,8 @@ __global__ __launch_bounds__(256) void kv_compact_kernel(MoveParams p) {
   }
 }
 
-// Page dst[i] takes what page src[i] holds. A block takes 256 chunks x 4 of one page of one layer's K or V.
+// Page dst[i] takes what page src[i] holds. A block takes 256 chunks x 4 of one page of one layer's K or V. As fast as a
+// copy: 64 pages of 128 KB in 28 layers 178 us, 5.3 TB/s (a 1 GiB copy 5.15).
 constexpr int kCopyPer = 4;
 __global__ __launch_bounds__(256) void copy_pages_kernel(MoveParams p) {
   const int i = blockIdx.y;

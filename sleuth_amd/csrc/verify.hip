@@ -13,9 +13,14 @@
 // 131,072 would come out one token off.
 //
 // Every node's logits are read once, whichever the walk needs, by one launch over chunks of all nodes (each chunk's
-// maximum and sum); a block per row then walks, and draws within the one chunk that its number falls into. What a
-// rejected child's probabilities leave has to be summed over a whole row of the vocabulary: a launch more, whose blocks
-// end at once for the rows that need none, and whose last one draws.
+// maximum and sum); a block per row then walks, and draws within the one chunk that its number falls into. Waiting for the
+// walk to know which nodes it needs would read less and take a launch a level. What a rejected child's probabilities leave
+// has to be summed over a whole row of the vocabulary: a launch more, whose blocks end at once for the rows that need
+// none, and whose last one draws. Calls of few chunks walk in the scan's own launch.
+//
+// us a call (and each launch): one greedy chain of 5 over 32,768 tokens 7.9; 32 sampled chains of 6 over 131,072 in bf16 with
+// the drafter's probabilities 44 (scan 22: VALU, 0.86 of the SIMDs' cycles; walk 11 and rest 15: latency, a chain of loads and
+// cross-lane sums); 8 trees of up to 40 over 100,003 in fp32 30 (scan 19: 3.5 TB/s, VALU 0.67; walk 12).
 #include <limits.h>
 
 #include "common.h"
@@ -26,6 +31,7 @@ namespace forge {
 constexpr int kVerifyChunk = 4096;  // elements of a row that a block takes
 constexpr int kScanThreads = 256, kWalkThreads = 512;
 constexpr int kVerifyNodes = FORGE_TREE_MAX_TOKENS;
+static_assert(2 * kWalkThreads >= kVerifyNodes, "a thread of the walk takes two nodes");
 
 struct VerifyParams {
   const void* logits;
@@ -433,7 +439,7 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
 
   // Each drafted token, its parent, and the logit and probability it is judged by; the first chunks' numbers are on their
   // way meanwhile.
-  constexpr int MINE = 2;
+  constexpr int MINE = 2;   // (nodes a thread: the launch sees to it)
   struct Drafted {
     int64_t token;
     int up;
@@ -544,14 +550,6 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
 #pragma unroll
   for (int y = 0; y < MINE; ++y)
     if (tid + y * THREADS < n) weigh(tid + y * THREADS, logit[y], prob[y]);
-  if (n > MINE * THREADS) {   // (a large tree's others)
-    for (int t = MINE * THREADS + tid; t < n; t += THREADS) judged(t, drafted(t), logit[0], prob[0]);
-    __syncthreads();
-    for (int t = MINE * THREADS + tid; t < n; t += THREADS) {
-      judged(t, drafted(t), logit[0], prob[0]);
-      weigh(t, logit[0], prob[0]);
-    }
-  }
   __syncthreads();
 
   // Who would be accepted if the walk came to its parent. With the drafter's probabilities that is known for first
@@ -869,7 +867,8 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
   p.B = B; p.T = T; p.V = V; p.C = verify_chunks(V);
   p.out = out; p.path = path; p.count = count;
   p.parts = reinterpret_cast<Part*>(at + ws.parts);
-  if ((ws_flags & FORGE_WS_ZEROED) && (int64_t)p.C * T * B <= 2 * device_cus()) p.counters = reinterpret_cast<unsigned*>(at);
+  if ((ws_flags & FORGE_WS_ZEROED) && T <= 2 * kScanThreads && (int64_t)p.C * T * B <= 2 * device_cus())
+    p.counters = reinterpret_cast<unsigned*>(at);
   p.state = reinterpret_cast<State*>(at + ws.state);
   p.rest = reinterpret_cast<double*>(at + ws.rest);
   const hipStream_t s = (hipStream_t)stream;

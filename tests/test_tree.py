@@ -554,6 +554,35 @@ def test_verify_over_a_large_vocabulary(probs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T, B, V, shape", [(1024, 1, 40, "tree"), (600, 2, 9, "chain"), (513, 1, 5000, "star"), (256, 2, 30, "forest")])
+@pytest.mark.parametrize("mode", ["greedy", "sampled", "probs"])
+def test_verify_large_trees(T, B, V, shape, mode):
+    parents, logits, q, tokens, u = _verify_inputs(B, T, V, SF, shape, mode == "probs", seed=T, spread=1.0)
+    heat = 0.0 if mode == "greedy" else 1.3
+    got = ops.verify_drafts(logits.cuda(), tokens.cuda(), parents=i32(parents), uniform=None if mode == "greedy" else u.cuda(),
+                            temperature=heat, draft_probs=None if q is None else q.cuda())
+    _same(got, _verify_want(logits, tokens, parents, u, [heat] * B, q, [T] * B))
+
+
+@pytest.mark.gpu
+def test_verify_on_the_streams_workspace():
+    """Calls of one launch and of two, of other operators on the same workspace between them, and again: its counters are zero
+    each time."""
+    small = _verify_inputs(2, 6, 9000, BF, "tree", True, seed=8)
+    large = _verify_inputs(40, 6, 20011, BF, "tree", False, seed=9)
+    case = (BF, 16, 8, 128, 16, [0, 400], 12, "tree", None, 0, 0)
+    cache, parents, qs, real = _tree_inputs(*case)
+    mask, _ = ops.tree_mask(i32(parents))
+    first = _call(cache, 16, qs, mask, None, [0, 400], 0.1)
+    for _ in range(3):
+        for p, logits, q, tokens, u in (small, large):
+            got = ops.verify_drafts(logits.cuda(), tokens.cuda(), parents=i32(p), uniform=u.cuda(), temperature=1.0,
+                                    draft_probs=None if q is None else q.cuda())
+            _same(got, _verify_want(logits, tokens, p, u, [1.0] * len(p), q, [6] * len(p)))
+        assert torch.equal(_call(cache, 16, qs, mask, None, [0, 400], 0.1), first)
+
+
+@pytest.mark.gpu
 def test_verify_forms():
     """A chain by default, one tree for all, a temperature for each row, short rows, probabilities of 16 bits and of T - 1 nodes,
     strided logits."""
