@@ -31,7 +31,7 @@ import torch
 
 from .kv_cache import KVCache
 from .paged_cache import OutOfPages, PagedKVCache
-from .tree import Drafts, verify
+from .tree import Drafts, TokenTree, verify
 
 
 @dataclass
@@ -121,8 +121,10 @@ class GraphDecoder:
         this decoder then records (cache.keep says which nodes stand)."""
         if self._graph is not None and (parents is not None) != self._trees:
             raise ValueError("this decoder was recorded for " + ("trees" if self._trees else "chains"))
-        self._trees = parents is not None
+        if parents is not None and len(TokenTree._rows(parents, 1)[0]) != self.T:
+            raise ValueError(f"this decoder takes trees of {self.T} nodes")   # (its graph reads their buffers)
         self.cache.set_tree(parents)
+        self._trees = parents is not None
         return self._launch(tokens)
 
 

@@ -323,6 +323,23 @@ def test_fork_books():
     assert cache.free_pages == 3
 
 
+@pytest.mark.gpu
+@torch.no_grad()
+def test_a_recorded_tree_keeps_its_size():
+    model = make("cuda")
+    dec = GraphDecoder(model, 64, torch.float32, 3)
+    model(torch.tensor([REPEATING], device="cuda"), cache=dec.cache)
+    tokens = torch.tensor([3, 9, 4], device="cuda")
+    for parents in ([-1, 0], [-1, 0, 0, 1]):
+        with pytest.raises(ValueError, match="3 nodes"):
+            dec.verify(tokens, parents)
+    want = dec.verify(tokens, [-1, 0, 0]).clone()
+    for parents in ([-1, 0], torch.tensor([-1, 0, 0, 1])):
+        with pytest.raises(ValueError, match="3 nodes"):
+            dec.verify(tokens, parents)
+    assert torch.equal(dec.verify(tokens, [-1, 0, 0]), want)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @torch.no_grad()
 def test_trees_over_forked_rows(device):
