@@ -288,12 +288,15 @@ class PagedKVCache:
         n = [int(x) for x in count.tolist()]
         if len(n) != self.batch or min(n) < 0 or max(n) > path.shape[1] or any(r + x > self.max_len for r, x in zip(self._rows, n)):
             raise ValueError(f"keep needs paths and counts of {self.batch} rows that fit the cache")
+        P = self.page_size
+        into = [self._table[b][j] for b, (r, x) in enumerate(zip(self._rows, n)) if x for j in range(r // P, (r + x - 1) // P + 1)]
+        if -1 in into or len(set(into)) < len(into):
+            raise ValueError("keep is for nodes that the last pass has stored, in pages of their row")
         if self.device.type == "cuda":
             from . import ops
 
             ops.kv_compact_paged(self.k, self.v, self.page_table, self.seq_lens, path, count)
         else:
-            P = self.page_size
             for b, (r, x) in enumerate(zip(self._rows, n)):
                 of, to = r + path[b, :x].long(), r + torch.arange(x)
                 pages = self.page_table[b].long()

@@ -323,6 +323,26 @@ def test_fork_books():
     assert cache.free_pages == 3
 
 
+def test_keep_takes_what_a_pass_has_stored():
+    cache = PagedKVCache([(1, 32)], 2, 64, "cpu", torch.float32, 16)
+    cache.set_new([14, 0])
+    cache.reserve(14)
+    cache.advance(14)
+    cache.set_new([5, 0])
+    cache.set_tree([-1, 0, 0, 2, 1])
+    cache.reserve(5)
+    cache.advance(5)
+    cache.fork(0, 1)      # (shares the nodes' pages too)
+    path = torch.tensor([[0, 2, 3, -1, -1]] * 2, dtype=torch.int32)
+    for counts in ([3, 3], [3, 2]):
+        with pytest.raises(ValueError, match="stored"):
+            cache.keep(path, torch.tensor(counts))
+    assert cache.keep(path, torch.tensor([3, 0])) == [3, 0] and cache.seq_lens_host == [17, 14]
+    cache.release(1)
+    with pytest.raises(ValueError, match="stored"):
+        cache.keep(path, torch.tensor([0, 1]))
+
+
 @pytest.mark.gpu
 @torch.no_grad()
 def test_a_recorded_tree_keeps_its_size():
