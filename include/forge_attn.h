@@ -433,7 +433,7 @@ int forge_verify_drafts(int dtype, int B, int T, int V, const void* logits, int6
  * forge_kv_compact: an accepted branch closes up. Slot base + i of row b takes the key and value of slot base +
  * path[b][i], for i < counts[b]; path as forge_verify_drafts leaves it (rising; an entry below its place i, or beyond the
  * cache, moves nothing, nor do positions without a page). Cache arguments as in forge_attn_tree. Rows must not share the
- * pages that are written.
+ * pages that are written, no two caches share memory (one that is named twice is refused).
  * forge_copy_pages: page dst[i] takes what page src[i] holds, i < n, in K and V of every layer (pools as in
  * forge_attn_paged). Numbers outside the pool copy nothing. No page may be named in dst twice, or in both src and dst of
  * different i.

@@ -2,6 +2,9 @@
 // closing up in the cache (forge_kv_compact), copies of whole pages (forge_copy_pages).
 #include <limits.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "common.h"
 #include "forge_internal.h"
 
@@ -172,6 +175,13 @@ static const char* move_setup(MoveParams& p, int esize, int layers, const void* 
   p.K = K; p.chunks = D * esize / 16;
   return nullptr;
 }
+// A cache named twice would be moved by two blocks at once, one of which may read what the other has moved already.
+static bool named_twice(int layers, const void* const* k, const void* const* v) {
+  std::vector<const void*> all(k, k + layers);
+  all.insert(all.end(), v, v + layers);
+  if (!std::is_sorted(all.begin(), all.end())) std::sort(all.begin(), all.end());
+  return std::adjacent_find(all.begin(), all.end()) != all.end();
+}
 static int take_layers(MoveParams& p, int l0, int layers, const void* const* k, const void* const* v) {
   const int n = layers - l0 < kMoveLayers ? layers - l0 : kMoveLayers;
   for (int l = 0; l < n; ++l) {
@@ -226,6 +236,11 @@ extern "C" int forge_kv_compact(int esize, int layers, int B, int K, int D, cons
   if (!path || !counts || s_path < 0) return set_error("null path or counts");
   const int64_t limit = page_table ? max_pages * page_size : page_size;
   if (limit > INT_MAX) return set_error("rows are limited to 2^31 - 1 keys");
+  try {
+    if (named_twice(layers, k, v)) return set_error("a cache is named twice: its keys would move twice");
+  } catch (...) {
+    return set_error("no memory");
+  }
   p.limit = (int)limit;
   p.table = page_table; p.spt = s_table; p.npages = n_pages;
   p.page_shift = page_table ? __builtin_ctz((unsigned)page_size) : 31;

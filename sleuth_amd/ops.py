@@ -1035,6 +1035,9 @@ def _pointers(ptrs: list[int]):
 
 
 def _compact(groups, dev, B, where, path, counts, s_path, T) -> None:
+    named = [p for _, kp, vp in groups for p in (*kp, *vp)]
+    if len(set(named)) < len(named):
+        raise ValueError("a cache is named twice: its keys would move twice")
     with _guard(dev):
         for k, kp, vp in groups:
             st = lib().forge_kv_compact(k.element_size(), len(kp), B, k.shape[1], k.shape[3], _pointers(kp), _pointers(vp),
@@ -1054,8 +1057,8 @@ def kv_compact(k_caches, v_caches, path: torch.Tensor, count: torch.Tensor, *, p
                pos_dev: torch.Tensor | None = None, row_pos: torch.Tensor | None = None) -> None:
     """The accepted branch of a verified tree closes up, in every layer: slot base_b + i of the contiguous caches
     [B,K,max_len,D] (lists of the layers' tensors) takes the key and value of slot base_b + path[b, i], for i < count[b]
-    (verify_drafts' path and count). What an entry below its own place i, or beyond the cache, names moves nothing. One launch
-    for all layers of a shape."""
+    (verify_drafts' path and count). What an entry below its own place i, or beyond the cache, names moves nothing. No two of
+    the tensors may share memory. One launch for all layers of a shape."""
     st = host().kv_compact(k_caches, v_caches, path, count, pos, pos_dev, row_pos)
     if st is not None:
         return check(st, "forge_kv_compact")

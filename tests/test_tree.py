@@ -132,6 +132,12 @@ def test_kv_compact_refusals(bad, why):
     _refused(_compact_call(**bad), why)
 
 
+@pytest.mark.parametrize("k, v", [([1, 2, 3], [4, 5, 1]), ([2, 1, 2], [4, 5, 6]), ([1], [1]), ([3, 2, 1], [6, 4, 4])])
+def test_kv_compact_refuses_a_cache_named_twice(k, v):
+    k, v = (_pointers(*(FAKE + 4096 * i for i in x)) for x in (k, v))
+    _refused(_compact_call(layers=len(k), k=k, v=v), "twice")
+
+
 def test_moves_of_nothing():
     assert _compact_call(layers=0) == _compact_call(B=0) == _compact_call(T=0, path=None) == 0
     f = _lib.lib().forge_copy_pages
@@ -791,6 +797,21 @@ def test_kv_compact_positions_and_arguments():
         a.update(bad)
         with pytest.raises(ValueError):
             ops.kv_compact(**a)
+
+
+@pytest.mark.gpu
+def test_a_cache_named_twice_stays_as_it_is():
+    x, y = (torch.randn(2, 4, 48, 32, generator=gen(i)).cuda() for i in range(2))
+    path, count = i32([[0, 2, 5], [0, 1, 4]]), i32([3, 3])
+    table = i32([[0], [1]])
+    pool = [t[:, :, :32].contiguous() for t in (x, y)]
+    before = [t.clone() for t in (x, y, *pool)]
+    for ks, vs in (([x], [x]), ([x, x], [y, y.clone()]), ([x, y], [y, x]), ([x, x[:, :2]], [y, y[:, :2]])):
+        with pytest.raises(ValueError, match="twice"):
+            ops.kv_compact(ks, vs, path, count, pos=10)
+    with pytest.raises(ValueError, match="twice"):
+        ops.kv_compact_paged([pool[0]] * 2, [pool[1]] * 2, table, i32([10, 10]), path, count)
+    assert all(torch.equal(a, b) for a, b in zip(before, (x, y, *pool)))
 
 
 @pytest.mark.gpu
