@@ -1117,6 +1117,8 @@ def copy_pages(k_pools, v_pools, src, dst) -> None:
             raise ValueError(f"src and dst must be int32 [n] tensors on {dev}")
         src, dst = src.contiguous(), dst.contiguous()
     else:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("lists of pages are copied to the GPU: a recording takes tensors")
         src, dst = [int(x) for x in src], [int(x) for x in dst]
         if len(src) != len(dst) or any(not 0 <= x < n_pages for x in src + dst):
             raise ValueError(f"src and dst must be page numbers of a pool of {n_pages}, as many of one as of the other")

@@ -815,6 +815,18 @@ def test_a_cache_named_twice_stays_as_it_is():
 
 
 @pytest.mark.gpu
+def test_page_lists_are_not_recorded():
+    kp, vp = torch.zeros(4, 2, 16, 32, device="cuda"), torch.ones(4, 2, 16, 32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="recording"):
+            ops.copy_pages([kp], [vp], [0], [1])
+        out = kp + 1
+    g.replay()
+    assert torch.equal(out, kp + 1)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype, shapes, page, n", [(BF, [(8, 128)] * 3, 16, 1), (SF, [(4, 32)], 32, 7), (HF, [(2, 256), (4, 64)], 64, 3),
                                                     (BF, [(1, 512)] * 70, 16, 2), (BF, [(3, 8)], 128, 5)])
 def test_copy_pages(dtype, shapes, page, n):
