@@ -3,6 +3,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <functional>
 #include <vector>
 
 #include "common.h"
@@ -177,9 +178,23 @@ static const char* move_setup(MoveParams& p, int esize, int layers, const void* 
 }
 // A cache named twice would be moved by two blocks at once, one of which may read what the other has moved already.
 static bool named_twice(int layers, const void* const* k, const void* const* v) {
+  const std::less<const void*> before;
+  const auto rises = [&](const void* const* x) {
+    for (int l = 1; l < layers; ++l)
+      if (!before(x[l - 1], x[l])) return false;
+    return true;
+  };
+  if (rises(k) && rises(v)) {   // (as allocated one after the other: no memory of its own needed)
+    for (int i = 0, j = 0; i < layers && j < layers;) {
+      if (k[i] == v[j]) return true;
+      if (before(k[i], v[j])) ++i;
+      else ++j;
+    }
+    return false;
+  }
   std::vector<const void*> all(k, k + layers);
   all.insert(all.end(), v, v + layers);
-  if (!std::is_sorted(all.begin(), all.end())) std::sort(all.begin(), all.end());
+  std::sort(all.begin(), all.end(), before);
   return std::adjacent_find(all.begin(), all.end()) != all.end();
 }
 static int take_layers(MoveParams& p, int l0, int layers, const void* const* k, const void* const* v) {
