@@ -414,7 +414,7 @@ int forge_attn_tree(int dtype, int B, int T, int H, int K, int D, const void* q,
  * Out: count[b] how many nodes stand, node 0 included (0 for a row without nodes); path [B, T] int32 those nodes in
  * order; out [B, T] int64 the row's count[b] new tokens (the accepted ones', then the drawn one); -1 behind them.
  * All sums in 64 bits. workspace: forge_verify_drafts_workspace_bytes(...) bytes, 256-byte aligned, separate for calls
- * that may overlap. ws_flags as in forge_attn_paged (small calls then take one launch less). V at most 2^22 - 8.
+ * that may overlap. ws_flags as in forge_attn_paged (small greedy calls then take one launch less). V at most 2^22 - 8.
  */
 size_t forge_verify_drafts_workspace_bytes(int B, int T, int V, int draft_probs);
 int forge_verify_drafts(int dtype, int B, int T, int V, const void* logits, int64_t s_logits_b,

@@ -16,7 +16,7 @@
 // maximum and sum); a block per row then walks, and draws within the one chunk that its number falls into. Waiting for the
 // walk to know which nodes it needs would read less and take a launch a level. What a rejected child's probabilities leave
 // has to be summed over a whole row of the vocabulary: a launch more, whose blocks end at once for the rows that need
-// none, and whose last one draws. Calls of few chunks walk in the scan's own launch.
+// none, and whose last one draws. Greedy calls of few chunks walk in the scan's own launch.
 //
 // us a call (and each launch): one greedy chain of 5 over 32,768 tokens 7.9; 32 sampled chains of 6 over 131,072 in bf16 with
 // the drafter's probabilities 44 (scan 22: VALU, 0.86 of the SIMDs' cycles; walk 11 and rest 15: latency, a chain of loads and
@@ -711,8 +711,7 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
   }
 }
 
-// The scan, a block a chunk. FUSED: the block that ends a row's scan walks it too, where blocks are few and a second launch
-// would cost more than the walk's registers take from the scan's occupancy.
+// The scan, a block a chunk. FUSED (greedy calls of few chunks): the block that ends a row's scan walks it too.
 template <typename T, typename Q, bool FUSED>
 __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -805,7 +804,7 @@ template <typename T, typename Q> static int launch_verify(const VerifyParams& p
   const size_t lds = WalkLds::bytes(p.T, p.C);
   const dim3 scan(p.C, p.T, p.B);
   if (p.counters) {
-    hipLaunchKernelGGL((verify_scan_kernel<T, Q, true>), scan, dim3(kScanThreads), lds, s, p);
+    hipLaunchKernelGGL((verify_scan_kernel<T, float, true>), scan, dim3(kScanThreads), lds, s, p);
   } else {
     hipLaunchKernelGGL((verify_scan_kernel<T, float, false>), scan, dim3(kScanThreads), 0, s, p);
     if (const int st = check_launch()) return st;
@@ -867,7 +866,11 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
   p.B = B; p.T = T; p.V = V; p.C = verify_chunks(V);
   p.out = out; p.path = path; p.count = count;
   p.parts = reinterpret_cast<Part*>(at + ws.parts);
-  if ((ws_flags & FORGE_WS_ZEROED) && T <= 2 * kScanThreads && (int64_t)p.C * T * B <= 2 * device_cus())
+  // One launch saves an eager caller the time of making the second, 3 us; its walk waits for a counter and has half the
+  // threads. us, two launches / one, 6 nodes over 32,768 tokens, greedy, recorded: 54 chunks 7.0 / 6.6, 108 7.2 / 7.2, 216 7.3 /
+  // 8.5, 432 7.5 / 10.8, 1,296 8.4 / 18.8 (eager, 45 chunks 11.5 / 8.1); sampled 54 12.6 / 13.4, 216 12.8 / 15.0; with
+  // probabilities, 198 16.5 / 18.7.
+  if ((ws_flags & FORGE_WS_ZEROED) && !warm && T <= 2 * kScanThreads && (int64_t)p.C * T * B <= device_cus() / 2)
     p.counters = reinterpret_cast<unsigned*>(at);
   p.state = reinterpret_cast<State*>(at + ws.state);
   p.rest = reinterpret_cast<double*>(at + ws.rest);
