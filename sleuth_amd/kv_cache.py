@@ -39,7 +39,23 @@ def _set_tree(cache, parents) -> None:
         tree = cache._trees[len(rows[0])] = TokenTree(rows, cache.batch, cache.device)
     else:
         tree.set(rows)
-    cache.tree = tree
+    cache.tree = cache._last_tree = tree
+
+
+def _kept(cache, path: torch.Tensor, count: torch.Tensor, nodes: list[int]) -> list[int]:
+    """The counts of a keep, whose paths must name each row's stored nodes (the first nodes[b] of its tree) in rising order."""
+    B = cache.batch
+    if path.dim() != 2 or path.shape[0] != B or count.shape != (B,) or path.device != count.device:
+        raise ValueError(f"keep needs path [B, T] and count [B] of {B} rows on one device")
+    both = torch.cat([count[:, None], path], 1).tolist()   # (one copy to the host)
+    n = [row[0] for row in both]
+    if min(n) < 0 or max(n) > path.shape[1] or any(r + x > cache.max_len for r, x in zip(cache._rows, n)):
+        raise ValueError(f"keep needs paths and counts of {B} rows that fit the cache")
+    for row, x, most in zip(both, n, nodes):
+        at = [-1] + row[1:x + 1]
+        if at[-1] >= most or any(a >= b for a, b in zip(at, at[1:])):
+            raise ValueError("keep is for nodes that the last pass has stored, in rising order")
+    return n
 
 
 class KVCache:
@@ -62,6 +78,7 @@ class KVCache:
         self._rows_dev: torch.Tensor | None = None   # device mirror, made when rows differ
         self._history: torch.Tensor | None = None
         self.tree: TokenTree | None = None
+        self._last_tree: TokenTree | None = None   # (what keep is about, also once tree is None again)
         self._trees: dict[int, TokenTree] = {}
         # static (graph) mode
         self.static = False
@@ -147,6 +164,7 @@ class KVCache:
         the position (pos and pos_t), so nothing moves here; nor with a tree, whose nodes stand once keep says so."""
         if self.static or self.tree is not None:
             return
+        self._last_tree = None
         self._rows = [r + n for r in self._rows]
         if self._rows_dev is not None:
             self._rows_dev.add_(n)
@@ -159,10 +177,10 @@ class KVCache:
 
     def keep(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
         """Of the last pass's nodes, path[b, :count[b]] stand (tree.verify): their keys and values close up behind the row, which
-        grows by count[b]. Returns the counts."""
-        n = [int(x) for x in count.tolist()]
-        if len(n) != self.batch or min(n) < 0 or max(n) > path.shape[1] or any(r + x > self.max_len for r, x in zip(self._rows, n)):
-            raise ValueError(f"keep needs paths and counts of {self.batch} rows that fit the cache")
+        grows by count[b]. Returns the counts. ValueError, and nothing changed, where a path names what is no node of the row's
+        tree, or does not rise. Once for each pass."""
+        T = self._last_tree.T if self._last_tree is not None else 0
+        n = _kept(self, path, count, [min(T, self.max_len - r) for r in self._rows])
         if self.k[0].is_cuda:
             from . import ops
 
@@ -180,7 +198,7 @@ class KVCache:
     def reset(self) -> None:
         self.pos = 0
         self.static = False
-        self.tree = None
+        self.tree = self._last_tree = None
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()

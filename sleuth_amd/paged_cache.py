@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from .kv_cache import _set_tree
+from .kv_cache import _kept, _set_tree
 from .tree import TokenTree
 
 
@@ -61,7 +61,9 @@ class PagedKVCache:
         self._free = list(range(n - 1, -1, -1))
         self._users = [0] * n         # rows that hold a page
         self.tree: TokenTree | None = None
+        self._last_tree: TokenTree | None = None   # (what keep is about, also once tree is None again)
         self._trees: dict[int, TokenTree] = {}
+        self._forked: set[int] = set()   # rows that no pass has run since they were forked: the nodes behind them are another row's
         self._rows = [0] * batch
         self._least = [0] * batch     # rows cannot be rewound below this: pages that it would see were given back
         self._new: list[int] | None = None
@@ -130,6 +132,7 @@ class PagedKVCache:
         P = self.page_size
         need = []
         users = {}
+        self._forked.clear()
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
             if r + n > self.max_len:
                 raise ValueError(f"KV cache full ({self.max_len} tokens)")
@@ -179,6 +182,7 @@ class PagedKVCache:
             raise ValueError(f"row {into} must be empty, and another than {row}")
         if self._recording():
             raise RuntimeError("fork a paged cache's rows outside of a recorded graph")
+        self._forked.add(into)
         self._table[into] = list(self._table[row])
         for page in self._table[into]:
             if page >= 0:
@@ -270,6 +274,7 @@ class PagedKVCache:
             return   # (its nodes stand once keep says so)
         if self._recording():
             raise RuntimeError("advance a paged cache outside of a recorded graph: its lengths are the host's too")
+        self._last_tree = None
         new = self.new_tokens(n)
         self._rows = [r + x for r, x in zip(self._rows, new)]
         if self._new is None:
@@ -284,10 +289,9 @@ class PagedKVCache:
 
     def keep(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
         """KVCache.keep: path[b, :count[b]] of the last pass's nodes stand and close up; pages behind the rows' new ends come
-        back. Returns the counts."""
-        n = [int(x) for x in count.tolist()]
-        if len(n) != self.batch or min(n) < 0 or max(n) > path.shape[1] or any(r + x > self.max_len for r, x in zip(self._rows, n)):
-            raise ValueError(f"keep needs paths and counts of {self.batch} rows that fit the cache")
+        back. Returns the counts. A row's nodes are its real tokens of that pass (set_new); one forked since has none."""
+        T = self._last_tree.T if self._last_tree is not None else 0
+        n = _kept(self, path, count, [0 if b in self._forked else x for b, x in enumerate(self.new_tokens(T))])
         P = self.page_size
         into = [self._table[b][j] for b, (r, x) in enumerate(zip(self._rows, n)) if x for j in range(r // P, (r + x - 1) // P + 1)]
         if -1 in into or len(set(into)) < len(into):
@@ -312,7 +316,7 @@ class PagedKVCache:
         for b in range(self.batch):
             self.release(b)
         self._new = None
-        self.tree = None
+        self.tree = self._last_tree = None
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()

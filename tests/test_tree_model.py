@@ -343,6 +343,74 @@ def test_keep_takes_what_a_pass_has_stored():
         cache.keep(path, torch.tensor([0, 1]))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("paged", [False, True])
+def test_keep_takes_real_nodes_in_order(device, paged):
+    """A path that names padding, what is no node of the tree, or nodes out of order is refused and nothing moves; nor are
+    there nodes without a tree, behind a fork, or once other tokens are in."""
+    if paged:
+        cache = PagedKVCache([(1, 32)], 2, 64, device, torch.float32, 16)
+        cache.set_new([4, 9])
+        cache.reserve(9)
+        cache.advance(9)
+        cache.set_new([2, 5])
+    else:
+        cache = KVCache([(1, 32)], 2, 64, device, torch.float32)
+        cache.set_lengths([4, 9])
+    path = [[0, 1, -1, -1, -1], [0, 2, 3, -1, -1]]
+
+    def keep(path, count):
+        return cache.keep(torch.tensor(path, dtype=torch.int32, device=device), torch.tensor(count, dtype=torch.int32, device=device))
+
+    with pytest.raises(ValueError, match="stored"):
+        keep(path, [1, 0])                       # no tree yet
+    cache.set_tree([-1, 0, 0, 2, 1])
+    if paged:
+        cache.reserve(5)
+    for pool in (*cache.k, *cache.v):
+        pool.copy_(torch.arange(pool.numel(), device=device).view_as(pool))
+    cache.advance(5)
+    before = [pool.clone() for pool in (*cache.k, *cache.v)]
+    least = ([-1, 1, -1, -1, -1], [0, 5, -1, -1, -1], [0, 2 ** 31 - 1, -1, -1, -1], [1, 0, -1, -1, -1], [0, 0, -1, -1, -1])
+    for bad in least + (([0, 4, -1, -1, -1],) if paged else ()):   # (the row's pass had two real tokens)
+        with pytest.raises(ValueError, match="stored"):
+            keep([bad, path[1]], [2, 3])
+    with pytest.raises(ValueError, match="keep"):
+        keep(path[:1], [1])
+    with pytest.raises(ValueError, match="keep"):
+        cache.keep(torch.tensor(path[0], dtype=torch.int32, device=device), torch.tensor([1, 0], dtype=torch.int32, device=device))
+    assert all(torch.equal(x, y) for x, y in zip(before, (*cache.k, *cache.v))) and cache.seq_lens_host == [4, 9]
+    cache.set_tree(None)                         # (the nodes are still the last pass's)
+    assert keep(path, [2, 3]) == [2, 3] and cache.seq_lens_host == [6, 12]
+    cache.advance(1)                             # a pass of plain tokens
+    with pytest.raises(ValueError, match="stored"):
+        keep(path, [1, 0])
+
+
+def test_a_forks_nodes_are_the_other_rows():
+    """Nodes that lie in a shared page close up for the row whose pass stored them: a fork made since would keep what that
+    has moved already."""
+    cache = PagedKVCache([(1, 32)], 2, 64, "cpu", torch.float32, 16)
+    cache.set_new([4, 0])
+    cache.reserve(4)
+    cache.advance(4)
+    cache.set_new(None)
+    cache.set_tree([-1, 0, 0, 2, 1])
+    path = torch.tensor([[0, 2, 3, -1, -1], [0, 1, 4, -1, -1]], dtype=torch.int32)
+    cache.release(1)
+    cache.reserve(5)
+    cache.release(1)
+    cache.advance(5)
+    cache.fork(0, 1)
+    assert cache.keep(path, torch.tensor([3, 0])) == [3, 0]
+    with pytest.raises(ValueError, match="stored"):
+        cache.keep(path, torch.tensor([0, 3]))
+    assert cache.seq_lens_host == [7, 4]
+    cache.reserve(5)                             # row 1 gets pages of its own, and a pass
+    cache.advance(5)
+    assert cache.keep(path, torch.tensor([0, 3])) == [0, 3]
+
+
 @pytest.mark.gpu
 @torch.no_grad()
 def test_a_recorded_tree_keeps_its_size():
