@@ -51,7 +51,7 @@ from .config import ModelConfig
 from .norm import RMSNorm
 from .rope import apply_rope
 from .taps import make_tap, tap_active
-from .tree import tree_mask
+from .tree import static_tree_mask, tree_mask
 
 DECODE_MAX_T = 16
 _HIP_HEAD_DIMS = (32, 64, 128, 256, 512)   # 512 (Gemma 4's full layers) in bf16/fp16 only
@@ -542,7 +542,9 @@ class Attention(nn.Module):
         out = torch.zeros_like(q)
         paged = getattr(cache, "paged", False)
         T = q.shape[2]
-        lens = [int(cache.pos_t)] * q.shape[0] if getattr(cache, "static", False) else cache.seq_lens_host
+        static = getattr(cache, "static", False)   # (a recorded graph: no row's length is the host's)
+        lens = [cache.length - T] * q.shape[0] if static else cache.seq_lens_host
+        sees = static_tree_mask(tree, cache.pos_t, cache.length, self.window, self.sinks) if static else None
         for b, (L, n) in enumerate(zip(lens, cache.new_tokens(T) if paged else [T] * q.shape[0])):
             if not n:
                 continue
@@ -551,7 +553,9 @@ class Attention(nn.Module):
             else:
                 kb, vb, held = cache.k[self.layer_idx][b, :, :L + n], cache.v[self.layer_idx][b, :, :L + n], True
             rep = self.n_heads // self.n_kv
-            if tree is not None:
+            if sees is not None:
+                see = sees[b]
+            elif tree is not None:
                 see = tree_mask(tree, b, L, n, self.window, self.sinks, q.device) & held
             else:
                 see = self._mask(n, L + n, L, q.device) & held

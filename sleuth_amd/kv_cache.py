@@ -42,6 +42,15 @@ def _set_tree(cache, parents) -> None:
     cache.tree = cache._last_tree = tree
 
 
+def _native(cache) -> bool:
+    """Whether moves within a cache are the library's: on the GPU, as for the attention (SLEUTH_AMD_NO_HIP=1 keeps to torch),
+    where its 16-byte pieces fit."""
+    from .attention import hip_disabled
+
+    return cache.device.type == "cuda" and not hip_disabled() and cache.k[0].dtype in (torch.bfloat16, torch.float16, torch.float32) and \
+        all(k.shape[3] * k.element_size() % 16 == 0 for k in cache.k)
+
+
 def _kept(cache, path: torch.Tensor, count: torch.Tensor, nodes: list[int]) -> list[int]:
     """The counts of a keep, whose paths must name each row's stored nodes (the first nodes[b] of its tree) in rising order."""
     B = cache.batch
@@ -181,7 +190,7 @@ class KVCache:
         tree, or does not rise. Once for each pass."""
         T = self._last_tree.T if self._last_tree is not None else 0
         n = _kept(self, path, count, [min(T, self.max_len - r) for r in self._rows])
-        if self.k[0].is_cuda:
+        if _native(self):
             from . import ops
 
             where = dict(row_pos=self.seq_lens) if self.ragged else dict(pos=self.pos)

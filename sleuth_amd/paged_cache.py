@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from .kv_cache import _kept, _set_tree
+from .kv_cache import _kept, _native, _set_tree
 from .tree import TokenTree
 
 
@@ -167,7 +167,7 @@ class PagedKVCache:
         if not pages:
             return
         src, dst = [a for a, _ in pages], [b for _, b in pages]
-        if self.device.type == "cuda":
+        if _native(self):
             from . import ops
 
             ops.copy_pages(self.k, self.v, src, dst)
@@ -296,13 +296,13 @@ class PagedKVCache:
         into = [self._table[b][j] for b, (r, x) in enumerate(zip(self._rows, n)) if x for j in range(r // P, (r + x - 1) // P + 1)]
         if -1 in into or len(set(into)) < len(into):
             raise ValueError("keep is for nodes that the last pass has stored, in pages of their row")
-        if self.device.type == "cuda":
+        if _native(self):
             from . import ops
 
             ops.kv_compact_paged(self.k, self.v, self.page_table, self.seq_lens, path, count)
         else:
             for b, (r, x) in enumerate(zip(self._rows, n)):
-                of, to = r + path[b, :x].long(), r + torch.arange(x)
+                of, to = r + path[b, :x].long(), r + torch.arange(x, device=self.device)
                 pages = self.page_table[b].long()
                 for pool in (*self.k, *self.v):
                     pool[pages[to // P], :, to % P] = pool[pages[of // P], :, of % P]

@@ -75,14 +75,20 @@ class TokenTree:
             raise ValueError(f"these buffers hold trees of {self.T} nodes, not {len(rows[0])}")
         self.rows = rows
         self.parents.copy_(torch.tensor(rows, dtype=torch.int32).clamp(-1, self.T))
-        if self.device.type == "cuda":
+        from .attention import hip_disabled
+
+        if self.device.type == "cuda" and not hip_disabled():
             from . import ops
 
             mask, depth = ops.tree_mask(self.parents)
             self.mask.copy_(mask)
             self.depth.copy_(depth)
-        else:   # (the torch path asks see())
-            self.depth.copy_(torch.tensor([_ancestors(r)[1] for r in rows], dtype=torch.int32))
+        else:
+            trees = [_ancestors(r) for r in rows]
+            bits = torch.zeros(self.batch, self.T, 64 * self.mask.shape[2], dtype=torch.int64)
+            bits[..., :self.T] = torch.stack([see for see, _ in trees])
+            self.mask.copy_((bits.view(*self.mask.shape, 64) << torch.arange(64)).sum(-1))
+            self.depth.copy_(torch.tensor([depth for _, depth in trees], dtype=torch.int32))
 
     def see(self, row: int) -> torch.Tensor:
         """bool [T, T]: which nodes each node of a row sees."""
@@ -98,6 +104,22 @@ def tree_mask(tree: TokenTree, row: int, base: int, n: int, window: int, sinks: 
         pos = torch.cat([torch.arange(base), own])
         see &= (pos[None] > own[:, None] - window) | (pos < sinks)[None]
     return see.to(device)
+
+
+def static_tree_mask(tree: TokenTree, pos_t: torch.Tensor, length: int, window: int, sinks: int) -> torch.Tensor:
+    """tree_mask of all rows against a static cache's `length` slots, bool [B, T, length], by the device's own numbers (a
+    recorded graph computes it anew)."""
+    T, dev = tree.T, tree.device
+    slot = torch.arange(length, device=dev)
+    off = slot - pos_t
+    new, at = (off >= 0) & (off < T), off.clamp(0, T - 1)
+    among = ((tree.mask[..., None] >> torch.arange(64, device=dev)) & 1).flatten(-2)[..., :T].bool()
+    see = torch.where(new, among.index_select(2, at), off < 0)
+    if window:
+        own = pos_t + tree.depth
+        pos = torch.where(new, own.index_select(1, at), slot)
+        see &= (pos[:, None] > own[..., None] - window) | (pos < sinks)[:, None]
+    return see
 
 
 def verify(logits: torch.Tensor, tokens: torch.Tensor, *, parents: torch.Tensor | None = None, uniform: torch.Tensor | None = None,

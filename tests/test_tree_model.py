@@ -7,6 +7,7 @@ import random
 import pytest
 import torch
 
+from sleuth_amd import ops
 from sleuth_amd.config import ModelConfig
 from sleuth_amd.gated import GatedAttention
 from sleuth_amd.generate import (GraphDecoder, generate, generate_batch, ngram_draft, ngram_tree_draft, speculative_generate)
@@ -341,6 +342,100 @@ def test_keep_takes_what_a_pass_has_stored():
     cache.release(1)
     with pytest.raises(ValueError, match="stored"):
         cache.keep(path, torch.tensor([0, 1]))
+
+
+class _NoLibrary:
+    def __getattr__(self, name):
+        raise AssertionError(f"{name}: the library was called for")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@torch.no_grad()
+def test_trees_keep_to_torch_where_the_library_is_off(kind, monkeypatch):
+    """SLEUTH_AMD_NO_HIP=1: passes of trees, what they keep, forks and their copies, the generators; nothing calls the library."""
+    monkeypatch.setenv("SLEUTH_AMD_NO_HIP", "1")
+    for name in ("lib", "host"):
+        monkeypatch.setattr(ops, name, lambda: _NoLibrary())
+    for paged in (False, True):
+        model = make("cuda", **KINDS[kind])
+        cache = (PagedKVCache if paged else KVCache).for_model(model, 1, 64, **({"page_size": 16} if paged else {}))
+        prompt, tokens, parents = list(range(1, 16)), [3, 9, 4, 8], [-1, 0, 0, 2]
+        model(torch.tensor([prompt], device="cuda"), cache=cache)
+        cache.set_tree(parents)
+        logits = model(torch.tensor([tokens], device="cuda"), cache=cache).logits[0]
+        assert {blk.attn.last_path for blk in model.blocks} == {"torch"}
+        for t in range(4):
+            assert (logits[t] - _branch_logits(model, prompt, tokens, parents, t)).abs().max() < TOL
+        cache.keep(torch.tensor([[0, 2, 3, -1]], dtype=torch.int32, device="cuda"), torch.tensor([3], dtype=torch.int32, device="cuda"))
+        cache.set_tree(None)
+        after = model(torch.tensor([[7]], device="cuda"), cache=cache).logits[0, -1]
+        assert (after - model(torch.tensor([prompt + [3, 4, 8, 7]], device="cuda")).logits[0, -1]).abs().max() < TOL
+    test_samples_of_a_prompt("cuda", "sinks" if kind == "sinks" else "full")
+    want = generate(model, REPEATING, 20).new_ids
+    for graph in (False, True):
+        got = speculative_generate(model, REPEATING, 20, k=6, draft=_tree_of_truth(model, lambda i: i % 2 == 0), cuda_graph=graph,
+                                   trees=graph)
+        assert got.new_ids == want and got.stats["speculative"]["accepted"] >= 10
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", KINDS)
+@torch.no_grad()
+def test_a_static_tree_pass_in_torch(device, kind, monkeypatch):
+    """A static cache's tree, whose mask is the device's to compute, is the tree of a cache whose length the host knows."""
+    monkeypatch.setenv("SLEUTH_AMD_NO_HIP", "1")
+    model = make(device, **KINDS[kind])
+    rng = random.Random(5)
+    T = 9
+    for past in (0, 1, 12, 55):
+        parents, tokens = make_parents(rng, T, "tree"), torch.tensor([[rng.randrange(64) for _ in range(T)]], device=device)
+        logits = []
+        for static in (False, True):
+            cache = KVCache.for_model(model, 1, 64, tokens_per_step=T)
+            if past:
+                model(torch.tensor([[(3 * i) % 64 for i in range(past)]], device=device), cache=cache)
+            cache.set_tree(parents)
+            cache.static = static
+            cache.pos_t.fill_(cache.pos)
+            logits.append(model(tokens, cache=cache).logits)
+        assert (logits[0] - logits[1]).abs().max() < TOL
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tree_masks_in_torch(device, monkeypatch):
+    monkeypatch.setenv("SLEUTH_AMD_NO_HIP", "1")
+    rng = random.Random(2)
+    for T in (1, 63, 64, 65, 130):
+        rows = [make_parents(rng, T, shape) for shape in ("tree", "chain", "forest")]
+        tree = TokenTree(rows, 3, torch.device(device))
+        assert tree.mask.tolist() == [mask_of(p, T)[0] for p in rows]
+        assert tree.depth.tolist() == [mask_of(p, T)[1] for p in rows]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("paged", [False, True])
+def test_caches_of_odd_heads_move_in_torch(device, paged):
+    """Heads that are no 16-byte pieces run on the torch path, and so do their trees' moves and their forks' copies."""
+    kw = dict(page_size=16) if paged else {}
+    cache = (PagedKVCache if paged else KVCache)([(2, 6)], 2, 32, device, torch.float32, **kw)
+    if paged:
+        cache.set_new([6, 0])
+        cache.reserve(6)
+        cache.advance(6)
+        cache.k[0][cache.page_table[0, 0].item()] = torch.arange(16., device=device)[:, None]
+        cache.fork(0, 1)
+        cache.set_new(None)
+    else:
+        cache.pos = 6
+        cache.k[0].copy_(torch.arange(32., device=device)[:, None].expand(2, 2, 32, 6))
+    cache.set_tree([-1, 0, 0, 2])
+    if paged:
+        cache.reserve(4)
+    path = torch.tensor([[0, 2, 3, -1], [0, 1, -1, -1]], dtype=torch.int32, device=device)
+    assert cache.keep(path, torch.tensor([3, 2], dtype=torch.int32, device=device)) == [3, 2]
+    rows = [cache.row(0, b, 9)[0] if paged else cache.k[0][b] for b in range(2)]
+    assert rows[0][0, 5:9, 0].tolist() == [5, 6, 8, 9] and rows[1][1, 5:8, 3].tolist() == [5, 6, 7]
 
 
 @pytest.mark.parametrize("device", DEVICES)
