@@ -633,30 +633,36 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
     int* gone = l.child;     // the rejected children's tokens and weights, and chunks that are summed again
     double* weights = l.zs;
     int* again = l.sib;
-    __shared__ int ngone, nagain;
+    __shared__ int nagain;
+    int ngone = 0;
     __syncthreads();
-    if (tid == 0) ngone = nagain = 0;
+    if (tid == 0) nagain = 0;
     for (int c = tid; c < p.C; c += THREADS) {
       const Part x = keep ? l.parts[at * p.C + c] : load_part<FUSED>(parts + at * p.C + c);
       masses[c] = x.m > kNegInf ? x.z * weight(x.m, top, s) : 0.0;
     }
     __syncthreads();
     if (!probs) {
-      for (int j = at + 1 + tid; j < n; j += THREADS)
-        if (l.par[j] == at && l.es[j] > 0.0) {
-          const int g = atomicAdd(&ngone, 1);
+      // (in the nodes' order, in which their weights are added up: every wave counts them, and keeps its own nodes')
+      for (int j0 = at + 1; j0 < n; j0 += kWave) {
+        const int j = j0 + lane;
+        const bool mine = j < n && l.par[j] == at && l.es[j] > 0.0;
+        const uint64_t all = __ballot(mine);
+        if (mine && (j0 - at - 1) / kWave % WAVES == tid / kWave) {
+          const int g = ngone + __popcll(all & ((1ull << lane) - 1));
           gone[g] = l.tok[j];
           weights[g] = l.es[j];
         }
+        ngone += __popcll(all);
+      }
       __syncthreads();
       // a chunk that loses all but a thousandth of its sum is summed again: the difference could leave what is not there
-      const int most_gone = ngone;
-      for (int g = tid; g < most_gone; g += THREADS) {
+      for (int g = tid; g < ngone; g += THREADS) {
         const int c = (gone[g] + row.shift) / kVerifyChunk;
         double out_of = 0.0;
         bool first = true;
 #pragma unroll 4
-        for (int h = 0; h < most_gone; ++h) {
+        for (int h = 0; h < ngone; ++h) {
           const bool here = (gone[h] + row.shift) / kVerifyChunk == c;
           first &= !here || h >= g;
           out_of += here ? weights[h] : 0.0;
@@ -675,9 +681,8 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
 #pragma unroll
       for (int u = 0; u < PER / E; ++u) row.piece(i0 + u * E, reinterpret_cast<float(&)[E]>(x[u * E]));
       unsigned cut = 0;
-      const int most_gone = ngone;
 #pragma unroll 4
-      for (int g = 0; g < most_gone; ++g) {
+      for (int g = 0; g < ngone; ++g) {
         const int d = gone[g] - i0;
         cut |= (unsigned)d < PER ? 1u << (d & 31) : 0u;
       }

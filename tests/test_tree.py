@@ -589,6 +589,28 @@ def test_verify_on_the_streams_workspace():
 
 
 @pytest.mark.gpu
+def test_rejected_tokens_are_taken_out_in_order():
+    """A star of 459 drafts, all rejected: 458 of weight 2^-54, then one of weight 1. What is left of 3 + 2^-46 + 458 2^-54 is
+    2 + 2^-46 if they are added up in their order: half of it passes the first of what stays, 1, and not 1 + 2^-46, the second.
+    With the weight of 1 before others, those are lost to its rounding, half of what is left is up to 2^-45.2 more, and the third
+    would be the token."""
+    V, T = 1000, 460
+    x = torch.full((V,), -math.inf)
+    x[[10, 20, 900]] = 0.0
+    x[11] = -46 * math.log(2)
+    x[100:558] = -54 * math.log(2)
+    tokens = torch.tensor([[0, *range(100, 558), 20]])
+    logits = x.expand(1, T, V).cuda()
+    u = torch.full((1, T), 0.9)
+    u[0, 0] = 0.5
+    args = logits, tokens.cuda()
+    kw = dict(parents=i32([[-1] + [0] * (T - 1)]), uniform=u.cuda(), temperature=1.0)
+    for _ in range(50):
+        out, path, count = ops.verify_drafts(*args, **kw)
+        assert (out[0, 0].item(), count.item()) == (11, 1)
+
+
+@pytest.mark.gpu
 def test_verify_forms():
     """A chain by default, one tree for all, a temperature for each row, short rows, probabilities of 16 bits and of T - 1 nodes,
     strided logits."""
