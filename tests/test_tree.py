@@ -14,7 +14,7 @@ import torch
 from paged_oracle import Paged, assert_close, attend64, norm_rope64
 from sleuth_amd import _lib, ops
 from sleuth_amd.rope import rope_tables
-from tree_oracle import bits_to_bool, chain_of, compact_row, make_parents, mask_of, tree_see, verify_row
+from tree_oracle import bits_to_bool, chain_of, compact_row, make_parents, mask_of, tree_see, tree_see_long, verify_row
 
 BF, HF, SF = torch.bfloat16, torch.float16, torch.float32
 
@@ -360,6 +360,57 @@ def test_attn_tree(case):
         assert not got[b, n:].any()
 
 
+@pytest.mark.parametrize("base, n, window, sinks", [(0, 1, 0, 0), (0, 30, 4, 2), (90, 40, 20, 5), (200, 33, 300, 4), (50, 30, 7, 60)])
+def test_who_sees_whom_by_rows(base, n, window, sinks):
+    parents = make_parents(random.Random(n), n, "tree")
+    among = torch.tensor([[j in chain_of(parents, t) for j in range(n)] for t in range(n)])
+    depth = mask_of(parents, n)[1] if window else None
+    assert torch.equal(tree_see_long(base, n, among, depth, window, sinks), tree_see(base, n, among, depth, window, sinks))
+
+
+# What long batches take on 256 CUs: the chunk kernel's parts planned on the device, in one round or two, with windows or not; its
+# windowed calls that are not planned; the split kernel's blocks of 32 rows
+LONG = [
+    (BF, 16, 8, 128, 16, [9000, 200, 4100, 0, 8999, 1500, 6000, 333], 64, "tree", [64, 64, 1, 7, 64, 0, 50, 64], 0, 0),
+    (BF, 16, 8, 128, 0, [9000, 5200, 7100, 800, 8999, 9000, 6000, 8333], 60, "forest", None, 0, 0),
+    (BF, 16, 8, 128, 16, [1900 - 7 * i for i in range(40)], 64, "tree", [64 - i % 7 for i in range(40)], 0, 0),
+    (BF, 16, 8, 128, 16, [2400 - 9 * i if i % 13 else 30 * i for i in range(40)], 64, "tree", [64 - i % 5 * 13 for i in range(40)], 1900, 4),
+    (HF, 12, 4, 64, 32, [13000, 12900, 500, 0, 7000, 64, 9000, 13000], 64, "tree", [64, 3, 64, 64, 64, 64, 0, 64], 0, 0),
+    (BF, 8, 1, 256, 16, [9000, 8000, 100, 7000, 8500, 5, 31, 4000] * 2, 26, "tree", None, 0, 0),
+    (BF, 16, 1, 512, 64, [7000, 10, 6500, 6999], 40, "tree", [40, 40, 9, 40], 0, 0),
+    (SF, 16, 8, 128, 16, [4600, 4200, 100, 3000, 4600, 17, 4500, 2000], 64, "tree", None, 0, 0),
+    (BF, 8, 1, 256, 16, [5000, 700, 1030, 1100, 3000, 0, 2047, 900], 26, "tree", [26, 26, 1, 26, 0, 26, 13, 26], 1024, 4),
+    (HF, 8, 2, 256, 0, [700, 5, 1030, 3000] * 3, 40, "chain", None, 300, 64),
+    (HF, 8, 2, 256, 0, [700, 5, 1030, 3000] * 3, 40, "chain", None, 9, 2),
+    (SF, 16, 4, 64, 16, [3000, 40, 700, 1200] * 4, 40, "tree", [40, 7, 40, 0] * 4, 250, 10),
+    (BF, 16, 1, 512, 16, [900, 31, 1500], 26, "tree", None, 256, 4),
+    (BF, 16, 8, 128, 16, [2000 - 97 * i for i in range(16)], 12, "tree", [12 - i % 4 for i in range(16)], 0, 0),
+    (SF, 16, 8, 64, 0, [1900 - 90 * i for i in range(16)], 12, "tree", None, 0, 0),
+    (HF, 16, 8, 128, 32, [3000 - 101 * i for i in range(24)], 12, "tree", None, 700, 4),
+    (BF, 8, 1, 256, 16, [4300 - 100 * i for i in range(16)], 4, "forest", [4 - i % 3 for i in range(16)], 0, 0),
+    (BF, 16, 8, 32, 16, [4000 - 60 * i for i in range(16)], 14, "tree", None, 0, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LONG, ids=lambda c: _id((*c[:5], f"{len(c[5])}x{max(c[5])}", *c[6:8], *c[9:])))
+def test_attn_tree_over_long_batches(case):
+    dtype, H, K, D, page, pasts, T, shape, news, window, sinks = case
+    cache, parents, q, real = _tree_inputs(*case)
+    mask, depth = ops.tree_mask(i32(parents))
+    among, depths = bits_to_bool(mask.cpu(), T), depth.tolist()
+    got = _call(cache, page, q, mask, depth if window else None, pasts, D ** -0.5, window=window, sinks=sinks,
+                new_lens=i32(news) if news is not None else None)
+    for b, n in enumerate(real):
+        assert not got[b, n:].any()
+        if n:
+            see = tree_see_long(pasts[b], n, among[b][:n, :n], depths[b], window, sinks) & cache.held[b][None]
+            assert_close(got[b, :n], *attend64(q[b, :, :n], cache.k[b], cache.v[b], see, D ** -0.5), f"row {b}")
+    again = _call(cache, page, q, mask, depth if window else None, pasts, D ** -0.5, window=window, sinks=sinks,
+                  new_lens=i32(news) if news is not None else None)
+    assert torch.equal(got, again)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype, heads, page, T", [(BF, (16, 8, 128), 16, 40), (BF, (16, 8, 128), 0, 100), (SF, (8, 4, 32), 0, 33),
                                                    (HF, (8, 1, 256), 64, 24), (BF, (16, 1, 512), 16, 70)])
@@ -585,6 +636,29 @@ def test_verify_on_the_streams_workspace():
             got = ops.verify_drafts(logits.cuda(), tokens.cuda(), parents=i32(p), uniform=u.cuda(), temperature=1.0,
                                     draft_probs=None if q is None else q.cuda())
             _same(got, _verify_want(logits, tokens, p, u, [1.0] * len(p), q, [6] * len(p)))
+        assert torch.equal(_call(cache, 16, qs, mask, None, [0, 400], 0.1), first)
+
+
+@pytest.mark.gpu
+def test_greedy_calls_of_one_launch():
+    """Greedy calls that walk in the scan's launch (few chunks: up to half the CUs) and ones just above, rows of no node, of some
+    and of more than there are, one chunk a row and several, and other operators on the stream's workspace between them: each
+    call leaves its counters at zero, whatever its sizes."""
+    case = (BF, 16, 8, 128, 16, [0, 400], 12, "tree", None, 0, 0)
+    cache, parents, qs, real = _tree_inputs(*case)
+    mask, _ = ops.tree_mask(i32(parents))
+    first = _call(cache, 16, qs, mask, None, [0, 400], 0.1)
+    news, real = [8, 0, 1, 3, 99, -4], [8, 0, 1, 3, 8, 0]
+    calls = [(6, 8, 900, BF, "tree", news, real), (6, 8, 5000, SF, "chain", news, real), (6, 8, 9000, HF, "tree", news, real),
+             (2, 6, 9000, BF, "tree", None, [6] * 2), (1, 1, 4000, SF, "chain", [0], [0]), (1, 1, 4000, SF, "chain", [1], [1]),
+             (1, 100, 300, HF, "tree", None, [100]), (2, 64, 3000, BF, "star", [64, 7], [64, 7]), (128, 1, 50, BF, "chain", None, [1] * 128),
+             (1, 5, 32768, BF, "chain", None, [5])]
+    inputs = [_verify_inputs(B, T, V, dtype, shape, False, seed=V) for B, T, V, dtype, shape, _, _ in calls]
+    wants = [_verify_want(x[1], x[3], x[0], None, [0.0] * c[0], None, c[6]) for c, x in zip(calls, inputs)]
+    for _ in range(3):
+        for (B, T, V, dtype, shape, lens, _), (p, logits, _, tokens, _), want in zip(calls, inputs, wants):
+            for _ in range(2):
+                _same(ops.verify_drafts(logits.cuda(), tokens.cuda(), parents=i32(p), new_lens=None if lens is None else i32(lens)), want)
         assert torch.equal(_call(cache, 16, qs, mask, None, [0, 400], 0.1), first)
 
 

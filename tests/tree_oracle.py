@@ -59,6 +59,14 @@ def tree_see(base: int, n: int, among: torch.Tensor, depth: list[int] | None, wi
     return see
 
 
+def tree_see_long(base: int, n: int, among: torch.Tensor, depth: list[int] | None, window: int, sinks: int) -> torch.Tensor:
+    """tree_see by whole rows, for long caches."""
+    at = base + (torch.tensor(depth[:n]) if depth else torch.zeros(n, dtype=torch.long))
+    pos = torch.cat([torch.arange(base), at])
+    see = torch.cat([torch.ones(n, base, dtype=torch.bool), among], 1)
+    return see & ((pos[None] > at[:, None] - window) | (pos < sinks)[None]) if window else see
+
+
 def verify_row(logits: torch.Tensor, tokens: list[int], parents: list[int], u: list[float] | None, heat: float,
                probs: torch.Tensor | None, n: int) -> tuple[list[int], list[int]]:
     """(new tokens, path) of one row: logits [T, V], probs [>= T - 1, V] or None, n real nodes."""
