@@ -132,7 +132,6 @@ class PagedKVCache:
         P = self.page_size
         need = []
         users = {}
-        self._forked.clear()
         for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
             if r + n > self.max_len:
                 raise ValueError(f"KV cache full ({self.max_len} tokens)")
@@ -147,20 +146,22 @@ class PagedKVCache:
                             need.append((b, j))
                             users[page] = left - 1
         if not need:
+            self._forked.clear()
             return
         if self._recording():
             raise RuntimeError("reserve a paged cache's pages before recording a graph")
         if len(need) > len(self._free):
             raise OutOfPages(f"KV cache out of pages ({len(need)} needed, {len(self._free)} of {self.n_pages} free)")
-        copies = []
-        for b, j in need:
-            old, page = self._table[b][j], self._free.pop()
+        given = [(b, j, self._table[b][j], page) for (b, j), page in zip(need, reversed(self._free))]
+        self._copy([(old, page) for _, _, old, page in given if old >= 0])
+        # (the books last: a row whose copy failed must not find itself alone on an empty page)
+        del self._free[-len(given):]
+        for b, j, old, page in given:
             self._table[b][j] = page
             self._users[page] = 1
             if old >= 0:
                 self._users[old] -= 1
-                copies.append((old, page))
-        self._copy(copies)
+        self._forked.clear()
         self._put_table()
 
     def _copy(self, pages: list[tuple[int, int]]) -> None:

@@ -482,6 +482,37 @@ def test_keep_takes_real_nodes_in_order(device, paged):
         keep(path, [1, 0])
 
 
+def test_a_copy_that_fails_leaves_the_books():
+    """Out of memory, say, while a shared page is copied: the rows still share it, and the next reserve copies it."""
+    cache = PagedKVCache([(1, 32)], 3, 64, "cpu", torch.float32, 16)
+    cache.set_new([20, 0, 0])
+    cache.reserve(20)
+    cache.advance(20)
+    cache.fork(0, 1)
+    cache.fork(0, 2)
+    shared = cache.page_table[0, 1].item()
+    cache.v[0][shared] = 5.0
+    copy = cache._copy
+
+    def fails(pages):
+        raise torch.cuda.OutOfMemoryError("no memory")
+
+    cache._copy = fails
+    cache.set_new([20, 1, 0])                    # copies and new pages
+    free, table = list(cache._free), [list(x) for x in cache._table]
+    for _ in range(2):
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            cache.reserve(20)
+        assert (cache._free, cache._table, cache.page_table.tolist()) == (free, table, table) and cache._users[shared] == 3
+    cache._copy = copy
+    cache.reserve(20)
+    assert (cache._users[shared], cache.page_table[2, 1].item()) == (1, shared)
+    assert len({cache._table[b][1] for b in range(3)}) == 3
+    assert all((cache.v[0][cache._table[b][1]] == 5.0).all() for b in range(3))
+    cache.reset()
+    assert sorted(cache._free) == list(range(cache.n_pages)) and not any(cache._users)
+
+
 def test_a_forks_nodes_are_the_other_rows():
     """Nodes that lie in a shared page close up for the row whose pass stored them: a fork made since would keep what that
     has moved already."""
