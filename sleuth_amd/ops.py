@@ -1095,6 +1095,17 @@ def kv_compact_paged(k_pools, v_pools, page_table: torch.Tensor, row_pos: torch.
                  count, s_path, path.shape[1])
 
 
+def _page_numbers(src, dst, n_pages: int) -> tuple[list[int], list[int]]:
+    """copy_pages' lists, checked."""
+    src, dst = [int(x) for x in src], [int(x) for x in dst]
+    if len(src) != len(dst) or any(not 0 <= x < n_pages for x in src + dst):
+        raise ValueError(f"src and dst must be page numbers of a pool of {n_pages}, as many of one as of the other")
+    written = set(dst)
+    if len(written) < len(dst) or not written.isdisjoint(src):
+        raise ValueError("a page may be written once, and not be read as well")
+    return src, dst
+
+
 def copy_pages(k_pools, v_pools, src, dst) -> None:
     """Page dst[i] takes what page src[i] holds, in K and V of every layer (lists of pools [n_pages,K,page_size,D]): rows that
     fork, or write to a page they share. src and dst are lists of page numbers, which are checked (in the pool, none written
@@ -1119,12 +1130,7 @@ def copy_pages(k_pools, v_pools, src, dst) -> None:
     else:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("lists of pages are copied to the GPU: a recording takes tensors")
-        src, dst = [int(x) for x in src], [int(x) for x in dst]
-        if len(src) != len(dst) or any(not 0 <= x < n_pages for x in src + dst):
-            raise ValueError(f"src and dst must be page numbers of a pool of {n_pages}, as many of one as of the other")
-        if len(set(dst)) < len(dst) or any(x in set(src) for x in dst):
-            raise ValueError("a page may be written once, and not be read as well")
-        both = torch.tensor([src, dst], dtype=torch.int32).to(dev)
+        both = torch.tensor(_page_numbers(src, dst, n_pages), dtype=torch.int32).to(dev)
         src, dst = both[0], both[1]
     if not len(src):
         return
