@@ -89,11 +89,14 @@ class GraphDecoder:
             self._logits = self._pass()
         self._graph = g
 
+    def _room(self) -> None:
+        if self.cache.pos + self.T > self.cache.max_len:
+            raise ValueError(f"KV cache full ({self.cache.max_len} tokens)")
+
     @torch.no_grad()
     def _launch(self, tokens: torch.Tensor) -> torch.Tensor:
         c = self.cache
-        if c.pos + self.T > c.max_len:
-            raise ValueError(f"KV cache full ({c.max_len} tokens)")
+        self._room()
         self._ids.copy_(tokens.view(1, self.T))
         c.pos_t.fill_(c.pos)
         c.static = True
@@ -123,6 +126,7 @@ class GraphDecoder:
             raise ValueError("this decoder was recorded for " + ("trees" if self._trees else "chains"))
         if parents is not None and len(TokenTree._rows(parents, 1)[0]) != self.T:
             raise ValueError(f"this decoder takes trees of {self.T} nodes")   # (its graph reads their buffers)
+        self._room()   # (what is refused leaves the cache's tree as it was)
         self.cache.set_tree(parents)
         self._trees = parents is not None
         return self._launch(tokens)

@@ -554,6 +554,23 @@ def test_a_recorded_tree_keeps_its_size():
     assert torch.equal(dec.verify(tokens, [-1, 0, 0]), want)
 
 
+@pytest.mark.gpu
+@torch.no_grad()
+def test_a_refused_tree_is_not_set():
+    model = make("cuda")
+    dec = GraphDecoder(model, 16, torch.float32, 3)
+    model(torch.tensor([REPEATING[:12]], device="cuda"), cache=dec.cache)
+    tokens = torch.tensor([3, 9, 4], device="cuda")
+    dec.verify(tokens, [-1, 0, 0])
+    dec.cache.keep(torch.tensor([[0, 1, -1]], dtype=torch.int32, device="cuda"), torch.tensor([2], dtype=torch.int32, device="cuda"))
+    dec.cache.set_tree(None)
+    with pytest.raises(ValueError, match="full"):
+        dec.verify(tokens, [-1, 0, 0])
+    assert dec.cache.tree is None
+    model(torch.tensor([[5]], device="cuda"), cache=dec.cache)
+    assert dec.cache.pos == 15
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @torch.no_grad()
 def test_trees_over_forked_rows(device):
