@@ -213,7 +213,7 @@ template <typename T> __device__ __forceinline__ Row<T> logits_row(const VerifyP
 // with the temperature's scale in one part and a polynomial through seven points (1.2e-10), the exponent added as a whole
 // number, and nothing below 2^-1000: 19 instructions a logit, which are what it waits for (a bf16 logit comes from memory
 // in half that time). The argmax is looked for where it decides, at temperature 0.
-template <typename T> __device__ __forceinline__ Part scan_chunk(const VerifyParams& p, int b, int t, int c) {
+template <typename T, bool GREEDY> __device__ __forceinline__ Part scan_chunk(const VerifyParams& p, int b, int t, int c) {
   constexpr int E = Row<T>::E, U = kVerifyChunk / kScanThreads / E, WAVES = kScanThreads / kWave;
   const Row<T> row = logits_row<T>(p, b, t);
   const int first = c * kVerifyChunk - row.shift;
@@ -234,10 +234,9 @@ template <typename T> __device__ __forceinline__ Part scan_chunk(const VerifyPar
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) m = fmaxf(m, wm[w]);
-  const double heat = p.heat(b);
   double z = 0.0;
   int i = 0;
-  if (!(heat > 0.0)) {
+  if (GREEDY || !(p.heat(b) > 0.0)) {
     i = p.V;
 #pragma unroll
     for (int u = U - 1; u >= 0; --u)
@@ -425,17 +424,17 @@ struct WalkLds {
 };
 
 // A row's walk, by one block: from the chunks' numbers to its new tokens. Latency: what is read hangs on what was read
-// before, the tokens, their logits, the chunks' numbers, the one chunk that the draw falls into.
+// before, the tokens, their logits, the chunks' numbers, the one chunk that the draw falls into. FUSED: behind the scan, in its
+// launch, greedily.
 template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinline__ void walk_row(const VerifyParams& p, int b, char* smem) {
   constexpr int PER = kVerifyChunk / THREADS, WAVES = THREADS / kWave;
   const WalkLds l(smem, p.T, p.C);
   const int n = p.nodes(b), tid = threadIdx.x, lane = tid % kWave;
   int64_t* out = p.out + (int64_t)b * p.T;
   int32_t* path = p.path + (int64_t)b * p.T;
-  const double heat = p.heat(b);
-  const bool warm = heat > 0.0;
-  const Scale s = row_scale(p, b);
-  const Q* probs = static_cast<const Q*>(p.probs);
+  const bool warm = !FUSED && p.heat(b) > 0.0;
+  const Scale s = FUSED ? Scale{} : row_scale(p, b);
+  const Q* probs = FUSED ? nullptr : static_cast<const Q*>(p.probs);
 
   // Each drafted token, its parent, and the logit and probability it is judged by; the first chunks' numbers are on their
   // way meanwhile.
@@ -638,7 +637,7 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
     __syncthreads();
     if (tid == 0) nagain = 0;
     for (int c = tid; c < p.C; c += THREADS) {
-      const Part x = keep ? l.parts[at * p.C + c] : load_part<FUSED>(parts + at * p.C + c);
+      const Part x = keep ? l.parts[at * p.C + c] : parts[at * p.C + c];
       masses[c] = x.m > kNegInf ? x.z * weight(x.m, top, s) : 0.0;
     }
     __syncthreads();
@@ -717,12 +716,12 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
 }
 
 // The scan, a block a chunk. FUSED (greedy calls of few chunks): the block that ends a row's scan walks it too.
-template <typename T, typename Q, bool FUSED>
+template <typename T, bool FUSED>
 __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int c = blockIdx.x, t = blockIdx.y, b = blockIdx.z, n = p.nodes(b);
   if (t < n) {
-    const Part x = scan_chunk<T>(p, b, t, c);
+    const Part x = scan_chunk<T, FUSED>(p, b, t, c);
     Part* to = p.parts + ((int64_t)b * p.T + t) * p.C + c;
     if constexpr (!FUSED) {
       if (threadIdx.x == 0) *to = x;
@@ -741,7 +740,7 @@ __global__ __launch_bounds__(kScanThreads) void verify_scan_kernel(VerifyParams 
   } else if (!FUSED || n > 0 || t > 0 || c > 0) {
     return;
   }
-  if constexpr (FUSED) walk_row<T, Q, kScanThreads, true>(p, b, smem);
+  if constexpr (FUSED) walk_row<T, float, kScanThreads, true>(p, b, smem);
 }
 template <typename T, typename Q> __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -809,9 +808,9 @@ template <typename T, typename Q> static int launch_verify(const VerifyParams& p
   const size_t lds = WalkLds::bytes(p.T, p.C);
   const dim3 scan(p.C, p.T, p.B);
   if (p.counters) {
-    hipLaunchKernelGGL((verify_scan_kernel<T, float, true>), scan, dim3(kScanThreads), lds, s, p);
+    hipLaunchKernelGGL((verify_scan_kernel<T, true>), scan, dim3(kScanThreads), lds, s, p);
   } else {
-    hipLaunchKernelGGL((verify_scan_kernel<T, float, false>), scan, dim3(kScanThreads), 0, s, p);
+    hipLaunchKernelGGL((verify_scan_kernel<T, false>), scan, dim3(kScanThreads), 0, s, p);
     if (const int st = check_launch()) return st;
     hipLaunchKernelGGL((verify_walk_kernel<T, Q>), dim3(p.B), dim3(kWalkThreads), lds, s, p);
   }
@@ -872,9 +871,9 @@ extern "C" int forge_verify_drafts(int dtype, int B, int T, int V, const void* l
   p.out = out; p.path = path; p.count = count;
   p.parts = reinterpret_cast<Part*>(at + ws.parts);
   // One launch saves an eager caller the time of making the second, 3 us; its walk waits for a counter and has half the
-  // threads. us, two launches / one, 6 nodes over 32,768 tokens, greedy, recorded: 54 chunks 7.0 / 6.6, 108 7.2 / 7.2, 216 7.3 /
-  // 8.5, 432 7.5 / 10.8, 1,296 8.4 / 18.8 (eager, 45 chunks 11.5 / 8.1); sampled 54 12.6 / 13.4, 216 12.8 / 15.0; with
-  // probabilities, 198 16.5 / 18.7.
+  // threads. us, two launches / one, 6 nodes over 32,768 tokens, greedy, recorded: 54 chunks 7.0 / 5.8, 108 7.2 / 6.3, 216 7.3 /
+  // 7.7, 432 7.6 / 10.0, 1,296 8.4 / 17.4 (eager, 45 chunks 11.5 / 8.1). Sampled calls gain nothing (54 chunks 12.6 / 13.4, 216
+  // 12.8 / 15.0; with probabilities, 198 16.5 / 18.7): without their walk the kernel has 38 registers in place of 181.
   if ((ws_flags & FORGE_WS_ZEROED) && !warm && T <= 2 * kScanThreads && (int64_t)p.C * T * B <= device_cus() / 2)
     p.counters = reinterpret_cast<unsigned*>(at);
   p.state = reinterpret_cast<State*>(at + ws.state);
