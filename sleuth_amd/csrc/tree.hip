@@ -14,7 +14,7 @@ namespace forge {
 // ---------------------------------------------------------------- who sees whom
 // vis(t) = {t} and vis(parent of t). Doubling: after k rounds a node has its 2^k nearest ancestors, itself among them, and
 // knows the one after those, whose set it takes next; a chain of 1,024 takes ten rounds, a usual tree three. One block a
-// row. Bound by its start and the rounds' barriers: 1.9 us for a row of 12 nodes, 5.2 for 64 rows of 256.
+// row. Bound by its start and the rounds, a barrier and a row of LDS each: 1.9 us for a row of 12 nodes, 5.2 for 64 rows of 256.
 template <int W> __global__ __launch_bounds__(1024) void tree_mask_kernel(const int32_t* parents, int64_t spb,
                                                                         const int32_t* new_lens, int T, uint64_t* mask,
                                                                         int32_t* depth) {

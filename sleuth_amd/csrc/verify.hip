@@ -594,6 +594,7 @@ template <typename T, typename Q, int THREADS, bool FUSED> __device__ __forceinl
     int t = l.child[at];
     if (t >= p.T) break;
     if (warm && probs && !l.yes[t]) {
+      // (a sibling more is a row of the vocabulary more, by this one block: 52 us at 131,072 tokens in bf16)
       taken = l.zs[at];
       for (t = l.sib[t]; t < p.T; t = l.sib[t]) {
         const Rest<T, Q> rest(p, b, at, taken, l.most[at], s);
