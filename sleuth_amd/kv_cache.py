@@ -42,13 +42,16 @@ def _set_tree(cache, parents) -> None:
     cache.tree = cache._last_tree = tree
 
 
+def _pieces(shapes: list[tuple[int, int]], dtype: torch.dtype) -> bool:
+    """Whether heads of these shapes are the library's to move: whole pieces of 16 bytes, of its types."""
+    return dtype in (torch.bfloat16, torch.float16, torch.float32) and all(hd * dtype.itemsize % 16 == 0 for _, hd in shapes)
+
+
 def _native(cache) -> bool:
-    """Whether moves within a cache are the library's: on the GPU, as for the attention (SLEUTH_AMD_NO_HIP=1 keeps to torch),
-    where its 16-byte pieces fit."""
+    """Whether moves within a cache are the library's: on the GPU, as for the attention (SLEUTH_AMD_NO_HIP=1 keeps to torch)."""
     from .attention import hip_disabled
 
-    return cache.device.type == "cuda" and not hip_disabled() and cache.k[0].dtype in (torch.bfloat16, torch.float16, torch.float32) and \
-        all(k.shape[3] * k.element_size() % 16 == 0 for k in cache.k)
+    return cache.pieces and cache.device.type == "cuda" and not hip_disabled()
 
 
 def _kept(cache, path: torch.Tensor, count: torch.Tensor, nodes: list[int]) -> list[int]:
@@ -56,12 +59,12 @@ def _kept(cache, path: torch.Tensor, count: torch.Tensor, nodes: list[int]) -> l
     B = cache.batch
     if path.dim() != 2 or path.shape[0] != B or count.shape != (B,) or path.device != count.device:
         raise ValueError(f"keep needs path [B, T] and count [B] of {B} rows on one device")
-    both = torch.cat([count[:, None], path], 1).tolist()   # (one copy to the host)
-    n = [row[0] for row in both]
+    both = torch.cat([count[:, None], path], 1).cpu()   # (one copy to the host)
+    n = both[:, 0].tolist()
     if min(n) < 0 or max(n) > path.shape[1] or any(r + x > cache.max_len for r, x in zip(cache._rows, n)):
         raise ValueError(f"keep needs paths and counts of {B} rows that fit the cache")
-    for row, x, most in zip(both, n, nodes):
-        at = [-1] + row[1:x + 1]
+    for row, x, most in zip(both[:, 1:max(n) + 1].tolist(), n, nodes):
+        at = [-1] + row[:x]
         if at[-1] >= most or any(a >= b for a, b in zip(at, at[1:])):
             raise ValueError("keep is for nodes that the last pass has stored, in rising order")
     return n
@@ -83,6 +86,7 @@ class KVCache:
             self.v.append(self._arena[half + off:half + off + n].view(batch, kv, max_len, hd))
             off += n
         self.max_len, self.batch, self.device = max_len, batch, dev
+        self.pieces = _pieces(shapes, dtype)
         self._rows = [0] * batch
         self._rows_dev: torch.Tensor | None = None   # device mirror, made when rows differ
         self._history: torch.Tensor | None = None

@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import torch
 
-from .kv_cache import _kept, _native, _set_tree
+from .kv_cache import _kept, _native, _pieces, _set_tree
 from .tree import TokenTree
 
 
@@ -46,6 +46,7 @@ class PagedKVCache:
             raise ValueError("n_pages must be positive")
         dev = torch.device(device)
         self.batch, self.max_len, self.device, self.page_size, self.n_pages = batch, max_len, dev, page_size, n
+        self.pieces = _pieces(shapes, dtype)
         sizes = [n * kv * page_size * hd for kv, hd in shapes]
         half = sum(sizes)
         self._arena = torch.zeros(2 * half, device=dev, dtype=dtype)   # [all K | all V]
@@ -132,7 +133,8 @@ class PagedKVCache:
         P = self.page_size
         need = []
         users = {}
-        for b, (r, n) in enumerate(zip(self._rows, self.new_tokens(T))):
+        new = self.new_tokens(T)
+        for b, (r, n) in enumerate(zip(self._rows, new)):
             if r + n > self.max_len:
                 raise ValueError(f"KV cache full ({self.max_len} tokens)")
             if n:
@@ -146,7 +148,7 @@ class PagedKVCache:
                             need.append((b, j))
                             users[page] = left - 1
         if not need:
-            self._forked.clear()
+            self._forked.difference_update(b for b, n in enumerate(new) if n)
             return
         if self._recording():
             raise RuntimeError("reserve a paged cache's pages before recording a graph")
@@ -161,7 +163,7 @@ class PagedKVCache:
             self._users[page] = 1
             if old >= 0:
                 self._users[old] -= 1
-        self._forked.clear()
+        self._forked.difference_update(b for b, n in enumerate(new) if n)
         self._put_table()
 
     def _copy(self, pages: list[tuple[int, int]]) -> None:

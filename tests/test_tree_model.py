@@ -532,6 +532,11 @@ def test_a_forks_nodes_are_the_other_rows():
     with pytest.raises(ValueError, match="stored"):
         cache.keep(path, torch.tensor([0, 3]))
     assert cache.seq_lens_host == [7, 4]
+    cache.set_new([1, 0])                        # a pass that row 1 sits out
+    cache.reserve(1)
+    cache.set_new(None)
+    with pytest.raises(ValueError, match="stored"):
+        cache.keep(path, torch.tensor([0, 3]))
     cache.reserve(5)                             # row 1 gets pages of its own, and a pass
     cache.advance(5)
     assert cache.keep(path, torch.tensor([0, 3])) == [0, 3]
