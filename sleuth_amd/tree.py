@@ -47,6 +47,15 @@ def _ancestors(parents: list[int]) -> tuple[torch.Tensor, list[int]]:
     return see, depth
 
 
+def _packed(parents: list[int]) -> tuple[torch.Tensor, list[int]]:
+    """ops.tree_mask's bits [T, words] and depths of one tree."""
+    see, depth = _ancestors(parents)
+    T = len(parents)
+    bits = torch.zeros(T, -(-T // 64), 64, dtype=torch.int64)
+    bits.view(T, -1)[:, :T] = see
+    return (bits << torch.arange(64)).sum(-1), depth
+
+
 class TokenTree:
     """The trees of one pass, in buffers that a recorded graph may read: set() fills them anew for trees of as many nodes."""
 
@@ -84,11 +93,9 @@ class TokenTree:
             self.mask.copy_(mask)
             self.depth.copy_(depth)
         else:
-            trees = [_ancestors(r) for r in rows]
-            bits = torch.zeros(self.batch, self.T, 64 * self.mask.shape[2], dtype=torch.int64)
-            bits[..., :self.T] = torch.stack([see for see, _ in trees])
-            self.mask.copy_((bits.view(*self.mask.shape, 64) << torch.arange(64)).sum(-1))
-            self.depth.copy_(torch.tensor([depth for _, depth in trees], dtype=torch.int32))
+            masks, depths = zip(*(_packed(r) for r in rows))
+            self.mask.copy_(torch.stack(masks))
+            self.depth.copy_(torch.tensor(depths, dtype=torch.int32))
 
     def see(self, row: int) -> torch.Tensor:
         """bool [T, T]: which nodes each node of a row sees."""
