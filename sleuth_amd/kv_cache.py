@@ -39,7 +39,8 @@ def _set_tree(cache, parents) -> None:
         tree = cache._trees[len(rows[0])] = TokenTree(rows, cache.batch, cache.device)
     else:
         tree.set(rows)
-    cache.tree = cache._last_tree = tree
+    cache.tree = tree
+    cache._set_nodes = tree.T
 
 
 def _pieces(shapes: list[tuple[int, int]], dtype: torch.dtype) -> bool:
@@ -91,7 +92,8 @@ class KVCache:
         self._rows_dev: torch.Tensor | None = None   # device mirror, made when rows differ
         self._history: torch.Tensor | None = None
         self.tree: TokenTree | None = None
-        self._last_tree: TokenTree | None = None   # (what keep is about, also once tree is None again)
+        # nodes of the tree that was set last and of the one that a pass ran last (a replayed pass is not seen here): keep's
+        self._set_nodes = self._ran_nodes = 0
         self._trees: dict[int, TokenTree] = {}
         # static (graph) mode
         self.static = False
@@ -175,9 +177,12 @@ class KVCache:
     def advance(self, n: int) -> None:
         """All layers have stored n more tokens per row. In static mode the caller owns
         the position (pos and pos_t), so nothing moves here; nor with a tree, whose nodes stand once keep says so."""
-        if self.static or self.tree is not None:
+        if self.tree is not None:
+            self._ran_nodes = self.tree.T
             return
-        self._last_tree = None
+        if self.static:
+            return
+        self._set_nodes = self._ran_nodes = 0
         self._rows = [r + n for r in self._rows]
         if self._rows_dev is not None:
             self._rows_dev.add_(n)
@@ -192,7 +197,7 @@ class KVCache:
         """Of the last pass's nodes, path[b, :count[b]] stand (tree.verify): their keys and values close up behind the row, which
         grows by count[b]. Returns the counts. ValueError, and nothing changed, where a path names what is no node of the row's
         tree, or does not rise. Once for each pass."""
-        T = self._last_tree.T if self._last_tree is not None else 0
+        T = max(self._set_nodes, self._ran_nodes)
         n = _kept(self, path, count, [min(T, self.max_len - r) for r in self._rows])
         if _native(self):
             from . import ops
@@ -211,7 +216,8 @@ class KVCache:
     def reset(self) -> None:
         self.pos = 0
         self.static = False
-        self.tree = self._last_tree = None
+        self.tree = None
+        self._set_nodes = self._ran_nodes = 0
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()

@@ -62,7 +62,7 @@ class PagedKVCache:
         self._free = list(range(n - 1, -1, -1))
         self._users = [0] * n         # rows that hold a page
         self.tree: TokenTree | None = None
-        self._last_tree: TokenTree | None = None   # (what keep is about, also once tree is None again)
+        self._set_nodes = self._ran_nodes = 0   # (KVCache's)
         self._trees: dict[int, TokenTree] = {}
         self._forked: set[int] = set()   # rows that no pass has run since they were forked: the nodes behind them are another row's
         self._rows = [0] * batch
@@ -274,10 +274,11 @@ class PagedKVCache:
     def advance(self, n: int) -> None:
         """All layers have stored this pass's tokens."""
         if self.tree is not None:
+            self._ran_nodes = self.tree.T
             return   # (its nodes stand once keep says so)
         if self._recording():
             raise RuntimeError("advance a paged cache outside of a recorded graph: its lengths are the host's too")
-        self._last_tree = None
+        self._set_nodes = self._ran_nodes = 0
         new = self.new_tokens(n)
         self._rows = [r + x for r, x in zip(self._rows, new)]
         if self._new is None:
@@ -293,7 +294,7 @@ class PagedKVCache:
     def keep(self, path: torch.Tensor, count: torch.Tensor) -> list[int]:
         """KVCache.keep: path[b, :count[b]] of the last pass's nodes stand and close up; pages behind the rows' new ends come
         back. Returns the counts. A row's nodes are its real tokens of that pass (set_new); one forked since has none."""
-        T = self._last_tree.T if self._last_tree is not None else 0
+        T = max(self._set_nodes, self._ran_nodes)
         n = _kept(self, path, count, [0 if b in self._forked else x for b, x in enumerate(self.new_tokens(T))])
         P = self.page_size
         into = [self._table[b][j] for b, (r, x) in enumerate(zip(self._rows, n)) if x for j in range(r // P, (r + x - 1) // P + 1)]
@@ -319,7 +320,8 @@ class PagedKVCache:
         for b in range(self.batch):
             self.release(b)
         self._new = None
-        self.tree = self._last_tree = None
+        self.tree = None
+        self._set_nodes = self._ran_nodes = 0
 
     def nbytes(self) -> int:
         return self._arena.numel() * self._arena.element_size()

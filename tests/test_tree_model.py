@@ -475,7 +475,8 @@ def test_keep_takes_real_nodes_in_order(device, paged):
     with pytest.raises(ValueError, match="keep"):
         cache.keep(torch.tensor(path[0], dtype=torch.int32, device=device), torch.tensor([1, 0], dtype=torch.int32, device=device))
     assert all(torch.equal(x, y) for x, y in zip(before, (*cache.k, *cache.v))) and cache.seq_lens_host == [4, 9]
-    cache.set_tree(None)                         # (the nodes are still the last pass's)
+    cache.set_tree([-1, 0])                      # (the nodes are still the last pass's)
+    cache.set_tree(None)
     assert keep(path, [2, 3]) == [2, 3] and cache.seq_lens_host == [6, 12]
     cache.advance(1)                             # a pass of plain tokens
     with pytest.raises(ValueError, match="stored"):
